@@ -17,8 +17,10 @@
  * headers and static_asserts equal sizeof/offsetof for every field.
  *
  * Extensions (appended after the reference's last enumerator so every existing numeric value is
- * unchanged): DTYPE gains INT64 (argmax indices); OP_TYPE gains ARGMAX, FUSED_ELEMENTWISE,
- * SOFTMAX_CROSS_ENTROPY, SOFTMAX and LOG_SOFTMAX.
+ * unchanged): DTYPE gains INT64 (argmax indices) and the 16-bit FLOAT16 and BFLOAT16 (logits and
+ * matrices of the operators that say so); OP_TYPE gains ARGMAX, FUSED_ELEMENTWISE,
+ * SOFTMAX_CROSS_ENTROPY, SOFTMAX, LOG_SOFTMAX and TOKEN_LOGPROB. NewtonSchulz and Muon have no
+ * counterpart in the reference.
  */
 #ifndef PLAST_ABI_H
 #define PLAST_ABI_H
@@ -42,7 +44,7 @@ typedef uint64_t u64;
 /* `KernelParams.dim` value that selects a reduction over every element (reduce_ops.c:69). */
 #define PLAST_DIM_ALL (PLAST_MAX_NDIM + 1)
 
-typedef enum DTYPE { INT32 = 0, FLOAT32 = 1, INT64 = 2 } DTYPE;
+typedef enum DTYPE { INT32 = 0, FLOAT32 = 1, INT64 = 2, FLOAT16 = 3, BFLOAT16 = 4 } DTYPE;
 
 /* Device tag. The reference's second value is spelled CUDA; here it is simply "the GPU". */
 typedef enum DEVICE { CPU = 0, GPU = 1 } DEVICE;
@@ -121,6 +123,7 @@ typedef enum OP_TYPE {
   SOFTMAX_CROSS_ENTROPY,
   SOFTMAX,
   LOG_SOFTMAX,
+  TOKEN_LOGPROB,
   PLAST_NUM_OP_TYPES
 } OP_TYPE;
 
@@ -181,6 +184,27 @@ typedef struct AdamW {
   Arena *data_arena;
   Arena *optimizer_arena;
 } AdamW;
+
+/* Newton-Schulz orthogonalisation: X = G / (|G| + eps) with the Frobenius norm, then `steps` times
+ * A = X X^T, X = a X + (b A + c A A) X, on the side with fewer rows. */
+typedef struct NewtonSchulz {
+  float a;
+  float b;
+  float c;
+  float eps;
+  int steps;
+} NewtonSchulz;
+
+/* Muon: m += (1 - momentum)(g - m), u = nesterov ? g + momentum (m - g) : m, O = Newton-Schulz(u),
+ * p = p (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) O. `m` as in Adam. */
+typedef struct Muon {
+  float lr;
+  float momentum;
+  float weight_decay;
+  int nesterov;
+  NewtonSchulz rule;
+  Tensor **m;
+} Muon;
 
 #ifdef __cplusplus
 }

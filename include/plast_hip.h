@@ -99,6 +99,32 @@ PLAST_HIP_KERNEL_PAIR(softmax_cross_entropy)
 PLAST_HIP_KERNEL_PAIR(softmax)
 PLAST_HIP_KERNEL_PAIR(log_softmax)
 
+/* Log-probabilities of given tokens with the rows' entropies, and optionally each row's most likely
+ * tokens: no reference op. A row's distribution is p = softmax(x / T) over its last axis.
+ * inputs: [0] x, FLOAT32, FLOAT16 or BFLOAT16, any rank and leading strides, the last axis
+ *             contiguous; its N rows are the leading axes in row-major order;
+ *         [1] tokens, N INT32;
+ *         [2] stats, 2 N FLOAT32 (written by forward: the row's largest logit m and
+ *             log2 sum exp((x - m) / T); read by backward);
+ *         [3] entropy, N FLOAT32 (written by forward, read by backward; its grad is the upstream
+ *             gradient of the entropy, none counts as zero);
+ *         [4] top_logp, N * top FLOAT32, and [5] top_ids, N * top INT32: only where top > 0.
+ * output: logp, N FLOAT32 (its grad is the upstream gradient, none counts as zero). All but x and
+ * its grad are contiguous.
+ * params.dim: top, 0 .. PLAST_TOP_MAX; params.fval: T, finite and above 0; params.keepdim: 1 makes
+ * the backward overwrite x->grad, 0 accumulate into it.
+ *   logp = log p[token], entropy = -sum p log p, the alternatives' ids and log p in descending
+ *   order of their logits (equal logits: the lower id first; NaN above all).
+ * A negative token marks padding: the row is not read, and gets logp 0, entropy 0, alternatives
+ * (-1, -inf) and a zero gradient. A token of at least the row's length has logp NaN and a NaN
+ * gradient. A row of -inf alone has logp -inf, entropy 0 and a zero gradient; a NaN or +inf logit
+ * makes its row NaN. Rows shorter than top are filled up with (-1, -inf).
+ * Backward, x->grad of x's type and shape (any leading strides):
+ *   dx[j] (+)= (u ((j == token) - p[j]) - h p[j] (log p[j] + H)) / T
+ * for upstream u of logp and h of the entropy H. */
+#define PLAST_TOP_MAX 32
+PLAST_HIP_KERNEL_PAIR(token_logprob)
+
 #undef PLAST_HIP_KERNEL_PAIR
 
 /* ------------------------------------------------------------------ fused-chain tape --------- */
@@ -231,6 +257,33 @@ void softmax_cross_entropy_step_noalloc_hip(const float *logits, const i32 *labe
                                             const float *dloss, float *stats, float *loss,
                                             float *dlogits, float *dbias, float *mean_loss, u64 N,
                                             u64 C);
+
+/* ------------------------------------------------------------------ log-probability step ----- */
+
+/* token_logprob's forward and backward (without alternatives) in one pass, for upstream gradients
+ * that are known beforehand: each logit is read once and each gradient written once (rows that do
+ * not fit a workgroup's registers are read twice). dlogp or dentropy may be NULL (zero);
+ * dx, of x's type and shape, is written, not accumulated. All results are the same bits on every
+ * call. */
+void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor *dlogp,
+                            const Tensor *dentropy, Tensor *logp, Tensor *entropy, Tensor *dx,
+                            float temperature);
+
+/* ------------------------------------------------------------------ orthogonalised updates --- */
+
+/* out = the Newton-Schulz iteration of g, a matrix [rows, cols] or a stack [count, rows, cols] of
+ * them, each by itself: FLOAT32, FLOAT16 or BFLOAT16, any strides (out's must not overlap); out has
+ * g's type and shape and may be g itself. The iteration runs on
+ * float32-grade products: every factor is held as a pair of 16-bit floats, 22 significant bits,
+ * summed in 32 bits; entries of an iterate beyond 15 (a diverging rule) overflow to inf or NaN.
+ * No counterpart in the reference. */
+void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule);
+/* One Muon step over `num_parameters` contiguous FLOAT32 matrices of any shapes (other ranks are
+ * refused; parameters that are NULL or have no grad are skipped). Moments as in adam_step_hip:
+ * allocated and zeroed by this library when optimizer->m is NULL (freed by plast_hip_muon_release),
+ * else the caller's. Matrices of one shape run through the same launches. */
+void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters);
+void plast_hip_muon_release(Muon *optimizer, int num_parameters);
 
 /* ------------------------------------------------------------------ pack / host transfer ----- */
 

@@ -11,8 +11,8 @@ import ctypes as C
 MAX_NDIM = 8
 DIM_ALL = MAX_NDIM + 1  # reduce over every element (src/kernels/cpu/reduce_ops.c:69)
 
-# DTYPE (include/core/tensor.h:8, INT64 appended)
-INT32, FLOAT32, INT64 = 0, 1, 2
+# DTYPE (include/core/tensor.h:8, INT64 and the 16-bit floats appended)
+INT32, FLOAT32, INT64, FLOAT16, BFLOAT16 = 0, 1, 2, 3, 4
 # DEVICE (include/core/arena.h:16)
 CPU, GPU = 0, 1
 
@@ -22,6 +22,7 @@ OP_NAMES = [
     "TAN", "VIEW", "TRANSPOSE", "UNSQUEEZE", "SQUEEZE", "EXPAND", "FLATTEN", "BROADCAST", "MEAN",
     "MIN", "MAX", "SUM", "CONV2D", "MATMUL_RELU", "MATMUL_BIAS_RELU", "CONV_RELU",
     "ARGMAX", "FUSED_ELEMENTWISE", "SOFTMAX_CROSS_ENTROPY", "SOFTMAX", "LOG_SOFTMAX",
+    "TOKEN_LOGPROB",
 ]
 OP = {name: i for i, name in enumerate(OP_NAMES)}
 
@@ -143,6 +144,20 @@ class AdamW(C.Structure):
                 ("epsilon", C.c_float), ("weight_decay", C.c_float), ("t", C.c_int),
                 ("m", TensorPP), ("v", TensorPP), ("data_arena", C.POINTER(Arena)),
                 ("optimizer_arena", C.POINTER(Arena))]
+
+
+# Newton-Schulz and Muon (include/plast_abi.h; no reference counterpart)
+class NewtonSchulz(C.Structure):
+    _fields_ = [("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("eps", C.c_float),
+                ("steps", C.c_int)]
+
+
+class Muon(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float),
+                ("nesterov", C.c_int), ("rule", NewtonSchulz), ("m", TensorPP)]
+
+
+TOP_MAX = 32  # alternatives of token_logprob (PLAST_TOP_MAX)
 
 
 def params(dim: int = 0, keepdim: int = 0, fval: float = 0.0) -> KernelParams:

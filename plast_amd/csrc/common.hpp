@@ -418,6 +418,7 @@ bool broadcast_shape(const Tensor *a, const Tensor *b, uint64_t *shape, int *ran
 
 uint64_t numel(const Tensor *t);
 bool same_shape(const Tensor *a, const Tensor *b);
+inline bool is_half(const Tensor *t) { return t->dtype == FLOAT16 || t->dtype == BFLOAT16; }
 // Row-major contiguity with every stride checked (size-1 axes ignored).
 bool contiguous(const Tensor *t);
 

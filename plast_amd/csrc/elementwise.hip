@@ -275,6 +275,10 @@ void view_like_backward(Tensor **in, const Tensor *out, const char *where) {
   if (!ensure_init()) return;
   Tensor *a = in[0];
   if (!a->requires_grad || !out->grad || !a->grad) return;
+  if (is_half(a->grad) || is_half(out->grad)) {
+    report_error(where, "gradients of 16-bit views are not accumulated");
+    return;
+  }
   reshape_accumulate(static_cast<float *>(a->grad->data),
                      static_cast<const float *>(out->grad->data), numel(a), where);
   finish(where);
@@ -394,6 +398,10 @@ void transpose_hip_forward(const Tensor **inputs, Tensor *output, KernelParams p
 void transpose_hip_backward(Tensor **inputs, const Tensor *output, KernelParams params) {
   Tensor *a = inputs[0];
   if (!a->requires_grad || !output->grad || !a->grad) return;
+  if (is_half(a->grad) || is_half(output->grad)) {
+    report_error("transpose_hip_backward", "gradients of 16-bit views are not accumulated");
+    return;
+  }
   transpose_backward_hip(static_cast<float *>(a->grad->data),
                          static_cast<const float *>(output->grad->data), a->shape,
                          a->grad->strides, output->grad->strides, a->ndim, params.dim,

@@ -47,6 +47,7 @@ Op make_op(OP_TYPE t) {
     SLOT(SOFTMAX_CROSS_ENTROPY, softmax_cross_entropy)
     SLOT(SOFTMAX, softmax)
     SLOT(LOG_SOFTMAX, log_softmax)
+    SLOT(TOKEN_LOGPROB, token_logprob)
 #undef SLOT
   default:
     break;  // MATMUL, CONV2D and their fused epilogues have no GPU slot here

@@ -80,8 +80,10 @@ struct CopyBody : ScalarBody<CopyBody> {
 uint64_t elem_words(DTYPE d) { return d == INT64 ? 2 : 1; }
 
 // Space over tensor t viewed as 4-byte words: operand `strided` follows t's strides, the other
-// operand is the contiguous image. False when t has more axes than a space can hold.
+// operand is the contiguous image. False when t has more axes than a space can hold, or elements of
+// two bytes.
 bool word_space(const Tensor *t, Space &s, int strided) {
+  if (is_half(t)) return false;
   const uint64_t w = elem_words(t->dtype);
   const int rank = int(t->ndim) + (w > 1 ? 1 : 0);
   if (rank > kMaxRank) return false;
@@ -107,7 +109,8 @@ bool word_space(const Tensor *t, Space &s, int strided) {
 bool pack_into(const Tensor *t, void *dst, const char *where) {
   Space s;
   if (!word_space(t, s, 0)) {
-    report_error(where, "rank %llu is too large", (unsigned long long)t->ndim);
+    report_error(where, "a strided tensor of rank %llu and dtype %d cannot be packed",
+                 (unsigned long long)t->ndim, int(t->dtype));
     return false;
   }
   const void *ins[1] = {t->data};
@@ -124,14 +127,17 @@ bool unpack_from(const void *src, Tensor *t, const char *where) {
     }
   Space s;
   if (!word_space(t, s, 1)) {
-    report_error(where, "rank %llu is too large", (unsigned long long)t->ndim);
+    report_error(where, "a strided tensor of rank %llu and dtype %d cannot be packed",
+                 (unsigned long long)t->ndim, int(t->dtype));
     return false;
   }
   const void *ins[1] = {src};
   return launch_elementwise(CopyBody{}, ins, t->data, s, where);
 }
 
-uint64_t tensor_bytes(const Tensor *t) { return numel(t) * 4 * elem_words(t->dtype); }
+uint64_t tensor_bytes(const Tensor *t) {
+  return is_half(t) ? numel(t) * 2 : numel(t) * 4 * elem_words(t->dtype);
+}
 
 }  // namespace
 }  // namespace plast

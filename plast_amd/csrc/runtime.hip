@@ -536,7 +536,9 @@ void arena_memcpy_d2d_hip(void *dest, const void *src, u64 size) {
 
 // ---- fill hooks (include/kernels/cuda/cuda_tensor_init.h:9-11)
 
-static uint64_t dtype_bytes(DTYPE d) { return d == INT64 ? 8 : 4; }
+static uint64_t dtype_bytes(DTYPE d) {
+  return d == INT64 ? 8 : d == FLOAT16 || d == BFLOAT16 ? 2 : 4;
+}
 
 void zeros_hip(Tensor *t, u64 num_elements) {
   if (!t || !ensure_init()) return;

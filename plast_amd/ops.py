@@ -8,7 +8,7 @@ import ctypes as C
 import numpy as np
 
 from . import abi
-from .abi import DIM_ALL, FLOAT32, INT32, INT64, KernelParams
+from .abi import BFLOAT16, DIM_ALL, FLOAT32, INT32, INT64, KernelParams
 from .runtime import DeviceTensor, backward, forward, lib
 
 
@@ -99,6 +99,49 @@ def softmax_cross_entropy(logits: DeviceTensor, labels: DeviceTensor, requires_g
     return loss, stats
 
 
+def bfloat16_bits(values) -> np.ndarray:
+    """The bit patterns (uint16, what a BFLOAT16 tensor's host image holds) of float32 values rounded
+    to the nearest bfloat16, ties to even."""
+    v = np.ascontiguousarray(values, np.float32)
+    b = v.view(np.uint32).astype(np.uint64)
+    b = ((b + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(v), np.uint16(0x7FC0), b)
+
+
+def bfloat16_values(bits) -> np.ndarray:
+    """The float32 values of bfloat16 bit patterns."""
+    return (np.ascontiguousarray(bits, np.uint16).astype(np.uint32) << 16).view(np.float32)
+
+
+def token_logprob(x: DeviceTensor, tokens: DeviceTensor, temperature: float = 1.0, top: int = 0,
+                  requires_grad: bool = False):
+    """Log-probability of each row's token under softmax(x / temperature) and the row's entropy, with
+    the `top` most likely alternatives. Returns (inputs, logp, params): `inputs` are
+    [x, tokens, stats, entropy] and, with top > 0, top_logp and top_ids; backward("token_logprob",
+    inputs, logp, params) accumulates into x's gradient from those of logp and entropy."""
+    lead = abi.shape_of(x.t)[:-1]
+    stats = DeviceTensor(lead + (2,), FLOAT32, zero=False)
+    entropy = DeviceTensor(lead, FLOAT32, requires_grad, zero=False)
+    logp = DeviceTensor(lead, FLOAT32, requires_grad, zero=False)
+    inputs = [x, tokens, stats, entropy]
+    if top:
+        inputs += [DeviceTensor(lead + (top,), FLOAT32, zero=False),
+                   DeviceTensor(lead + (top,), INT32, zero=False)]
+    p = KernelParams(top, 0, temperature)
+    forward("token_logprob", inputs, logp, p)
+    return inputs, logp, p
+
+
+def newton_schulz(g: DeviceTensor, steps: int = 5, a: float = 3.4445, b: float = -4.7750,
+                  c: float = 2.0315, eps: float = 1e-7) -> DeviceTensor:
+    """The orthogonalised g, a matrix or a stack of matrices (newton_schulz_hip)."""
+    out = DeviceTensor(abi.shape_of(g.t), g.dtype, zero=False)
+    rule = abi.NewtonSchulz(a, b, c, eps, steps)
+    lib().newton_schulz_hip(C.byref(g.t), C.byref(out.t), C.byref(rule))
+    lib().check("newton_schulz")
+    return out
+
+
 def make_tape(instructions, num_inputs: int) -> abi.FusedTape:
     """instructions: list of (op_name, src, idx, acc_rhs, imm)."""
     tape = abi.FusedTape()
@@ -117,5 +160,5 @@ def fused(tape: abi.FusedTape, inputs, shape) -> DeviceTensor:
 
 
 __all__ = ["binary", "unary", "reduce", "transpose", "permute", "expand", "softmax_cross_entropy",
-           "make_tape", "fused", "broadcast_shape", "reduced_shape", "backward", "forward", "lib",
+           "token_logprob", "newton_schulz", "bfloat16_bits", "bfloat16_values", "BFLOAT16", "make_tape", "fused", "broadcast_shape", "reduced_shape", "backward", "forward", "lib",
            "DeviceTensor", "np", "INT32"]

@@ -14,17 +14,21 @@ from pathlib import Path
 import numpy as np
 
 from . import abi
-from .abi import FLOAT32, GPU, INT32, INT64, KernelParams, Tensor, TensorP, TensorPP
+from .abi import (BFLOAT16, FLOAT16, FLOAT32, GPU, INT32, INT64, KernelParams, Tensor, TensorP,
+                  TensorPP)
 
 LIB_PATH = Path(__file__).resolve().parent / "libplast_hip.so"
 
-_NP_DTYPE = {FLOAT32: np.float32, INT32: np.int32, INT64: np.int64}
-_DT_OF_NP = {np.dtype(np.float32): FLOAT32, np.dtype(np.int32): INT32, np.dtype(np.int64): INT64}
+# numpy has no bfloat16: a BFLOAT16 tensor's host image holds its bit patterns
+_NP_DTYPE = {FLOAT32: np.float32, INT32: np.int32, INT64: np.int64, FLOAT16: np.float16,
+             BFLOAT16: np.uint16}
+_DT_OF_NP = {np.dtype(np.float32): FLOAT32, np.dtype(np.int32): INT32, np.dtype(np.int64): INT64,
+             np.dtype(np.float16): FLOAT16, np.dtype(np.uint16): BFLOAT16}
 
 OP_NAMES = ["add", "sub", "mul", "div", "exp", "log", "neg", "abs", "sin", "cos", "tan",
             "leaky_relu", "sum", "mean", "max", "min", "argmax", "view", "flatten", "squeeze",
             "unsqueeze", "expand", "broadcast", "transpose", "fused_elementwise",
-            "softmax_cross_entropy", "softmax", "log_softmax"]
+            "softmax_cross_entropy", "softmax", "log_softmax", "token_logprob"]
 
 
 class PlastHipError(RuntimeError):
@@ -83,6 +87,10 @@ class Library:
             "adam_step_hip": ([C.POINTER(abi.Adam), TensorPP, C.c_int], None),
             "adamw_step_hip": ([C.POINTER(abi.AdamW), TensorPP, C.c_int], None),
             "zero_grad_hip": ([TensorP], None),
+            "token_logprob_step_hip": ([C.c_void_p] * 7 + [C.c_float], None),
+            "newton_schulz_hip": ([C.c_void_p] * 3, None),
+            "muon_step_hip": ([C.c_void_p, C.c_void_p, C.c_int], None),
+            "plast_hip_muon_release": ([C.POINTER(abi.Muon), C.c_int], None),
             "plast_hip_adam_release": ([C.POINTER(abi.Adam), C.c_int], None),
             "plast_hip_adamw_release": ([C.POINTER(abi.AdamW), C.c_int], None),
             "hip_tensor_pack_init": ([C.POINTER(abi.HipTensorPack), TensorP], None),
