@@ -4,6 +4,20 @@
 // With G on the side with m <= n rows (transposed where it has more rows than columns) and
 // X = G / (|G| + eps), Frobenius norm, each of `steps` iterations is
 //   A = X X^T (m x m),  S = b A + c A A (m x m),  X = a X + S X (m x n).
+// A and S are symmetric: their products compute the tiles on and below the diagonal and store each twice.
+//
+// The products run on the matrix units. fp32's own matrix instructions reach a sixteenth of fp16's rate,
+// so every factor v is kept as two fp16, hi = round(v) and lo = round(v - hi), 22 significant bits (and a
+// scale that keeps lo above fp16's subnormals: X and A times 2^12, S times 2^11), and a product is three
+// instructions, hi hi + hi lo + lo hi, summed in fp32. What is left out, lo lo, is below 2^-22 of the
+// product. The iteration in 64 bits is met to 4e-7 of the result at [256, 256] and [300, 800], where
+// fp32 factors (24 bits, but one rounding per addition) meet it to 1.5e-6 and 1.8e-6.
+//
+// Layout of a factor ("lines"): each row is cut into lines of 128 bytes, a line holding 32 columns' hi
+// and then their lo: what a workgroup's tile needs of a row in one step of the sum is one whole line, read
+// from HBM, staged in LDS and read from there in 16-byte units. Rows and columns are padded with zeros to
+// whole tiles, so the product has no bounds to check. Both operands of each product are read along their
+// rows, X X^T, A A^T and S (X^T)^T, so X is kept in both orders; the update writes both.
 #include <cfloat>
 #include <cmath>
 #include <cstdlib>
@@ -17,7 +31,11 @@ namespace plast {
 namespace {
 
 constexpr int kNsBlock = 256;
-constexpr uint32_t kNormParts = 64;  // workgroups that share a matrix's norm
+constexpr uint32_t kNormParts = 1024;  // most workgroups that share a matrix's norm
+constexpr int kPointers = 64;          // matrices of a launch that have pointers of their own
+
+typedef f16_t h8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 // A stack of matrices with any strides, in elements.
 struct Stack {
@@ -26,126 +44,560 @@ struct Stack {
   int64_t sb, s0, s1;
 };
 
-// |G|^2 in 64 bits, where neither the squares nor their sum overflow or vanish: one partial sum
-// per workgroup, then one per matrix in norm_scale.
-template <class T>
-__global__ __launch_bounds__(kNsBlock) void norm_kernel(Stack G, double *part) {
+struct MuonRule {
+  float momentum, keep, scale;  // keep: 1 - lr decay; scale: lr sqrt(max(1, rows / cols))
+  int nesterov;
+};
+// The matrices of a Muon launch.
+struct MuonSet {
+  const float *g[kPointers];
+  float *m[kPointers], *p[kPointers];
+  MuonRule rule;
+};
+__device__ __forceinline__ float muon_update(float g, float m, const MuonRule &R) {
+  return R.nesterov ? (1.0f - R.momentum) * g + R.momentum * m : m;
+}
+
+// ------------------------------------------------------------------------- norms
+
+__device__ __forceinline__ double block_sum(double s) {
   __shared__ double lds[kNsBlock / 64];
-  const T *g = static_cast<const T *>(G.data) + int64_t(blockIdx.y) * G.sb;
-  double s = 0.0;
-  for (uint32_t i = blockIdx.x; i < G.rows; i += gridDim.x)
-    for (uint32_t j = threadIdx.x; j < G.cols; j += kNsBlock) {
-      const double v = double(float(g[int64_t(i) * G.s0 + int64_t(j) * G.s1]));
-      s += v * v;
-    }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < kNsBlock / 64; ++k) s += lds[k];
-    part[uint64_t(blockIdx.y) * kNormParts + blockIdx.x] = s;
-  }
+  s = lds[0];
+  for (int k = 1; k < kNsBlock / 64; ++k) s += lds[k];
+  return s;
 }
 
-// 1 / (|G| + eps) of matrix b from its partial sums, by every thread.
-__device__ __forceinline__ double norm_scale(const double *part, uint32_t b, uint32_t parts, float eps) {
-  double s = 0.0;
-  for (uint32_t k = 0; k < parts; ++k) s += part[uint64_t(b) * kNormParts + k];
-  return 1.0 / (sqrt(s) + double(eps));
-}
-
-// X[b] [m, n] = G[b] * scale, transposed where G has more rows than columns.
+// |G|^2 in 64 bits, where neither the squares nor their sum overflow or vanish: one partial sum per
+// workgroup.
 template <class T>
-__global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, const double *part, uint32_t parts,
-                                                         float eps, float *X, uint32_t m, uint32_t n) {
-  const uint32_t b = blockIdx.z, i = blockIdx.y, j = blockIdx.x * kNsBlock + threadIdx.x;
-  if (j >= n) return;
-  const double scale = norm_scale(part, b, parts, eps);
+__global__ __launch_bounds__(kNsBlock) void norm_kernel(Stack G, MagicDiv cols, double *part) {
+  const T *g = static_cast<const T *>(G.data) + int64_t(blockIdx.y) * G.sb;
+  const uint32_t n = G.rows * G.cols, stride = gridDim.x * kNsBlock;  // below 2^32
+  double s = 0.0;
+  for (uint64_t at = uint64_t(blockIdx.x) * kNsBlock + threadIdx.x; at < n; at += stride) {
+    const uint32_t i = cols.div(uint32_t(at)), j = uint32_t(at) - i * G.cols;
+    const double v = double(float(g[int64_t(i) * G.s0 + int64_t(j) * G.s1]));
+    s += v * v;
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) part[uint64_t(blockIdx.y) * kNormParts + blockIdx.x] = s;
+}
+
+// Muon's: the momentum is updated in the same pass, and the norm is the update's.
+__global__ __launch_bounds__(kNsBlock) void momentum_kernel(MuonSet S, uint64_t n, double *part) {
+  const float *g = S.g[blockIdx.y];
+  float *m = S.m[blockIdx.y];
+  const bool vec = ((uintptr_t(g) | uintptr_t(m)) & 15) == 0;
+  const uint64_t n4 = vec ? n / 4 : 0, at = uint64_t(blockIdx.x) * kNsBlock + threadIdx.x;
+  const uint64_t stride = uint64_t(gridDim.x) * kNsBlock;
+  const float b = S.rule.momentum;
+  double s = 0.0;
+  for (uint64_t i = at; i < n4; i += stride) {
+    const f4 gi = reinterpret_cast<const f4 *>(g)[i];
+    f4 v = reinterpret_cast<const f4 *>(m)[i];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      v[c] = b * v[c] + (1.0f - b) * gi[c];
+      const double u = double(muon_update(gi[c], v[c], S.rule));
+      s += u * u;
+    }
+    reinterpret_cast<f4 *>(m)[i] = v;
+  }
+  for (uint64_t i = n4 * 4 + at; i < n; i += stride) {
+    const float v = b * m[i] + (1.0f - b) * g[i];
+    m[i] = v;
+    const double u = double(muon_update(g[i], v, S.rule));
+    s += u * u;
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) part[uint64_t(blockIdx.y) * kNormParts + blockIdx.x] = s;
+}
+
+// |G| of matrix b from its partial sums, for a workgroup.
+__device__ __forceinline__ double norm_of(const double *part, uint32_t b, uint32_t parts) {
+  double s = 0.0;
+  for (uint32_t k = threadIdx.x; k < parts; k += kNsBlock) s += part[uint64_t(b) * kNormParts + k];
+  return sqrt(block_sum(s));
+}
+
+// ------------------------------------------------------------------------- lines
+
+constexpr float kScaleX = 4096.0f, kScaleA = 4096.0f, kScaleS = 2048.0f;
+
+// The power of two that X is kept times. 2^12 where |X| = |G| / (|G| + eps) is about 1. A smaller |G|
+// leaves a small X, whose iterates grow by up to `growth` bits in all, a being their largest factor: it is
+// raised by the bits that X lacks, less those that it may still grow by and has no room for.
+__device__ __forceinline__ double scale_of_x(double norm, float eps, int growth) {
+  const double x = norm / (norm + double(eps));
+  int lacks = x > 0.0 && x < 0.5 ? -ilogb(x) - 1 : 0;
+  lacks = lacks > 110 ? 110 : lacks;
+  const int grows = lacks < growth ? lacks : growth;
+  return ldexp(double(kScaleX), lacks - (grows > 3 ? grows - 3 : 0));
+}
+
+// A stack of factors in lines: `rows` padded rows of `pitch` bytes.
+struct Lines {
+  char *data;
+  uint64_t pitch, next;  // bytes from one row, one matrix to the next
+};
+__device__ __forceinline__ char *line_at(const Lines &L, uint32_t b, uint32_t row, uint32_t col) {
+  return L.data + b * L.next + row * L.pitch + (col >> 5) * 128 + (col & 31) * 2;
+}
+// Eight columns (a multiple of 8) of a row.
+__device__ __forceinline__ void put8(char *at, const float *v) {
+  h8 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    hi[e] = f16_t(v[e]);
+    lo[e] = f16_t(v[e] - float(hi[e]));
+  }
+  *reinterpret_cast<h8 *>(at) = hi;
+  *reinterpret_cast<h8 *>(at + 64) = lo;
+}
+__device__ __forceinline__ void get8(const char *at, float *v) {
+  const h8 hi = *reinterpret_cast<const h8 *>(at), lo = *reinterpret_cast<const h8 *>(at + 64);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = float(hi[e]) + float(lo[e]);
+}
+
+// X and X^T in lines from the source, a 64x64 tile per workgroup, padding included.
+template <class T, bool MUON>
+__global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, const double *part,
+                                                         uint32_t parts, float eps, int growth, Lines X,
+                                                         Lines XT, float *xscale) {
+  __shared__ float tile[64][65];
+  const uint32_t b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of the source
+  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth);
+  const double scale = sx / (norm + double(eps));
+  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) xscale[b] = float(sx);
   const bool tall = G.rows > G.cols;
   const T *g = static_cast<const T *>(G.data) + int64_t(b) * G.sb;
-  const float v = float(g[int64_t(tall ? j : i) * G.s0 + int64_t(tall ? i : j) * G.s1]);
-  X[(uint64_t(b) * m + i) * n + j] = float(double(v) * scale);
+  for (uint32_t e = threadIdx.x; e < 64 * 64; e += kNsBlock) {
+    const uint32_t r = r0 + e / 64, c = c0 + e % 64;
+    float v = 0.0f;
+    if (r < G.rows && c < G.cols) {
+      if constexpr (MUON) {
+        const uint64_t at = uint64_t(r) * G.cols + c;
+        v = muon_update(S.g[b][at], S.m[b][at], S.rule);
+      } else {
+        v = float(g[int64_t(r) * G.s0 + int64_t(c) * G.s1]);
+      }
+    }
+    tile[e / 64][e % 64] = float(double(v) * scale);
+  }
+  __syncthreads();
+  const Lines &R = tall ? XT : X, &C = tall ? X : XT;
+  for (uint32_t e = threadIdx.x; e < 64 * 8; e += kNsBlock) {
+    const uint32_t r = e / 8, c = e % 8 * 8;
+    float v[8], w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v[k] = tile[r][c + k];
+      w[k] = tile[c + k][r];
+    }
+    put8(line_at(R, b, r0 + r, c0 + c), v);
+    put8(line_at(C, b, c0 + r, r0 + c), w);
+  }
 }
 
-template <class T>
-__global__ __launch_bounds__(kNsBlock) void finish_kernel(const float *X, uint32_t m, uint32_t n, Stack O) {
-  const uint32_t b = blockIdx.z, i = blockIdx.y, j = blockIdx.x * kNsBlock + threadIdx.x;
-  if (j >= n) return;
-  const bool tall = O.rows > O.cols;
-  T *o = static_cast<T *>(const_cast<void *>(O.data)) + int64_t(b) * O.sb;
-  o[int64_t(tall ? j : i) * O.s0 + int64_t(tall ? i : j) * O.s1] = T(X[(uint64_t(b) * m + i) * n + j]);
-}
+// ------------------------------------------------------------------------- products
 
-// C = alpha A B + beta D over row-major C, D [p, q]; A[i, k] and B[k, j] by strides. 64x64 tiles,
-// 4x4 outputs a lane, both operands staged through LDS.
+enum Mode { Gram, Square, Update, Final };
+
+// Where the last step's result goes: out[b][i, j] (O), or p = p keep - scale * it.
 struct Product {
-  const float *a, *b, *d;
-  float *c;
-  uint32_t p, q, k;
-  int64_t a0, a1, b0, b1;      // strides
-  uint64_t ab, bb, cb;         // from one matrix of the stack to the next
-  float alpha, beta;
+  Lines u, v;         // the factors: C[i, j] = sum_k u[i, k] v[j, k]
+  Lines in, in_t;     // the term added: A (Square), X and X^T (Update, Final)
+  Lines out, out_t;   // the result and its transpose
+  uint32_t lines;     // of a row
+  uint32_t ti, tj;    // tiles
+  uint32_t parts;     // the sum is cut into so many pieces
+  float *partial;     // their sums, when there are several
+  float alpha, beta;  // result = alpha * sum + beta * term, in the result's scale, of
+  const float *xscale;  // X's scale in Gram and Final: by 1 / its square, 1 / it
+  Stack o;
 };
-__global__ __launch_bounds__(kNsBlock) void product_kernel(Product P) {
-  __shared__ float la[16][64 + 4], lb[16][64 + 4];
-  const uint32_t i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-  const float *a = P.a + blockIdx.z * P.ab, *b = P.b + blockIdx.z * P.bb;
-  const int ti = threadIdx.x / 16, tj = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (uint32_t k0 = 0; k0 < P.k; k0 += 16) {
-    for (int e = threadIdx.x; e < 16 * 64; e += kNsBlock) {
-      const uint32_t kk = e % 16, r = e / 16;
-      la[kk][r] = i0 + r < P.p && k0 + kk < P.k ? a[int64_t(i0 + r) * P.a0 + int64_t(k0 + kk) * P.a1] : 0.0f;
-      lb[kk][r] = j0 + r < P.q && k0 + kk < P.k ? b[int64_t(k0 + kk) * P.b0 + int64_t(j0 + r) * P.b1] : 0.0f;
-    }
-    __syncthreads();
-    for (int kk = 0; kk < 16; ++kk)
-      for (int u = 0; u < 4; ++u)
-        for (int v = 0; v < 4; ++v)
-          acc[u][v] = __builtin_fmaf(la[kk][ti * 4 + u], lb[kk][tj * 4 + v], acc[u][v]);
-    __syncthreads();
+
+// A block of 32x32 sums as the matrix unit leaves it: register r of a lane holds row
+// 8 (r / 4) + 4 (lane / 32) + r % 4 of column lane % 32. It goes through LDS, so that rows and columns
+// both leave as whole lines.
+constexpr int kBlockLds = 32 * 33;
+// Orders a wave's writes to its part of LDS before its lanes' reads of each other's.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+template <class T, Mode M, bool MUON>
+__device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, float *lds, f16v acc, uint32_t b,
+                                          uint32_t i0, uint32_t j0, bool mirror) {
+  const uint32_t lane = threadIdx.x & 63;
+  float alpha = P.alpha, beta = P.beta;
+  if constexpr (M == Gram || M == Final) {
+    const float unscale = 1.0f / P.xscale[b];  // a power of two
+    alpha *= unscale;
+    if constexpr (M == Gram) alpha *= unscale;
+    else beta *= unscale;
   }
-  for (int u = 0; u < 4; ++u)
-    for (int v = 0; v < 4; ++v) {
-      const uint32_t i = i0 + ti * 4 + u, j = j0 + tj * 4 + v;
-      if (i >= P.p || j >= P.q) continue;
-      const uint64_t at = blockIdx.z * P.cb + uint64_t(i) * P.q + j;
-      P.c[at] = P.alpha * acc[u][v] + (P.d ? P.beta * P.d[at] : 0.0f);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) lds[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * 33 + lane % 32] = alpha * acc[r];
+  wave_sync();
+  const uint32_t r = lane / 2, c = lane % 2 * 16;
+  if constexpr (M == Final) {
+    const bool tall = P.o.rows > P.o.cols;  // then the result is the transpose
+    if (!tall) {
+      float v[16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) get8(line_at(P.in, b, i0 + r, j0 + c + 8 * h), v + 8 * h);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) lds[r * 33 + c + e] += beta * v[e];
+    } else {
+      float v[16];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) get8(line_at(P.in_t, b, j0 + r, i0 + c + 8 * h), v + 8 * h);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) lds[(c + e) * 33 + r] += beta * v[e];
     }
+    wave_sync();
+    const uint32_t k = lane % 32;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const uint32_t q = 2 * e + lane / 32;
+      const float v = tall ? lds[k * 33 + q] : lds[q * 33 + k];
+      const uint32_t row = (tall ? j0 : i0) + q, col = (tall ? i0 : j0) + k;
+      if (row >= P.o.rows || col >= P.o.cols) continue;
+      if constexpr (MUON) {
+        float *p = S.p[b] + uint64_t(row) * P.o.cols + col;
+        *p = *p * S.rule.keep - S.rule.scale * v;
+      } else {
+        T *o = static_cast<T *>(const_cast<void *>(P.o.data)) + int64_t(b) * P.o.sb;
+        o[int64_t(row) * P.o.s0 + int64_t(col) * P.o.s1] = T(v);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[8], t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = lds[r * 33 + c + 8 * h + e];
+      if constexpr (M != Gram) {
+        get8(line_at(P.in, b, i0 + r, j0 + c + 8 * h), t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(beta, t[e], v[e]);
+      }
+      put8(line_at(P.out, b, i0 + r, j0 + c + 8 * h), v);
+    }
+    if (mirror)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[8], t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = lds[(c + 8 * h + e) * 33 + r];
+        if constexpr (M != Gram) {
+          get8(line_at(P.in_t, b, j0 + r, i0 + c + 8 * h), t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(beta, t[e], v[e]);
+        }
+        put8(line_at(P.out_t, b, j0 + r, i0 + c + 8 * h), v);
+      }
+  }
+  wave_sync();
 }
 
-void product(const Product &P, uint32_t count) {
-  product_kernel<<<dim3(ceil_div(P.q, 64), ceil_div(P.p, 64), count), kNsBlock, 0, stream()>>>(P);
+// Tile number -> (i, j): all of them, or those on and below the diagonal, row by row.
+template <Mode M>
+__device__ __forceinline__ void tile_at(uint32_t t, uint32_t ti, uint32_t &i, uint32_t &j) {
+  if constexpr (M == Gram || M == Square) {
+    i = uint32_t((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    while (i * (i + 1) / 2 > t) --i;
+    j = t - i * (i + 1) / 2;
+  } else {
+    i = t % ti;
+    j = t / ti;
+  }
 }
 
-// The iteration over `count` matrices G into O, in a workspace of ns_bytes(count, m, n) bytes.
-uint64_t ns_bytes(uint64_t count, uint64_t m, uint64_t n) {
-  return count * (kNormParts * sizeof(double) + (2 * m * n + 2 * m * m) * sizeof(float));
+// One tile of BM x BN outputs over one piece of the sum, by waves of WM x WN. Two stages of LDS: while
+// the waves multiply one line of every row, the next lines are on their way into the other (loads straight
+// to LDS; lane l of a load fills bytes 16 l of its 1 KiB, so a row's eight 16-byte units are permuted by
+// choosing what each lane reads: unit c lies at c ^ (row % 8), which spreads the reads of eight rows over all
+// banks).
+template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Product P, MuonSet S) {
+  constexpr int NW = (BM / WM) * (BN / WN), LOADS = (BM + BN) / 8 / NW, FA = WM / 32, FB = WN / 32;
+  constexpr uint32_t STAGE = (BM + BN) * 128;
+  constexpr uint32_t LDS = 2 * STAGE > NW * kBlockLds * 4 ? 2 * STAGE : NW * kBlockLds * 4;
+  __shared__ __align__(128) char lds[LDS];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr bool sym = M == Gram || M == Square;
+  const uint32_t tiles = sym ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj;
+  const uint32_t id = xcd_block(blockIdx.x, gridDim.x);
+  const uint32_t b = id / (tiles * P.parts), rest = id - b * tiles * P.parts;
+  const uint32_t part = rest / tiles, t = rest - part * tiles;
+  uint32_t ti, tj;
+  tile_at<M>(t, P.ti, ti, tj);
+  const uint32_t first = uint32_t(uint64_t(P.lines) * part / P.parts);
+  const uint32_t last = uint32_t(uint64_t(P.lines) * (part + 1) / P.parts);
+
+  // this wave's loads: rows 8 q .. 8 q + 7 of the stage, q = wave * LOADS + k
+  const char *src[LOADS];
+#pragma unroll
+  for (int k = 0; k < LOADS; ++k) {
+    const uint32_t r = (wave * LOADS + k) * 8;
+    const bool first_operand = r < BM;
+    const Lines &L = first_operand ? P.u : P.v;
+    const uint32_t row = (first_operand ? ti * BM + r : tj * BN + r - BM) + lane / 8;
+    src[k] = L.data + b * L.next + row * L.pitch + ((lane % 8) ^ (lane / 8)) * 16;
+  }
+  const auto fetch = [&](uint32_t line, uint32_t stage) {
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k)
+      __builtin_amdgcn_global_load_lds(
+          reinterpret_cast<const __attribute__((address_space(1))) uint32_t *>(reinterpret_cast<uintptr_t>(src[k] + line * 128)),
+          reinterpret_cast<__attribute__((address_space(3))) uint32_t *>(
+              uint32_t(reinterpret_cast<uintptr_t>(&lds[stage * STAGE + (wave * LOADS + k) * 1024]))),
+          16, 0, 0);
+  };
+  const uint32_t wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
+  f16v acc[FA][FB];
+#pragma unroll
+  for (int a = 0; a < FA; ++a)
+#pragma unroll
+    for (int c = 0; c < FB; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][c][r] = 0.0f;
+
+  fetch(first, 0);
+  uint32_t stage = 0;
+  for (uint32_t line = first; line < last; ++line, stage ^= 1) {
+    __syncthreads();  // the line has arrived, and every wave is done with the other stage
+    if (line + 1 < last) fetch(line + 1, stage ^ 1);
+    const char *base = lds + stage * STAGE;
+    const uint32_t row = lane % 32, key = row % 8;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {  // 16 columns each
+      h8 ua[FA][2], vb[FB][2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const uint32_t unit = ((p * 4 + g * 2 + lane / 32) ^ key) * 16;
+#pragma unroll
+        for (int a = 0; a < FA; ++a)
+          ua[a][p] = *reinterpret_cast<const h8 *>(base + (wi + a * 32 + row) * 128 + unit);
+#pragma unroll
+        for (int c = 0; c < FB; ++c)
+          vb[c][p] = *reinterpret_cast<const h8 *>(base + (BM + wj + c * 32 + row) * 128 + unit);
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int a = 0; a < FA; ++a)
+#pragma unroll
+          for (int c = 0; c < FB; ++c)
+            acc[a][c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ua[a][q == 2], vb[c][q == 1], acc[a][c], 0, 0, 0);
+    }
+  }
+  const uint32_t i0 = ti * BM + wi, j0 = tj * BN + wj;
+  if (P.parts > 1) {
+    f4 *to = reinterpret_cast<f4 *>(P.partial) +
+             ((uint64_t(id) * NW + wave) * (FA * FB) * 4) * 64 + lane;
+#pragma unroll
+    for (int a = 0; a < FA; ++a)
+#pragma unroll
+      for (int c = 0; c < FB; ++c)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          to[((a * FB + c) * 4 + q) * 64] = f4{acc[a][c][4 * q], acc[a][c][4 * q + 1], acc[a][c][4 * q + 2],
+                                               acc[a][c][4 * q + 3]};
+    return;
+  }
+  __syncthreads();  // the stages become the blocks' way out
+  float *way = reinterpret_cast<float *>(lds) + wave * kBlockLds;
+#pragma unroll
+  for (int a = 0; a < FA; ++a)
+#pragma unroll
+    for (int c = 0; c < FB; ++c)
+      put_block<T, M, MUON>(P, S, way, acc[a][c], b, i0 + a * 32, j0 + c * 32, !sym || ti != tj);
 }
-void iterate(const Stack &G, DTYPE type, const Stack &O, uint32_t count, const NewtonSchulz &rule,
-             void *work) {
-  const uint32_t m = G.rows < G.cols ? G.rows : G.cols, n = G.rows < G.cols ? G.cols : G.rows;
-  const uint64_t mn = uint64_t(m) * n, mm = uint64_t(m) * m;
-  double *part = static_cast<double *>(work);
-  float *x = reinterpret_cast<float *>(part + uint64_t(count) * kNormParts), *y = x + count * mn;
-  float *a = y + count * mn, *s = a + count * mm;
-  const uint32_t parts = G.rows < kNormParts ? G.rows : kNormParts;
-  const dim3 grid(ceil_div(n, kNsBlock), m, count);
-  with_float_type(type, [&](auto t) {
-    norm_kernel<decltype(t)><<<dim3(parts, count), kNsBlock, 0, stream()>>>(G, part);
-    start_kernel<decltype(t)><<<grid, kNsBlock, 0, stream()>>>(G, part, parts, rule.eps, x, m, n);
-  });
+
+// Adds the pieces of a sum: a wave per 32x32 block.
+template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
+  constexpr int FA = WM / 32, FB = WN / 32, NB = (BM / 32) * (BN / 32);
+  __shared__ float lds[kNsBlock / 64 * kBlockLds];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr bool sym = M == Gram || M == Square;
+  const uint32_t tiles = sym ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj;
+  const uint32_t id = blockIdx.x * (kNsBlock / 64) + wave;  // NB is a multiple of 4: whole workgroups
+  const uint32_t block = id % NB, tile = id / NB, b = tile / tiles, t = tile - b * tiles;
+  uint32_t ti, tj;
+  tile_at<M>(t, P.ti, ti, tj);
+  f16v acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+  for (uint32_t part = 0; part < P.parts; ++part) {
+    const f4 *from = reinterpret_cast<const f4 *>(P.partial) +
+                     ((uint64_t(b * P.parts + part) * tiles + t) * NB + block) * 4 * 64 + lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f4 v = from[q * 64];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[4 * q + c] += v[c];
+    }
+  }
+  const uint32_t w = block / (FA * FB), a = block % (FA * FB) / FB, c = block % FB;
+  const uint32_t i0 = ti * BM + w / (BN / WN) * WM + a * 32, j0 = tj * BN + w % (BN / WN) * WN + c * 32;
+  put_block<T, M, MUON>(P, S, lds + wave * kBlockLds, acc, b, i0, j0, !sym || ti != tj);
+}
+
+// No steps: the result is X.
+template <class T, bool MUON>
+__global__ __launch_bounds__(kNsBlock) void copy_out_kernel(Lines X, Lines XT, const float *xscale, Stack O,
+                                                            MuonSet S) {
+  const uint32_t b = blockIdx.z, i = blockIdx.y, j = blockIdx.x * kNsBlock + threadIdx.x;
+  if (j >= O.cols) return;
+  const char *at = line_at(O.rows > O.cols ? XT : X, b, i, j);
+  const float v = (float(*reinterpret_cast<const f16_t *>(at)) + float(*reinterpret_cast<const f16_t *>(at + 64))) /
+                  xscale[b];
+  if constexpr (MUON) {
+    float *p = S.p[b] + uint64_t(i) * O.cols + j;
+    *p = *p * S.rule.keep - S.rule.scale * v;
+  } else {
+    T *o = static_cast<T *>(const_cast<void *>(O.data)) + int64_t(b) * O.sb;
+    o[int64_t(i) * O.s0 + int64_t(j) * O.s1] = T(v);
+  }
+}
+
+// ------------------------------------------------------------------------- host
+
+// How a shape runs: the tile, and the pieces each product's sum is cut into.
+struct Plan {
+  uint32_t m, n, mp, np;  // extents, and padded to whole tiles
+  uint32_t tile;
+  uint32_t gram, square, update;  // pieces
+};
+
+// The pieces that leave the fewest rounds of `slots` workgroups, each a share of the sum: cutting costs
+// a write and a read of the tile per piece, about six lines' time.
+uint32_t pieces(uint64_t tiles, uint32_t lines, uint64_t slots) {
+  uint32_t best = 1;
+  double least = 1e300;
+  for (uint32_t s = 1; s <= 16 && s <= lines; ++s) {
+    const double rounds = double((tiles * s + slots - 1) / slots);
+    const double t = rounds * (double(lines) / s + 4.0) + (s > 1 ? 6.0 * s * double(tiles) / double(slots) + 4.0 : 0.0);
+    if (t < least * 0.98) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
+}
+
+uint32_t round_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
+
+Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count) {
+  Plan p;
+  p.m = rows < cols ? rows : cols;
+  p.n = rows < cols ? cols : rows;
+  const uint64_t work = uint64_t(p.m) * p.n * count;
+  p.tile = p.m > 512 && work >= uint64_t(1) << 24 ? 256 : p.m > 128 && work >= uint64_t(1) << 19 ? 128 : 64;
+  p.mp = round_up(p.m, p.tile);
+  p.np = round_up(p.n, p.tile);
+  const uint64_t ti = p.mp / p.tile, tj = p.np / p.tile, sym = ti * (ti + 1) / 2;
+  const uint64_t slots = uint64_t(num_cus()) * (p.tile == 256 ? 1 : 2);
+  p.gram = pieces(sym * count, p.np / 32, slots);
+  p.square = pieces(sym * count, p.mp / 32, slots);
+  p.update = pieces(ti * tj * count, p.mp / 32, slots);
+  return p;
+}
+
+// Bytes of a workspace for `count` matrices: norms, X and X^T twice, A and S, and the pieces' sums.
+uint64_t ns_bytes(const Plan &p, uint64_t count) {
+  const uint64_t ti = p.mp / p.tile, tj = p.np / p.tile, sym = ti * (ti + 1) / 2;
+  uint64_t part = 0;
+  for (uint64_t t : {p.gram > 1 ? sym * p.gram : 0, p.square > 1 ? sym * p.square : 0,
+                     p.update > 1 ? ti * tj * p.update : 0})
+    part = t > part ? t : part;
+  return count * (kNormParts * 8 + 128 + 4 * (4 * uint64_t(p.mp) * p.np + 2 * uint64_t(p.mp) * p.mp +
+                                        part * p.tile * p.tile));
+}
+
+template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
+void launch_product(const Product &P, const MuonSet &S, uint32_t count) {
+  constexpr int NW = (BM / WM) * (BN / WN);
+  const uint32_t tiles = (M == Gram || M == Square ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj) * count;
+  product_kernel<T, M, MUON, BM, BN, WM, WN><<<tiles * P.parts, 64 * NW, 0, stream()>>>(P, S);
+  if (P.parts > 1)
+    join_kernel<T, M, MUON, BM, BN, WM, WN>
+        <<<tiles * (BM / 32) * (BN / 32) / (kNsBlock / 64), kNsBlock, 0, stream()>>>(P, S);
+}
+template <class T, Mode M, bool MUON>
+void product(const Plan &plan, const Product &P, const MuonSet &S, uint32_t count) {
+  if (plan.tile == 256) launch_product<T, M, MUON, 256, 256, 128, 64>(P, S, count);
+  else if (plan.tile == 128) launch_product<T, M, MUON, 128, 128, 64, 64>(P, S, count);
+  else launch_product<T, M, MUON, 64, 64, 32, 32>(P, S, count);
+}
+
+// The iteration over `count` matrices: from G into O, or of a Muon set into its parameters.
+template <class T, bool MUON>
+void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S, uint32_t count,
+             const NewtonSchulz &rule, void *work) {
+  const uint64_t mn = 4 * uint64_t(plan.mp) * plan.np, mm = 4 * uint64_t(plan.mp) * plan.mp;
+  double *norms = static_cast<double *>(work);
+  float *xscale = reinterpret_cast<float *>(norms + uint64_t(count) * kNormParts);
+  char *at = static_cast<char *>(work) + uint64_t(count) * (kNormParts * 8 + 128);
+  const auto take = [&](uint64_t bytes, uint64_t pitch) {
+    Lines l{at, pitch, bytes};
+    at += count * bytes;
+    return l;
+  };
+  Lines x = take(mn, 4 * uint64_t(plan.np)), y = take(mn, 4 * uint64_t(plan.np));
+  Lines xt = take(mn, 4 * uint64_t(plan.mp)), yt = take(mn, 4 * uint64_t(plan.mp));
+  const Lines a = take(mm, 4 * uint64_t(plan.mp)), s = take(mm, 4 * uint64_t(plan.mp));
+  float *partial = reinterpret_cast<float *>(at);
+
+  const uint64_t size = uint64_t(G.rows) * G.cols;
+  uint64_t parts = (size + 8 * kNsBlock - 1) / (8 * kNsBlock), most = 4096 / count + 1;
+  parts = parts > most ? most : parts;
+  const uint32_t np = uint32_t(parts > kNormParts ? kNormParts : parts);
+  if constexpr (MUON) momentum_kernel<<<dim3(np, count), kNsBlock, 0, stream()>>>(S, size, norms);
+  else norm_kernel<T><<<dim3(np, count), kNsBlock, 0, stream()>>>(G, MagicDiv::make(G.cols), norms);
+  const float most_growth = std::fabs(rule.a) > 1.0f ? std::ceil(std::log2(std::fabs(rule.a)) * float(rule.steps)) : 0.0f;
+  const int growth = int(most_growth < 110.0f ? most_growth : 110.0f);
+  const bool tall = G.rows > G.cols;
+  const dim3 grid((tall ? plan.mp : plan.np) / 64, (tall ? plan.np : plan.mp) / 64, count);
+  start_kernel<T, MUON><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, growth, x, xt, xscale);
+  const uint32_t ti = plan.mp / plan.tile, tj = plan.np / plan.tile;
   for (int k = 0; k < rule.steps; ++k) {
-    product(Product{x, x, nullptr, a, m, m, n, n, 1, 1, n, mn, mn, mm, 1.0f, 0.0f}, count);
-    product(Product{a, a, a, s, m, m, m, m, 1, m, 1, mm, mm, mm, rule.c, rule.b}, count);
-    product(Product{s, x, x, y, m, n, m, m, 1, n, 1, mm, mn, mn, 1.0f, rule.a}, count);
-    float *z = x;
-    x = y, y = z;
+    Product P;
+    memset(&P, 0, sizeof P);
+    P.partial = partial;
+    P.xscale = xscale;
+    P.ti = ti, P.tj = ti;
+    P.u = P.v = x, P.out = P.out_t = a, P.lines = plan.np / 32, P.parts = plan.gram;
+    P.alpha = kScaleA;
+    product<float, Gram, false>(plan, P, S, count);
+    P.u = P.v = P.in = P.in_t = a, P.out = P.out_t = s, P.lines = plan.mp / 32, P.parts = plan.square;
+    P.alpha = rule.c * (kScaleS / (kScaleA * kScaleA)), P.beta = rule.b * (kScaleS / kScaleA);
+    product<float, Square, false>(plan, P, S, count);
+    P.u = s, P.v = P.in_t = xt, P.in = x, P.out = y, P.out_t = yt, P.tj = tj, P.parts = plan.update;
+    P.alpha = 1.0f / kScaleS, P.beta = rule.a;
+    if (k + 1 < rule.steps) {
+      product<float, Update, false>(plan, P, S, count);
+      Lines z = x;
+      x = y, y = z;
+      z = xt, xt = yt, yt = z;
+    } else {
+      P.o = O;
+      product<T, Final, MUON>(plan, P, S, count);
+    }
   }
-  with_float_type(type, [&](auto t) {
-    finish_kernel<decltype(t)><<<grid, kNsBlock, 0, stream()>>>(x, m, n, O);
-  });
+  if (rule.steps == 0)
+    copy_out_kernel<T, MUON><<<dim3(ceil_div(O.cols, kNsBlock), O.rows, count), kNsBlock, 0, stream()>>>(x, xt, xscale, O, S);
 }
 
 bool check_rule(const NewtonSchulz *r, const char *where) {
@@ -165,9 +617,10 @@ constexpr uint64_t kMaxExtent = 65535;             // of a matrix
 constexpr uint64_t kNsBytes = uint64_t(8) << 30;  // workspace that stacks are cut to
 
 // Matrices that go through the launches together.
-uint64_t stack_share(uint64_t count, uint64_t bytes_each) {
-  uint64_t c = kNsBytes / bytes_each;
-  c = c < 1 ? 1 : c > 65535 ? 65535 : c;
+uint64_t stack_share(uint64_t count, uint32_t rows, uint32_t cols) {
+  const uint64_t mn = uint64_t(round_up(rows, 256)) * round_up(cols, 256);
+  uint64_t c = kNsBytes / (16 * mn + 16 * mn);
+  c = c < 1 ? 1 : c > 4096 ? 4096 : c;
   return count < c ? count : c;
 }
 
@@ -215,26 +668,6 @@ bool overlapping(const Tensor *t) {
 }
 
 // ------------------------------------------------------------------------- Muon
-
-struct MuonRule {
-  float momentum, keep, scale;  // keep: 1 - lr decay; scale: lr sqrt(max(1, rows / cols))
-  int nesterov;
-};
-
-__global__ __launch_bounds__(kNsBlock) void momentum_kernel(const float *g, float *m, float *u, uint64_t n,
-                                                            MuonRule R) {
-  for (uint64_t i = uint64_t(blockIdx.x) * kNsBlock + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kNsBlock) {
-    const float gi = g[i];
-    const float v = R.momentum * m[i] + (1.0f - R.momentum) * gi;
-    m[i] = v;
-    u[i] = R.nesterov ? (1.0f - R.momentum) * gi + R.momentum * v : v;
-  }
-}
-
-__global__ __launch_bounds__(kNsBlock) void apply_kernel(float *p, const float *o, uint64_t n, MuonRule R) {
-  for (uint64_t i = uint64_t(blockIdx.x) * kNsBlock + threadIdx.x; i < n; i += uint64_t(gridDim.x) * kNsBlock)
-    p[i] = p[i] * R.keep - R.scale * o[i];
-}
 
 // Moment arrays that the library made (freed by plast_hip_muon_release).
 std::mutex g_muon_mu;
@@ -302,15 +735,20 @@ void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule) {
     return;
   }
   if (numel(g) == 0 || !ensure_init()) return;
-  const uint64_t m = G.rows < G.cols ? G.rows : G.cols, n = G.rows < G.cols ? G.cols : G.rows;
-  const uint64_t share = stack_share(count, ns_bytes(1, m, n)), item = float_bytes(g);
-  void *work = workspace(ns_bytes(share, m, n));
+  const uint64_t share = stack_share(count, G.rows, G.cols), item = float_bytes(g);
+  const Plan plan = make_plan(G.rows, G.cols, share);
+  void *work = workspace(ns_bytes(plan, share));
   if (!work) return;
+  MuonSet none;
+  memset(&none, 0, sizeof none);
   for (uint64_t b = 0; b < count; b += share) {
     Stack Gb = G, Ob = O;
     Gb.data = static_cast<const char *>(G.data) + int64_t(b) * G.sb * int64_t(item);
     Ob.data = static_cast<const char *>(O.data) + int64_t(b) * O.sb * int64_t(item);
-    iterate(Gb, g->dtype, Ob, uint32_t(count - b < share ? count - b : share), *rule, work);
+    with_float_type(g->dtype, [&](auto t) {
+      iterate<decltype(t), false>(plan, Gb, Ob, none, uint32_t(count - b < share ? count - b : share), *rule,
+                                  work);
+    });
   }
   finish(where);
 }
@@ -351,32 +789,28 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
         same.push_back(j);
         done[j] = 1;
       }
-    const uint64_t rows = first->shape[0], cols = first->shape[1], size = rows * cols;
-    const uint64_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    const uint64_t each = ns_bytes(1, m, n) + size * sizeof(float);
-    const uint64_t share = stack_share(same.size(), each);
-    char *work = static_cast<char *>(workspace(share * each));
+    const uint32_t rows = uint32_t(first->shape[0]), cols = uint32_t(first->shape[1]);
+    uint64_t share = stack_share(same.size(), rows, cols);
+    if (share > kPointers) share = kPointers;
+    const Plan plan = make_plan(rows, cols, share);
+    void *work = workspace(ns_bytes(plan, share));
     if (!work) return;
-    float *u = reinterpret_cast<float *>(work + ns_bytes(share, m, n));
-    MuonRule R;
-    R.momentum = optimizer->momentum;
-    R.nesterov = optimizer->nesterov;
-    R.keep = 1.0f - optimizer->lr * optimizer->weight_decay;
-    R.scale = optimizer->lr * sqrtf(rows > cols ? float(rows) / float(cols) : 1.0f);
-    const Stack U{u, uint32_t(rows), uint32_t(cols), int64_t(size), int64_t(cols), 1};
-    const unsigned grid = unsigned(size < (uint64_t(1) << 20) ? ceil_div(size, kNsBlock) : 4096);
+    MuonSet S;
+    memset(&S, 0, sizeof S);
+    S.rule.momentum = optimizer->momentum;
+    S.rule.nesterov = optimizer->nesterov;
+    S.rule.keep = 1.0f - optimizer->lr * optimizer->weight_decay;
+    S.rule.scale = optimizer->lr * sqrtf(rows > cols ? float(rows) / float(cols) : 1.0f);
+    const Stack shape{nullptr, rows, cols, 0, int64_t(cols), 1};
     for (size_t b = 0; b < same.size(); b += share) {
       const size_t c = same.size() - b < share ? same.size() - b : share;
       for (size_t j = 0; j < c; ++j) {
         const Tensor *p = parameters[same[b + j]];
-        momentum_kernel<<<grid, kNsBlock, 0, stream()>>>(
-            static_cast<const float *>(p->grad->data), static_cast<float *>(optimizer->m[same[b + j]]->data),
-            u + j * size, size, R);
+        S.p[j] = static_cast<float *>(p->data);
+        S.g[j] = static_cast<const float *>(p->grad->data);
+        S.m[j] = static_cast<float *>(optimizer->m[same[b + j]]->data);
       }
-      iterate(U, FLOAT32, U, uint32_t(c), optimizer->rule, work);
-      for (size_t j = 0; j < c; ++j)
-        apply_kernel<<<grid, kNsBlock, 0, stream()>>>(static_cast<float *>(parameters[same[b + j]]->data),
-                                                      u + j * size, size, R);
+      iterate<float, true>(plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
     }
   }
   finish(where);
