@@ -76,28 +76,73 @@ struct RowRef {
   __device__ __forceinline__ float shift() const { return far ? 0.0f : __builtin_fmaf(c, m, -cm); }
 };
 
-// Adds a logit's terms to s and w; a masked logit (z = -inf) adds nothing.
-__device__ __forceinline__ void add_terms(float z, float &s, float &w) {
-  const float e = __builtin_amdgcn_exp2f(z);
-  s += e;
-  w = __builtin_fmaf(e, fmaxf(z, -FLT_MAX), w);
+// 16 bytes of a row.
+template <class T>
+struct Unit {
+  static constexpr uint32_t E = 16 / sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(E)));
+  typedef vec any __attribute__((aligned(sizeof(T))));  // at any element's address
+  typedef float floats __attribute__((ext_vector_type(E)));
+};
+template <class T>
+__device__ __forceinline__ typename Unit<T>::vec load_unit(const T *p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const typename Unit<T>::any *>(p));
+}
+template <class T>
+__device__ __forceinline__ typename Unit<T>::floats to_floats(typename Unit<T>::vec v) {
+  return __builtin_convertvector(v, typename Unit<T>::floats);
+}
+// The largest of a unit, NaN if one is.
+template <class F>
+__device__ __forceinline__ float unit_max(F f) {
+  constexpr int E = sizeof(F) / sizeof(float);
+  float g = f[0];
+#pragma unroll
+  for (int e = 1; e + 1 < E; e += 2) g = __builtin_elementwise_maximum(__builtin_elementwise_maximum(g, f[e]), f[e + 1]);
+  return __builtin_elementwise_maximum(g, f[E - 1]);
 }
 
-template <int W>
-__device__ __forceinline__ float block_reduce(float v, float *lds, bool maximum) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    const float o = __shfl_xor(v, m);
-    v = maximum ? fmaxf(v, o) : v + o;
+// A lane's share of s and w, against a reference of its own that grows with the logits it meets: cm is
+// c times the largest so far, but at least -1e38, so that it stays finite (a row whose largest logit is not
+// in range is worked out by the exact path below).
+struct Running {
+  float m = -kInf, cm = -1e38f, s = 0.0f, w = 0.0f;
+  __device__ __forceinline__ void refer(float to) {
+    const float d = cm - to, f = __builtin_amdgcn_exp2f(d);
+    w = f * __builtin_fmaf(d, s, w);
+    s *= f;
+    cm = to;
   }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  float r = lds[0];
+  __device__ __forceinline__ void grow(float c, float g) {
+    m = __builtin_elementwise_maximum(m, g);  // NaN stays
+    refer(fmaxf(c * m, -1e38f));
+  }
+  __device__ __forceinline__ void add(float c, float x) {
+    // below 2^-200 nothing is added, and a masked logit's -inf meets no 0
+    const float z = fmaxf(__builtin_fmaf(x, c, -cm), -200.0f);
+    const float e = __builtin_amdgcn_exp2f(z);
+    s += e;
+    w = __builtin_fmaf(e, z, w);
+  }
+};
+__device__ __forceinline__ Running wave_join(Running r) {
+  float m = r.m, cm = r.cm;
 #pragma unroll
-  for (int k = 1; k < W; ++k) r = maximum ? fmaxf(r, lds[k]) : r + lds[k];
+  for (int d = 32; d >= 1; d >>= 1) {
+    m = __builtin_elementwise_maximum(m, __shfl_xor(m, d));
+    cm = fmaxf(cm, __shfl_xor(cm, d));
+  }
+  r.refer(cm);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    r.s += __shfl_xor(r.s, d);
+    r.w += __shfl_xor(r.w, d);
+  }
+  r.m = m;
   return r;
 }
+// Whether the running form holds for a row with this largest logit.
+__device__ __forceinline__ bool in_range(float c, float m) { return m == -kInf || fabsf(c * m) < 1e38f; }
 
 // A logit's place in the order of alternatives: larger first, equal logits (both zeros too) by the
 // lower index, NaN above all. No key is 0.
@@ -140,44 +185,88 @@ __device__ __forceinline__ void pad_out(const TokenArgs &A, uint32_t row) {
   A.stats[2 * row + 1] = 0.0f;
 }
 
-// One workgroup per row: the maximum, then the sums, then an argmax per alternative.
-template <class T>
-__global__ __launch_bounds__(kRowBlock) void fwd_kernel(TokenArgs A) {
-  __shared__ float lds[4];
-  __shared__ uint64_t keys[4];
-  const uint32_t row = blockIdx.x, V = A.vocab;
-  const int32_t token = A.tokens[row];
-  const uint32_t top = A.top;
-  if (token < 0) {
-    if (threadIdx.x == 0) pad_out(A, row);
-    if (threadIdx.x < top) {
-      A.top_logp[uint64_t(row) * top + threadIdx.x] = -kInf;
-      A.top_ids[uint64_t(row) * top + threadIdx.x] = -1;
+// ------------------------------------------------------------------------- forward
+
+constexpr uint32_t kList = 256;  // candidates that are kept while a row is read
+
+// What the W waves that share a row hold in LDS.
+template <int W>
+struct RowLds {
+  float red[W][4];
+  uint64_t keys[W];
+  float group[64];
+  float threshold;
+  uint32_t count[2], ties;
+  uint64_t list[2][kList];
+};
+
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+template <int W>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (W == 1) wave_sync();
+  else __syncthreads();
+}
+
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t k = uint32_t(key >> 32);
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+// An alternative at its place, by one lane; no key: the row is shorter than its alternatives.
+__device__ __forceinline__ void put_top(const TokenArgs &A, uint32_t row, uint32_t k, uint64_t key, float m, float l0) {
+  const uint64_t at = uint64_t(row) * A.top + k;
+  A.top_ids[at] = key ? int32_t(0xffffffffu - uint32_t(key)) : -1;
+  A.top_logp[at] = key ? log_p(A, key_value(key), m, l0) : -kInf;
+}
+
+// The exact path, for rows with NaN, infinite or out-of-range logits and for alternatives that the list
+// could not hold: the maximum, then the sums, then an argmax per alternative, each a pass over the row.
+template <class T, int W>
+__device__ __forceinline__ void exact_row(const TokenArgs &A, const T *x, uint32_t row, int32_t token, uint32_t gl,
+                                       RowLds<W> &L, bool stats, float m, float l0) {
+  constexpr uint32_t NL = 64 * W;
+  const uint32_t V = A.vocab, wave = gl / 64;
+  const auto together = [&](float v, bool maximum) {
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      const float o = __shfl_xor(v, d);
+      v = maximum ? fmaxf(v, o) : v + o;
     }
-    return;
+    row_sync<W>();
+    if (gl % 64 == 0) L.red[wave][0] = v;
+    row_sync<W>();
+    v = L.red[0][0];
+    for (int k = 1; k < W; ++k) v = maximum ? fmaxf(v, L.red[k][0]) : v + L.red[k][0];
+    return v;
+  };
+  if (stats) {
+    m = -kInf;
+    for (uint32_t j = gl; j < V; j += NL) m = fmaxf(m, float(x[j]));
+    m = together(m, true);
+    const RowRef ref(A.c, m);
+    float s = 0.0f, w = 0.0f;
+    bool nan = false;
+    for (uint32_t j = gl; j < V; j += NL) {
+      const float v = float(x[j]);
+      nan = nan || v != v;
+      const float z = ref.z(v), e = __builtin_amdgcn_exp2f(z);
+      s += e;
+      w = __builtin_fmaf(e, fmaxf(z, -FLT_MAX), w);
+    }
+    s = together(nan ? __builtin_nanf("") : s, false);
+    w = together(w, false);
+    if (s != s) m = s;  // a NaN or an infinite logit
+    l0 = log2f(s) - ref.shift();
+    if (gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, m, s, w);
   }
-  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
-  float m = -kInf;
-  for (uint32_t j = threadIdx.x; j < V; j += kRowBlock) m = fmaxf(m, float(x[j]));
-  m = block_reduce<4>(m, lds, true);
-  const RowRef ref(A.c, m);
-  float s = 0.0f, w = 0.0f;
-  bool nan = false;
-  for (uint32_t j = threadIdx.x; j < V; j += kRowBlock) {
-    const float v = float(x[j]);
-    nan = nan || v != v;
-    if (m != -kInf) add_terms(ref.z(v), s, w);
-  }
-  if (nan) s = __builtin_nanf("");
-  s = block_reduce<4>(s, lds, false);
-  w = block_reduce<4>(w, lds, false);
-  if (s != s) m = s;  // a NaN or an infinite logit
-  if (threadIdx.x == 0)
-    row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, m, s, w);
   uint64_t last = ~uint64_t(0);
-  for (uint32_t k = 0; k < top; ++k) {
+  for (uint32_t k = 0; k < A.top; ++k) {
     uint64_t best = 0;
-    for (uint32_t j = threadIdx.x; j < V; j += kRowBlock) {
+    for (uint32_t j = gl; j < V; j += NL) {
       const uint64_t key = order_key(float(x[j]), j);
       if (key < last && key > best) best = key;
     }
@@ -186,17 +275,336 @@ __global__ __launch_bounds__(kRowBlock) void fwd_kernel(TokenArgs A) {
       const uint64_t o = __shfl_xor((unsigned long long)best, d);
       best = o > best ? o : best;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) keys[threadIdx.x >> 6] = best;
-    __syncthreads();
-    for (int d = 0; d < 4; ++d) best = keys[d] > best ? keys[d] : best;
-    if (threadIdx.x == 0) {
-      const uint64_t at = uint64_t(row) * top + k;
-      const uint32_t j = 0xffffffffu - uint32_t(best);
-      A.top_ids[at] = best ? int32_t(j) : -1;
-      A.top_logp[at] = best ? log_p(A, float(x[j]), m, log2f(s) - ref.shift()) : -kInf;
+    row_sync<W>();
+    if (gl % 64 == 0) L.keys[wave] = best;
+    row_sync<W>();
+    for (int d = 0; d < W; ++d) best = L.keys[d] > best ? L.keys[d] : best;
+    if (gl == 0) {
+      put_top(A, row, k, best, m, l0);
+      if (best && uint32_t(best >> 32) == 0xffffffffu) A.top_logp[uint64_t(row) * A.top + k] = __builtin_nanf("");
     }
     last = best;
+  }
+}
+
+// Keeps the largest candidates of a row while it is read. A bound under which no logit can be among the
+// `top` largest starts as the top-th largest of 64 lane groups' maxima over the first logits (so many
+// logits at least reach it), and is raised to the top-th candidate whenever as many logits again have been
+// read; only logits above it go to the list, a few times `top` in all.
+template <int W>
+struct Candidates {
+  static constexpr uint32_t NL = 64 * W;
+  RowLds<W> &L;
+  uint32_t gl, top, cur = 0;
+  float bound = kInf;  // logits above it are candidates
+  bool lost = false;   // the list was too short
+  __device__ __forceinline__ Candidates(RowLds<W> &l, uint32_t g, uint32_t t) : L(l), gl(g), top(t) {}
+
+  __device__ __forceinline__ void push(float v, uint32_t j) {
+    const uint32_t at = atomicAdd(&L.count[cur], 1u);
+    if (at < kList) L.list[cur][at] = order_key(v, j);
+  }
+  __device__ __forceinline__ void clear() {
+    if (gl == 0) L.count[0] = L.count[1] = L.ties = 0;
+  }
+  // The bound from every lane's maximum over the first logits; clear() comes before it.
+  __device__ __forceinline__ void start(float lane_max) {
+    float v = lane_max;
+    if constexpr (W > 1) {
+#pragma unroll
+      for (int d = W / 2; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+      if (gl % W == 0) L.group[gl / W] = v;
+      row_sync<W>();
+      v = L.group[gl % 64];
+    } else {
+      row_sync<W>();
+    }
+    const uint32_t lane = gl % 64;
+    uint32_t before = 0;
+#pragma unroll 8
+    for (uint32_t d = 0; d < 64; ++d) {
+      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), d));
+      before += o > v || (o == v && d < lane);
+    }
+    const uint64_t at = __ballot(before == top - 1);
+    bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), __ffsll((unsigned long long)at) - 1));
+  }
+  // After start()'s logits: those above the bound are in the list and `equal` counts this lane's at it. The
+  // lowest of the equal ones are found by rereading the row from its start where there are many (a mask).
+  template <class T, class F>
+  __device__ __forceinline__ void take_equal(uint32_t equal, F &&push_equal, const T *x, uint32_t from, uint32_t to) {
+    if (equal) atomicAdd(&L.ties, equal);
+    row_sync<W>();
+    const uint32_t above = L.count[0], ties = L.ties;
+    row_sync<W>();
+    if (above > kList) {
+      give_up();
+      return;
+    }
+    if (above >= top || ties == 0) return;
+    if (above + ties <= kList) {
+      push_equal();
+      row_sync<W>();
+      return;
+    }
+    if (gl < 64) {
+      uint32_t want = top - above, at = above;
+      for (uint32_t j0 = from; want && j0 < to; j0 += 64) {
+        const uint32_t j = j0 + gl;
+        const float v = j < to ? float(x[j]) : __builtin_nanf("");
+        const uint64_t hit = __ballot(v == bound);
+        const uint32_t place = __popcll(hit & ((uint64_t(1) << gl) - 1));
+        if (v == bound && place < want) L.list[0][at + place] = order_key(v, j);
+        const uint32_t n = min(uint32_t(__popcll(hit)), want);
+        want -= n;
+        at += n;
+      }
+      if (gl == 0) L.count[0] = at;
+    }
+    row_sync<W>();
+  }
+  __device__ __forceinline__ void give_up() {
+    lost = true;
+    bound = kInf;
+  }
+  // The place of a candidate among the list's.
+  __device__ __forceinline__ uint32_t rank(uint64_t key, uint32_t n) const {
+    uint32_t r = 0;
+#pragma unroll 4
+    for (uint32_t k = 0; k < n; ++k) r += L.list[cur][k] > key;
+    return r;
+  }
+  // Drops all but the `top` largest and raises the bound to the last of them.
+  __device__ __forceinline__ void raise() {
+    row_sync<W>();
+    const uint32_t n = L.count[cur];
+    if (n > kList) give_up();
+    if (lost || n <= top) {
+      row_sync<W>();
+      return;
+    }
+    for (uint32_t i = gl; i < n; i += NL) {
+      const uint64_t key = L.list[cur][i];
+      const uint32_t r = rank(key, n);
+      if (r < top) L.list[1 - cur][r] = key;
+      if (r == top - 1) L.threshold = key_value(key);
+    }
+    if (gl == 0) L.count[1 - cur] = top;
+    cur = 1 - cur;
+    row_sync<W>();
+    bound = L.threshold;
+  }
+};
+
+// A piece of a row, where rows are cut because there are few: what it found, for the last to finish.
+struct Piece {
+  float m, cm, s, w;
+  uint32_t lost, found;
+  uint64_t keys[PLAST_TOP_MAX];
+};
+struct Pieces {
+  uint32_t n;
+  Piece *found;      // [rows][n]
+  uint32_t *tickets;  // [rows], zero between launches
+};
+constexpr uint32_t kTickets = 4096;
+__device__ uint32_t g_tickets[kTickets];
+
+// W waves per row (or piece of one), four rows per workgroup where W is 1. One pass: a lane's units of 16 bytes
+// come four at a time. What bounds it is the read for fp32 and the vector units for the 16-bit types: of a
+// logit's ten issue slots four are the exponential.
+template <class T, int W, bool TOP, bool CUT>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A, Pieces P) {
+  constexpr uint32_t NL = 64 * W, E = Unit<T>::E, U = 4;
+  __shared__ RowLds<W> lds[W == 1 ? 4 : 1];
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t gl = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+  RowLds<W> &L = lds[W == 1 ? wave : 0];
+  const uint32_t row = W == 1 ? blockIdx.x * 4 + wave : CUT ? blockIdx.x / P.n : blockIdx.x;
+  const uint32_t piece = CUT ? blockIdx.x - row * P.n : 0, pieces = CUT ? P.n : 1;
+  if (W == 1 && row >= A.rows) return;
+  const int32_t token = A.tokens[row];
+  if (token < 0) {
+    if (piece == 0) {
+      if (gl == 0) pad_out(A, row);
+      if (TOP && gl < A.top) put_top(A, row, gl, 0, 0.0f, 0.0f);
+    }
+    return;
+  }
+  const uint32_t V = A.vocab, units = V / E;
+  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
+  const uint32_t from = uint32_t(uint64_t(units) * piece / pieces), to = uint32_t(uint64_t(units) * (piece + 1) / pieces);
+  // the logits after the last unit, one a lane
+  const bool has_tail = piece == pieces - 1 && gl < V - units * E;
+  const uint32_t tail_at = units * E + gl;
+  const float tail = has_tail ? float(x[tail_at]) : -kInf;
+  const bool tail_first = to - from <= NL * U;  // then it is among the first logits
+  const float c = A.c;
+  Running r;
+  Candidates<W> top(L, gl, A.top);
+  if constexpr (TOP) top.clear();
+  uint32_t batch = 0;
+  uint32_t q0 = from;
+  do {
+    typename Unit<T>::vec v[U];
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t q = q0 + u * NL + gl;
+      if (q < to) v[u] = load_unit(x + uint64_t(q) * E);
+    }
+    float most = tail_first ? tail : -kInf;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t q = q0 + u * NL + gl;
+      if (q >= to) continue;
+      const auto f = to_floats<T>(v[u]);
+      const float g = unit_max(f);
+      if (!(g <= r.m)) r.grow(c, g);
+#pragma unroll
+      for (uint32_t e = 0; e < E; ++e) r.add(c, f[e]);
+      if constexpr (TOP) {
+        most = fmaxf(most, g);
+        if (batch && g > top.bound) {
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e)
+            if (f[e] > top.bound) top.push(f[e], q * E + e);
+        }
+      }
+    }
+    if constexpr (TOP) {
+      if (batch == 0) {
+        top.start(most);
+        uint32_t equal = 0;
+        const auto each = [&](auto &&visit) {
+#pragma unroll
+          for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t q = q0 + u * NL + gl;
+            if (q >= to) continue;
+            const auto f = to_floats<T>(v[u]);
+            if (unit_max(f) >= top.bound)
+#pragma unroll
+              for (uint32_t e = 0; e < E; ++e) visit(f[e], q * E + e);
+          }
+          if (tail_first && has_tail) visit(tail, tail_at);
+        };
+        each([&](float a, uint32_t j) {
+          if (a > top.bound) top.push(a, j);
+          else if (a == top.bound) ++equal;
+        });
+        top.take_equal(
+            equal, [&] { each([&](float a, uint32_t j) { if (a == top.bound) top.push(a, j); }); }, x, from * E,
+            tail_first && piece == pieces - 1 ? V : min(q0 + NL * U, to) * E);
+      } else if (((batch + 1) & batch) == 0) {
+        top.raise();
+      }
+    }
+    ++batch;
+    q0 += NL * U;
+  } while (q0 < to);
+  if (has_tail) {
+    if (!(tail <= r.m)) r.grow(c, tail);
+    r.add(c, tail);
+    if (TOP && !tail_first && tail > top.bound) top.push(tail, tail_at);
+  }
+  r = wave_join(r);
+  if constexpr (W > 1) {
+    if (gl % 64 == 0) {
+      L.red[gl / 64][0] = r.m;
+      L.red[gl / 64][1] = r.cm;
+      L.red[gl / 64][2] = r.s;
+      L.red[gl / 64][3] = r.w;
+    }
+    __syncthreads();
+    r.m = L.red[0][0], r.cm = L.red[0][1], r.s = L.red[0][2], r.w = L.red[0][3];
+    for (int k = 1; k < W; ++k) {
+      Running o;
+      o.m = L.red[k][0], o.cm = L.red[k][1], o.s = L.red[k][2], o.w = L.red[k][3];
+      const float cm = fmaxf(r.cm, o.cm);
+      r.refer(cm);
+      o.refer(cm);
+      r.m = __builtin_elementwise_maximum(r.m, o.m);
+      r.s += o.s;
+      r.w += o.w;
+    }
+  } else {
+    row_sync<W>();
+  }
+  uint32_t found = 0;
+  if constexpr (TOP) {
+    found = L.count[top.cur];
+    if (found > kList) top.give_up();
+  }
+  if constexpr (CUT) {
+    __shared__ bool is_last;
+    Piece *mine = P.found + uint64_t(row) * P.n;
+    if (gl == 0) {
+      mine[piece].m = r.m, mine[piece].cm = r.cm, mine[piece].s = r.s, mine[piece].w = r.w;
+      mine[piece].lost = top.lost, mine[piece].found = min(found, A.top);
+    }
+    if (TOP && !top.lost)
+      for (uint32_t i = gl; i < found; i += NL) {
+        const uint64_t key = L.list[top.cur][i];
+        const uint32_t k = top.rank(key, found);
+        if (k < A.top) mine[piece].keys[k] = key;
+      }
+    __threadfence();
+    __syncthreads();
+    if (gl == 0) is_last = atomicAdd(&P.tickets[row], 1u) == P.n - 1;
+    __syncthreads();
+    if (!is_last) return;
+    if (gl == 0) __hip_atomic_store(&P.tickets[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __threadfence();
+    // a wave's lanes take the pieces; the merged sums are the same whoever comes last
+    Running o;
+    const uint32_t lane = gl % 64;
+    bool lost = false;
+    if (lane < P.n) {
+      o.m = mine[lane].m, o.cm = mine[lane].cm, o.s = mine[lane].s, o.w = mine[lane].w;
+      lost = mine[lane].lost != 0;
+    }
+    r = wave_join(o);
+    top.lost = __any(lost);
+    if (TOP && !top.lost) {
+      // no logit below a piece's last candidate can be among the largest
+      uint64_t least = lane < P.n && mine[lane].found == A.top ? mine[lane].keys[A.top - 1] : 0;
+#pragma unroll
+      for (int d = 32; d >= 1; d >>= 1) {
+        const uint64_t k = __shfl_xor((unsigned long long)least, d);
+        least = k > least ? k : least;
+      }
+      top.cur = 0;
+      if (gl == 0) L.count[0] = 0;
+      __syncthreads();
+      for (uint32_t i = gl; i < P.n * A.top; i += NL) {
+        const uint32_t p = i / A.top, k = i - p * A.top;
+        if (k >= mine[p].found) continue;
+        const uint64_t key = mine[p].keys[k];
+        if (key >= least) {
+          const uint32_t at = atomicAdd(&L.count[0], 1u);
+          if (at < kList) L.list[0][at] = key;
+        }
+      }
+      __syncthreads();
+      found = L.count[0];
+      if (found > kList) top.give_up();
+    }
+  }
+  const bool exact = !in_range(c, r.m);
+  if (exact || top.lost) {
+    const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
+    if (!exact && gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, r.m, r.s, r.w);
+    exact_row<T, W>(A, x, row, token, gl, L, exact, r.m, l0);
+    return;
+  }
+  if (gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, r.m, r.s, r.w);
+  if constexpr (TOP) {
+    const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
+    for (uint32_t i = gl; i < found; i += NL) {
+      const uint64_t key = L.list[top.cur][i];
+      const uint32_t k = top.rank(key, found);
+      if (k < A.top) put_top(A, row, k, key, r.m, l0);
+    }
+    if (gl >= found && gl < A.top) put_top(A, row, gl, 0, r.m, l0);
   }
 }
 
@@ -317,10 +725,50 @@ bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *t
   return true;
 }
 
-void launch_forward(const TokenArgs &A, DTYPE type) {
+uint32_t *tickets(const char *where) {
+  static uint32_t *at = nullptr;
+  if (at) return at;
+  void *p = nullptr;
+  const hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(g_tickets));
+  if (e != hipSuccess) {
+    report_error(where, "hipGetSymbolAddress: %s", hipGetErrorString(e));
+    return nullptr;
+  }
+  return at = static_cast<uint32_t *>(p);
+}
+
+template <class T, bool TOP>
+bool launch_rows(const TokenArgs &A, const char *where) {
+  const uint64_t unit = 16 / sizeof(T), units = A.vocab / unit;
+  Pieces P{1, nullptr, nullptr};
+  // waves of a row: enough rows, or enough waves to a row, to fill the chip
+  if (A.rows >= 2048 || units <= 256) {
+    fwd_kernel<T, 1, TOP, false><<<ceil_div(A.rows, 4), 256, 0, stream()>>>(A, P);
+    return true;
+  }
+  uint64_t cut = units / 1024;
+  if (cut > 512 / A.rows) cut = 512 / A.rows;
+  if (cut > 32) cut = 32;
+  if (cut > 1) {
+    P.n = uint32_t(cut);
+    P.tickets = tickets(where);
+    P.found = static_cast<Piece *>(partials(uint64_t(A.rows) * cut * sizeof(Piece), where));
+    if (!P.tickets || !P.found) return false;
+    fwd_kernel<T, 4, TOP, true><<<A.rows * P.n, 256, 0, stream()>>>(A, P);
+  } else if (A.rows < 512 && units > 1024) {
+    fwd_kernel<T, 16, TOP, false><<<A.rows, 1024, 0, stream()>>>(A, P);
+  } else {
+    fwd_kernel<T, 4, TOP, false><<<A.rows, 256, 0, stream()>>>(A, P);
+  }
+  return true;
+}
+
+bool launch_forward(const TokenArgs &A, DTYPE type, const char *where) {
+  bool ok = false;
   with_float_type(type, [&](auto t) {
-    fwd_kernel<decltype(t)><<<A.rows, kRowBlock, 0, stream()>>>(A);
+    ok = A.top ? launch_rows<decltype(t), true>(A, where) : launch_rows<decltype(t), false>(A, where);
   });
+  return ok;
 }
 
 void launch_backward(const TokenArgs &A, DTYPE type, bool add) {
@@ -390,7 +838,7 @@ void token_logprob_hip_forward(const Tensor **inputs, Tensor *output, KernelPara
     A.top_ids = static_cast<int32_t *>(ids->data);
   }
   if (A.rows == 0 || !ensure_init()) return;
-  launch_forward(A, inputs[0]->dtype);
+  if (!launch_forward(A, inputs[0]->dtype, where)) return;
   finish(where);
 }
 
@@ -436,7 +884,7 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
     return;
   A.stats = static_cast<float *>(partials(2 * N * sizeof(float), where));
   if (!A.stats) return;
-  launch_forward(A, x->dtype);
+  if (!launch_forward(A, x->dtype, where)) return;
   launch_backward(A, x->dtype, false);
   finish(where);
 }
