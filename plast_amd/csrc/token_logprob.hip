@@ -14,6 +14,7 @@
 //   B = h ln2 / (T s),  A = (u + h H) / (T s) - B log2 s.
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "half_types.hpp"
 
@@ -56,7 +57,7 @@ struct TokenArgs {
   float *top_logp;
   int32_t *top_ids;
   uint32_t top;
-  uint32_t rows, vocab;
+  uint32_t first_row, rows, vocab;  // first_row: of a launch, where one cannot hold all
   float c;      // log2(e) / T
   float inv_t;  // 1 / T
   RowMap map;
@@ -91,6 +92,15 @@ __device__ __forceinline__ typename Unit<T>::vec load_unit(const T *p) {
 template <class T>
 __device__ __forceinline__ typename Unit<T>::floats to_floats(typename Unit<T>::vec v) {
   return __builtin_convertvector(v, typename Unit<T>::floats);
+}
+// Holds a unit as it was read: without it the compiler keeps a 16-bit unit's floats, twice the registers, from
+// one use to the next.
+template <class V>
+__device__ __forceinline__ void keep_raw(V &v) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  words w = __builtin_bit_cast(words, v);
+  asm volatile("" : "+v"(w));
+  v = __builtin_bit_cast(V, w);
 }
 // The largest of a unit, NaN if one is.
 template <class F>
@@ -158,14 +168,19 @@ __device__ __forceinline__ float log_p(const TokenArgs &A, float x, float m, flo
   return m == -kInf ? -kInf : (x - m) * A.inv_t - kLn2 * l0;
 }
 
+__device__ __forceinline__ void put_stats(const TokenArgs &A, uint32_t row, float m, float l0) {
+  if (!A.stats) return;  // the step keeps none
+  A.stats[2 * row] = m;
+  A.stats[2 * row + 1] = l0;
+}
+
 // The row's results, by one lane. s and w are over the whole row.
 __device__ __forceinline__ void row_out(const TokenArgs &A, uint32_t row, int32_t token, float x_token,
                                         float m, float s, float w) {
   if (m == -kInf) {  // no logit that is not -inf
     A.logp[row] = uint32_t(token) < A.vocab ? -kInf : __builtin_nanf("");
     A.entropy[row] = 0.0f;
-    A.stats[2 * row] = -kInf;
-    A.stats[2 * row + 1] = 0.0f;
+    put_stats(A, row, -kInf, 0.0f);
     return;
   }
   const float l = log2f(s);
@@ -174,15 +189,13 @@ __device__ __forceinline__ void row_out(const TokenArgs &A, uint32_t row, int32_
   const float l0 = l - ref.shift();
   A.logp[row] = uint32_t(token) < A.vocab ? log_p(A, x_token, m, l0) : __builtin_nanf("");
   A.entropy[row] = h < 0.0f ? 0.0f : h;
-  A.stats[2 * row] = m;
-  A.stats[2 * row + 1] = l0;
+  put_stats(A, row, m, l0);
 }
 
 __device__ __forceinline__ void pad_out(const TokenArgs &A, uint32_t row) {
   A.logp[row] = 0.0f;
   A.entropy[row] = 0.0f;
-  A.stats[2 * row] = -kInf;
-  A.stats[2 * row + 1] = 0.0f;
+  put_stats(A, row, -kInf, 0.0f);
 }
 
 // ------------------------------------------------------------------------- forward
@@ -608,34 +621,265 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   }
 }
 
-// One workgroup per row.
+// ------------------------------------------------------------------------- backward
+
+// A row's gradient: dx = onehot - 2^z (a + b z).
+struct RowGrad {
+  RowRef ref;
+  float a, b, onehot;
+  __device__ __forceinline__ RowGrad(const TokenArgs &A, uint32_t row, int32_t token, float m, float l, float entropy)
+      : ref(A.c, m) {
+    const float u = A.dlogp ? A.dlogp[row] : 0.0f, h = A.dentropy ? A.dentropy[row] : 0.0f;
+    const float r = A.inv_t * __builtin_amdgcn_exp2f(-l);  // 1 / (T s)
+    b = h * kLn2 * r;
+    a = uint32_t(token) < A.vocab ? (u + h * entropy) * r - b * l : __builtin_nanf("");
+    onehot = u * A.inv_t;
+  }
+  __device__ __forceinline__ float at(float x) const {
+    const float z = fmaxf(ref.z(x), -200.0f);  // 2^-200 is 0, and a masked logit's z stays finite
+    return -__builtin_amdgcn_exp2f(z) * __builtin_fmaf(b, z, a);
+  }
+};
+
+// A row in units that start at 16-byte boundaries of its gradient, where the stores go (the reads take any
+// address): unit q holds elements first .. first + E - 1, of which those inside the row count.
+template <class T>
+struct RowUnits {
+  static constexpr uint32_t E = Unit<T>::E;
+  int32_t shift;
+  uint32_t V;
+  __device__ __forceinline__ RowUnits(const T *g, uint32_t v)
+      : shift(int32_t(uint32_t(reinterpret_cast<uintptr_t>(g) / sizeof(T)) % E)), V(v) {}
+  __device__ __forceinline__ int32_t first(uint32_t q) const { return int32_t(q * E) - shift; }
+  __device__ __forceinline__ bool whole(int32_t j) const { return j >= 0 && j + int32_t(E) <= int32_t(V); }
+  // A unit's elements; those outside the row are -inf.
+  __device__ __forceinline__ typename Unit<T>::vec load(const T *x, int32_t j) const {
+    if (whole(j)) return load_unit(x + j);
+    typename Unit<T>::vec v;
+#pragma unroll
+    for (int32_t e = 0; e < int32_t(E); ++e) v[e] = j + e >= 0 && j + e < int32_t(V) ? x[j + e] : T(-kInf);
+    return v;
+  }
+  template <bool ADD>
+  __device__ __forceinline__ void store(T *g, int32_t j, typename Unit<T>::floats f) const {
+    if (whole(j)) {
+      typename Unit<T>::vec *to = reinterpret_cast<typename Unit<T>::vec *>(g + j);
+      if constexpr (ADD) f += to_floats<T>(__builtin_nontemporal_load(to));
+      __builtin_nontemporal_store(__builtin_convertvector(f, typename Unit<T>::vec), to);
+      return;
+    }
+#pragma unroll
+    for (int32_t e = 0; e < int32_t(E); ++e)
+      if (j + e >= 0 && j + e < int32_t(V)) g[j + e] = T(ADD ? f[e] + float(g[j + e]) : f[e]);
+  }
+};
+// Units of the longest row of v elements, whatever its address.
+template <class T>
+constexpr uint32_t most_units(uint32_t v) {
+  return (v + 2 * (Unit<T>::E - 1)) / Unit<T>::E;
+}
+
 template <class T, bool ADD>
-__global__ __launch_bounds__(kRowBlock) void bwd_kernel(TokenArgs A) {
-  const uint32_t row = blockIdx.x, V = A.vocab;
+__device__ __forceinline__ void grad_unit(const RowUnits<T> &R, const RowGrad &G, const T *x, T *dx, int32_t token,
+                                          int32_t j) {
+  auto f = to_floats<T>(R.load(x, j));
+#pragma unroll
+  for (int32_t e = 0; e < int32_t(R.E); ++e) {
+    f[e] = G.at(f[e]);
+    if (token == j + e) f[e] += G.onehot;
+  }
+  R.template store<ADD>(dx, j, f);
+}
+
+// Rows of many units: a workgroup takes BWD_UNITS units a lane of one row, whose constants are uniform.
+constexpr uint32_t kBwdUnits = 2;
+template <class T, bool ADD>
+__global__ __launch_bounds__(kRowBlock) void bwd_kernel(TokenArgs A, uint32_t chunks) {
+  const uint32_t block_row = blockIdx.x / chunks, row = A.first_row + block_row;
+  const uint32_t q0 = (blockIdx.x - block_row * chunks) * kBwdUnits * kRowBlock + threadIdx.x;
   const int32_t token = A.tokens[row];
   const RowAt at = row_at(A.map, row);
   T *dx = static_cast<T *>(A.dx) + at.g;
+  const RowUnits<T> R(dx, A.vocab);
   const float m = A.stats[2 * row];
-  const RowRef ref(A.c, m);
-  const float l = A.stats[2 * row + 1] + ref.shift();
   if (token < 0 || m == -kInf) {
-    if (!ADD)
-      for (uint32_t j = threadIdx.x; j < V; j += kRowBlock) dx[j] = T(0.0f);
+    if (ADD) return;
+    typename Unit<T>::floats none = 0.0f;
+#pragma unroll
+    for (uint32_t u = 0; u < kBwdUnits; ++u) {
+      const int32_t j = R.first(q0 + u * kRowBlock);
+      if (j < int32_t(A.vocab)) R.template store<false>(dx, j, none);
+    }
     return;
   }
   const T *x = static_cast<const T *>(A.x) + at.x;
-  const float u = A.dlogp ? A.dlogp[row] : 0.0f, h = A.dentropy ? A.dentropy[row] : 0.0f;
-  const float r = A.inv_t * __builtin_amdgcn_exp2f(-l);  // 1 / (T s)
-  const float b = h * kLn2 * r;
-  float a = (u + h * A.entropy[row]) * r - b * l;
-  if (uint32_t(token) >= V) a = __builtin_nanf("");
-  for (uint32_t j = threadIdx.x; j < V; j += kRowBlock) {
-    const float z = fmaxf(ref.z(float(x[j])), -300.0f);  // 2^-300 = 0; masked logits stay finite
-    float d = -__builtin_amdgcn_exp2f(z) * __builtin_fmaf(b, z, a);
-    if (j == uint32_t(token)) d += u * A.inv_t;
-    if (ADD) d += float(dx[j]);
-    dx[j] = T(d);
+  const RowGrad G(A, row, token, m, A.stats[2 * row + 1] + RowRef(A.c, m).shift(), A.entropy[row]);
+#pragma unroll
+  for (uint32_t u = 0; u < kBwdUnits; ++u) {
+    const int32_t j = R.first(q0 + u * kRowBlock);
+    if (j < int32_t(A.vocab)) grad_unit<T, ADD>(R, G, x, dx, token, j);
   }
+}
+
+// Short rows: one unit a lane, whatever rows a workgroup's lanes fall into.
+template <class T, bool ADD>
+__global__ __launch_bounds__(kRowBlock) void bwd_short_kernel(TokenArgs A, MagicDiv units) {
+  const uint64_t at_unit = uint64_t(blockIdx.x) * kRowBlock + threadIdx.x;
+  if (at_unit >= uint64_t(A.rows) * units.d) return;
+  const uint32_t row = units.div(uint32_t(at_unit)), q = uint32_t(at_unit) - row * units.d;
+  const int32_t token = A.tokens[row];
+  const RowAt at = row_at(A.map, row);
+  T *dx = static_cast<T *>(A.dx) + at.g;
+  const RowUnits<T> R(dx, A.vocab);
+  const int32_t j = R.first(q);
+  if (j >= int32_t(A.vocab)) return;
+  const float m = A.stats[2 * row];
+  if (token < 0 || m == -kInf) {
+    typename Unit<T>::floats none = 0.0f;
+    if (!ADD) R.template store<false>(dx, j, none);
+    return;
+  }
+  const RowGrad G(A, row, token, m, A.stats[2 * row + 1] + RowRef(A.c, m).shift(), A.entropy[row]);
+  grad_unit<T, ADD>(R, G, static_cast<const T *>(A.x) + at.x, dx, token, j);
+}
+
+// ------------------------------------------------------------------------- rows in registers
+
+// The largest and the sum over the L lanes that share a row.
+template <int L>
+__device__ __forceinline__ float lanes_max(float v, float *lds) {
+#pragma unroll
+  for (int d = (L < 64 ? L : 64) / 2; d >= 1; d >>= 1) v = __builtin_elementwise_maximum(v, __shfl_xor(v, d));
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int k = 1; k < L / 64; ++k) v = __builtin_elementwise_maximum(v, lds[k]);
+  }
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v, float *lds) {
+#pragma unroll
+  for (int d = (L < 64 ? L : 64) / 2; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int k = 1; k < L / 64; ++k) v += lds[k];
+  }
+  return v;
+}
+
+// Forward and gradient (GRAD), or the forward alone, of rows that L lanes hold in N units each: one read, one
+// write. Rows of up to a wave's lanes share workgroups.
+template <class T, int L, int N, bool GRAD>
+__global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(TokenArgs A) {
+  constexpr uint32_t B = L > kRowBlock ? L : kRowBlock, E = Unit<T>::E;
+  constexpr uint32_t ROWS = L > 64 ? 1 : B / L;
+  static_assert(L <= 64 || L == B, "a row has a workgroup or lanes of a wave");
+  __shared__ float lds[3][16];
+  const uint32_t V = A.vocab, gl = threadIdx.x % L;
+  const uint32_t r = blockIdx.x * ROWS + threadIdx.x / L;
+  const bool valid = ROWS == 1 || r < A.rows;
+  const uint32_t row = valid ? r : A.rows - 1;
+  const int32_t token = A.tokens[row];
+  const RowAt at = row_at(A.map, row);
+  const T *x = static_cast<const T *>(A.x) + at.x;
+  T *dx = static_cast<T *>(A.dx) + at.g;
+  const RowUnits<T> R(GRAD ? dx : x, V);
+  typename Unit<T>::vec v[N];
+  if (token >= 0) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const int32_t j = R.first(u * L + gl);
+      if (j < int32_t(V)) v[u] = R.load(x, j);
+      else v[u] = T(-kInf);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < N; ++u) v[u] = T(-kInf);
+  }
+  const float x_token = gl == 0 && uint32_t(token) < V ? float(x[token]) : 0.0f;
+  float m = -kInf;
+#pragma unroll
+  for (int u = 0; u < N; ++u) m = __builtin_elementwise_maximum(m, unit_max(to_floats<T>(v[u])));
+  m = lanes_max<L>(m, lds[0]);
+  const RowRef ref(A.c, m);
+  float s = 0.0f, w = 0.0f;
+  if (m != -kInf) {
+    const auto sums = [&](auto far) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        keep_raw(v[u]);
+        const auto f = to_floats<T>(v[u]);
+#pragma unroll
+        for (uint32_t e = 0; e < E; ++e) {
+          const float z = fmaxf(far ? (f[e] - m) * A.c : __builtin_fmaf(f[e], A.c, -ref.cm), -200.0f);
+          const float p = __builtin_amdgcn_exp2f(z);
+          s += p;
+          w = __builtin_fmaf(p, z, w);
+        }
+      }
+    };
+    if (ref.far) sums(std::true_type{});
+    else sums(std::false_type{});
+  }
+  s = lanes_sum<L>(s, lds[1]);
+  w = lanes_sum<L>(w, lds[2]);
+  if (!(fabsf(m) <= FLT_MAX) && m != -kInf) m = __builtin_nanf("");  // a NaN or an infinite logit
+  const float l = log2f(s);
+  if (gl == 0 && valid) {
+    if (token < 0) pad_out(A, row);
+    else row_out(A, row, token, x_token, m, s, w);
+  }
+  if constexpr (GRAD) {
+    if (!valid) return;
+    if (m == -kInf) {  // padding too
+      typename Unit<T>::floats none = 0.0f;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const int32_t j = R.first(u * L + gl);
+        if (j < int32_t(V)) R.template store<false>(dx, j, none);
+      }
+      return;
+    }
+    const float h = kLn2 * (l - w / s);
+    const RowGrad G(A, row, token, m, l, h < 0.0f ? 0.0f : h);
+    const auto grads = [&](auto far) {
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const int32_t j = R.first(u * L + gl);
+        if (j >= int32_t(V)) continue;
+        keep_raw(v[u]);
+        auto f = to_floats<T>(v[u]);
+#pragma unroll
+        for (int32_t e = 0; e < int32_t(E); ++e) {
+          const float z = fmaxf(far ? (f[e] - m) * A.c : __builtin_fmaf(f[e], A.c, -ref.cm), -200.0f);
+          f[e] = -__builtin_amdgcn_exp2f(z) * __builtin_fmaf(G.b, z, G.a);
+          if (token == j + e) f[e] += G.onehot;
+        }
+        R.template store<false>(dx, j, f);
+      }
+    };
+    if (ref.far) grads(std::true_type{});
+    else grads(std::false_type{});
+  }
+}
+
+// f(lanes, units) for rows of `units` units that registers can hold; false for longer ones.
+template <class F>
+bool with_held_shape(uint32_t units, F &&f) {
+  using std::integral_constant;
+  const auto call = [&](auto l, auto n) { f(l, n); return true; };
+#define HELD(l, n) \
+  if (units <= l * n) return call(integral_constant<int, l>{}, integral_constant<int, n>{});
+  HELD(2, 4) HELD(4, 4) HELD(8, 4) HELD(16, 4) HELD(32, 4) HELD(64, 4) HELD(256, 4) HELD(512, 4) HELD(1024, 4)
+  HELD(1024, 8) HELD(1024, 16)
+#undef HELD
+  return false;
 }
 
 // ------------------------------------------------------------------------- host
@@ -741,6 +985,16 @@ template <class T, bool TOP>
 bool launch_rows(const TokenArgs &A, const char *where) {
   const uint64_t unit = 16 / sizeof(T), units = A.vocab / unit;
   Pieces P{1, nullptr, nullptr};
+  if constexpr (!TOP)
+    if (most_units<T>(A.vocab) <= 256) {
+      with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto n) {
+        constexpr int L = decltype(lanes)::value;
+        if constexpr (L <= 64)
+          held_kernel<T, L, decltype(n)::value, false>
+              <<<ceil_div(A.rows, kRowBlock / L), kRowBlock, 0, stream()>>>(A);
+      });
+      return true;
+    }
   // waves of a row: enough rows, or enough waves to a row, to fill the chip
   if (A.rows >= 2048 || units <= 256) {
     fwd_kernel<T, 1, TOP, false><<<ceil_div(A.rows, 4), 256, 0, stream()>>>(A, P);
@@ -771,10 +1025,28 @@ bool launch_forward(const TokenArgs &A, DTYPE type, const char *where) {
   return ok;
 }
 
+template <class T, bool ADD>
+void launch_bwd(const TokenArgs &A) {
+  const uint32_t units = most_units<T>(A.vocab);
+  if (units < 128 && uint64_t(A.rows) * units < uint64_t(1) << 32) {
+    bwd_short_kernel<T, ADD><<<ceil_div(uint64_t(A.rows) * units, kRowBlock), kRowBlock, 0, stream()>>>(
+        A, MagicDiv::make(units));
+    return;
+  }
+  const uint32_t chunks = ceil_div(units, kBwdUnits * kRowBlock);
+  const uint64_t most = max_blocks(kRowBlock) / chunks;  // rows of one launch
+  TokenArgs part = A;
+  for (uint64_t r = 0; r < A.rows; r += most) {
+    part.first_row = uint32_t(r);
+    part.rows = uint32_t(A.rows - r < most ? A.rows - r : most);
+    bwd_kernel<T, ADD><<<part.rows * chunks, kRowBlock, 0, stream()>>>(part, chunks);
+  }
+}
+
 void launch_backward(const TokenArgs &A, DTYPE type, bool add) {
   with_float_type(type, [&](auto t) {
-    if (add) bwd_kernel<decltype(t), true><<<A.rows, kRowBlock, 0, stream()>>>(A);
-    else bwd_kernel<decltype(t), false><<<A.rows, kRowBlock, 0, stream()>>>(A);
+    if (add) launch_bwd<decltype(t), true>(A);
+    else launch_bwd<decltype(t), false>(A);
   });
 }
 
@@ -882,6 +1154,18 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
   if (!upstream(dlogp, N, &A.dlogp, where) || !upstream(dentropy, N, &A.dentropy, where) || N == 0 ||
       !ensure_init())
     return;
+  bool held = false;
+  with_float_type(x->dtype, [&](auto t) {
+    typedef decltype(t) T;
+    held = with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto units) {
+      constexpr int L = decltype(lanes)::value, B = L > kRowBlock ? L : kRowBlock;
+      held_kernel<T, L, decltype(units)::value, true><<<ceil_div(N, L > 64 ? 1 : B / L), B, 0, stream()>>>(A);
+    });
+  });
+  if (held) {
+    finish(where);
+    return;
+  }
   A.stats = static_cast<float *>(partials(2 * N * sizeof(float), where));
   if (!A.stats) return;
   if (!launch_forward(A, x->dtype, where)) return;
