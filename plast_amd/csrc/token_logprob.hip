@@ -300,22 +300,43 @@ __device__ __forceinline__ void exact_row(const TokenArgs &A, const T *x, uint32
   }
 }
 
-// Keeps the largest candidates of a row while it is read. A bound under which no logit can be among the
-// `top` largest starts as the top-th largest of 64 lane groups' maxima over the first logits (so many
-// logits at least reach it), and is raised to the top-th candidate whenever as many logits again have been
-// read; only logits above it go to the list, a few times `top` in all.
-template <int W>
+// Finds the `top` largest logits of a row while it is read, by units: a unit's key is its largest logit and its
+// number, and the largest logits all lie in the `top` units of the largest keys (a logit of another unit has
+// `top` logits before it, those units' largest). A bound under which no unit counts starts as the top-th
+// largest of 16, 32 or 64 lane groups' maxima over the first logits, twice `top` groups at least, and is raised to
+// the top-th unit whenever as many logits again have been read; only units above it go to the list, some
+// top ln(units) in all, and an ascending row raises it more often. Logits after the last whole unit are units
+// of their own.
+template <class T, int W>
 struct Candidates {
-  static constexpr uint32_t NL = 64 * W;
+  static constexpr uint32_t NL = 64 * W, E = Unit<T>::E;
   RowLds<W> &L;
-  uint32_t gl, top, cur = 0;
-  float bound = kInf;  // logits above it are candidates
+  const T *x;
+  uint32_t gl, top, units, cur = 0;
+  float bound = kInf;  // units above it are candidates
   bool lost = false;   // the list was too short
-  __device__ __forceinline__ Candidates(RowLds<W> &l, uint32_t g, uint32_t t) : L(l), gl(g), top(t) {}
+  uint32_t held = 0;   // its length, where a wave has its own
+  __device__ __forceinline__ Candidates(RowLds<W> &l, const T *row, uint32_t g, uint32_t t, uint32_t n)
+      : L(l), x(row), gl(g), top(t), units(n) {}
 
-  __device__ __forceinline__ void push(float v, uint32_t j) {
-    const uint32_t at = atomicAdd(&L.count[cur], 1u);
-    if (at < kList) L.list[cur][at] = order_key(v, j);
+  // By whole waves: the lanes that `hot` names add theirs.
+  __device__ __forceinline__ void push(bool hot, float v, uint32_t number) {
+    const uint64_t hits = __ballot(hot);
+    if (!hits) return;
+    const uint32_t n = __popcll(hits), before = __popcll(hits & ((uint64_t(1) << (gl & 63)) - 1));
+    uint32_t at = held;
+    if constexpr (W == 1) {
+      held += n;
+    } else {
+      if ((gl & 63) == 0) at = atomicAdd(&L.count[cur], n);
+      at = __builtin_amdgcn_readfirstlane(at);
+    }
+    if (hot && at + before < kList) L.list[cur][at + before] = order_key(v, number);
+  }
+  __device__ __forceinline__ uint32_t listed() const { return W == 1 ? held : L.count[cur]; }
+  __device__ __forceinline__ void relist(uint32_t n, uint32_t list) {
+    if constexpr (W == 1) held = n;
+    else if (gl == 0) L.count[list] = n;
   }
   __device__ __forceinline__ void clear() {
     if (gl == 0) L.count[0] = L.count[1] = L.ties = 0;
@@ -332,23 +353,31 @@ struct Candidates {
     } else {
       row_sync<W>();
     }
-    const uint32_t lane = gl % 64;
     uint32_t before = 0;
-#pragma unroll 8
-    for (uint32_t d = 0; d < 64; ++d) {
-      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), d));
-      before += o > v || (o == v && d < lane);
-    }
-    const uint64_t at = __ballot(before == top - 1);
-    bound = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), __ffsll((unsigned long long)at) - 1));
+    const auto count = [&](auto groups) {
+      constexpr uint32_t G = decltype(groups)::value;
+#pragma unroll
+      for (uint32_t d = 32; d >= G; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+#pragma unroll
+      for (uint32_t d = 0; d < G; ++d) before += __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), d)) > v;
+    };
+    if (top <= 8) count(std::integral_constant<uint32_t, 16>{});
+    else if (top <= 16) count(std::integral_constant<uint32_t, 32>{});
+    else count(std::integral_constant<uint32_t, 64>{});
+    // the top-th largest: the smallest that fewer than `top` exceed
+    v = before < top ? v : kInf;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v = fminf(v, __shfl_xor(v, d));
+    bound = v;
   }
-  // After start()'s logits: those above the bound are in the list and `equal` counts this lane's at it. The
-  // lowest of the equal ones are found by rereading the row from its start where there are many (a mask).
-  template <class T, class F>
-  __device__ __forceinline__ void take_equal(uint32_t equal, F &&push_equal, const T *x, uint32_t from, uint32_t to) {
+  // After start()'s logits: the units above the bound are in the list and `equal` counts this lane's at it. The
+  // lowest of the equal ones are found by rereading the units from..to and the tail where there are many (a
+  // mask).
+  template <class F>
+  __device__ __forceinline__ void take_equal(uint32_t equal, F &&push_equal, uint32_t from, uint32_t to, uint32_t tail) {
     if (equal) atomicAdd(&L.ties, equal);
     row_sync<W>();
-    const uint32_t above = L.count[0], ties = L.ties;
+    const uint32_t above = listed(), ties = L.ties;
     row_sync<W>();
     if (above > kList) {
       give_up();
@@ -360,27 +389,28 @@ struct Candidates {
       row_sync<W>();
       return;
     }
-    if (gl < 64) {
-      uint32_t want = top - above, at = above;
-      for (uint32_t j0 = from; want && j0 < to; j0 += 64) {
-        const uint32_t j = j0 + gl;
-        const float v = j < to ? float(x[j]) : __builtin_nanf("");
+    uint32_t want = top - above, at = above;
+    if (gl < 64)
+      for (uint32_t n0 = from; want && n0 < to + tail; n0 += 64) {
+        const uint32_t n = n0 + gl;
+        float v = __builtin_nanf("");
+        if (n < to) v = unit_max(to_floats<T>(load_unit(x + uint64_t(n) * E)));
+        else if (n < to + tail) v = float(x[uint64_t(to) * E + (n - to)]);
         const uint64_t hit = __ballot(v == bound);
         const uint32_t place = __popcll(hit & ((uint64_t(1) << gl) - 1));
-        if (v == bound && place < want) L.list[0][at + place] = order_key(v, j);
-        const uint32_t n = min(uint32_t(__popcll(hit)), want);
-        want -= n;
-        at += n;
+        if (v == bound && place < want) L.list[0][at + place] = order_key(v, n);
+        const uint32_t got = min(uint32_t(__popcll(hit)), want);
+        want -= got;
+        at += got;
       }
-      if (gl == 0) L.count[0] = at;
-    }
+    relist(at, 0);
     row_sync<W>();
   }
   __device__ __forceinline__ void give_up() {
     lost = true;
     bound = kInf;
   }
-  // The place of a candidate among the list's.
+  // The place of a candidate among the list's n.
   __device__ __forceinline__ uint32_t rank(uint64_t key, uint32_t n) const {
     uint32_t r = 0;
 #pragma unroll 4
@@ -390,7 +420,7 @@ struct Candidates {
   // Drops all but the `top` largest and raises the bound to the last of them.
   __device__ __forceinline__ void raise() {
     row_sync<W>();
-    const uint32_t n = L.count[cur];
+    const uint32_t n = listed();
     if (n > kList) give_up();
     if (lost || n <= top) {
       row_sync<W>();
@@ -402,25 +432,61 @@ struct Candidates {
       if (r < top) L.list[1 - cur][r] = key;
       if (r == top - 1) L.threshold = key_value(key);
     }
-    if (gl == 0) L.count[1 - cur] = top;
+    relist(top, 1 - cur);
     cur = 1 - cur;
     row_sync<W>();
     bound = L.threshold;
+  }
+  // The units' logits in their place: the list holds logits from here on.
+  __device__ __forceinline__ void open() {
+    raise();
+    if (lost) return;
+    const uint32_t n = listed(), old = cur;
+    const float least = n == top ? bound : -kInf;  // the top-th logit is no smaller
+    row_sync<W>();
+    cur = 1 - cur;
+    relist(0, cur);
+    row_sync<W>();
+    for (uint32_t i0 = 0; i0 < n * E; i0 += NL) {
+      const uint32_t i = i0 + gl;
+      bool hot = i < n * E;
+      float v = 0.0f;
+      uint32_t j = 0;
+      if (hot) {
+        const uint32_t number = 0xffffffffu - uint32_t(L.list[old][i / E]), e = i % E;
+        j = number < units ? number * E + e : units * E + (number - units);
+        hot = number < units || e == 0;
+        v = float(x[j]);
+        hot = hot && v >= least;
+      }
+      push(hot, v, j);
+    }
+    row_sync<W>();
   }
 };
 
 // A piece of a row, where rows are cut because there are few: what it found, for the last to finish.
 struct Piece {
   float m, cm, s, w;
-  uint32_t lost, found;
   uint64_t keys[PLAST_TOP_MAX];
+  uint32_t lost;  // the list was too short
 };
+// The XCDs' L2 caches are not coherent: what a workgroup leaves for another goes past them, store by store (a
+// fence would write back and drop the whole cache: 46 us instead of 9 with 384 workgroups).
+template <class V>
+__device__ __forceinline__ void put_shared(V *p, V v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class V>
+__device__ __forceinline__ V get_shared(const V *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 struct Pieces {
   uint32_t n;
   Piece *found;      // [rows][n]
   uint32_t *tickets;  // [rows], zero between launches
 };
-constexpr uint32_t kTickets = 4096;
+constexpr uint32_t kTickets = 4096, kMaxPieces = 32;
 __device__ uint32_t g_tickets[kTickets];
 
 // W waves per row (or piece of one), four rows per workgroup where W is 1. One pass: a lane's units of 16 bytes
@@ -437,6 +503,19 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   const uint32_t piece = CUT ? blockIdx.x - row * P.n : 0, pieces = CUT ? P.n : 1;
   if (W == 1 && row >= A.rows) return;
   const int32_t token = A.tokens[row];
+  const uint32_t V = A.vocab, units = V / E;
+  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
+  const uint32_t from = uint32_t(uint64_t(units) * piece / pieces), to = uint32_t(uint64_t(units) * (piece + 1) / pieces);
+  // where rows are few, their first units are on their way before the token is known
+  typename Unit<T>::vec v[U];
+  const auto fetch = [&](uint32_t q0) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t q = q0 + u * NL + gl;
+      if (q < to) v[u] = load_unit(x + uint64_t(q) * E);
+    }
+  };
+  if constexpr (W > 1) fetch(from);
   if (token < 0) {
     if (piece == 0) {
       if (gl == 0) pad_out(A, row);
@@ -444,31 +523,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
     }
     return;
   }
-  const uint32_t V = A.vocab, units = V / E;
-  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
-  const uint32_t from = uint32_t(uint64_t(units) * piece / pieces), to = uint32_t(uint64_t(units) * (piece + 1) / pieces);
+  const float x_token = uint32_t(token) < V ? float(x[token]) : 0.0f;
   // the logits after the last unit, one a lane
   const bool has_tail = piece == pieces - 1 && gl < V - units * E;
-  const uint32_t tail_at = units * E + gl;
-  const float tail = has_tail ? float(x[tail_at]) : -kInf;
+  const float tail = has_tail ? float(x[units * E + gl]) : -kInf;
   const bool tail_first = to - from <= NL * U;  // then it is among the first logits
   const float c = A.c;
   Running r;
-  Candidates<W> top(L, gl, A.top);
+  Candidates<T, W> top(L, x, gl, A.top, units);
   if constexpr (TOP) top.clear();
   uint32_t batch = 0;
   uint32_t q0 = from;
   do {
-    typename Unit<T>::vec v[U];
-#pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-      const uint32_t q = q0 + u * NL + gl;
-      if (q < to) v[u] = load_unit(x + uint64_t(q) * E);
-    }
+    if (W == 1 || batch) fetch(q0);
     float most = tail_first ? tail : -kInf;
+    float largest[U];  // of each unit
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
       const uint32_t q = q0 + u * NL + gl;
+      largest[u] = -kInf;
       if (q >= to) continue;
       const auto f = to_floats<T>(v[u]);
       const float g = unit_max(f);
@@ -476,39 +549,38 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
 #pragma unroll
       for (uint32_t e = 0; e < E; ++e) r.add(c, f[e]);
       if constexpr (TOP) {
+        largest[u] = g;
         most = fmaxf(most, g);
-        if (batch && g > top.bound) {
-#pragma unroll
-          for (uint32_t e = 0; e < E; ++e)
-            if (f[e] > top.bound) top.push(f[e], q * E + e);
-        }
       }
     }
     if constexpr (TOP) {
       if (batch == 0) {
         top.start(most);
-        uint32_t equal = 0;
-        const auto each = [&](auto &&visit) {
+        const bool tail_now = tail_first && has_tail;
+        uint32_t equal = tail_now && tail == top.bound;
+        top.push(tail_now && tail > top.bound, tail, units + gl);
 #pragma unroll
-          for (uint32_t u = 0; u < U; ++u) {
-            const uint32_t q = q0 + u * NL + gl;
-            if (q >= to) continue;
-            const auto f = to_floats<T>(v[u]);
-            if (unit_max(f) >= top.bound)
-#pragma unroll
-              for (uint32_t e = 0; e < E; ++e) visit(f[e], q * E + e);
-          }
-          if (tail_first && has_tail) visit(tail, tail_at);
-        };
-        each([&](float a, uint32_t j) {
-          if (a > top.bound) top.push(a, j);
-          else if (a == top.bound) ++equal;
-        });
+        for (uint32_t u = 0; u < U; ++u) {
+          const uint32_t q = q0 + u * NL + gl;
+          top.push(largest[u] > top.bound, largest[u], q);
+          equal += q < to && largest[u] == top.bound;
+        }
         top.take_equal(
-            equal, [&] { each([&](float a, uint32_t j) { if (a == top.bound) top.push(a, j); }); }, x, from * E,
-            tail_first && piece == pieces - 1 ? V : min(q0 + NL * U, to) * E);
-      } else if (((batch + 1) & batch) == 0) {
-        top.raise();
+            equal,
+            [&] {
+              top.push(tail_now && tail == top.bound, tail, units + gl);
+#pragma unroll
+              for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t q = q0 + u * NL + gl;
+                top.push(q < to && largest[u] == top.bound, largest[u], q);
+              }
+            },
+            from, min(q0 + NL * U, to), tail_first && piece == pieces - 1 ? V - units * E : 0);
+      } else {
+        if (__any(most > top.bound))
+#pragma unroll
+          for (uint32_t u = 0; u < U; ++u) top.push(largest[u] > top.bound, largest[u], q0 + u * NL + gl);
+        if (((batch + 1) & batch) == 0 || (W == 1 && top.listed() > kList / 2)) top.raise();
       }
     }
     ++batch;
@@ -517,8 +589,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   if (has_tail) {
     if (!(tail <= r.m)) r.grow(c, tail);
     r.add(c, tail);
-    if (TOP && !tail_first && tail > top.bound) top.push(tail, tail_at);
   }
+  if (TOP && !tail_first) top.push(has_tail && tail > top.bound, tail, units + gl);
   r = wave_join(r);
   if constexpr (W > 1) {
     if (gl % 64 == 0) {
@@ -544,42 +616,59 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   }
   uint32_t found = 0;
   if constexpr (TOP) {
-    found = L.count[top.cur];
-    if (found > kList) top.give_up();
+    top.open();
+    found = top.listed();
   }
   if constexpr (CUT) {
     __shared__ bool is_last;
     Piece *mine = P.found + uint64_t(row) * P.n;
     if (gl == 0) {
-      mine[piece].m = r.m, mine[piece].cm = r.cm, mine[piece].s = r.s, mine[piece].w = r.w;
-      mine[piece].lost = top.lost, mine[piece].found = min(found, A.top);
+      put_shared(&mine[piece].m, r.m);
+      put_shared(&mine[piece].cm, r.cm);
+      put_shared(&mine[piece].s, r.s);
+      put_shared(&mine[piece].w, r.w);
+      put_shared(&mine[piece].lost, uint32_t(top.lost));
     }
-    if (TOP && !top.lost)
+    if (TOP && !top.lost) {
       for (uint32_t i = gl; i < found; i += NL) {
         const uint64_t key = L.list[top.cur][i];
         const uint32_t k = top.rank(key, found);
-        if (k < A.top) mine[piece].keys[k] = key;
+        if (k < A.top) put_shared(&mine[piece].keys[k], key);
       }
-    __threadfence();
+      if (gl >= found && gl < A.top) put_shared(&mine[piece].keys[gl], uint64_t(0));
+    }
+    // every wave's stores have reached the memory that the XCDs share before the ticket is drawn
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (gl == 0) is_last = atomicAdd(&P.tickets[row], 1u) == P.n - 1;
+    if (gl == 0)
+      is_last = __hip_atomic_fetch_add(&P.tickets[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == P.n - 1;
     __syncthreads();
     if (!is_last) return;
-    if (gl == 0) __hip_atomic_store(&P.tickets[row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __threadfence();
+    if (gl == 0) put_shared(&P.tickets[row], 0u);
     // a wave's lanes take the pieces; the merged sums are the same whoever comes last
     Running o;
     const uint32_t lane = gl % 64;
-    bool lost = false;
+    uint32_t lost = 0;
+    uint64_t least = 0, keys[kMaxPieces * PLAST_TOP_MAX / NL];
     if (lane < P.n) {
-      o.m = mine[lane].m, o.cm = mine[lane].cm, o.s = mine[lane].s, o.w = mine[lane].w;
-      lost = mine[lane].lost != 0;
+      o.m = get_shared(&mine[lane].m), o.cm = get_shared(&mine[lane].cm);
+      o.s = get_shared(&mine[lane].s), o.w = get_shared(&mine[lane].w);
+      if constexpr (TOP) {
+        lost = get_shared(&mine[lane].lost);
+        least = get_shared(&mine[lane].keys[A.top - 1]);
+      }
+    }
+    if constexpr (TOP) {
+#pragma unroll
+      for (uint32_t t = 0; t < kMaxPieces * PLAST_TOP_MAX / NL; ++t) {
+        const uint32_t i = gl + t * NL, p = i / A.top;
+        keys[t] = p < P.n ? get_shared(&mine[p].keys[i - p * A.top]) : 0;
+      }
     }
     r = wave_join(o);
-    top.lost = __any(lost);
+    top.lost = __any(lost != 0);
     if (TOP && !top.lost) {
       // no logit below a piece's last candidate can be among the largest
-      uint64_t least = lane < P.n && mine[lane].found == A.top ? mine[lane].keys[A.top - 1] : 0;
 #pragma unroll
       for (int d = 32; d >= 1; d >>= 1) {
         const uint64_t k = __shfl_xor((unsigned long long)least, d);
@@ -588,15 +677,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
       top.cur = 0;
       if (gl == 0) L.count[0] = 0;
       __syncthreads();
-      for (uint32_t i = gl; i < P.n * A.top; i += NL) {
-        const uint32_t p = i / A.top, k = i - p * A.top;
-        if (k >= mine[p].found) continue;
-        const uint64_t key = mine[p].keys[k];
-        if (key >= least) {
+#pragma unroll
+      for (uint32_t t = 0; t < kMaxPieces * PLAST_TOP_MAX / NL; ++t)
+        if (keys[t] && keys[t] >= least) {
           const uint32_t at = atomicAdd(&L.count[0], 1u);
-          if (at < kList) L.list[0][at] = key;
+          if (at < kList) L.list[0][at] = keys[t];
         }
-      }
       __syncthreads();
       found = L.count[0];
       if (found > kList) top.give_up();
@@ -605,11 +691,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   const bool exact = !in_range(c, r.m);
   if (exact || top.lost) {
     const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
-    if (!exact && gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, r.m, r.s, r.w);
+    if (!exact && gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w);
     exact_row<T, W>(A, x, row, token, gl, L, exact, r.m, l0);
     return;
   }
-  if (gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, r.m, r.s, r.w);
+  if (gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w);
   if constexpr (TOP) {
     const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
     for (uint32_t i = gl; i < found; i += NL) {
@@ -996,13 +1082,13 @@ bool launch_rows(const TokenArgs &A, const char *where) {
       return true;
     }
   // waves of a row: enough rows, or enough waves to a row, to fill the chip
-  if (A.rows >= 2048 || units <= 256) {
+  if (units <= 256 || (A.rows >= 8192 && units < 4096)) {
     fwd_kernel<T, 1, TOP, false><<<ceil_div(A.rows, 4), 256, 0, stream()>>>(A, P);
     return true;
   }
   uint64_t cut = units / 1024;
   if (cut > 512 / A.rows) cut = 512 / A.rows;
-  if (cut > 32) cut = 32;
+  if (cut > kMaxPieces) cut = kMaxPieces;
   if (cut > 1) {
     P.n = uint32_t(cut);
     P.tickets = tickets(where);
