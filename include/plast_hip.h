@@ -275,7 +275,7 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
  * them, each by itself: FLOAT32, FLOAT16 or BFLOAT16, any strides (out's must not overlap); out has
  * g's type and shape and may be g itself. The iteration runs on
  * float32-grade products: every factor is held as a pair of 16-bit floats, 22 significant bits,
- * summed in 32 bits; entries of an iterate beyond 15 (a diverging rule) overflow to inf or NaN.
+ * summed in 32 bits. A rule that takes a singular value in [0, 1] beyond 4 is refused.
  * No counterpart in the reference. */
 void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule);
 /* One Muon step over `num_parameters` contiguous FLOAT32 matrices of any shapes (other ranks are

@@ -5,13 +5,21 @@
 // X = G / (|G| + eps), Frobenius norm, each of `steps` iterations is
 //   A = X X^T (m x m),  S = b A + c A A (m x m),  X = a X + S X (m x n).
 // A and S are symmetric: their products compute the tiles on and below the diagonal and store each twice.
+// Two steps can go at once: with P = a I + S the next X is P X and its A is P A P, all m x m, so that
+//   PA = a A + S A,  A' = a PA + S PA,  S' = b A' + c A' A',  Q = a (S + S') + S' S,  X'' = a^2 X + Q X,
+// polynomials of A that commute: their products are symmetric too. X is formed anew every second step, as an
+// error of A' (of 2^-24, say) grows by a^2 with each step that goes without.
 //
 // The products run on the matrix units. fp32's own matrix instructions reach a sixteenth of fp16's rate,
 // so every factor v is kept as two fp16, hi = round(v) and lo = round(v - hi), 22 significant bits (and a
-// scale that keeps lo above fp16's subnormals: X and A times 2^12, S times 2^11), and a product is three
+// scale that keeps lo above fp16's subnormals), and a product is three
 // instructions, hi hi + hi lo + lo hi, summed in fp32. What is left out, lo lo, is below 2^-22 of the
 // product. The iteration in 64 bits is met to 4e-7 of the result at [256, 256] and [300, 800], where
 // fp32 factors (24 bits, but one rounding per addition) meet it to 1.5e-6 and 1.8e-6.
+//
+// Matrices of bfloat16 take hi alone, one instruction a product: bf16 keeps 8 bits of the input and of the result, so
+// factors of 11 stay below the rounding that the input already had. The result is off by 1.4e-3 before its own
+// rounding of 1.7e-3 (all in bf16: 1.1e-2), for a third of the arithmetic: 6 x 2605 x 1001 596 us instead of 1027.
 //
 // Layout of a factor ("lines"): each row is cut into lines of 128 bytes, a line holding 32 columns' hi
 // and then their lo: what a workgroup's tile needs of a row in one step of the sum is one whole line, read
@@ -22,6 +30,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 #include <unordered_set>
 #include <vector>
 
@@ -126,17 +135,21 @@ __device__ __forceinline__ double norm_of(const double *part, uint32_t b, uint32
 
 // ------------------------------------------------------------------------- lines
 
-constexpr float kScaleX = 4096.0f, kScaleA = 4096.0f, kScaleS = 2048.0f;
+// The powers of two that X, A (and P A) and S (and Q) are kept times: 2^12, 2^12 and 2^11 for rules whose singular
+// values stay around 1, less where the iteration leaves them no room below fp16's 65504.
+struct Scales {
+  float x, a, s;
+};
 
-// The power of two that X is kept times. 2^12 where |X| = |G| / (|G| + eps) is about 1. A smaller |G|
+// The power of two that one X is kept times: `scale` where |X| = |G| / (|G| + eps) is about 1. A smaller |G|
 // leaves a small X, whose iterates grow by up to `growth` bits in all, a being their largest factor: it is
 // raised by the bits that X lacks, less those that it may still grow by and has no room for.
-__device__ __forceinline__ double scale_of_x(double norm, float eps, int growth) {
+__device__ __forceinline__ double scale_of_x(double norm, float eps, int growth, float scale) {
   const double x = norm / (norm + double(eps));
   int lacks = x > 0.0 && x < 0.5 ? -ilogb(x) - 1 : 0;
   lacks = lacks > 110 ? 110 : lacks;
   const int grows = lacks < growth ? lacks : growth;
-  return ldexp(double(kScaleX), lacks - (grows > 3 ? grows - 3 : 0));
+  return ldexp(double(scale), lacks - (grows > 3 ? grows - 3 : 0));
 }
 
 // A stack of factors in lines: `rows` padded rows of `pitch` bytes.
@@ -144,10 +157,13 @@ struct Lines {
   char *data;
   uint64_t pitch, next;  // bytes from one row, one matrix to the next
 };
+// PL: 2 for pairs, 1 for hi alone, 64 columns a line.
+template <int PL>
 __device__ __forceinline__ char *line_at(const Lines &L, uint32_t b, uint32_t row, uint32_t col) {
-  return L.data + b * L.next + row * L.pitch + (col >> 5) * 128 + (col & 31) * 2;
+  return L.data + b * L.next + row * L.pitch + (PL == 2 ? (col >> 5) * 128 + (col & 31) * 2 : col * 2);
 }
 // Eight columns (a multiple of 8) of a row.
+template <int PL>
 __device__ __forceinline__ void put8(char *at, const float *v) {
   h8 hi, lo;
 #pragma unroll
@@ -156,22 +172,30 @@ __device__ __forceinline__ void put8(char *at, const float *v) {
     lo[e] = f16_t(v[e] - float(hi[e]));
   }
   *reinterpret_cast<h8 *>(at) = hi;
-  *reinterpret_cast<h8 *>(at + 64) = lo;
+  if constexpr (PL == 2) *reinterpret_cast<h8 *>(at + 64) = lo;
 }
+template <int PL>
 __device__ __forceinline__ void get8(const char *at, float *v) {
-  const h8 hi = *reinterpret_cast<const h8 *>(at), lo = *reinterpret_cast<const h8 *>(at + 64);
+  const h8 hi = *reinterpret_cast<const h8 *>(at);
+  h8 lo = f16_t(0.0f);
+  if constexpr (PL == 2) lo = *reinterpret_cast<const h8 *>(at + 64);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = float(hi[e]) + float(lo[e]);
 }
+template <int PL>
+__device__ __forceinline__ float get1(const char *at) {
+  const float hi = float(*reinterpret_cast<const f16_t *>(at));
+  return PL == 2 ? hi + float(*reinterpret_cast<const f16_t *>(at + 64)) : hi;
+}
 
 // X and X^T in lines from the source, a 64x64 tile per workgroup, padding included.
-template <class T, bool MUON>
+template <class T, bool MUON, int PL>
 __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, const double *part,
-                                                         uint32_t parts, float eps, int growth, Lines X,
-                                                         Lines XT, float *xscale) {
+                                                         uint32_t parts, float eps, int growth,
+                                                         float base, Lines X, Lines XT, float *xscale) {
   __shared__ float tile[64][65];
   const uint32_t b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of the source
-  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth);
+  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth, base);
   const double scale = sx / (norm + double(eps));
   if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) xscale[b] = float(sx);
   const bool tall = G.rows > G.cols;
@@ -199,13 +223,15 @@ __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, con
       v[k] = tile[r][c + k];
       w[k] = tile[c + k][r];
     }
-    put8(line_at(R, b, r0 + r, c0 + c), v);
-    put8(line_at(C, b, c0 + r, r0 + c), w);
+    put8<PL>(line_at<PL>(R, b, r0 + r, c0 + c), v);
+    put8<PL>(line_at<PL>(C, b, c0 + r, r0 + c), w);
   }
 }
 
 // ------------------------------------------------------------------------- products
 
+// X X^T; a product of two symmetric factors that commute (polynomials of one matrix), with terms added; an
+// update of X; the last one.
 enum Mode { Gram, Square, Update, Final };
 
 // Where the last step's result goes: out[b][i, j] (O), or p = p keep - scale * it.
@@ -217,7 +243,8 @@ struct Product {
   uint32_t ti, tj;    // tiles
   uint32_t parts;     // the sum is cut into so many pieces
   float *partial;     // their sums, when there are several
-  float alpha, beta;  // result = alpha * sum + beta * term, in the result's scale, of
+  Lines in2;          // another term (Square), where it has data
+  float alpha, beta, gamma;  // result = alpha sum + beta term + gamma term2, in the result's scale, of
   const float *xscale;  // X's scale in Gram and Final: by 1 / its square, 1 / it
   Stack o;
 };
@@ -232,7 +259,7 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-template <class T, Mode M, bool MUON>
+template <class T, Mode M, bool MUON, int PL>
 __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, float *lds, f16v acc, uint32_t b,
                                           uint32_t i0, uint32_t j0, bool mirror) {
   const uint32_t lane = threadIdx.x & 63;
@@ -252,13 +279,13 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
     if (!tall) {
       float v[16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) get8(line_at(P.in, b, i0 + r, j0 + c + 8 * h), v + 8 * h);
+      for (int h = 0; h < 2; ++h) get8<PL>(line_at<PL>(P.in, b, i0 + r, j0 + c + 8 * h), v + 8 * h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) lds[r * 33 + c + e] += beta * v[e];
     } else {
       float v[16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) get8(line_at(P.in_t, b, j0 + r, i0 + c + 8 * h), v + 8 * h);
+      for (int h = 0; h < 2; ++h) get8<PL>(line_at<PL>(P.in_t, b, j0 + r, i0 + c + 8 * h), v + 8 * h);
 #pragma unroll
       for (int e = 0; e < 16; ++e) lds[(c + e) * 33 + r] += beta * v[e];
     }
@@ -285,25 +312,30 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = lds[r * 33 + c + 8 * h + e];
       if constexpr (M != Gram) {
-        get8(line_at(P.in, b, i0 + r, j0 + c + 8 * h), t);
+        get8<PL>(line_at<PL>(P.in, b, i0 + r, j0 + c + 8 * h), t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(beta, t[e], v[e]);
       }
-      put8(line_at(P.out, b, i0 + r, j0 + c + 8 * h), v);
+      if (M == Square && P.in2.data) {
+        get8<PL>(line_at<PL>(P.in2, b, i0 + r, j0 + c + 8 * h), t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(P.gamma, t[e], v[e]);
+      }
+      put8<PL>(line_at<PL>(P.out, b, i0 + r, j0 + c + 8 * h), v);
+      if (M != Gram && mirror)  // the transpose's lines take the same sums
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lds[r * 33 + c + 8 * h + e] = v[e];
     }
-    if (mirror)
+    if (mirror) {
+      wave_sync();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float v[8], t[8];
+        float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = lds[(c + 8 * h + e) * 33 + r];
-        if constexpr (M != Gram) {
-          get8(line_at(P.in_t, b, j0 + r, i0 + c + 8 * h), t);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(beta, t[e], v[e]);
-        }
-        put8(line_at(P.out_t, b, j0 + r, i0 + c + 8 * h), v);
+        put8<PL>(line_at<PL>(P.out_t, b, j0 + r, i0 + c + 8 * h), v);
       }
+    }
   }
   wave_sync();
 }
@@ -325,9 +357,9 @@ __device__ __forceinline__ void tile_at(uint32_t t, uint32_t ti, uint32_t &i, ui
 // One tile of BM x BN outputs over one piece of the sum, by waves of WM x WN. Two stages of LDS: while
 // the waves multiply one line of every row, the next lines are on their way into the other (loads straight
 // to LDS; lane l of a load fills bytes 16 l of its 1 KiB, so a row's eight 16-byte units are permuted by
-// choosing what each lane reads: unit c lies at c ^ (row % 8), which spreads the reads of eight rows over all
-// banks).
-template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
+// choosing what each lane reads: unit c lies at c ^ (row / 2 % 8). A 16-byte LDS read is served for lanes 0-3, 12-15,
+// 20-27 of a half wave together, then for the others, from 64 banks: this spreads either set over all of them).
+template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Product P, MuonSet S) {
   constexpr int NW = (BM / WM) * (BN / WN), LOADS = (BM + BN) / 8 / NW, FA = WM / 32, FB = WN / 32;
   constexpr uint32_t STAGE = (BM + BN) * 128;
@@ -352,7 +384,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
     const bool first_operand = r < BM;
     const Lines &L = first_operand ? P.u : P.v;
     const uint32_t row = (first_operand ? ti * BM + r : tj * BN + r - BM) + lane / 8;
-    src[k] = L.data + b * L.next + row * L.pitch + ((lane % 8) ^ (lane / 8)) * 16;
+    src[k] = L.data + b * L.next + row * L.pitch + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
   }
   const auto fetch = [&](uint32_t line, uint32_t stage) {
 #pragma unroll
@@ -378,12 +410,12 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
     __syncthreads();  // the line has arrived, and every wave is done with the other stage
     if (line + 1 < last) fetch(line + 1, stage ^ 1);
     const char *base = lds + stage * STAGE;
-    const uint32_t row = lane % 32, key = row % 8;
+    const uint32_t row = lane % 32, key = (row >> 1) & 7;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {  // 16 columns each
-      h8 ua[FA][2], vb[FB][2];
+    for (int g = 0; g < 4 / PL; ++g) {  // 16 columns each
+      h8 ua[FA][PL], vb[FB][PL];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
+      for (int p = 0; p < PL; ++p) {
         const uint32_t unit = ((p * 4 + g * 2 + lane / 32) ^ key) * 16;
 #pragma unroll
         for (int a = 0; a < FA; ++a)
@@ -393,7 +425,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
           vb[c][p] = *reinterpret_cast<const h8 *>(base + (BM + wj + c * 32 + row) * 128 + unit);
       }
 #pragma unroll
-      for (int q = 0; q < 3; ++q)
+      for (int q = 0; q < (PL == 2 ? 3 : 1); ++q)
 #pragma unroll
         for (int a = 0; a < FA; ++a)
 #pragma unroll
@@ -421,11 +453,106 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
   for (int a = 0; a < FA; ++a)
 #pragma unroll
     for (int c = 0; c < FB; ++c)
-      put_block<T, M, MUON>(P, S, way, acc[a][c], b, i0 + a * 32, j0 + c * 32, !sym || ti != tj);
+      put_block<T, M, MUON, PL>(P, S, way, acc[a][c], b, i0 + a * 32, j0 + c * 32, !sym || ti != tj);
+}
+
+// Small products: a workgroup per 32x32 tile, whose eight waves each take a share of the sum straight from memory (a
+// tile's factors are read by few others) and meet in LDS. One launch a product, where tiles of 64 leave most of the
+// chip idle or need a second launch to join pieces.
+constexpr int kSmallWaves = 8;
+template <class T, Mode M, bool MUON, int PL>
+__global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product P, MuonSet S) {
+  __shared__ float lds[kSmallWaves][kBlockLds];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr bool sym = M == Gram || M == Square;
+  const uint32_t tiles = sym ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj;
+  const uint32_t b = blockIdx.x / tiles, t = blockIdx.x - b * tiles;
+  uint32_t ti, tj;
+  tile_at<M>(t, P.ti, ti, tj);
+  const uint32_t first = P.lines * wave / kSmallWaves, last = P.lines * (wave + 1) / kSmallWaves;
+  const uint32_t i0 = ti * 32, j0 = tj * 32;
+  const char *u = P.u.data + b * P.u.next + (i0 + lane % 32) * P.u.pitch + lane / 32 * 16;
+  const char *v = P.v.data + b * P.v.next + (j0 + lane % 32) * P.v.pitch + lane / 32 * 16;
+  f16v acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+  for (uint32_t line = first; line < last; ++line) {
+    h8 ua[4 / PL][PL], vb[4 / PL][PL];
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+      for (int g = 0; g < 4 / PL; ++g) {
+        ua[g][p] = *reinterpret_cast<const h8 *>(u + line * 128 + p * 64 + g * 32);
+        vb[g][p] = *reinterpret_cast<const h8 *>(v + line * 128 + p * 64 + g * 32);
+      }
+#pragma unroll
+    for (int g = 0; g < 4 / PL; ++g)
+#pragma unroll
+      for (int q = 0; q < (PL == 2 ? 3 : 1); ++q)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ua[g][q == 2], vb[g][q == 1], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) lds[wave][(8 * (r / 4) + 4 * (lane / 32) + r % 4) * 33 + lane % 32] = acc[r];
+  __syncthreads();
+  // the waves' sums, two outputs a thread, back into the first wave's tile
+  for (uint32_t e = threadIdx.x; e < 32 * 32; e += 64 * kSmallWaves) {
+    const uint32_t at = e / 32 * 33 + e % 32;
+    float sum = lds[0][at];
+#pragma unroll
+    for (int w = 1; w < kSmallWaves; ++w) sum += lds[w][at];
+    lds[0][at] = sum;
+  }
+  __syncthreads();
+  // as put_block, an eighth of the tile a wave: rows by the first waves, the transpose's by the others
+  float alpha = P.alpha, beta = P.beta;
+  if constexpr (M == Gram || M == Final) {
+    const float unscale = 1.0f / P.xscale[b];
+    alpha *= unscale;
+    if constexpr (M == Gram) alpha *= unscale;
+    else beta *= unscale;
+  }
+  const float *tile = lds[0];
+  if constexpr (M == Final) {
+    const bool tall = P.o.rows > P.o.cols;
+    for (uint32_t e = threadIdx.x; e < 32 * 32; e += 64 * kSmallWaves) {
+      const uint32_t q = e / 32, k = e % 32;
+      const uint32_t row = (tall ? j0 : i0) + q, col = (tall ? i0 : j0) + k;
+      const char *at = tall ? line_at<PL>(P.in_t, b, j0 + q, i0 + k) : line_at<PL>(P.in, b, i0 + q, j0 + k);
+      const float term = get1<PL>(at);
+      const float r = __builtin_fmaf(beta, term, alpha * (tall ? tile[k * 33 + q] : tile[q * 33 + k]));
+      if (row >= P.o.rows || col >= P.o.cols) continue;
+      if constexpr (MUON) {
+        float *p = S.p[b] + uint64_t(row) * P.o.cols + col;
+        *p = *p * S.rule.keep - S.rule.scale * r;
+      } else {
+        T *o = static_cast<T *>(const_cast<void *>(P.o.data)) + int64_t(b) * P.o.sb;
+        o[int64_t(row) * P.o.s0 + int64_t(col) * P.o.s1] = T(r);
+      }
+    }
+  } else {
+    const uint32_t half = threadIdx.x / 256, e = threadIdx.x % 256;
+    if (e >= 128 || (half && sym && ti == tj)) return;
+    const uint32_t r = e / 4, c = e % 4 * 8;
+    const uint32_t row = (half ? j0 : i0) + r, col = (half ? i0 : j0) + c;
+    float w[8], x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = alpha * (half ? tile[(c + k) * 33 + r] : tile[r * 33 + c + k]);
+    if constexpr (M != Gram) {
+      get8<PL>(line_at<PL>(half ? P.in_t : P.in, b, row, col), x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = __builtin_fmaf(beta, x[k], w[k]);
+    }
+    if (M == Square && P.in2.data) {
+      get8<PL>(line_at<PL>(P.in2, b, row, col), x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = __builtin_fmaf(P.gamma, x[k], w[k]);
+    }
+    put8<PL>(line_at<PL>(half ? P.out_t : P.out, b, row, col), w);
+  }
 }
 
 // Adds the pieces of a sum: a wave per 32x32 block.
-template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
+template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
   constexpr int FA = WM / 32, FB = WN / 32, NB = (BM / 32) * (BN / 32);
   __shared__ float lds[kNsBlock / 64 * kBlockLds];
@@ -451,18 +578,17 @@ __global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
   }
   const uint32_t w = block / (FA * FB), a = block % (FA * FB) / FB, c = block % FB;
   const uint32_t i0 = ti * BM + w / (BN / WN) * WM + a * 32, j0 = tj * BN + w % (BN / WN) * WN + c * 32;
-  put_block<T, M, MUON>(P, S, lds + wave * kBlockLds, acc, b, i0, j0, !sym || ti != tj);
+  put_block<T, M, MUON, PL>(P, S, lds + wave * kBlockLds, acc, b, i0, j0, !sym || ti != tj);
 }
 
 // No steps: the result is X.
-template <class T, bool MUON>
+template <class T, bool MUON, int PL>
 __global__ __launch_bounds__(kNsBlock) void copy_out_kernel(Lines X, Lines XT, const float *xscale, Stack O,
                                                             MuonSet S) {
   const uint32_t b = blockIdx.z, i = blockIdx.y, j = blockIdx.x * kNsBlock + threadIdx.x;
   if (j >= O.cols) return;
-  const char *at = line_at(O.rows > O.cols ? XT : X, b, i, j);
-  const float v = (float(*reinterpret_cast<const f16_t *>(at)) + float(*reinterpret_cast<const f16_t *>(at + 64))) /
-                  xscale[b];
+  const char *at = line_at<PL>(O.rows > O.cols ? XT : X, b, i, j);
+  const float v = get1<PL>(at) / xscale[b];
   if constexpr (MUON) {
     float *p = S.p[b] + uint64_t(i) * O.cols + j;
     *p = *p * S.rule.keep - S.rule.scale * v;
@@ -474,21 +600,29 @@ __global__ __launch_bounds__(kNsBlock) void copy_out_kernel(Lines X, Lines XT, c
 
 // ------------------------------------------------------------------------- host
 
-// How a shape runs: the tile, and the pieces each product's sum is cut into.
+// How a product runs: its tiles, and the pieces its sums are cut into.
+struct Tiling {
+  uint32_t tile, parts;
+};
+// How a shape runs.
 struct Plan {
   uint32_t m, n, mp, np;  // extents, and padded to whole tiles
-  uint32_t tile;
-  uint32_t gram, square, update;  // pieces
+  Tiling gram, square, update;
+  uint32_t planes;  // of a factor
+  bool pairs;       // steps go by pairs
+  Scales scale;
 };
 
-// The pieces that leave the fewest rounds of `slots` workgroups, each a share of the sum: cutting costs
-// a write and a read of the tile per piece, about six lines' time.
-uint32_t pieces(uint64_t tiles, uint32_t lines, uint64_t slots) {
+// The pieces that leave the fewest rounds of `slots` workgroups, each a share of the sum. In lines' time, a round
+// costs four beside its lines, and cutting the launch that joins the pieces, twelve (four of 256 wide tiles' longer
+// ones), and eight per round of pieces
+// (256 x 256 in 64 wide tiles without that: 177 us instead of 128; 6 x 1001 x 2605 in 128 wide ones 1216 and 1132).
+uint32_t pieces(uint64_t tiles, uint32_t lines, uint64_t slots, double join) {
   uint32_t best = 1;
   double least = 1e300;
   for (uint32_t s = 1; s <= 16 && s <= lines; ++s) {
     const double rounds = double((tiles * s + slots - 1) / slots);
-    const double t = rounds * (double(lines) / s + 4.0) + (s > 1 ? 6.0 * s * double(tiles) / double(slots) + 4.0 : 0.0);
+    const double t = rounds * (double(lines) / s + 4.0) + (s > 1 ? join + 8.0 * s * double(tiles) / double(slots) : 0.0);
     if (t < least * 0.98) {
       least = t;
       best = s;
@@ -497,56 +631,131 @@ uint32_t pieces(uint64_t tiles, uint32_t lines, uint64_t slots) {
   return best;
 }
 
+// Tiles of 64 and below: sums of up to 32 lines over up to 512 tiles of 32 go to the small products (256 x 256:
+// 88 us instead of 128, 512 x 512 130 and 185; but 64 x 8000, 250 lines, 354 and 149, 20 x 300 x 300, 1100 tiles, 318
+// and 181).
+Tiling tiling(uint32_t tile, uint32_t rows, uint32_t cols, bool sym, uint64_t count, uint32_t lines) {
+  const auto tiles = [&](uint64_t t) { return (sym ? rows / t * (rows / t + 1) / 2 : rows / t * (cols / t)) * count; };
+  if (tile == 64 && lines <= 32 && tiles(32) <= 512) return {32, 1};
+  return {tile, pieces(tiles(tile), lines, uint64_t(num_cus()) * (tile == 256 ? 1 : 2), tile == 256 ? 4.0 : 12.0)};
+}
+
 uint32_t round_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
-Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count) {
+// The rule followed for singular values in [0, 1]: the scales that give each factor room, and whether two steps'
+// factor, P' P - a^2, has room at the scale of S; `most` is the largest singular value met.
+struct RuleRange {
+  Scales scale;
+  bool pairs;
+  double most;
+};
+RuleRange follow(const NewtonSchulz &r) {
+  double x = 1.0, a = 1.0, s = 0.0, q = 0.0;
+  for (int k = 0; k <= 4096; ++k) {
+    double v = double(k) / 4096.0, before = 0.0;
+    for (int i = 0; i < r.steps; ++i) {
+      const double l = v * v, p = r.a + r.b * l + r.c * l * l;
+      a = std::fmax(a, std::fmax(l, std::fabs(p * l)));
+      s = std::fmax(s, std::fabs(r.b * l + r.c * l * l));
+      if (i % 2) q = std::fmax(q, std::fabs(before * p - double(r.a) * r.a));
+      before = p;
+      v *= p;
+      x = std::fmax(x, std::fabs(v));
+    }
+  }
+  const auto fit = [](double most, int bits) {
+    while (bits > -100 && !(std::ldexp(most, bits) <= 32768.0)) --bits;
+    return float(std::ldexp(1.0, bits));
+  };
+  const Scales to{fit(x, 12), fit(a, 12), fit(s, 11)};
+  return RuleRange{to, q * to.s <= 32768.0, x};
+}
+// The same, worked out when the rule is another than the last call's (45 us on the host).
+RuleRange range_of(const NewtonSchulz &r) {
+  static std::mutex mu;
+  static NewtonSchulz last{};
+  static RuleRange range{};
+  static bool any = false;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!any || memcmp(&last, &r, sizeof r) != 0) {
+    range = follow(r);
+    last = r;
+    any = true;
+  }
+  return range;
+}
+
+Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz &rule, uint32_t planes) {
   Plan p;
+  p.planes = planes;
   p.m = rows < cols ? rows : cols;
   p.n = rows < cols ? cols : rows;
+  // 256 wide tiles read each factor least often, 128 wide ones leave fewer workgroups without work: 4096 x 4096 4.39
+  // and 4.83 ms, 2048 x 2048 909 and 839 us, 24 x 1024 x 1024 2.31 and 2.25 ms; 64 wide ones go on with that: 1024 x 1024
+  // 262 us (128: 324), 512 x 4096 246 (321), 2048 x 2048 913.
   const uint64_t work = uint64_t(p.m) * p.n * count;
-  p.tile = p.m > 512 && work >= uint64_t(1) << 24 ? 256 : p.m > 128 && work >= uint64_t(1) << 19 ? 128 : 64;
-  p.mp = round_up(p.m, p.tile);
-  p.np = round_up(p.n, p.tile);
-  const uint64_t ti = p.mp / p.tile, tj = p.np / p.tile, sym = ti * (ti + 1) / 2;
-  const uint64_t slots = uint64_t(num_cus()) * (p.tile == 256 ? 1 : 2);
-  p.gram = pieces(sym * count, p.np / 32, slots);
-  p.square = pieces(sym * count, p.mp / 32, slots);
-  p.update = pieces(ti * tj * count, p.mp / 32, slots);
+  const uint32_t tile = p.m > 2048 && work >= uint64_t(1) << 23 ? 256 : p.m > 128 && work >= uint64_t(3) << 20 ? 128 : 64;
+  // Two steps at once cost three more m x m products and one product of X X^T and one update of X less: 1.5 m^2 n
+  // multiplications less for 1.5 m^3 more, and one launch more (4096 x 16384: 13.6 -> 10.4 ms, 6 x 2605 x 1001 in fp32 1.34 ->
+  // 1.18; under 2^30 the launch costs more). With factors of 11 bits the two would cost accuracy, 2.5e-3 for 1.4e-3.
+  const RuleRange range = range_of(rule);
+  p.scale = range.scale;
+  p.pairs = range.pairs && planes == 2 && rule.steps >= 2 && uint64_t(p.m) * p.m * (p.n - p.m) * count >= uint64_t(1) << 30;
+  p.mp = round_up(p.m, tile);
+  p.np = round_up(p.n, tile);
+  p.gram = tiling(tile, p.mp, p.mp, true, count, p.np * planes / 64);
+  p.square = tiling(tile, p.mp, p.mp, true, count, p.mp * planes / 64);
+  p.update = tiling(tile, p.mp, p.np, false, count, p.mp * planes / 64);
   return p;
 }
 
 // Bytes of a workspace for `count` matrices: norms, X and X^T twice, A and S, and the pieces' sums.
 uint64_t ns_bytes(const Plan &p, uint64_t count) {
-  const uint64_t ti = p.mp / p.tile, tj = p.np / p.tile, sym = ti * (ti + 1) / 2;
-  uint64_t part = 0;
-  for (uint64_t t : {p.gram > 1 ? sym * p.gram : 0, p.square > 1 ? sym * p.square : 0,
-                     p.update > 1 ? ti * tj * p.update : 0})
-    part = t > part ? t : part;
-  return count * (kNormParts * 8 + 128 + 4 * (4 * uint64_t(p.mp) * p.np + 2 * uint64_t(p.mp) * p.mp +
-                                        part * p.tile * p.tile));
+  uint64_t part = 0;  // floats of a product's pieces
+  const auto need = [&](const Tiling &t, uint64_t rows, uint64_t cols, bool sym) {
+    if (t.parts == 1) return;
+    const uint64_t ti = rows / t.tile, tj = cols / t.tile;
+    const uint64_t n = (sym ? ti * (ti + 1) / 2 : ti * tj) * t.parts * t.tile * t.tile;
+    part = n > part ? n : part;
+  };
+  need(p.gram, p.mp, p.mp, true);
+  need(p.square, p.mp, p.mp, true);
+  need(p.update, p.mp, p.np, false);
+  return count * (kNormParts * 8 + 128 + 4 * part +
+                  2 * p.planes * (4 * uint64_t(p.mp) * p.np + (p.pairs ? 4 : 2) * uint64_t(p.mp) * p.mp));
 }
 
-template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
+template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
 void launch_product(const Product &P, const MuonSet &S, uint32_t count) {
   constexpr int NW = (BM / WM) * (BN / WN);
   const uint32_t tiles = (M == Gram || M == Square ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj) * count;
-  product_kernel<T, M, MUON, BM, BN, WM, WN><<<tiles * P.parts, 64 * NW, 0, stream()>>>(P, S);
+  product_kernel<T, M, MUON, PL, BM, BN, WM, WN><<<tiles * P.parts, 64 * NW, 0, stream()>>>(P, S);
   if (P.parts > 1)
-    join_kernel<T, M, MUON, BM, BN, WM, WN>
+    join_kernel<T, M, MUON, PL, BM, BN, WM, WN>
         <<<tiles * (BM / 32) * (BN / 32) / (kNsBlock / 64), kNsBlock, 0, stream()>>>(P, S);
 }
-template <class T, Mode M, bool MUON>
-void product(const Plan &plan, const Product &P, const MuonSet &S, uint32_t count) {
-  if (plan.tile == 256) launch_product<T, M, MUON, 256, 256, 128, 64>(P, S, count);
-  else if (plan.tile == 128) launch_product<T, M, MUON, 128, 128, 64, 64>(P, S, count);
-  else launch_product<T, M, MUON, 64, 64, 32, 32>(P, S, count);
+template <class T, Mode M, bool MUON, int PL>
+void product(const Plan &plan, const Tiling &how, Product &P, const MuonSet &S, uint32_t count) {
+  P.parts = how.parts;
+  P.ti = plan.mp / how.tile;
+  P.tj = (M == Gram || M == Square ? plan.mp : plan.np) / how.tile;
+  if (how.tile == 32) {
+    const uint32_t tiles = (M == Gram || M == Square ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj) * count;
+    small_product_kernel<T, M, MUON, PL><<<tiles, 64 * kSmallWaves, 0, stream()>>>(P, S);
+  } else if (how.tile == 256) {
+    launch_product<T, M, MUON, PL, 256, 256, 128, 64>(P, S, count);
+  } else if (how.tile == 128) {
+    launch_product<T, M, MUON, PL, 128, 128, 64, 64>(P, S, count);
+  } else {
+    launch_product<T, M, MUON, PL, 64, 64, 32, 32>(P, S, count);
+  }
 }
 
 // The iteration over `count` matrices: from G into O, or of a Muon set into its parameters.
-template <class T, bool MUON>
+template <class T, bool MUON, int PL>
 void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S, uint32_t count,
              const NewtonSchulz &rule, void *work) {
-  const uint64_t mn = 4 * uint64_t(plan.mp) * plan.np, mm = 4 * uint64_t(plan.mp) * plan.mp;
+  const uint64_t mn = 2 * PL * uint64_t(plan.mp) * plan.np, mm = 2 * PL * uint64_t(plan.mp) * plan.mp;
   double *norms = static_cast<double *>(work);
   float *xscale = reinterpret_cast<float *>(norms + uint64_t(count) * kNormParts);
   char *at = static_cast<char *>(work) + uint64_t(count) * (kNormParts * 8 + 128);
@@ -555,9 +764,11 @@ void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S,
     at += count * bytes;
     return l;
   };
-  Lines x = take(mn, 4 * uint64_t(plan.np)), y = take(mn, 4 * uint64_t(plan.np));
-  Lines xt = take(mn, 4 * uint64_t(plan.mp)), yt = take(mn, 4 * uint64_t(plan.mp));
-  const Lines a = take(mm, 4 * uint64_t(plan.mp)), s = take(mm, 4 * uint64_t(plan.mp));
+  Lines x = take(mn, 2 * PL * uint64_t(plan.np)), y = take(mn, 2 * PL * uint64_t(plan.np));
+  Lines xt = take(mn, 2 * PL * uint64_t(plan.mp)), yt = take(mn, 2 * PL * uint64_t(plan.mp));
+  const Lines a = take(mm, 2 * PL * uint64_t(plan.mp)), s = take(mm, 2 * PL * uint64_t(plan.mp));
+  const Lines pa = plan.pairs ? take(mm, 2 * PL * uint64_t(plan.mp)) : Lines{};
+  const Lines s2 = plan.pairs ? take(mm, 2 * PL * uint64_t(plan.mp)) : Lines{};
   float *partial = reinterpret_cast<float *>(at);
 
   const uint64_t size = uint64_t(G.rows) * G.cols;
@@ -570,34 +781,53 @@ void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S,
   const int growth = int(most_growth < 110.0f ? most_growth : 110.0f);
   const bool tall = G.rows > G.cols;
   const dim3 grid((tall ? plan.mp : plan.np) / 64, (tall ? plan.np : plan.mp) / 64, count);
-  start_kernel<T, MUON><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, growth, x, xt, xscale);
-  const uint32_t ti = plan.mp / plan.tile, tj = plan.np / plan.tile;
-  for (int k = 0; k < rule.steps; ++k) {
-    Product P;
-    memset(&P, 0, sizeof P);
-    P.partial = partial;
-    P.xscale = xscale;
-    P.ti = ti, P.tj = ti;
-    P.u = P.v = x, P.out = P.out_t = a, P.lines = plan.np / 32, P.parts = plan.gram;
-    P.alpha = kScaleA;
-    product<float, Gram, false>(plan, P, S, count);
-    P.u = P.v = P.in = P.in_t = a, P.out = P.out_t = s, P.lines = plan.mp / 32, P.parts = plan.square;
-    P.alpha = rule.c * (kScaleS / (kScaleA * kScaleA)), P.beta = rule.b * (kScaleS / kScaleA);
-    product<float, Square, false>(plan, P, S, count);
-    P.u = s, P.v = P.in_t = xt, P.in = x, P.out = y, P.out_t = yt, P.tj = tj, P.parts = plan.update;
-    P.alpha = 1.0f / kScaleS, P.beta = rule.a;
-    if (k + 1 < rule.steps) {
-      product<float, Update, false>(plan, P, S, count);
+  start_kernel<T, MUON, PL><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, growth, plan.scale.x, x, xt, xscale);
+  const float sa = plan.scale.a, ss = plan.scale.s;
+  Product P;
+  memset(&P, 0, sizeof P);
+  P.partial = partial;
+  P.xscale = xscale;
+  const auto gram = [&] {
+    P.u = P.v = x, P.out = P.out_t = a, P.lines = plan.np * PL / 64, P.alpha = sa;
+    product<float, Gram, false, PL>(plan, plan.gram, P, S, count);
+  };
+  // to = coef u v + beta in + gamma in2, of scales su, sv, so, si and s2
+  const auto square = [&](const Lines &to, float so, float coef, const Lines &u, float su, const Lines &v, float sv,
+                          float beta, const Lines &in, float si, float gamma = 0.0f, Lines in2 = Lines{}, float s2 = 1.0f) {
+    P.u = u, P.v = v, P.in = P.in_t = in, P.in2 = in2, P.out = P.out_t = to;
+    P.lines = plan.mp * PL / 64;
+    P.alpha = coef * (so / (su * sv)), P.beta = beta * (so / si), P.gamma = gamma * (so / s2);
+    product<float, Square, false, PL>(plan, plan.square, P, S, count);
+  };
+  for (int k = 0; k < rule.steps;) {
+    const int steps = plan.pairs && k + 2 <= rule.steps ? 2 : 1;
+    gram();
+    square(s, ss, rule.c, a, sa, a, sa, rule.b, a, sa);
+    Lines q = s;
+    float identity = rule.a;
+    if (steps == 2) {
+      square(pa, sa, 1.0f, s, ss, a, sa, rule.a, a, sa);
+      square(a, sa, 1.0f, s, ss, pa, sa, rule.a, pa, sa);
+      square(s2, ss, rule.c, a, sa, a, sa, rule.b, a, sa);
+      square(pa, ss, 1.0f, s2, ss, s, ss, rule.a, s, ss, rule.a, s2, ss);
+      q = pa;
+      identity *= rule.a;
+    }
+    k += steps;
+    P.u = q, P.v = P.in_t = xt, P.in = x, P.out = y, P.out_t = yt, P.lines = plan.mp * PL / 64;
+    P.alpha = 1.0f / ss, P.beta = identity;
+    if (k < rule.steps) {
+      product<float, Update, false, PL>(plan, plan.update, P, S, count);
       Lines z = x;
       x = y, y = z;
       z = xt, xt = yt, yt = z;
     } else {
       P.o = O;
-      product<T, Final, MUON>(plan, P, S, count);
+      product<T, Final, MUON, PL>(plan, plan.update, P, S, count);
     }
   }
   if (rule.steps == 0)
-    copy_out_kernel<T, MUON><<<dim3(ceil_div(O.cols, kNsBlock), O.rows, count), kNsBlock, 0, stream()>>>(x, xt, xscale, O, S);
+    copy_out_kernel<T, MUON, PL><<<dim3(ceil_div(O.cols, kNsBlock), O.rows, count), kNsBlock, 0, stream()>>>(x, xt, xscale, O, S);
 }
 
 bool check_rule(const NewtonSchulz *r, const char *where) {
@@ -608,6 +838,11 @@ bool check_rule(const NewtonSchulz *r, const char *where) {
   if (r->steps < 0 || r->steps > 1000 || !(r->eps >= 0.0f) || !std::isfinite(r->a) ||
       !std::isfinite(r->b) || !std::isfinite(r->c) || !std::isfinite(r->eps)) {
     report_error(where, "a rule needs 0 to 1000 steps, finite coefficients and eps of at least 0");
+    return false;
+  }
+  const double most = range_of(*r).most;
+  if (!(most <= 4.0)) {
+    report_error(where, "the rule diverges: it takes singular values of 0 to 1 to %g", most);
     return false;
   }
   return true;
@@ -736,7 +971,7 @@ void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule) {
   }
   if (numel(g) == 0 || !ensure_init()) return;
   const uint64_t share = stack_share(count, G.rows, G.cols), item = float_bytes(g);
-  const Plan plan = make_plan(G.rows, G.cols, share);
+  const Plan plan = make_plan(G.rows, G.cols, share, *rule, g->dtype == BFLOAT16 ? 1 : 2);
   void *work = workspace(ns_bytes(plan, share));
   if (!work) return;
   MuonSet none;
@@ -746,7 +981,8 @@ void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule) {
     Gb.data = static_cast<const char *>(G.data) + int64_t(b) * G.sb * int64_t(item);
     Ob.data = static_cast<const char *>(O.data) + int64_t(b) * O.sb * int64_t(item);
     with_float_type(g->dtype, [&](auto t) {
-      iterate<decltype(t), false>(plan, Gb, Ob, none, uint32_t(count - b < share ? count - b : share), *rule,
+      typedef decltype(t) T;
+      iterate<T, false, std::is_same_v<T, bf16_t> ? 1 : 2>(plan, Gb, Ob, none, uint32_t(count - b < share ? count - b : share), *rule,
                                   work);
     });
   }
@@ -792,7 +1028,7 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
     const uint32_t rows = uint32_t(first->shape[0]), cols = uint32_t(first->shape[1]);
     uint64_t share = stack_share(same.size(), rows, cols);
     if (share > kPointers) share = kPointers;
-    const Plan plan = make_plan(rows, cols, share);
+    const Plan plan = make_plan(rows, cols, share, optimizer->rule, 2);
     void *work = workspace(ns_bytes(plan, share));
     if (!work) return;
     MuonSet S;
@@ -810,7 +1046,7 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
         S.g[j] = static_cast<const float *>(p->grad->data);
         S.m[j] = static_cast<float *>(optimizer->m[same[b + j]]->data);
       }
-      iterate<float, true>(plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
+      iterate<float, true, 2>(plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
     }
   }
   finish(where);

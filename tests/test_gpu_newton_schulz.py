@@ -104,6 +104,39 @@ def test_strong_directions_and_low_rank(shape):
         near(run(g, "f32"), iterate(g), 3.3e-4, "f32", f"{name} {shape}")
 
 
+@pytest.mark.parametrize("shape", [(1, 700, 3000), (1, 3000, 700), (2, 530, 2700), (1, 1030, 2100)])
+def test_large(shape):
+    """Sizes from which the products run in the largest tiles and two steps go at once, the strong directions
+    of a gradient among them."""
+    print(f"newton_schulz large {shape}", flush=True)
+    rng = np.random.RandomState(7)
+    g = rng.randn(*shape).astype(np.float32)
+    g[0] += (rng.randn(shape[1], 8) @ rng.randn(8, shape[2])).astype(np.float32)
+    for kind, steps in (("f32", 5), ("f32", 4), ("bf16", 5)):
+        h = load(store(g, kind))
+        got = run(h, kind, steps)
+        for b in range(shape[0]):
+            near(got[b], iterate(h[b], steps), 2e-5, kind, f"{kind} {shape}[{b}] {steps} steps")
+
+
+@pytest.mark.parametrize("rule", [(1.5, -0.5, 0.0), (2.0, -1.5, 0.5), (5.5, -12.0, 7.5)])
+def test_other_rules(rule):
+    """The last one takes singular values to 1e5 and is refused."""
+    rt = _rt()
+    rng = np.random.RandomState(8)
+    g = rng.randn(1030, 2100).astype(np.float32)
+    x = rt.DeviceTensor.from_numpy(g)
+    out = rt.DeviceTensor(g.shape, zero=False)
+    r = abi.NewtonSchulz(*rule, EPS, 4)
+    rt.lib().newton_schulz_hip(C.byref(x.t), C.byref(out.t), C.byref(r))
+    if rule[0] > 5:
+        with pytest.raises(rt.PlastHipError, match="diverges"):
+            rt.lib().check("newton_schulz")
+        return
+    rt.lib().check("newton_schulz")
+    near(out.numpy(), iterate(g, 4, *rule), 2e-5, "f32", f"{rule}")
+
+
 def test_steps_and_extremes():
     rng = np.random.RandomState(2)
     g = rng.randn(70, 90).astype(np.float32)

@@ -141,6 +141,8 @@ def rule(**kw):
     (T((8, 8)), T((8, 8)), rule(steps=-1), "0 to 1000 steps"),
     (T((8, 8)), T((8, 8)), rule(a=float("nan")), "finite coefficients"),
     (T((8, 8)), T((8, 8)), rule(eps=-1.0), "eps"),
+    (T((8, 8)), T((8, 8)), rule(a=5.5, b=-12.0, c=7.5), "diverges"),
+    (T((8, 8)), T((8, 8)), rule(a=1e30), "diverges"),
 ])
 def test_newton_schulz_refuses(L, g, out, r, match):
     L.plast_hip_clear_error()
