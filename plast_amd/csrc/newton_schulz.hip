@@ -1015,22 +1015,38 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
                    "of its shape", k);
       return;
     }
+  // the parameters of each shape, and a workspace for the largest, before anything is written
+  struct Group {
+    std::vector<int> which;
+    uint64_t share;
+    Plan plan;
+  };
   std::vector<char> done(size_t(num_parameters), 0);
+  std::vector<Group> groups;
+  uint64_t bytes = 0;
   for (int k = 0; k < num_parameters; ++k) {
     const Tensor *first = parameters[k];
     if (done[k] || !first || !first->grad || numel(first) == 0) continue;
-    std::vector<int> same;  // the parameters of this shape
+    Group g;
     for (int j = k; j < num_parameters; ++j)
       if (!done[j] && parameters[j] && parameters[j]->grad && same_shape(parameters[j], first)) {
-        same.push_back(j);
+        g.which.push_back(j);
         done[j] = 1;
       }
     const uint32_t rows = uint32_t(first->shape[0]), cols = uint32_t(first->shape[1]);
-    uint64_t share = stack_share(same.size(), rows, cols);
-    if (share > kPointers) share = kPointers;
-    const Plan plan = make_plan(rows, cols, share, optimizer->rule, 2);
-    void *work = workspace(ns_bytes(plan, share));
-    if (!work) return;
+    g.share = stack_share(g.which.size(), rows, cols);
+    if (g.share > kPointers) g.share = kPointers;
+    g.plan = make_plan(rows, cols, g.share, optimizer->rule, 2);
+    const uint64_t need = ns_bytes(g.plan, g.share);
+    bytes = need > bytes ? need : bytes;
+    groups.push_back(std::move(g));
+  }
+  if (groups.empty()) return;
+  void *work = workspace(bytes);
+  if (!work) return;
+  for (const Group &group : groups) {
+    const Tensor *first = parameters[group.which[0]];
+    const uint32_t rows = uint32_t(first->shape[0]), cols = uint32_t(first->shape[1]);
     MuonSet S;
     memset(&S, 0, sizeof S);
     S.rule.momentum = optimizer->momentum;
@@ -1038,15 +1054,15 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
     S.rule.keep = 1.0f - optimizer->lr * optimizer->weight_decay;
     S.rule.scale = optimizer->lr * sqrtf(rows > cols ? float(rows) / float(cols) : 1.0f);
     const Stack shape{nullptr, rows, cols, 0, int64_t(cols), 1};
-    for (size_t b = 0; b < same.size(); b += share) {
-      const size_t c = same.size() - b < share ? same.size() - b : share;
+    for (size_t b = 0; b < group.which.size(); b += group.share) {
+      const size_t c = group.which.size() - b < group.share ? group.which.size() - b : group.share;
       for (size_t j = 0; j < c; ++j) {
-        const Tensor *p = parameters[same[b + j]];
-        S.p[j] = static_cast<float *>(p->data);
-        S.g[j] = static_cast<const float *>(p->grad->data);
-        S.m[j] = static_cast<float *>(optimizer->m[same[b + j]]->data);
+        const int at = group.which[b + j];
+        S.p[j] = static_cast<float *>(parameters[at]->data);
+        S.g[j] = static_cast<const float *>(parameters[at]->grad->data);
+        S.m[j] = static_cast<float *>(optimizer->m[at]->data);
       }
-      iterate<float, true, 2>(plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
+      iterate<float, true, 2>(group.plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
     }
   }
   finish(where);

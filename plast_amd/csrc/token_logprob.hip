@@ -174,9 +174,9 @@ __device__ __forceinline__ void put_stats(const TokenArgs &A, uint32_t row, floa
   A.stats[2 * row + 1] = l0;
 }
 
-// The row's results, by one lane. s and w are over the whole row.
+// The row's results, by one lane. s and w are over the whole row; `shift` is what every z holds beside c (x - m).
 __device__ __forceinline__ void row_out(const TokenArgs &A, uint32_t row, int32_t token, float x_token,
-                                        float m, float s, float w) {
+                                        float m, float s, float w, float shift) {
   if (m == -kInf) {  // no logit that is not -inf
     A.logp[row] = uint32_t(token) < A.vocab ? -kInf : __builtin_nanf("");
     A.entropy[row] = 0.0f;
@@ -184,9 +184,8 @@ __device__ __forceinline__ void row_out(const TokenArgs &A, uint32_t row, int32_
     return;
   }
   const float l = log2f(s);
-  const RowRef ref(A.c, m);
   const float h = kLn2 * (l - w / s);
-  const float l0 = l - ref.shift();
+  const float l0 = l - shift;
   A.logp[row] = uint32_t(token) < A.vocab ? log_p(A, x_token, m, l0) : __builtin_nanf("");
   A.entropy[row] = h < 0.0f ? 0.0f : h;
   put_stats(A, row, m, l0);
@@ -274,7 +273,7 @@ __device__ __forceinline__ void exact_row(const TokenArgs &A, const T *x, uint32
     w = together(w, false);
     if (s != s) m = s;  // a NaN or an infinite logit
     l0 = log2f(s) - ref.shift();
-    if (gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, m, s, w);
+    if (gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, m, s, w, ref.shift());
   }
   uint64_t last = ~uint64_t(0);
   for (uint32_t k = 0; k < A.top; ++k) {
@@ -499,9 +498,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t gl = W == 1 ? threadIdx.x & 63 : threadIdx.x;
   RowLds<W> &L = lds[W == 1 ? wave : 0];
-  const uint32_t row = W == 1 ? blockIdx.x * 4 + wave : CUT ? blockIdx.x / P.n : blockIdx.x;
-  const uint32_t piece = CUT ? blockIdx.x - row * P.n : 0, pieces = CUT ? P.n : 1;
-  if (W == 1 && row >= A.rows) return;
+  const uint32_t local = W == 1 ? blockIdx.x * 4 + wave : CUT ? blockIdx.x / P.n : blockIdx.x;
+  const uint32_t row = A.first_row + local;
+  const uint32_t piece = CUT ? blockIdx.x - local * P.n : 0, pieces = CUT ? P.n : 1;
+  if (W == 1 && local >= A.rows) return;
   const int32_t token = A.tokens[row];
   const uint32_t V = A.vocab, units = V / E;
   const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
@@ -691,11 +691,11 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   const bool exact = !in_range(c, r.m);
   if (exact || top.lost) {
     const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
-    if (!exact && gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w);
+    if (!exact && gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w, RowRef(c, r.m).shift());
     exact_row<T, W>(A, x, row, token, gl, L, exact, r.m, l0);
     return;
   }
-  if (gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w);
+  if (gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w, RowRef(c, r.m).shift());
   if constexpr (TOP) {
     const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
     for (uint32_t i = gl; i < found; i += NL) {
@@ -870,7 +870,7 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   const uint32_t V = A.vocab, gl = threadIdx.x % L;
   const uint32_t r = blockIdx.x * ROWS + threadIdx.x / L;
   const bool valid = ROWS == 1 || r < A.rows;
-  const uint32_t row = valid ? r : A.rows - 1;
+  const uint32_t row = A.first_row + (valid ? r : A.rows - 1);
   const int32_t token = A.tokens[row];
   const RowAt at = row_at(A.map, row);
   const T *x = static_cast<const T *>(A.x) + at.x;
@@ -919,7 +919,7 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   const float l = log2f(s);
   if (gl == 0 && valid) {
     if (token < 0) pad_out(A, row);
-    else row_out(A, row, token, x_token, m, s, w);
+    else row_out(A, row, token, x_token, m, s, w, ref.shift());
   }
   if constexpr (GRAD) {
     if (!valid) return;
@@ -955,6 +955,124 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   }
 }
 
+// The step over many long rows: a workgroup of 1024 lanes per CU that goes from row to row, the next one's units on
+// their way into a second set of registers while this one is worked on. Rows are handed out as workgroups
+// become free (in fixed turns the odd XCDs end some 8% after the even ones); a result does not depend on who works it
+// out. [32768, 32000] in fp32: 1436 us, 5.84 TB/s, instead of 1585 with a workgroup per row (two of them fit a CU); 16-bit
+// rows, whose two exponentials a logit leave the memory idle at one workgroup per CU, lose: 455 us and 425 at [16384,
+// 32000] in bf16. Rows are whole units, 16-byte aligned in the gradient (the others' bounds cost registers that the two sets
+// need).
+constexpr uint32_t kStreamLanes = 1024;
+__device__ uint32_t g_stream_rows[2];  // rows handed out, workgroups that are done; zero between launches
+template <class T, int N>
+__global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) {
+  constexpr uint32_t E = Unit<T>::E, L = kStreamLanes;
+  __shared__ float lds[2][3][16];
+  __shared__ uint32_t drawn[2];
+  const uint32_t V = A.vocab, gl = threadIdx.x, grid = gridDim.x;
+  typedef typename Unit<T>::vec vec;
+  const auto fetch = [&](vec (&v)[N], uint32_t row, int32_t token) {
+    const RowAt at = row_at(A.map, row);
+    const T *x = static_cast<const T *>(A.x) + at.x;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      v[u] = T(-kInf);
+      if (token >= 0 && (u * L + gl) * E < V) v[u] = load_unit(x + u * L * E + gl * E);
+    }
+  };
+  uint32_t row = blockIdx.x, next = blockIdx.x + grid, turn = 0;
+  int32_t token = A.tokens[row], next_token = next < A.rows ? A.tokens[next] : -1;
+  vec first[N], second[N];
+  fetch(first, row, token);
+  // one row; the next one's loads are issued first
+  const auto work = [&](vec (&v)[N], vec (&after)[N]) {
+    uint32_t ticket = 0;  // an increment, not an add: its result is waited for where it is used, below
+    if (gl == 0) ticket = atomicInc(&g_stream_rows[0], 0xffffffffu);
+    if (next < A.rows) fetch(after, next, next_token);
+    const RowAt at = row_at(A.map, row);
+    T *dx = static_cast<T *>(A.dx) + at.g;
+    const float x_token = gl == 0 && uint32_t(token) < V ? float((static_cast<const T *>(A.x) + at.x)[token]) : 0.0f;
+    float m = -kInf;
+#pragma unroll
+    for (int u = 0; u < N; ++u) m = __builtin_elementwise_maximum(m, unit_max(to_floats<T>(v[u])));
+    if (gl == 0) drawn[turn] = ticket + 2 * grid;
+    m = lanes_max<L>(m, lds[turn][0]);  // its barrier makes drawn[turn] visible too
+    const uint32_t after_next = __builtin_amdgcn_readfirstlane(drawn[turn]);
+    const int32_t after_token = after_next < A.rows ? A.tokens[after_next] : -1;
+    // c (x - m) rather than a fused c x - c m: one more instruction, and no logits out of its range
+    const auto exponent = [&](float x) { return fmaxf((x - m) * A.c, -200.0f); };
+    float s = 0.0f, w = 0.0f;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      if constexpr (sizeof(T) == 2) keep_raw(v[u]);
+      const auto f = to_floats<T>(v[u]);
+#pragma unroll
+      for (uint32_t e = 0; e < E; ++e) {
+        const float z = exponent(f[e]), p = __builtin_amdgcn_exp2f(z);
+        s += p;
+        w = __builtin_fmaf(p, z, w);
+      }
+    }
+    // both sums behind one barrier
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+      s += __shfl_xor(s, d);
+      w += __shfl_xor(w, d);
+    }
+    if (gl % 64 == 0) {
+      lds[turn][1][gl / 64] = s;
+      lds[turn][2][gl / 64] = w;
+    }
+    __syncthreads();
+    s = w = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < L / 64; ++k) {
+      s += lds[turn][1][k];
+      w += lds[turn][2][k];
+    }
+    if (!(fabsf(m) <= FLT_MAX) && m != -kInf) m = __builtin_nanf("");  // a NaN or an infinite logit
+    const float l = log2f(s), h = kLn2 * (l - w / s);
+    if (gl == 0) {
+      if (token < 0) pad_out(A, row);
+      else row_out(A, row, token, x_token, m, s, w, 0.0f);
+    }
+    RowGrad G(A, row, token, m, l, h < 0.0f ? 0.0f : h);
+    if (m == -kInf) G.a = G.b = G.onehot = 0.0f;  // padding too
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      const uint32_t j = (u * L + gl) * E;
+      if (j >= V) continue;
+      if constexpr (sizeof(T) == 2) keep_raw(v[u]);
+      auto f = to_floats<T>(v[u]);
+#pragma unroll
+      for (uint32_t e = 0; e < E; ++e) {
+        const float z = exponent(f[e]);
+        f[e] = -__builtin_amdgcn_exp2f(z) * __builtin_fmaf(G.b, z, G.a);
+      }
+      const uint32_t hit = uint32_t(token) - j;
+      if (hit < E)
+#pragma unroll
+        for (uint32_t e = 0; e < E; ++e) f[e] += hit == e ? G.onehot : 0.0f;
+      __builtin_nontemporal_store(__builtin_convertvector(f, vec), reinterpret_cast<vec *>(dx + u * L * E + gl * E));
+    }
+    row = next, token = next_token;
+    next = after_next, next_token = after_token;
+    turn ^= 1;
+  };
+  while (row < A.rows) {
+    work(first, second);
+    if (row >= A.rows) break;
+    work(second, first);
+  }
+  // the last workgroup leaves the counters at zero for the next launch
+  if (gl == 0) {
+    if (__hip_atomic_fetch_add(&g_stream_rows[1], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == grid - 1) {
+      __hip_atomic_store(&g_stream_rows[0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&g_stream_rows[1], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+}
+
 // f(lanes, units) for rows of `units` units that registers can hold; false for longer ones.
 template <class F>
 bool with_held_shape(uint32_t units, F &&f) {
@@ -987,7 +1105,7 @@ bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *t
     return false;
   }
   const uint64_t V = x->shape[x->ndim - 1], n = numel(x);
-  if (V < 1 || V >= uint64_t(1) << 31) {
+  if (V < 1 || V > (uint64_t(1) << 31) - 64) {  // unit numbers times their elements stay within 31 bits
     report_error(where, "rows of %llu logits are not supported", (unsigned long long)V);
     return false;
   }
@@ -1067,6 +1185,26 @@ uint32_t *tickets(const char *where) {
   return at = static_cast<uint32_t *>(p);
 }
 
+// launch(args, workgroups) for parts of the rows that one grid of `threads` lanes holds.
+template <class F>
+void by_parts(const TokenArgs &A, uint64_t rows_per_block, uint64_t threads, F &&launch) {
+  const uint64_t most = max_blocks(threads) * rows_per_block;
+  TokenArgs part = A;
+  for (uint64_t r = 0; r < A.rows; r += most) {
+    part.first_row = uint32_t(r);
+    part.rows = uint32_t(A.rows - r < most ? A.rows - r : most);
+    launch(part, ceil_div(part.rows, rows_per_block));
+  }
+}
+
+template <class T, int L, int U, bool GRAD>
+void launch_held(const TokenArgs &A) {
+  constexpr int B = L > kRowBlock ? L : kRowBlock;
+  by_parts(A, L > 64 ? 1 : B / L, B, [](const TokenArgs &part, unsigned blocks) {
+    held_kernel<T, L, U, GRAD><<<blocks, B, 0, stream()>>>(part);
+  });
+}
+
 template <class T, bool TOP>
 bool launch_rows(const TokenArgs &A, const char *where) {
   const uint64_t unit = 16 / sizeof(T), units = A.vocab / unit;
@@ -1075,15 +1213,17 @@ bool launch_rows(const TokenArgs &A, const char *where) {
     if (most_units<T>(A.vocab) <= 256) {
       with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto n) {
         constexpr int L = decltype(lanes)::value;
-        if constexpr (L <= 64)
-          held_kernel<T, L, decltype(n)::value, false>
-              <<<ceil_div(A.rows, kRowBlock / L), kRowBlock, 0, stream()>>>(A);
+        if constexpr (L <= 64) launch_held<T, L, decltype(n)::value, false>(A);
       });
       return true;
     }
-  // waves of a row: enough rows, or enough waves to a row, to fill the chip
+  // A wave a row where rows are many and not long, four where a wave would be alone with its row for long: [4096,
+  // 131072] in bf16 with 8 alternatives 224 us with one, 184 with four, [8192, 49999] in fp16 with 20 192 and 169;
+  // [20000, 5000] in bf16 with 5 56 and 117. Few rows are cut over up to 512 workgroups of 1024 units or more.
   if (units <= 256 || (A.rows >= 8192 && units < 4096)) {
-    fwd_kernel<T, 1, TOP, false><<<ceil_div(A.rows, 4), 256, 0, stream()>>>(A, P);
+    by_parts(A, 4, 256, [&](const TokenArgs &part, unsigned blocks) {
+      fwd_kernel<T, 1, TOP, false><<<blocks, 256, 0, stream()>>>(part, P);
+    });
     return true;
   }
   uint64_t cut = units / 1024;
@@ -1098,7 +1238,9 @@ bool launch_rows(const TokenArgs &A, const char *where) {
   } else if (A.rows < 512 && units > 1024) {
     fwd_kernel<T, 16, TOP, false><<<A.rows, 1024, 0, stream()>>>(A, P);
   } else {
-    fwd_kernel<T, 4, TOP, false><<<A.rows, 256, 0, stream()>>>(A, P);
+    by_parts(A, 1, 256, [&](const TokenArgs &part, unsigned blocks) {
+      fwd_kernel<T, 4, TOP, false><<<blocks, 256, 0, stream()>>>(part, P);
+    });
   }
   return true;
 }
@@ -1114,7 +1256,7 @@ bool launch_forward(const TokenArgs &A, DTYPE type, const char *where) {
 template <class T, bool ADD>
 void launch_bwd(const TokenArgs &A) {
   const uint32_t units = most_units<T>(A.vocab);
-  if (units < 128 && uint64_t(A.rows) * units < uint64_t(1) << 32) {
+  if (units < 128 && uint64_t(A.rows) * units < (uint64_t(1) << 32) - kRowBlock) {
     bwd_short_kernel<T, ADD><<<ceil_div(uint64_t(A.rows) * units, kRowBlock), kRowBlock, 0, stream()>>>(
         A, MagicDiv::make(units));
     return;
@@ -1134,6 +1276,15 @@ void launch_backward(const TokenArgs &A, DTYPE type, bool add) {
     if (add) launch_bwd<decltype(t), true>(A);
     else launch_bwd<decltype(t), false>(A);
   });
+}
+
+// Whether every row of the gradient is whole 16-byte units at 16-byte addresses.
+template <class T>
+bool whole_rows(const TokenArgs &A) {
+  constexpr int64_t E = Unit<T>::E;
+  bool whole = A.vocab % E == 0 && aligned16(A.dx);
+  for (int d = 0; d < A.map.rank; ++d) whole = whole && A.map.g[d] % E == 0;
+  return whole;
 }
 
 // The float vectors of a call.
@@ -1244,8 +1395,15 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
   with_float_type(x->dtype, [&](auto t) {
     typedef decltype(t) T;
     held = with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto units) {
-      constexpr int L = decltype(lanes)::value, B = L > kRowBlock ? L : kRowBlock;
-      held_kernel<T, L, decltype(units)::value, true><<<ceil_div(N, L > 64 ? 1 : B / L), B, 0, stream()>>>(A);
+      constexpr int L = decltype(lanes)::value;
+      constexpr int U = decltype(units)::value;
+      if constexpr (L == 1024 && U == 8 && sizeof(T) == 4) {
+        if (A.rows >= 4 * uint32_t(num_cus()) && whole_rows<T>(A)) {
+          held_stream_kernel<T, U><<<num_cus(), kStreamLanes, 0, stream()>>>(A);
+          return;
+        }
+      }
+      launch_held<T, L, U, true>(A);
     });
   });
   if (held) {

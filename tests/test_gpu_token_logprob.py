@@ -153,7 +153,8 @@ def test_gradient_and_step(kind, vocab):
         check_gradient(s.dx(), want, kind, f"step {kind} {n}x{vocab}")
 
 
-@pytest.mark.parametrize("rows, vocab", [(1500, 18), (700, 2052), (600, 8192), (520, 32000)])
+@pytest.mark.parametrize("rows, vocab", [(1500, 18), (700, 2052), (600, 8192), (520, 32000), (1300, 17000),
+                                         (1100, 16392)])
 @pytest.mark.parametrize("kind", list(KINDS))
 def test_step_over_more_rows_than_are_resident(kind, rows, vocab):
     rng = np.random.RandomState(rows)
