@@ -249,19 +249,54 @@ struct Product {
   Stack o;
 };
 
-// A block of 32x32 sums as the matrix unit leaves it: register r of a lane holds row
-// 8 (r / 4) + 4 (lane / 32) + r % 4 of column lane % 32. It goes through LDS, so that rows and columns
-// both leave as whole lines.
-constexpr int kBlockLds = 32 * 33;
+constexpr int kBlockLds = 32 * 33;  // floats of a block in LDS
 // Orders a wave's writes to its part of LDS before its lanes' reads of each other's.
 __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+// Tile number -> (i, j): all of them, or those on and below the diagonal, row by row.
+template <Mode M>
+__device__ __forceinline__ void tile_at(uint32_t t, uint32_t ti, uint32_t &i, uint32_t &j) {
+  if constexpr (M == Gram || M == Square) {
+    i = uint32_t((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= t) ++i;
+    while (i * (i + 1) / 2 > t) --i;
+    j = t - i * (i + 1) / 2;
+  } else {
+    i = t % ti;
+    j = t / ti;
+  }
+}
+
+// What a block's result adds to its sums, a lane's sixteen columns of a row.
+struct Term {
+  h8 hi[2], lo[2];
+};
+template <Mode M, int PL>
+__device__ __forceinline__ Term load_term(const Product &P, uint32_t b, uint32_t i0, uint32_t j0) {
+  const uint32_t lane = threadIdx.x & 63, r = lane / 2, c = lane % 2 * 16;
+  Term t;
+  if constexpr (M != Gram) {
+    const bool tall = M == Final && P.o.rows > P.o.cols;
+    const char *at = tall ? line_at<PL>(P.in_t, b, j0 + r, i0 + c) : line_at<PL>(P.in, b, i0 + r, j0 + c);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      t.hi[h] = reinterpret_cast<const h8 *>(at)[h];
+      if constexpr (PL == 2) t.lo[h] = reinterpret_cast<const h8 *>(at + 64)[h];
+      else t.lo[h] = f16_t(0.0f);
+    }
+  }
+  return t;
+}
+
+// A block of 32x32 sums as the matrix unit leaves it: register r of a lane holds row
+// 8 (r / 4) + 4 (lane / 32) + r % 4 of column lane % 32. It goes through LDS, so that rows and columns
+// both leave as whole lines.
 template <class T, Mode M, bool MUON, int PL>
-__device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, float *lds, f16v acc, uint32_t b,
-                                          uint32_t i0, uint32_t j0, bool mirror) {
+__device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, float *lds, f16v acc, const Term &term,
+                                          uint32_t b, uint32_t i0, uint32_t j0, bool mirror) {
   const uint32_t lane = threadIdx.x & 63;
   float alpha = P.alpha, beta = P.beta;
   if constexpr (M == Gram || M == Final) {
@@ -276,19 +311,9 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
   const uint32_t r = lane / 2, c = lane % 2 * 16;
   if constexpr (M == Final) {
     const bool tall = P.o.rows > P.o.cols;  // then the result is the transpose
-    if (!tall) {
-      float v[16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) get8<PL>(line_at<PL>(P.in, b, i0 + r, j0 + c + 8 * h), v + 8 * h);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) lds[r * 33 + c + e] += beta * v[e];
-    } else {
-      float v[16];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) get8<PL>(line_at<PL>(P.in_t, b, j0 + r, i0 + c + 8 * h), v + 8 * h);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) lds[(c + e) * 33 + r] += beta * v[e];
-    }
+    for (int e = 0; e < 16; ++e)
+      lds[tall ? (c + e) * 33 + r : r * 33 + c + e] += beta * (float(term.hi[e / 8][e % 8]) + float(term.lo[e / 8][e % 8]));
     wave_sync();
     const uint32_t k = lane % 32;
 #pragma unroll
@@ -310,11 +335,9 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
     for (int h = 0; h < 2; ++h) {
       float v[8], t[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = lds[r * 33 + c + 8 * h + e];
-      if constexpr (M != Gram) {
-        get8<PL>(line_at<PL>(P.in, b, i0 + r, j0 + c + 8 * h), t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(beta, t[e], v[e]);
+      for (int e = 0; e < 8; ++e) {
+        v[e] = lds[r * 33 + c + 8 * h + e];
+        if constexpr (M != Gram) v[e] = __builtin_fmaf(beta, float(term.hi[h][e]) + float(term.lo[h][e]), v[e]);
       }
       if (M == Square && P.in2.data) {
         get8<PL>(line_at<PL>(P.in2, b, i0 + r, j0 + c + 8 * h), t);
@@ -340,25 +363,14 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
   wave_sync();
 }
 
-// Tile number -> (i, j): all of them, or those on and below the diagonal, row by row.
-template <Mode M>
-__device__ __forceinline__ void tile_at(uint32_t t, uint32_t ti, uint32_t &i, uint32_t &j) {
-  if constexpr (M == Gram || M == Square) {
-    i = uint32_t((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);
-    while ((i + 1) * (i + 2) / 2 <= t) ++i;
-    while (i * (i + 1) / 2 > t) --i;
-    j = t - i * (i + 1) / 2;
-  } else {
-    i = t % ti;
-    j = t / ti;
-  }
-}
-
 // One tile of BM x BN outputs over one piece of the sum, by waves of WM x WN. Two stages of LDS: while
 // the waves multiply one line of every row, the next lines are on their way into the other (loads straight
 // to LDS; lane l of a load fills bytes 16 l of its 1 KiB, so a row's eight 16-byte units are permuted by
 // choosing what each lane reads: unit c lies at c ^ (row / 2 % 8). A 16-byte LDS read is served for lanes 0-3, 12-15,
-// 20-27 of a half wave together, then for the others, from 64 banks: this spreads either set over all of them).
+// 20-27 of a half wave together, then for the others, from 64 banks: this spreads either set over all of them). A ring of
+// five half-line stages, four of them on their way, measured the same within 2%, with 4096 x 4096 in 4.28 ms and 4.30: the
+// matrix units are at 1.1 PFLOP/s of fp16 in the long sums, what a large library product reaches here, and in the
+// short ones wait for the tiles' ways out, when all workgroups store at once (24 x 1024 x 1024: 35% busy).
 template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Product P, MuonSet S) {
   constexpr int NW = (BM / WM) * (BN / WN), LOADS = (BM + BN) / 8 / NW, FA = WM / 32, FB = WN / 32;
@@ -447,13 +459,46 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
                                                acc[a][c][4 * q + 3]};
     return;
   }
+  Term next = load_term<M, PL>(P, b, i0, j0);
   __syncthreads();  // the stages become the blocks' way out
   float *way = reinterpret_cast<float *>(lds) + wave * kBlockLds;
 #pragma unroll
-  for (int a = 0; a < FA; ++a)
+  for (int k = 0; k < FA * FB; ++k) {
+    const Term term = next;  // the next block's is on its way while this one leaves
+    if (k + 1 < FA * FB) next = load_term<M, PL>(P, b, i0 + (k + 1) / FB * 32, j0 + (k + 1) % FB * 32);
+    put_block<T, M, MUON, PL>(P, S, way, acc[k / FB][k % FB], term, b, i0 + k / FB * 32, j0 + k % FB * 32, !sym || ti != tj);
+  }
+}
+
+// Adds the pieces of a sum: a wave per 32x32 block.
+template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
+  constexpr int FA = WM / 32, FB = WN / 32, NB = (BM / 32) * (BN / 32);
+  __shared__ float lds[kNsBlock / 64 * kBlockLds];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr bool sym = M == Gram || M == Square;
+  const uint32_t tiles = sym ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj;
+  const uint32_t id = blockIdx.x * (kNsBlock / 64) + wave;  // NB is a multiple of 4: whole workgroups
+  const uint32_t block = id % NB, tile = id / NB, b = tile / tiles, t = tile - b * tiles;
+  uint32_t ti, tj;
+  tile_at<M>(t, P.ti, ti, tj);
+  const uint32_t w = block / (FA * FB), a = block % (FA * FB) / FB, c = block % FB;
+  const uint32_t i0 = ti * BM + w / (BN / WN) * WM + a * 32, j0 = tj * BN + w % (BN / WN) * WN + c * 32;
+  const Term term = load_term<M, PL>(P, b, i0, j0);
+  f16v acc;
 #pragma unroll
-    for (int c = 0; c < FB; ++c)
-      put_block<T, M, MUON, PL>(P, S, way, acc[a][c], b, i0 + a * 32, j0 + c * 32, !sym || ti != tj);
+  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+  for (uint32_t part = 0; part < P.parts; ++part) {
+    const f4 *from = reinterpret_cast<const f4 *>(P.partial) +
+                     ((uint64_t(b * P.parts + part) * tiles + t) * NB + block) * 4 * 64 + lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f4 v = from[q * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
+    }
+  }
+  put_block<T, M, MUON, PL>(P, S, lds + wave * kBlockLds, acc, term, b, i0, j0, !sym || ti != tj);
 }
 
 // Small products: a workgroup per 32x32 tile, whose eight waves each take a share of the sum straight from memory (a
@@ -473,6 +518,13 @@ __global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product
   const uint32_t i0 = ti * 32, j0 = tj * 32;
   const char *u = P.u.data + b * P.u.next + (i0 + lane % 32) * P.u.pitch + lane / 32 * 16;
   const char *v = P.v.data + b * P.v.next + (j0 + lane % 32) * P.v.pitch + lane / 32 * 16;
+  // the terms of the outputs that this thread will store, on their way while the sums are formed
+  const uint32_t half = threadIdx.x / 256, e8 = threadIdx.x % 256;
+  const bool stores = M == Final || (e8 < 128 && !(half && sym && ti == tj));
+  const uint32_t row8 = (half ? j0 : i0) + e8 / 4, col8 = (half ? i0 : j0) + e8 % 4 * 8;
+  float term[8];
+  if constexpr (M == Square || M == Update)
+    if (stores) get8<PL>(line_at<PL>(half ? P.in_t : P.in, b, row8, col8), term);
   f16v acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
@@ -530,55 +582,21 @@ __global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product
       }
     }
   } else {
-    const uint32_t half = threadIdx.x / 256, e = threadIdx.x % 256;
-    if (e >= 128 || (half && sym && ti == tj)) return;
-    const uint32_t r = e / 4, c = e % 4 * 8;
-    const uint32_t row = (half ? j0 : i0) + r, col = (half ? i0 : j0) + c;
+    if (!stores) return;
+    const uint32_t r = e8 / 4, c = e8 % 4 * 8;
     float w[8], x[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) w[k] = alpha * (half ? tile[(c + k) * 33 + r] : tile[r * 33 + c + k]);
-    if constexpr (M != Gram) {
-      get8<PL>(line_at<PL>(half ? P.in_t : P.in, b, row, col), x);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = __builtin_fmaf(beta, x[k], w[k]);
+    for (int k = 0; k < 8; ++k) {
+      w[k] = alpha * (half ? tile[(c + k) * 33 + r] : tile[r * 33 + c + k]);
+      if constexpr (M != Gram) w[k] = __builtin_fmaf(beta, term[k], w[k]);
     }
     if (M == Square && P.in2.data) {
-      get8<PL>(line_at<PL>(P.in2, b, row, col), x);
+      get8<PL>(line_at<PL>(P.in2, b, row8, col8), x);
 #pragma unroll
       for (int k = 0; k < 8; ++k) w[k] = __builtin_fmaf(P.gamma, x[k], w[k]);
     }
-    put8<PL>(line_at<PL>(half ? P.out_t : P.out, b, row, col), w);
+    put8<PL>(line_at<PL>(half ? P.out_t : P.out, b, row8, col8), w);
   }
-}
-
-// Adds the pieces of a sum: a wave per 32x32 block.
-template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
-  constexpr int FA = WM / 32, FB = WN / 32, NB = (BM / 32) * (BN / 32);
-  __shared__ float lds[kNsBlock / 64 * kBlockLds];
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr bool sym = M == Gram || M == Square;
-  const uint32_t tiles = sym ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj;
-  const uint32_t id = blockIdx.x * (kNsBlock / 64) + wave;  // NB is a multiple of 4: whole workgroups
-  const uint32_t block = id % NB, tile = id / NB, b = tile / tiles, t = tile - b * tiles;
-  uint32_t ti, tj;
-  tile_at<M>(t, P.ti, ti, tj);
-  f16v acc;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-  for (uint32_t part = 0; part < P.parts; ++part) {
-    const f4 *from = reinterpret_cast<const f4 *>(P.partial) +
-                     ((uint64_t(b * P.parts + part) * tiles + t) * NB + block) * 4 * 64 + lane;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f4 v = from[q * 64];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[4 * q + c] += v[c];
-    }
-  }
-  const uint32_t w = block / (FA * FB), a = block % (FA * FB) / FB, c = block % FB;
-  const uint32_t i0 = ti * BM + w / (BN / WN) * WM + a * 32, j0 = tj * BN + w % (BN / WN) * WN + c * 32;
-  put_block<T, M, MUON, PL>(P, S, lds + wave * kBlockLds, acc, b, i0, j0, !sym || ti != tj);
 }
 
 // No steps: the result is X.
