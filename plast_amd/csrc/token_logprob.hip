@@ -955,6 +955,44 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   }
 }
 
+// Alternatives of rows that a few lanes hold, one logit each: a logit's place is the number of those before it, counted
+// by passing the keys round. [60000, 18] in fp32 with 5: TINY us, a wave a row and its list in LDS 47.
+template <class T, int L>
+__global__ __launch_bounds__(kRowBlock) void tiny_kernel(TokenArgs A) {
+  const uint32_t gl = threadIdx.x % L, r = blockIdx.x * (kRowBlock / L) + threadIdx.x / L;
+  const bool valid = r < A.rows;
+  const uint32_t row = A.first_row + (valid ? r : A.rows - 1), V = A.vocab;
+  const int32_t token = A.tokens[row];
+  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
+  const bool mine = token >= 0 && gl < V;
+  const float v = mine ? float(x[gl]) : -kInf;
+  const uint32_t key = mine ? uint32_t(order_key(v, gl) >> 32) : 0;
+  float m = lanes_max<L>(v, nullptr);
+  const RowRef ref(A.c, m);
+  const float z = m == -kInf ? -200.0f : fmaxf(ref.z(v), -200.0f), e = __builtin_amdgcn_exp2f(z);
+  const float s = lanes_sum<L>(e, nullptr), w = lanes_sum<L>(e * z, nullptr);
+  uint32_t place = 0;
+#pragma unroll
+  for (int d = 1; d < L; ++d) {
+    const uint32_t o = __shfl_xor(key, d);
+    place += o > key || (o == key && (gl ^ d) < gl);
+  }
+  const float x_token = __shfl(v, token >= 0 && uint32_t(token) < V ? token : 0, L);
+  if (!(fabsf(m) <= FLT_MAX) && m != -kInf) m = __builtin_nanf("");  // a NaN or an infinite logit
+  if (!valid) return;
+  if (gl == 0) {
+    if (token < 0) pad_out(A, row);
+    else row_out(A, row, token, x_token, m, s, w, ref.shift());
+  }
+  const float l0 = log2f(s) - ref.shift();
+  if (mine && place < A.top) {
+    const uint64_t at = uint64_t(row) * A.top + place;
+    A.top_ids[at] = int32_t(gl);
+    A.top_logp[at] = log_p(A, v, m, l0);
+  }
+  for (uint32_t k = (token < 0 ? 0 : V) + gl; k < A.top; k += L) put_top(A, row, k, 0, m, l0);
+}
+
 // The step over many long rows: a workgroup of 1024 lanes per CU that goes from row to row, the next one's units on
 // their way into a second set of registers while this one is worked on. Rows are handed out as workgroups
 // become free (in fixed turns the odd XCDs end some 8% after the even ones); a result does not depend on who works it
@@ -1215,6 +1253,19 @@ bool launch_rows(const TokenArgs &A, const char *where) {
         constexpr int L = decltype(lanes)::value;
         if constexpr (L <= 64) launch_held<T, L, decltype(n)::value, false>(A);
       });
+      return true;
+    }
+  if constexpr (TOP)
+    if (A.vocab <= 64) {
+      const auto tiny = [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        by_parts(A, kRowBlock / L, kRowBlock, [](const TokenArgs &part, unsigned blocks) {
+          tiny_kernel<T, L><<<blocks, kRowBlock, 0, stream()>>>(part);
+        });
+      };
+      if (A.vocab <= 16) tiny(std::integral_constant<int, 16>{});
+      else if (A.vocab <= 32) tiny(std::integral_constant<int, 32>{});
+      else tiny(std::integral_constant<int, 64>{});
       return true;
     }
   // A wave a row where rows are many and not long, four where a wave would be alone with its row for long: [4096,

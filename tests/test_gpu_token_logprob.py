@@ -132,6 +132,23 @@ def test_few_long_rows_and_many_short(kind, rows, vocab):
 
 
 @pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("rows, vocab", [(300, 20011), (600, 9001), (2100, 2603), (8200, 4100), (20, 70001)])
+def test_alternatives_of_special_rows(kind, rows, vocab):
+    """Masked, tied, sorted and NaN rows among enough rows for each way of sharing a row."""
+    rng = np.random.RandomState(vocab)
+    for top, masked in ((20, 0.0), (32, 0.95)) if rows < 8000 else ((7, 0.3),):
+        print(f"special rows {kind} {rows}x{vocab} top {top}", flush=True)
+        x = special(logits(rng, rows, vocab, kind, masked), kind)
+        x[10:14] = x[0:4]
+        x[14, 5:] = -np.inf                    # fewer legal tokens than alternatives
+        x[15, : vocab - 4] = x[1, 0]           # the type's lowest value before a few others
+        tok = _tokens(rng, rows, vocab, 0.1)
+        tok[:16] = rng.randint(0, vocab, 16)
+        c = Case(x, kind, tok, 1.0, top).forward()
+        check_values(c.values(), exact(x, tok, 1.0, top), f"{kind} {rows}x{vocab} top {top}")
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("vocab", VOCABS + [131073])
 def test_gradient_and_step(kind, vocab):
     rng = np.random.RandomState(vocab + 1)
