@@ -175,17 +175,17 @@ __device__ __forceinline__ void put_stats(const TokenArgs &A, uint32_t row, floa
 }
 
 // The row's results, by one lane. s and w are over the whole row; `shift` is what every z holds beside c (x - m).
+// l0, log2 of s / 2^shift, may be given.
 __device__ __forceinline__ void row_out(const TokenArgs &A, uint32_t row, int32_t token, float x_token,
-                                        float m, float s, float w, float shift) {
+                                        float m, float s, float w, float shift, const float *exact_l0 = nullptr) {
   if (m == -kInf) {  // no logit that is not -inf
     A.logp[row] = uint32_t(token) < A.vocab ? -kInf : __builtin_nanf("");
     A.entropy[row] = 0.0f;
     put_stats(A, row, -kInf, 0.0f);
     return;
   }
-  const float l = log2f(s);
-  const float h = kLn2 * (l - w / s);
-  const float l0 = l - shift;
+  const float l0 = exact_l0 ? *exact_l0 : log2f(s) - shift;
+  const float h = kLn2 * ((l0 + shift) - w / s);
   A.logp[row] = uint32_t(token) < A.vocab ? log_p(A, x_token, m, l0) : __builtin_nanf("");
   A.entropy[row] = h < 0.0f ? 0.0f : h;
   put_stats(A, row, m, l0);
@@ -859,13 +859,23 @@ __device__ __forceinline__ float lanes_sum(float v, float *lds) {
   return v;
 }
 
+// log2 of s / 2^shift from the rest of s beside its `ones` largest terms of 2^shift each: log1p, rounded once where a
+// sum around 1 would lose what a likely token's log p, close to 0, consists of.
+__device__ __forceinline__ float log2_sum(float rest, float ones, float shift) {
+  constexpr float kLog2e = 1.44269504088896341f;
+  return log1pf(rest * __builtin_amdgcn_exp2f(-shift) + (ones - 1.0f)) * kLog2e;
+}
+
 // Forward and gradient (GRAD), or the forward alone, of rows that L lanes hold in N units each: one read, one
-// write. Rows of up to a wave's lanes share workgroups.
+// write. Rows of up to a wave's lanes share workgroups. In short rows, where a likely token can have nearly all of
+// the distribution, the largest logits' terms are counted apart from the others' sum (three instructions a logit: 14%
+// of the step's time if the long rows had it too).
 template <class T, int L, int N, bool GRAD>
 __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(TokenArgs A) {
   constexpr uint32_t B = L > kRowBlock ? L : kRowBlock, E = Unit<T>::E;
   constexpr uint32_t ROWS = L > 64 ? 1 : B / L;
   static_assert(L <= 64 || L == B, "a row has a workgroup or lanes of a wave");
+  constexpr bool APART = L <= 16;
   __shared__ float lds[3][16];
   const uint32_t V = A.vocab, gl = threadIdx.x % L;
   const uint32_t r = blockIdx.x * ROWS + threadIdx.x / L;
@@ -894,7 +904,9 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   for (int u = 0; u < N; ++u) m = __builtin_elementwise_maximum(m, unit_max(to_floats<T>(v[u])));
   m = lanes_max<L>(m, lds[0]);
   const RowRef ref(A.c, m);
+  const float ref_shift = ref.shift();
   float s = 0.0f, w = 0.0f;
+  uint32_t ones = 0;
   if (m != -kInf) {
     const auto sums = [&](auto far) {
 #pragma unroll
@@ -905,7 +917,12 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
         for (uint32_t e = 0; e < E; ++e) {
           const float z = fmaxf(far ? (f[e] - m) * A.c : __builtin_fmaf(f[e], A.c, -ref.cm), -200.0f);
           const float p = __builtin_amdgcn_exp2f(z);
-          s += p;
+          if constexpr (APART) {
+            ones += f[e] == m;
+            s += f[e] == m ? 0.0f : p;
+          } else {
+            s += p;
+          }
           w = __builtin_fmaf(p, z, w);
         }
       }
@@ -916,10 +933,18 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   s = lanes_sum<L>(s, lds[1]);
   w = lanes_sum<L>(w, lds[2]);
   if (!(fabsf(m) <= FLT_MAX) && m != -kInf) m = __builtin_nanf("");  // a NaN or an infinite logit
-  const float l = log2f(s);
+  float l0;
+  if constexpr (APART) {
+    const float n = lanes_sum<L>(float(ones), nullptr);
+    l0 = log2_sum(s, n, ref.shift());
+    s += n * __builtin_amdgcn_exp2f(ref.shift());
+  } else {
+    l0 = log2f(s) - ref.shift();
+  }
+  if (m != m) l0 = m;
   if (gl == 0 && valid) {
     if (token < 0) pad_out(A, row);
-    else row_out(A, row, token, x_token, m, s, w, ref.shift());
+    else row_out(A, row, token, x_token, m, s, w, ref.shift(), &l0);
   }
   if constexpr (GRAD) {
     if (!valid) return;
@@ -932,7 +957,7 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
       }
       return;
     }
-    const float h = kLn2 * (l - w / s);
+    const float l = l0 + ref_shift, h = kLn2 * (l - w / s);
     const RowGrad G(A, row, token, m, l, h < 0.0f ? 0.0f : h);
     const auto grads = [&](auto far) {
 #pragma unroll
@@ -956,7 +981,7 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
 }
 
 // Alternatives of rows that a few lanes hold, one logit each: a logit's place is the number of those before it, counted
-// by passing the keys round. [60000, 18] in fp32 with 5: TINY us, a wave a row and its list in LDS 47.
+// by passing the keys round. [60000, 18] in fp32 with 5: 26 us, a wave a row and its list in LDS 47.
 template <class T, int L>
 __global__ __launch_bounds__(kRowBlock) void tiny_kernel(TokenArgs A) {
   const uint32_t gl = threadIdx.x % L, r = blockIdx.x * (kRowBlock / L) + threadIdx.x / L;
@@ -970,6 +995,7 @@ __global__ __launch_bounds__(kRowBlock) void tiny_kernel(TokenArgs A) {
   float m = lanes_max<L>(v, nullptr);
   const RowRef ref(A.c, m);
   const float z = m == -kInf ? -200.0f : fmaxf(ref.z(v), -200.0f), e = __builtin_amdgcn_exp2f(z);
+  const float rest = lanes_sum<L>(v == m ? 0.0f : e, nullptr), ones = lanes_sum<L>(mine && v == m ? 1.0f : 0.0f, nullptr);
   const float s = lanes_sum<L>(e, nullptr), w = lanes_sum<L>(e * z, nullptr);
   uint32_t place = 0;
 #pragma unroll
@@ -978,13 +1004,13 @@ __global__ __launch_bounds__(kRowBlock) void tiny_kernel(TokenArgs A) {
     place += o > key || (o == key && (gl ^ d) < gl);
   }
   const float x_token = __shfl(v, token >= 0 && uint32_t(token) < V ? token : 0, L);
+  const float l0 = log2_sum(rest, ones, ref.shift());
   if (!(fabsf(m) <= FLT_MAX) && m != -kInf) m = __builtin_nanf("");  // a NaN or an infinite logit
   if (!valid) return;
   if (gl == 0) {
     if (token < 0) pad_out(A, row);
-    else row_out(A, row, token, x_token, m, s, w, ref.shift());
+    else row_out(A, row, token, x_token, m, s, w, ref.shift(), &l0);
   }
-  const float l0 = log2f(s) - ref.shift();
   if (mine && place < A.top) {
     const uint64_t at = uint64_t(row) * A.top + place;
     A.top_ids[at] = int32_t(gl);
