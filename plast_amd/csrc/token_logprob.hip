@@ -102,6 +102,12 @@ __device__ __forceinline__ void keep_raw(V &v) {
   asm volatile("" : "+v"(w));
   v = __builtin_bit_cast(V, w);
 }
+// A unit's sum by pairs: beside a largest term of 1, the fewer roundings the better.
+template <class F>
+__device__ __forceinline__ float unit_sum(F f) {
+  if constexpr (sizeof(F) == 32) return ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+  else return (f[0] + f[1]) + (f[2] + f[3]);
+}
 // The largest of a unit, NaN if one is.
 template <class F>
 __device__ __forceinline__ float unit_max(F f) {
@@ -127,12 +133,13 @@ struct Running {
     m = __builtin_elementwise_maximum(m, g);  // NaN stays
     refer(fmaxf(c * m, -1e38f));
   }
-  __device__ __forceinline__ void add(float c, float x) {
+  // A logit's term, which the caller adds to s.
+  __device__ __forceinline__ float term(float c, float x) {
     // below 2^-200 nothing is added, and a masked logit's -inf meets no 0
     const float z = fmaxf(__builtin_fmaf(x, c, -cm), -200.0f);
     const float e = __builtin_amdgcn_exp2f(z);
-    s += e;
     w = __builtin_fmaf(e, z, w);
+    return e;
   }
 };
 __device__ __forceinline__ Running wave_join(Running r) {
@@ -546,8 +553,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
       const auto f = to_floats<T>(v[u]);
       const float g = unit_max(f);
       if (!(g <= r.m)) r.grow(c, g);
+      auto terms = f;
 #pragma unroll
-      for (uint32_t e = 0; e < E; ++e) r.add(c, f[e]);
+      for (uint32_t e = 0; e < E; ++e) terms[e] = r.term(c, f[e]);
+      r.s += unit_sum(terms);
       if constexpr (TOP) {
         largest[u] = g;
         most = fmaxf(most, g);
@@ -588,7 +597,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   } while (q0 < to);
   if (has_tail) {
     if (!(tail <= r.m)) r.grow(c, tail);
-    r.add(c, tail);
+    r.s += r.term(c, tail);
   }
   if (TOP && !tail_first) top.push(has_tail && tail > top.bound, tail, units + gl);
   r = wave_join(r);
@@ -913,18 +922,20 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
       for (int u = 0; u < N; ++u) {
         keep_raw(v[u]);
         const auto f = to_floats<T>(v[u]);
+        auto terms = f;
 #pragma unroll
         for (uint32_t e = 0; e < E; ++e) {
           const float z = fmaxf(far ? (f[e] - m) * A.c : __builtin_fmaf(f[e], A.c, -ref.cm), -200.0f);
           const float p = __builtin_amdgcn_exp2f(z);
           if constexpr (APART) {
             ones += f[e] == m;
-            s += f[e] == m ? 0.0f : p;
+            terms[e] = f[e] == m ? 0.0f : p;
           } else {
-            s += p;
+            terms[e] = p;
           }
           w = __builtin_fmaf(p, z, w);
         }
+        s += unit_sum(terms);
       }
     };
     if (ref.far) sums(std::true_type{});
@@ -1070,12 +1081,14 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
     for (int u = 0; u < N; ++u) {
       if constexpr (sizeof(T) == 2) keep_raw(v[u]);
       const auto f = to_floats<T>(v[u]);
+      auto terms = f;
 #pragma unroll
       for (uint32_t e = 0; e < E; ++e) {
-        const float z = exponent(f[e]), p = __builtin_amdgcn_exp2f(z);
-        s += p;
-        w = __builtin_fmaf(p, z, w);
+        const float z = exponent(f[e]);
+        terms[e] = __builtin_amdgcn_exp2f(z);
+        w = __builtin_fmaf(terms[e], z, w);
       }
+      s += unit_sum(terms);
     }
     // both sums behind one barrier
 #pragma unroll
