@@ -87,6 +87,7 @@ __global__ __launch_bounds__(kNsBlock) void norm_kernel(Stack G, MagicDiv cols, 
   const T *g = static_cast<const T *>(G.data) + int64_t(blockIdx.y) * G.sb;
   const uint32_t n = G.rows * G.cols, stride = gridDim.x * kNsBlock;  // below 2^32
   double s = 0.0;
+#pragma unroll 4
   for (uint64_t at = uint64_t(blockIdx.x) * kNsBlock + threadIdx.x; at < n; at += stride) {
     const uint32_t i = cols.div(uint32_t(at)), j = uint32_t(at) - i * G.cols;
     const double v = double(float(g[int64_t(i) * G.s0 + int64_t(j) * G.s1]));
@@ -195,23 +196,29 @@ __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, con
                                                          float base, Lines X, Lines XT, float *xscale) {
   __shared__ float tile[64][65];
   const uint32_t b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of the source
-  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth, base);
-  const double scale = sx / (norm + double(eps));
-  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) xscale[b] = float(sx);
   const bool tall = G.rows > G.cols;
   const T *g = static_cast<const T *>(G.data) + int64_t(b) * G.sb;
-  for (uint32_t e = threadIdx.x; e < 64 * 64; e += kNsBlock) {
-    const uint32_t r = r0 + e / 64, c = c0 + e % 64;
-    float v = 0.0f;
+  float in[64 * 64 / kNsBlock];
+#pragma unroll
+  for (uint32_t k = 0; k < 64 * 64 / kNsBlock; ++k) {
+    const uint32_t e = k * kNsBlock + threadIdx.x, r = r0 + e / 64, c = c0 + e % 64;
+    in[k] = 0.0f;
     if (r < G.rows && c < G.cols) {
       if constexpr (MUON) {
         const uint64_t at = uint64_t(r) * G.cols + c;
-        v = muon_update(S.g[b][at], S.m[b][at], S.rule);
+        in[k] = muon_update(S.g[b][at], S.m[b][at], S.rule);
       } else {
-        v = float(g[int64_t(r) * G.s0 + int64_t(c) * G.s1]);
+        in[k] = float(g[int64_t(r) * G.s0 + int64_t(c) * G.s1]);
       }
     }
-    tile[e / 64][e % 64] = float(double(v) * scale);
+  }
+  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth, base);
+  const double scale = sx / (norm + double(eps));
+  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) xscale[b] = float(sx);
+#pragma unroll
+  for (uint32_t k = 0; k < 64 * 64 / kNsBlock; ++k) {
+    const uint32_t e = k * kNsBlock + threadIdx.x;
+    tile[e / 64][e % 64] = float(double(in[k]) * scale);
   }
   __syncthreads();
   const Lines &R = tall ? XT : X, &C = tall ? X : XT;
@@ -311,6 +318,15 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
   const uint32_t r = lane / 2, c = lane % 2 * 16;
   if constexpr (M == Final) {
     const bool tall = P.o.rows > P.o.cols;  // then the result is the transpose
+    const uint32_t row0 = (tall ? j0 : i0) + lane / 32, col = (tall ? i0 : j0) + lane % 32;
+    float old[16];  // the parameters, read together and ahead of their stores
+    if constexpr (MUON) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const uint32_t row = row0 + 2 * e;
+        old[e] = row < P.o.rows && col < P.o.cols ? S.p[b][uint64_t(row) * P.o.cols + col] : 0.0f;
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e)
       lds[tall ? (c + e) * 33 + r : r * 33 + c + e] += beta * (float(term.hi[e / 8][e % 8]) + float(term.lo[e / 8][e % 8]));
@@ -318,13 +334,11 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
     const uint32_t k = lane % 32;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const uint32_t q = 2 * e + lane / 32;
+      const uint32_t q = 2 * e + lane / 32, row = row0 + 2 * e;
       const float v = tall ? lds[k * 33 + q] : lds[q * 33 + k];
-      const uint32_t row = (tall ? j0 : i0) + q, col = (tall ? i0 : j0) + k;
       if (row >= P.o.rows || col >= P.o.cols) continue;
       if constexpr (MUON) {
-        float *p = S.p[b] + uint64_t(row) * P.o.cols + col;
-        *p = *p * S.rule.keep - S.rule.scale * v;
+        S.p[b][uint64_t(row) * P.o.cols + col] = old[e] * S.rule.keep - S.rule.scale * v;
       } else {
         T *o = static_cast<T *>(const_cast<void *>(P.o.data)) + int64_t(b) * P.o.sb;
         o[int64_t(row) * P.o.s0 + int64_t(col) * P.o.s1] = T(v);
