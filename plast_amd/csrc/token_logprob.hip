@@ -1282,8 +1282,20 @@ void launch_held(const TokenArgs &A) {
   });
 }
 
+// Workgroups that a row is cut over: few rows, up to 512 workgroups of 1024 units or more.
+uint32_t pieces_of(uint64_t rows, uint64_t vocab, uint64_t bytes) {
+  uint64_t cut = vocab * bytes / 16 / 1024;
+  if (cut > 512 / rows) cut = 512 / rows;
+  return uint32_t(cut > kMaxPieces ? kMaxPieces : cut < 1 ? 1 : cut);
+}
+uint64_t pieces_bytes(uint64_t rows, uint64_t vocab, uint64_t bytes) {
+  const uint32_t cut = pieces_of(rows, vocab, bytes);
+  return cut > 1 ? rows * cut * sizeof(Piece) : 0;
+}
+
+// `room`: pieces_bytes of memory, or null to take them from the workspace.
 template <class T, bool TOP>
-bool launch_rows(const TokenArgs &A, const char *where) {
+bool launch_rows(const TokenArgs &A, void *room, const char *where) {
   const uint64_t unit = 16 / sizeof(T), units = A.vocab / unit;
   Pieces P{1, nullptr, nullptr};
   if constexpr (!TOP)
@@ -1309,23 +1321,24 @@ bool launch_rows(const TokenArgs &A, const char *where) {
     }
   // A wave a row where rows are many and not long, four where a wave would be alone with its row for long: [4096,
   // 131072] in bf16 with 8 alternatives 224 us with one, 184 with four, [8192, 49999] in fp16 with 20 192 and 169;
-  // [20000, 5000] in bf16 with 5 56 and 117. Few rows are cut over up to 512 workgroups of 1024 units or more.
+  // [20000, 5000] in bf16 with 5 56 and 117.
   if (units <= 256 || (A.rows >= 8192 && units < 4096)) {
     by_parts(A, 4, 256, [&](const TokenArgs &part, unsigned blocks) {
       fwd_kernel<T, 1, TOP, false><<<blocks, 256, 0, stream()>>>(part, P);
     });
     return true;
   }
-  uint64_t cut = units / 1024;
-  if (cut > 512 / A.rows) cut = 512 / A.rows;
-  if (cut > kMaxPieces) cut = kMaxPieces;
-  if (cut > 1) {
-    P.n = uint32_t(cut);
+  P.n = pieces_of(A.rows, A.vocab, sizeof(T));
+  if (P.n > 1) {
+    if (!room) room = partials(pieces_bytes(A.rows, A.vocab, sizeof(T)), where);
+    P.found = static_cast<Piece *>(room);
     P.tickets = tickets(where);
-    P.found = static_cast<Piece *>(partials(uint64_t(A.rows) * cut * sizeof(Piece), where));
     if (!P.tickets || !P.found) return false;
     fwd_kernel<T, 4, TOP, true><<<A.rows * P.n, 256, 0, stream()>>>(A, P);
-  } else if (A.rows < 512 && units > 1024) {
+  } else if (A.rows < 512 && units >= 6000) {
+    // sixteen waves a row where a few hundred long ones leave the chip half empty: [300, 131072] in bf16 with 20
+    // alternatives 53 us with sixteen, 58 with four, [300, 32000] in fp32 15.8 and 16.7; but [500, 32000] in bf16 13.4 and
+    // 12.3, [500, 16000] with 5 19.9 and 13.0
     fwd_kernel<T, 16, TOP, false><<<A.rows, 1024, 0, stream()>>>(A, P);
   } else {
     by_parts(A, 1, 256, [&](const TokenArgs &part, unsigned blocks) {
@@ -1335,10 +1348,10 @@ bool launch_rows(const TokenArgs &A, const char *where) {
   return true;
 }
 
-bool launch_forward(const TokenArgs &A, DTYPE type, const char *where) {
+bool launch_forward(const TokenArgs &A, DTYPE type, void *room, const char *where) {
   bool ok = false;
   with_float_type(type, [&](auto t) {
-    ok = A.top ? launch_rows<decltype(t), true>(A, where) : launch_rows<decltype(t), false>(A, where);
+    ok = A.top ? launch_rows<decltype(t), true>(A, room, where) : launch_rows<decltype(t), false>(A, room, where);
   });
   return ok;
 }
@@ -1437,7 +1450,7 @@ void token_logprob_hip_forward(const Tensor **inputs, Tensor *output, KernelPara
     A.top_ids = static_cast<int32_t *>(ids->data);
   }
   if (A.rows == 0 || !ensure_init()) return;
-  if (!launch_forward(A, inputs[0]->dtype, where)) return;
+  if (!launch_forward(A, inputs[0]->dtype, nullptr, where)) return;
   finish(where);
 }
 
@@ -1500,9 +1513,12 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
     finish(where);
     return;
   }
-  A.stats = static_cast<float *>(partials(2 * N * sizeof(float), where));
-  if (!A.stats) return;
-  if (!launch_forward(A, x->dtype, where)) return;
+  // the statistics between the two, and the pieces of cut rows after them
+  const uint64_t stats = (2 * N * sizeof(float) + 255) / 256 * 256;
+  char *work = static_cast<char *>(partials(stats + pieces_bytes(N, A.vocab, float_bytes(x)), where));
+  if (!work) return;
+  A.stats = reinterpret_cast<float *>(work);
+  if (!launch_forward(A, x->dtype, work + stats, where)) return;
   launch_backward(A, x->dtype, false);
   finish(where);
 }

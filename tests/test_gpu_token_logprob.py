@@ -214,6 +214,24 @@ def test_strides_and_alignments(kind, vocab):
         check_gradient(s.dx(), want, kind, f"step {kind} {xs}")
 
 
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("rows", [1, 2, 40, 300])
+def test_step_over_rows_too_long_to_hold(kind, rows):
+    """The step's two passes: its statistics and the pieces of cut rows share one workspace."""
+    vocab = 70000 if kind == "f32" else 140003
+    rng = np.random.RandomState(rows)
+    x = special(logits(rng, rows, vocab, kind), kind)
+    tok = _tokens(rng, rows, vocab)
+    u, h = rng.randn(rows).astype(np.float32), rng.randn(rows).astype(np.float32)
+    want = exact(x, tok, 1.0, 0, u, h)
+    c = Case(x, kind, tok, 1.0, 0, u, h)
+    for k in range(3):
+        print(f"long step {kind} {rows}x{vocab} {k}", flush=True)
+        c.step()
+        check_values(c.values(), want, f"long step {kind} {rows}")
+        check_gradient(c.dx(), want, kind, f"long step {kind} {rows}")
+
+
 def test_broadcast_rows():
     """One row of logits for many tokens (stride 0): its gradient has rows of its own."""
     rng = np.random.RandomState(3)
