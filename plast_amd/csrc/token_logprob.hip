@@ -7,7 +7,8 @@
 //   log p_j = (x_j - m) / T - ln2 log2 s,  H = -sum_j p_j log p_j = ln2 (log2 s - w / s).
 // c m is rounded once and z_j = fma(c, x_j, -c m) once more: the first rounding, r = c m - round(c m),
 // moves every z_j alike, so p and H do not see it, and log p takes it out of log2 s again; the second is
-// relative to z_j itself, however large the logits are.
+// relative to z_j itself. r is at most half a step of c m: up to |c m| = kReach it is within 4 and 2^z_j in range;
+// beyond it z_j = c (x_j - m), whose difference is rounded relative to itself and r is 0.
 // Gradient for upstream u of log p[token] and h of H:
 //   dx_j = (u ([j = token] - p_j) - h p_j (log p_j + H)) / T
 //        = u / T [j = token] - 2^z_j (A + B z_j),
@@ -24,6 +25,9 @@ namespace {
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kRowBlock = 256;  // lanes of a workgroup
+// |c m| up to which c m and its rounding are used: a mask of -1e30 that a lane meets first, or that fills a row, has
+// an r of 1e22, and 2^r is no number. 2^27 leaves logits of 20 a temperature of 2.2e-7.
+constexpr float kReach = 0x1p27f;
 
 // Where row `r` of the leading axes starts, in elements, in x and in its gradient.
 struct RowMap {
@@ -63,12 +67,12 @@ struct TokenArgs {
   RowMap map;
 };
 
-// The exponent z of a logit. Where c m overflows, c (x - m) is taken instead.
+// The exponent z of a logit. Where c m is beyond kReach, c (x - m) is taken instead.
 struct RowRef {
   float c, m, cm;
   bool far;
   __device__ __forceinline__ RowRef(float c_, float m_) : c(c_), m(m_), cm(c_ * m_) {
-    far = !(fabsf(cm) < 1e38f);
+    far = !(fabsf(cm) < kReach);
   }
   __device__ __forceinline__ float z(float x) const {
     return far ? (x - m) * c : __builtin_fmaf(x, c, -cm);
@@ -119,10 +123,10 @@ __device__ __forceinline__ float unit_max(F f) {
 }
 
 // A lane's share of s and w, against a reference of its own that grows with the logits it meets: cm is
-// c times the largest so far, but at least -1e38, so that it stays finite (a row whose largest logit is not
-// in range is worked out by the exact path below).
+// c times the largest so far, but at least -kReach (a row whose largest logit is not in range is worked out by
+// the exact path below).
 struct Running {
-  float m = -kInf, cm = -1e38f, s = 0.0f, w = 0.0f;
+  float m = -kInf, cm = -kReach, s = 0.0f, w = 0.0f;
   __device__ __forceinline__ void refer(float to) {
     const float d = cm - to, f = __builtin_amdgcn_exp2f(d);
     w = f * __builtin_fmaf(d, s, w);
@@ -131,7 +135,7 @@ struct Running {
   }
   __device__ __forceinline__ void grow(float c, float g) {
     m = __builtin_elementwise_maximum(m, g);  // NaN stays
-    refer(fmaxf(c * m, -1e38f));
+    refer(fmaxf(c * m, -kReach));
   }
   // A logit's term, which the caller adds to s.
   __device__ __forceinline__ float term(float c, float x) {
@@ -159,7 +163,7 @@ __device__ __forceinline__ Running wave_join(Running r) {
   return r;
 }
 // Whether the running form holds for a row with this largest logit.
-__device__ __forceinline__ bool in_range(float c, float m) { return m == -kInf || fabsf(c * m) < 1e38f; }
+__device__ __forceinline__ bool in_range(float c, float m) { return m == -kInf || fabsf(c * m) < kReach; }
 
 // A logit's place in the order of alternatives: larger first, equal logits (both zeros too) by the
 // lower index, NaN above all. No key is 0.
@@ -242,46 +246,44 @@ __device__ __forceinline__ void put_top(const TokenArgs &A, uint32_t row, uint32
   A.top_logp[at] = key ? log_p(A, key_value(key), m, l0) : -kInf;
 }
 
-// The exact path, for rows with NaN, infinite or out-of-range logits and for alternatives that the list
-// could not hold: the maximum, then the sums, then an argmax per alternative, each a pass over the row.
+// The sums of a row with NaN, infinite or out-of-range logits, whose largest logit m the one pass has found (NaN
+// if one is): another pass, against m itself. Leaves m and l0, writes the row's results.
 template <class T, int W>
-__device__ __forceinline__ void exact_row(const TokenArgs &A, const T *x, uint32_t row, int32_t token, uint32_t gl,
-                                       RowLds<W> &L, bool stats, float m, float l0) {
+__device__ __forceinline__ void exact_sums(const TokenArgs &A, const T *x, uint32_t row, int32_t token, float x_token,
+                                           uint32_t gl, RowLds<W> &L, float &m, float &l0) {
+  constexpr uint32_t NL = 64 * W;
+  const uint32_t V = A.vocab;
+  const RowRef ref(A.c, m);
+  float s = 0.0f, w = 0.0f;
+  for (uint32_t j = gl; j < V; j += NL) {
+    const float z = ref.z(float(x[j])), e = __builtin_amdgcn_exp2f(z);
+    s += e;  // NaN for a NaN or a +inf logit
+    w = __builtin_fmaf(e, fmaxf(z, -FLT_MAX), w);
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    s += __shfl_xor(s, d);
+    w += __shfl_xor(w, d);
+  }
+  if constexpr (W > 1) {
+    row_sync<W>();
+    if (gl % 64 == 0) L.red[gl / 64][0] = s, L.red[gl / 64][1] = w;
+    row_sync<W>();
+    s = L.red[0][0], w = L.red[0][1];
+    for (int k = 1; k < W; ++k) s += L.red[k][0], w += L.red[k][1];
+  }
+  if (s != s) m = s;
+  l0 = log2f(s) - ref.shift();
+  if (gl == 0) row_out(A, row, token, x_token, m, s, w, ref.shift());
+}
+
+// The alternatives of a row with NaN or infinite logits, or of one that the list could not hold: an argmax each, a
+// pass over the row.
+template <class T, int W>
+__device__ __forceinline__ void exact_top(const TokenArgs &A, const T *x, uint32_t row, uint32_t gl, RowLds<W> &L, float m,
+                                          float l0) {
   constexpr uint32_t NL = 64 * W;
   const uint32_t V = A.vocab, wave = gl / 64;
-  const auto together = [&](float v, bool maximum) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      const float o = __shfl_xor(v, d);
-      v = maximum ? fmaxf(v, o) : v + o;
-    }
-    row_sync<W>();
-    if (gl % 64 == 0) L.red[wave][0] = v;
-    row_sync<W>();
-    v = L.red[0][0];
-    for (int k = 1; k < W; ++k) v = maximum ? fmaxf(v, L.red[k][0]) : v + L.red[k][0];
-    return v;
-  };
-  if (stats) {
-    m = -kInf;
-    for (uint32_t j = gl; j < V; j += NL) m = fmaxf(m, float(x[j]));
-    m = together(m, true);
-    const RowRef ref(A.c, m);
-    float s = 0.0f, w = 0.0f;
-    bool nan = false;
-    for (uint32_t j = gl; j < V; j += NL) {
-      const float v = float(x[j]);
-      nan = nan || v != v;
-      const float z = ref.z(v), e = __builtin_amdgcn_exp2f(z);
-      s += e;
-      w = __builtin_fmaf(e, fmaxf(z, -FLT_MAX), w);
-    }
-    s = together(nan ? __builtin_nanf("") : s, false);
-    w = together(w, false);
-    if (s != s) m = s;  // a NaN or an infinite logit
-    l0 = log2f(s) - ref.shift();
-    if (gl == 0) row_out(A, row, token, uint32_t(token) < V ? float(x[token]) : 0.0f, m, s, w, ref.shift());
-  }
   uint64_t last = ~uint64_t(0);
   for (uint32_t k = 0; k < A.top; ++k) {
     uint64_t best = 0;
@@ -697,22 +699,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
       if (found > kList) top.give_up();
     }
   }
-  const bool exact = !in_range(c, r.m);
-  if (exact || top.lost) {
-    const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
-    if (!exact && gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w, RowRef(c, r.m).shift());
-    exact_row<T, W>(A, x, row, token, gl, L, exact, r.m, l0);
-    return;
+  float m = r.m, l0;
+  if (!in_range(c, m)) {
+    exact_sums<T, W>(A, x, row, token, x_token, gl, L, m, l0);
+  } else {
+    const float shift = RowRef(c, m).shift();
+    l0 = log2f(r.s) - shift;
+    if (gl == 0) row_out(A, row, token, x_token, m, r.s, r.w, shift);
   }
-  if (gl == 0) row_out(A, row, token, x_token, r.m, r.s, r.w, RowRef(c, r.m).shift());
   if constexpr (TOP) {
-    const float l0 = log2f(r.s) - RowRef(c, r.m).shift();
+    if (m != m || top.lost) {
+      exact_top<T, W>(A, x, row, gl, L, m, l0);
+      return;
+    }
     for (uint32_t i = gl; i < found; i += NL) {
       const uint64_t key = L.list[top.cur][i];
       const uint32_t k = top.rank(key, found);
-      if (k < A.top) put_top(A, row, k, key, r.m, l0);
+      if (k < A.top) put_top(A, row, k, key, m, l0);
     }
-    if (gl >= found && gl < A.top) put_top(A, row, gl, 0, r.m, l0);
+    if (gl >= found && gl < A.top) put_top(A, row, gl, 0, m, l0);
   }
 }
 
