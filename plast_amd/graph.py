@@ -14,6 +14,9 @@ from . import abi
 from .abi import KernelParams
 from .runtime import DeviceTensor, lib
 
+# the first of an op's inputs that its forward writes: results beside the output, which later nodes may read
+WRITES_FROM = {"token_logprob": 2}
+
 
 class Graph:
     def __init__(self):
@@ -52,11 +55,13 @@ class Graph:
         n.params = p or KernelParams(0, 0, 0.0)
         self.nodes.append(n)
         output.t.creator = C.addressof(n)
+        for t in inputs[WRITES_FROM.get(op.lower(), len(inputs)):]:
+            t.t.creator = C.addressof(n)
         return output
 
     def build(self, root: DeviceTensor, fuse: bool = False) -> int:
-        """Topologically order the nodes reachable from root's creator (graph.c:30-39); with
-        fuse=True run the elementwise-chain pass. Returns the number of chains fused."""
+        """Topologically order the nodes reachable from root's creator (graph.c:30-39; a node whose results
+        are among its inputs is its own creator there and is not visited again); with fuse=True run the elementwise-chain pass. Returns the number of chains fused."""
         by_addr = {C.addressof(n): n for n in self.nodes}
         order: list[abi.Node] = []
         seen: set[int] = set()
