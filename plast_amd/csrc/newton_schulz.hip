@@ -17,9 +17,8 @@
 // product. The iteration in 64 bits is met to 4e-7 of the result at [256, 256] and [300, 800], where
 // fp32 factors (24 bits, but one rounding per addition) meet it to 1.5e-6 and 1.8e-6.
 //
-// Matrices of bfloat16 take hi alone, one instruction a product: bf16 keeps 8 bits of the input and of the result, so
-// factors of 11 stay below the rounding that the input already had. The result is off by 1.4e-3 before its own
-// rounding of 1.7e-3 (all in bf16: 1.1e-2), for a third of the arithmetic: 6 x 2605 x 1001 596 us instead of 1027.
+// All three types take pairs: with hi alone a bf16 matrix is off by 1.4e-3 before its own rounding (a norm of
+// 1.7e-3) instead of less than 1e-6.
 //
 // Layout of a factor ("lines"): each row is cut into lines of 128 bytes, a line holding 32 columns' hi
 // and then their lo: what a workgroup's tile needs of a row in one step of the sum is one whole line, read
@@ -30,7 +29,6 @@
 #include <cmath>
 #include <cstdlib>
 #include <mutex>
-#include <type_traits>
 #include <unordered_set>
 #include <vector>
 
@@ -158,13 +156,10 @@ struct Lines {
   char *data;
   uint64_t pitch, next;  // bytes from one row, one matrix to the next
 };
-// PL: 2 for pairs, 1 for hi alone, 64 columns a line.
-template <int PL>
 __device__ __forceinline__ char *line_at(const Lines &L, uint32_t b, uint32_t row, uint32_t col) {
-  return L.data + b * L.next + row * L.pitch + (PL == 2 ? (col >> 5) * 128 + (col & 31) * 2 : col * 2);
+  return L.data + b * L.next + row * L.pitch + (col >> 5) * 128 + (col & 31) * 2;
 }
 // Eight columns (a multiple of 8) of a row.
-template <int PL>
 __device__ __forceinline__ void put8(char *at, const float *v) {
   h8 hi, lo;
 #pragma unroll
@@ -173,24 +168,19 @@ __device__ __forceinline__ void put8(char *at, const float *v) {
     lo[e] = f16_t(v[e] - float(hi[e]));
   }
   *reinterpret_cast<h8 *>(at) = hi;
-  if constexpr (PL == 2) *reinterpret_cast<h8 *>(at + 64) = lo;
+  *reinterpret_cast<h8 *>(at + 64) = lo;
 }
-template <int PL>
 __device__ __forceinline__ void get8(const char *at, float *v) {
-  const h8 hi = *reinterpret_cast<const h8 *>(at);
-  h8 lo = f16_t(0.0f);
-  if constexpr (PL == 2) lo = *reinterpret_cast<const h8 *>(at + 64);
+  const h8 hi = *reinterpret_cast<const h8 *>(at), lo = *reinterpret_cast<const h8 *>(at + 64);
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = float(hi[e]) + float(lo[e]);
 }
-template <int PL>
 __device__ __forceinline__ float get1(const char *at) {
-  const float hi = float(*reinterpret_cast<const f16_t *>(at));
-  return PL == 2 ? hi + float(*reinterpret_cast<const f16_t *>(at + 64)) : hi;
+  return float(*reinterpret_cast<const f16_t *>(at)) + float(*reinterpret_cast<const f16_t *>(at + 64));
 }
 
 // X and X^T in lines from the source, a 64x64 tile per workgroup, padding included.
-template <class T, bool MUON, int PL>
+template <class T, bool MUON>
 __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, const double *part,
                                                          uint32_t parts, float eps, int growth,
                                                          float base, Lines X, Lines XT, float *xscale) {
@@ -230,8 +220,8 @@ __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, con
       v[k] = tile[r][c + k];
       w[k] = tile[c + k][r];
     }
-    put8<PL>(line_at<PL>(R, b, r0 + r, c0 + c), v);
-    put8<PL>(line_at<PL>(C, b, c0 + r, r0 + c), w);
+    put8(line_at(R, b, r0 + r, c0 + c), v);
+    put8(line_at(C, b, c0 + r, r0 + c), w);
   }
 }
 
@@ -281,18 +271,17 @@ __device__ __forceinline__ void tile_at(uint32_t t, uint32_t ti, uint32_t &i, ui
 struct Term {
   h8 hi[2], lo[2];
 };
-template <Mode M, int PL>
+template <Mode M>
 __device__ __forceinline__ Term load_term(const Product &P, uint32_t b, uint32_t i0, uint32_t j0) {
   const uint32_t lane = threadIdx.x & 63, r = lane / 2, c = lane % 2 * 16;
   Term t;
   if constexpr (M != Gram) {
     const bool tall = M == Final && P.o.rows > P.o.cols;
-    const char *at = tall ? line_at<PL>(P.in_t, b, j0 + r, i0 + c) : line_at<PL>(P.in, b, i0 + r, j0 + c);
+    const char *at = tall ? line_at(P.in_t, b, j0 + r, i0 + c) : line_at(P.in, b, i0 + r, j0 + c);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       t.hi[h] = reinterpret_cast<const h8 *>(at)[h];
-      if constexpr (PL == 2) t.lo[h] = reinterpret_cast<const h8 *>(at + 64)[h];
-      else t.lo[h] = f16_t(0.0f);
+      t.lo[h] = reinterpret_cast<const h8 *>(at + 64)[h];
     }
   }
   return t;
@@ -301,7 +290,7 @@ __device__ __forceinline__ Term load_term(const Product &P, uint32_t b, uint32_t
 // A block of 32x32 sums as the matrix unit leaves it: register r of a lane holds row
 // 8 (r / 4) + 4 (lane / 32) + r % 4 of column lane % 32. It goes through LDS, so that rows and columns
 // both leave as whole lines.
-template <class T, Mode M, bool MUON, int PL>
+template <class T, Mode M, bool MUON>
 __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, float *lds, f16v acc, const Term &term,
                                           uint32_t b, uint32_t i0, uint32_t j0, bool mirror) {
   const uint32_t lane = threadIdx.x & 63;
@@ -354,11 +343,11 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
         if constexpr (M != Gram) v[e] = __builtin_fmaf(beta, float(term.hi[h][e]) + float(term.lo[h][e]), v[e]);
       }
       if (M == Square && P.in2.data) {
-        get8<PL>(line_at<PL>(P.in2, b, i0 + r, j0 + c + 8 * h), t);
+        get8(line_at(P.in2, b, i0 + r, j0 + c + 8 * h), t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(P.gamma, t[e], v[e]);
       }
-      put8<PL>(line_at<PL>(P.out, b, i0 + r, j0 + c + 8 * h), v);
+      put8(line_at(P.out, b, i0 + r, j0 + c + 8 * h), v);
       if (M != Gram && mirror)  // the transpose's lines take the same sums
 #pragma unroll
         for (int e = 0; e < 8; ++e) lds[r * 33 + c + 8 * h + e] = v[e];
@@ -370,7 +359,7 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = lds[(c + 8 * h + e) * 33 + r];
-        put8<PL>(line_at<PL>(P.out_t, b, j0 + r, i0 + c + 8 * h), v);
+        put8(line_at(P.out_t, b, j0 + r, i0 + c + 8 * h), v);
       }
     }
   }
@@ -385,7 +374,7 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
 // five half-line stages, four of them on their way, measured the same within 2%, with 4096 x 4096 in 4.28 ms and 4.30: the
 // matrix units are at 1.1 PFLOP/s of fp16 in the long sums, what a large library product reaches here, and in the
 // short ones wait for the tiles' ways out, when all workgroups store at once (24 x 1024 x 1024: 35% busy).
-template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
+template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Product P, MuonSet S) {
   constexpr int NW = (BM / WM) * (BN / WN), LOADS = (BM + BN) / 8 / NW, FA = WM / 32, FB = WN / 32;
   constexpr uint32_t STAGE = (BM + BN) * 128;
@@ -438,10 +427,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
     const char *base = lds + stage * STAGE;
     const uint32_t row = lane % 32, key = (row >> 1) & 7;
 #pragma unroll
-    for (int g = 0; g < 4 / PL; ++g) {  // 16 columns each
-      h8 ua[FA][PL], vb[FB][PL];
+    for (int g = 0; g < 2; ++g) {  // 16 columns each
+      h8 ua[FA][2], vb[FB][2];
 #pragma unroll
-      for (int p = 0; p < PL; ++p) {
+      for (int p = 0; p < 2; ++p) {
         const uint32_t unit = ((p * 4 + g * 2 + lane / 32) ^ key) * 16;
 #pragma unroll
         for (int a = 0; a < FA; ++a)
@@ -451,7 +440,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
           vb[c][p] = *reinterpret_cast<const h8 *>(base + (BM + wj + c * 32 + row) * 128 + unit);
       }
 #pragma unroll
-      for (int q = 0; q < (PL == 2 ? 3 : 1); ++q)
+      for (int q = 0; q < 3; ++q)
 #pragma unroll
         for (int a = 0; a < FA; ++a)
 #pragma unroll
@@ -473,19 +462,19 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Pro
                                                acc[a][c][4 * q + 3]};
     return;
   }
-  Term next = load_term<M, PL>(P, b, i0, j0);
+  Term next = load_term<M>(P, b, i0, j0);
   __syncthreads();  // the stages become the blocks' way out
   float *way = reinterpret_cast<float *>(lds) + wave * kBlockLds;
 #pragma unroll
   for (int k = 0; k < FA * FB; ++k) {
     const Term term = next;  // the next block's is on its way while this one leaves
-    if (k + 1 < FA * FB) next = load_term<M, PL>(P, b, i0 + (k + 1) / FB * 32, j0 + (k + 1) % FB * 32);
-    put_block<T, M, MUON, PL>(P, S, way, acc[k / FB][k % FB], term, b, i0 + k / FB * 32, j0 + k % FB * 32, !sym || ti != tj);
+    if (k + 1 < FA * FB) next = load_term<M>(P, b, i0 + (k + 1) / FB * 32, j0 + (k + 1) % FB * 32);
+    put_block<T, M, MUON>(P, S, way, acc[k / FB][k % FB], term, b, i0 + k / FB * 32, j0 + k % FB * 32, !sym || ti != tj);
   }
 }
 
 // Adds the pieces of a sum: a wave per 32x32 block.
-template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
+template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
   constexpr int FA = WM / 32, FB = WN / 32, NB = (BM / 32) * (BN / 32);
   __shared__ float lds[kNsBlock / 64 * kBlockLds];
@@ -498,7 +487,7 @@ __global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
   tile_at<M>(t, P.ti, ti, tj);
   const uint32_t w = block / (FA * FB), a = block % (FA * FB) / FB, c = block % FB;
   const uint32_t i0 = ti * BM + w / (BN / WN) * WM + a * 32, j0 = tj * BN + w % (BN / WN) * WN + c * 32;
-  const Term term = load_term<M, PL>(P, b, i0, j0);
+  const Term term = load_term<M>(P, b, i0, j0);
   f16v acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
@@ -512,14 +501,14 @@ __global__ __launch_bounds__(kNsBlock) void join_kernel(Product P, MuonSet S) {
       for (int e = 0; e < 4; ++e) acc[4 * q + e] += v[e];
     }
   }
-  put_block<T, M, MUON, PL>(P, S, lds + wave * kBlockLds, acc, term, b, i0, j0, !sym || ti != tj);
+  put_block<T, M, MUON>(P, S, lds + wave * kBlockLds, acc, term, b, i0, j0, !sym || ti != tj);
 }
 
 // Small products: a workgroup per 32x32 tile, whose eight waves each take a share of the sum straight from memory (a
 // tile's factors are read by few others) and meet in LDS. One launch a product, where tiles of 64 leave most of the
 // chip idle or need a second launch to join pieces.
 constexpr int kSmallWaves = 8;
-template <class T, Mode M, bool MUON, int PL>
+template <class T, Mode M, bool MUON>
 __global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product P, MuonSet S) {
   __shared__ float lds[kSmallWaves][kBlockLds];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -538,23 +527,23 @@ __global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product
   const uint32_t row8 = (half ? j0 : i0) + e8 / 4, col8 = (half ? i0 : j0) + e8 % 4 * 8;
   float term[8];
   if constexpr (M == Square || M == Update)
-    if (stores) get8<PL>(line_at<PL>(half ? P.in_t : P.in, b, row8, col8), term);
+    if (stores) get8(line_at(half ? P.in_t : P.in, b, row8, col8), term);
   f16v acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
   for (uint32_t line = first; line < last; ++line) {
-    h8 ua[4 / PL][PL], vb[4 / PL][PL];
+    h8 ua[2][2], vb[2][2];
 #pragma unroll
-    for (int p = 0; p < PL; ++p)
+    for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int g = 0; g < 4 / PL; ++g) {
+      for (int g = 0; g < 2; ++g) {
         ua[g][p] = *reinterpret_cast<const h8 *>(u + line * 128 + p * 64 + g * 32);
         vb[g][p] = *reinterpret_cast<const h8 *>(v + line * 128 + p * 64 + g * 32);
       }
 #pragma unroll
-    for (int g = 0; g < 4 / PL; ++g)
+    for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int q = 0; q < (PL == 2 ? 3 : 1); ++q)
+      for (int q = 0; q < 3; ++q)
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ua[g][q == 2], vb[g][q == 1], acc, 0, 0, 0);
   }
 #pragma unroll
@@ -583,8 +572,8 @@ __global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product
     for (uint32_t e = threadIdx.x; e < 32 * 32; e += 64 * kSmallWaves) {
       const uint32_t q = e / 32, k = e % 32;
       const uint32_t row = (tall ? j0 : i0) + q, col = (tall ? i0 : j0) + k;
-      const char *at = tall ? line_at<PL>(P.in_t, b, j0 + q, i0 + k) : line_at<PL>(P.in, b, i0 + q, j0 + k);
-      const float term = get1<PL>(at);
+      const char *at = tall ? line_at(P.in_t, b, j0 + q, i0 + k) : line_at(P.in, b, i0 + q, j0 + k);
+      const float term = get1(at);
       const float r = __builtin_fmaf(beta, term, alpha * (tall ? tile[k * 33 + q] : tile[q * 33 + k]));
       if (row >= P.o.rows || col >= P.o.cols) continue;
       if constexpr (MUON) {
@@ -605,22 +594,22 @@ __global__ __launch_bounds__(64 * kSmallWaves) void small_product_kernel(Product
       if constexpr (M != Gram) w[k] = __builtin_fmaf(beta, term[k], w[k]);
     }
     if (M == Square && P.in2.data) {
-      get8<PL>(line_at<PL>(P.in2, b, row8, col8), x);
+      get8(line_at(P.in2, b, row8, col8), x);
 #pragma unroll
       for (int k = 0; k < 8; ++k) w[k] = __builtin_fmaf(P.gamma, x[k], w[k]);
     }
-    put8<PL>(line_at<PL>(half ? P.out_t : P.out, b, row8, col8), w);
+    put8(line_at(half ? P.out_t : P.out, b, row8, col8), w);
   }
 }
 
 // No steps: the result is X.
-template <class T, bool MUON, int PL>
+template <class T, bool MUON>
 __global__ __launch_bounds__(kNsBlock) void copy_out_kernel(Lines X, Lines XT, const float *xscale, Stack O,
                                                             MuonSet S) {
   const uint32_t b = blockIdx.z, i = blockIdx.y, j = blockIdx.x * kNsBlock + threadIdx.x;
   if (j >= O.cols) return;
-  const char *at = line_at<PL>(O.rows > O.cols ? XT : X, b, i, j);
-  const float v = get1<PL>(at) / xscale[b];
+  const char *at = line_at(O.rows > O.cols ? XT : X, b, i, j);
+  const float v = get1(at) / xscale[b];
   if constexpr (MUON) {
     float *p = S.p[b] + uint64_t(i) * O.cols + j;
     *p = *p * S.rule.keep - S.rule.scale * v;
@@ -640,7 +629,6 @@ struct Tiling {
 struct Plan {
   uint32_t m, n, mp, np;  // extents, and padded to whole tiles
   Tiling gram, square, update;
-  uint32_t planes;  // of a factor
   bool pairs;       // steps go by pairs
   Scales scale;
 };
@@ -717,9 +705,8 @@ RuleRange range_of(const NewtonSchulz &r) {
   return range;
 }
 
-Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz &rule, uint32_t planes) {
+Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz &rule) {
   Plan p;
-  p.planes = planes;
   p.m = rows < cols ? rows : cols;
   p.n = rows < cols ? cols : rows;
   // 256 wide tiles read each factor least often, 128 wide ones leave fewer workgroups without work: 4096 x 4096 4.39
@@ -729,15 +716,15 @@ Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz 
   const uint32_t tile = p.m > 2048 && work >= uint64_t(1) << 23 ? 256 : p.m > 128 && work >= uint64_t(3) << 20 ? 128 : 64;
   // Two steps at once cost three more m x m products and one product of X X^T and one update of X less: 1.5 m^2 n
   // multiplications less for 1.5 m^3 more, and one launch more (4096 x 16384: 13.6 -> 10.4 ms, 6 x 2605 x 1001 in fp32 1.34 ->
-  // 1.18; under 2^30 the launch costs more). With factors of 11 bits the two would cost accuracy, 2.5e-3 for 1.4e-3.
+  // 1.18; under 2^30 the launch costs more).
   const RuleRange range = range_of(rule);
   p.scale = range.scale;
-  p.pairs = range.pairs && planes == 2 && rule.steps >= 2 && uint64_t(p.m) * p.m * (p.n - p.m) * count >= uint64_t(1) << 30;
+  p.pairs = range.pairs && rule.steps >= 2 && uint64_t(p.m) * p.m * (p.n - p.m) * count >= uint64_t(1) << 30;
   p.mp = round_up(p.m, tile);
   p.np = round_up(p.n, tile);
-  p.gram = tiling(tile, p.mp, p.mp, true, count, p.np * planes / 64);
-  p.square = tiling(tile, p.mp, p.mp, true, count, p.mp * planes / 64);
-  p.update = tiling(tile, p.mp, p.np, false, count, p.mp * planes / 64);
+  p.gram = tiling(tile, p.mp, p.mp, true, count, p.np / 32);
+  p.square = tiling(tile, p.mp, p.mp, true, count, p.mp / 32);
+  p.update = tiling(tile, p.mp, p.np, false, count, p.mp / 32);
   return p;
 }
 
@@ -754,40 +741,40 @@ uint64_t ns_bytes(const Plan &p, uint64_t count) {
   need(p.square, p.mp, p.mp, true);
   need(p.update, p.mp, p.np, false);
   return count * (kNormParts * 8 + 128 + 4 * part +
-                  2 * p.planes * (4 * uint64_t(p.mp) * p.np + (p.pairs ? 4 : 2) * uint64_t(p.mp) * p.mp));
+                  4 * (4 * uint64_t(p.mp) * p.np + (p.pairs ? 4 : 2) * uint64_t(p.mp) * p.mp));
 }
 
-template <class T, Mode M, bool MUON, int PL, int BM, int BN, int WM, int WN>
+template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
 void launch_product(const Product &P, const MuonSet &S, uint32_t count) {
   constexpr int NW = (BM / WM) * (BN / WN);
   const uint32_t tiles = (M == Gram || M == Square ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj) * count;
-  product_kernel<T, M, MUON, PL, BM, BN, WM, WN><<<tiles * P.parts, 64 * NW, 0, stream()>>>(P, S);
+  product_kernel<T, M, MUON, BM, BN, WM, WN><<<tiles * P.parts, 64 * NW, 0, stream()>>>(P, S);
   if (P.parts > 1)
-    join_kernel<T, M, MUON, PL, BM, BN, WM, WN>
+    join_kernel<T, M, MUON, BM, BN, WM, WN>
         <<<tiles * (BM / 32) * (BN / 32) / (kNsBlock / 64), kNsBlock, 0, stream()>>>(P, S);
 }
-template <class T, Mode M, bool MUON, int PL>
+template <class T, Mode M, bool MUON>
 void product(const Plan &plan, const Tiling &how, Product &P, const MuonSet &S, uint32_t count) {
   P.parts = how.parts;
   P.ti = plan.mp / how.tile;
   P.tj = (M == Gram || M == Square ? plan.mp : plan.np) / how.tile;
   if (how.tile == 32) {
     const uint32_t tiles = (M == Gram || M == Square ? P.ti * (P.ti + 1) / 2 : P.ti * P.tj) * count;
-    small_product_kernel<T, M, MUON, PL><<<tiles, 64 * kSmallWaves, 0, stream()>>>(P, S);
+    small_product_kernel<T, M, MUON><<<tiles, 64 * kSmallWaves, 0, stream()>>>(P, S);
   } else if (how.tile == 256) {
-    launch_product<T, M, MUON, PL, 256, 256, 128, 64>(P, S, count);
+    launch_product<T, M, MUON, 256, 256, 128, 64>(P, S, count);
   } else if (how.tile == 128) {
-    launch_product<T, M, MUON, PL, 128, 128, 64, 64>(P, S, count);
+    launch_product<T, M, MUON, 128, 128, 64, 64>(P, S, count);
   } else {
-    launch_product<T, M, MUON, PL, 64, 64, 32, 32>(P, S, count);
+    launch_product<T, M, MUON, 64, 64, 32, 32>(P, S, count);
   }
 }
 
 // The iteration over `count` matrices: from G into O, or of a Muon set into its parameters.
-template <class T, bool MUON, int PL>
+template <class T, bool MUON>
 void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S, uint32_t count,
              const NewtonSchulz &rule, void *work) {
-  const uint64_t mn = 2 * PL * uint64_t(plan.mp) * plan.np, mm = 2 * PL * uint64_t(plan.mp) * plan.mp;
+  const uint64_t mn = 4 * uint64_t(plan.mp) * plan.np, mm = 4 * uint64_t(plan.mp) * plan.mp;
   double *norms = static_cast<double *>(work);
   float *xscale = reinterpret_cast<float *>(norms + uint64_t(count) * kNormParts);
   char *at = static_cast<char *>(work) + uint64_t(count) * (kNormParts * 8 + 128);
@@ -796,11 +783,11 @@ void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S,
     at += count * bytes;
     return l;
   };
-  Lines x = take(mn, 2 * PL * uint64_t(plan.np)), y = take(mn, 2 * PL * uint64_t(plan.np));
-  Lines xt = take(mn, 2 * PL * uint64_t(plan.mp)), yt = take(mn, 2 * PL * uint64_t(plan.mp));
-  const Lines a = take(mm, 2 * PL * uint64_t(plan.mp)), s = take(mm, 2 * PL * uint64_t(plan.mp));
-  const Lines pa = plan.pairs ? take(mm, 2 * PL * uint64_t(plan.mp)) : Lines{};
-  const Lines s2 = plan.pairs ? take(mm, 2 * PL * uint64_t(plan.mp)) : Lines{};
+  Lines x = take(mn, 4 * uint64_t(plan.np)), y = take(mn, 4 * uint64_t(plan.np));
+  Lines xt = take(mn, 4 * uint64_t(plan.mp)), yt = take(mn, 4 * uint64_t(plan.mp));
+  const Lines a = take(mm, 4 * uint64_t(plan.mp)), s = take(mm, 4 * uint64_t(plan.mp));
+  const Lines pa = plan.pairs ? take(mm, 4 * uint64_t(plan.mp)) : Lines{};
+  const Lines s2 = plan.pairs ? take(mm, 4 * uint64_t(plan.mp)) : Lines{};
   float *partial = reinterpret_cast<float *>(at);
 
   const uint64_t size = uint64_t(G.rows) * G.cols;
@@ -813,23 +800,23 @@ void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S,
   const int growth = int(most_growth < 110.0f ? most_growth : 110.0f);
   const bool tall = G.rows > G.cols;
   const dim3 grid((tall ? plan.mp : plan.np) / 64, (tall ? plan.np : plan.mp) / 64, count);
-  start_kernel<T, MUON, PL><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, growth, plan.scale.x, x, xt, xscale);
+  start_kernel<T, MUON><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, growth, plan.scale.x, x, xt, xscale);
   const float sa = plan.scale.a, ss = plan.scale.s;
   Product P;
   memset(&P, 0, sizeof P);
   P.partial = partial;
   P.xscale = xscale;
   const auto gram = [&] {
-    P.u = P.v = x, P.out = P.out_t = a, P.lines = plan.np * PL / 64, P.alpha = sa;
-    product<float, Gram, false, PL>(plan, plan.gram, P, S, count);
+    P.u = P.v = x, P.out = P.out_t = a, P.lines = plan.np / 32, P.alpha = sa;
+    product<float, Gram, false>(plan, plan.gram, P, S, count);
   };
   // to = coef u v + beta in + gamma in2, of scales su, sv, so, si and s2
   const auto square = [&](const Lines &to, float so, float coef, const Lines &u, float su, const Lines &v, float sv,
                           float beta, const Lines &in, float si, float gamma = 0.0f, Lines in2 = Lines{}, float s2 = 1.0f) {
     P.u = u, P.v = v, P.in = P.in_t = in, P.in2 = in2, P.out = P.out_t = to;
-    P.lines = plan.mp * PL / 64;
+    P.lines = plan.mp / 32;
     P.alpha = coef * (so / (su * sv)), P.beta = beta * (so / si), P.gamma = gamma * (so / s2);
-    product<float, Square, false, PL>(plan, plan.square, P, S, count);
+    product<float, Square, false>(plan, plan.square, P, S, count);
   };
   for (int k = 0; k < rule.steps;) {
     const int steps = plan.pairs && k + 2 <= rule.steps ? 2 : 1;
@@ -846,20 +833,20 @@ void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S,
       identity *= rule.a;
     }
     k += steps;
-    P.u = q, P.v = P.in_t = xt, P.in = x, P.out = y, P.out_t = yt, P.lines = plan.mp * PL / 64;
+    P.u = q, P.v = P.in_t = xt, P.in = x, P.out = y, P.out_t = yt, P.lines = plan.mp / 32;
     P.alpha = 1.0f / ss, P.beta = identity;
     if (k < rule.steps) {
-      product<float, Update, false, PL>(plan, plan.update, P, S, count);
+      product<float, Update, false>(plan, plan.update, P, S, count);
       Lines z = x;
       x = y, y = z;
       z = xt, xt = yt, yt = z;
     } else {
       P.o = O;
-      product<T, Final, MUON, PL>(plan, plan.update, P, S, count);
+      product<T, Final, MUON>(plan, plan.update, P, S, count);
     }
   }
   if (rule.steps == 0)
-    copy_out_kernel<T, MUON, PL><<<dim3(ceil_div(O.cols, kNsBlock), O.rows, count), kNsBlock, 0, stream()>>>(x, xt, xscale, O, S);
+    copy_out_kernel<T, MUON><<<dim3(ceil_div(O.cols, kNsBlock), O.rows, count), kNsBlock, 0, stream()>>>(x, xt, xscale, O, S);
 }
 
 bool check_rule(const NewtonSchulz *r, const char *where) {
@@ -1003,7 +990,7 @@ void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule) {
   }
   if (numel(g) == 0 || !ensure_init()) return;
   const uint64_t share = stack_share(count, G.rows, G.cols), item = float_bytes(g);
-  const Plan plan = make_plan(G.rows, G.cols, share, *rule, g->dtype == BFLOAT16 ? 1 : 2);
+  const Plan plan = make_plan(G.rows, G.cols, share, *rule);
   void *work = workspace(ns_bytes(plan, share));
   if (!work) return;
   MuonSet none;
@@ -1014,8 +1001,7 @@ void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule) {
     Ob.data = static_cast<const char *>(O.data) + int64_t(b) * O.sb * int64_t(item);
     with_float_type(g->dtype, [&](auto t) {
       typedef decltype(t) T;
-      iterate<T, false, std::is_same_v<T, bf16_t> ? 1 : 2>(plan, Gb, Ob, none, uint32_t(count - b < share ? count - b : share), *rule,
-                                  work);
+      iterate<T, false>(plan, Gb, Ob, none, uint32_t(count - b < share ? count - b : share), *rule, work);
     });
   }
   finish(where);
@@ -1068,7 +1054,7 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
     const uint32_t rows = uint32_t(first->shape[0]), cols = uint32_t(first->shape[1]);
     g.share = stack_share(g.which.size(), rows, cols);
     if (g.share > kPointers) g.share = kPointers;
-    g.plan = make_plan(rows, cols, g.share, optimizer->rule, 2);
+    g.plan = make_plan(rows, cols, g.share, optimizer->rule);
     const uint64_t need = ns_bytes(g.plan, g.share);
     bytes = need > bytes ? need : bytes;
     groups.push_back(std::move(g));
@@ -1094,7 +1080,7 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
         S.g[j] = static_cast<const float *>(parameters[at]->grad->data);
         S.m[j] = static_cast<float *>(optimizer->m[at]->data);
       }
-      iterate<float, true, 2>(group.plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
+      iterate<float, true>(group.plan, shape, shape, S, uint32_t(c), optimizer->rule, work);
     }
   }
   finish(where);
