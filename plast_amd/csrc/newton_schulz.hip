@@ -904,23 +904,6 @@ bool matrix_stack(const Tensor *t, Stack &S, uint64_t &count, const char *name, 
   return true;
 }
 
-// Whether two elements of t can lie at one address: an axis of several elements, in order of their
-// strides, steps no further than what the ones below it span.
-bool overlapping(const Tensor *t) {
-  uint64_t need = 1;
-  bool done[PLAST_MAX_NDIM] = {};
-  for (uint64_t k = 0; k < t->ndim; ++k) {
-    uint64_t at = t->ndim;
-    for (uint64_t d = 0; d < t->ndim; ++d)
-      if (!done[d] && (at == t->ndim || t->strides[d] < t->strides[at])) at = d;
-    done[at] = true;
-    if (t->shape[at] <= 1) continue;
-    if (t->strides[at] < need) return true;
-    need = t->strides[at] * t->shape[at];
-  }
-  return false;
-}
-
 // ------------------------------------------------------------------------- Muon
 
 // Moment arrays that the library made (freed by plast_hip_muon_release).
