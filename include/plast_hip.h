@@ -119,7 +119,7 @@ PLAST_HIP_KERNEL_PAIR(log_softmax)
  * (-1, -inf) and a zero gradient. A token of at least the row's length has logp NaN and a NaN
  * gradient. A row of -inf alone has logp -inf, entropy 0 and a zero gradient; a NaN or +inf logit
  * makes its row NaN. Rows shorter than top are filled up with (-1, -inf).
- * Backward, x->grad of x's type and shape (any leading strides):
+ * Backward, x->grad of x's type and shape (any leading strides whose rows do not overlap):
  *   dx[j] (+)= (u ((j == token) - p[j]) - h p[j] (log p[j] + H)) / T
  * for upstream u of logp and h of the entropy H. */
 #define PLAST_TOP_MAX 32

@@ -1228,11 +1228,10 @@ bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *t
       report_error(where, "the gradient of x must have x's type and shape and a contiguous last axis");
       return false;
     }
-    for (int d = 0; d < s.rank; ++d)
-      if (x->shape[d] > 1 && dx->strides[d] < V) {
-        report_error(where, "rows of x's gradient overlap along axis %d", d);
-        return false;
-      }
+    if (overlapping(dx)) {
+      report_error(where, "rows of x's gradient overlap");
+      return false;
+    }
   }
   if (n) collapse(s);
   A.x = x->data;
