@@ -115,7 +115,7 @@ PLAST_HIP_KERNEL_PAIR(log_softmax)
  * the backward overwrite x->grad, 0 accumulate into it.
  *   logp = log p[token], entropy = -sum p log p, the alternatives' ids and log p in descending
  *   order of their logits (equal logits: the lower id first; NaN above all).
- * A negative token marks padding: the row is not read, and gets logp 0, entropy 0, alternatives
+ * A negative token marks padding: whatever its row holds, it gets logp 0, entropy 0, alternatives
  * (-1, -inf) and a zero gradient. A token of at least the row's length has logp NaN and a NaN
  * gradient. A row of -inf alone has logp -inf, entropy 0 and a zero gradient; a NaN or +inf logit
  * makes its row NaN. Rows shorter than top are filled up with (-1, -inf).

@@ -63,3 +63,23 @@ def test_gradient_and_step_under_finite_masks(kind, rows, vocab):
         s = Case(x, kind, tok, temp, 0, u, h).step()
         check_values(s.values(), want, f"step {kind} {rows}x{vocab} {temp}")
         check_gradient(s.dx(), want, kind, f"step {kind} {rows}x{vocab} {temp}")
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("rows, vocab", [(60, 18), (60, 300), (60, 20011), (1100, 20000), (600, 9001), (2, 131072),
+                                         (60, 140003)])
+def test_padding_whatever_its_rows_hold(kind, rows, vocab):
+    rng = np.random.RandomState(rows + vocab)
+    x, tok = logits(rng, rows, vocab, kind), rng.randint(0, vocab, rows)
+    tok[::2] = [-1, -2 ** 31][rows % 4 // 2]
+    x[::2] = np.resize(np.array([np.nan, np.inf, -np.inf, 1e4], np.float32), (len(x[::2]), vocab))
+    u, h = rng.randn(rows).astype(np.float32), rng.randn(rows).astype(np.float32)
+    print(f"padding {kind} {rows}x{vocab}", flush=True)
+    want = exact(x, tok, 1.0, 4, u, h)
+    assert not want["dx"][::2].any() and not want["logp"][::2].any() and not want["entropy"][::2].any()
+    c = Case(x, kind, tok, 1.0, 4, u, h).forward().backward()
+    check_values(c.values(), want, f"padding {kind}")
+    check_gradient(c.dx(), want, kind, f"padding {kind}")
+    s = Case(x, kind, tok, 1.0, 0, u, h).step()
+    check_values(s.values(), want, f"padding step {kind}")
+    check_gradient(s.dx(), want, kind, f"padding step {kind}")
