@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/plast_hip.h"
 #include "launch_rules.hpp"
@@ -419,6 +420,15 @@ bool broadcast_shape(const Tensor *a, const Tensor *b, uint64_t *shape, int *ran
 uint64_t numel(const Tensor *t);
 bool same_shape(const Tensor *a, const Tensor *b);
 inline bool is_half(const Tensor *t) { return t->dtype == FLOAT16 || t->dtype == BFLOAT16; }
+// The fp32 ops' check of what they write or accumulate into (nulls pass): 16-bit tensors hold half the bytes.
+inline bool no_half(std::initializer_list<const Tensor *> tensors, const char *where) {
+  for (const Tensor *t : tensors)
+    if (t && is_half(t)) {
+      report_error(where, "a result or gradient has the 16-bit dtype %d", int(t->dtype));
+      return false;
+    }
+  return true;
+}
 // Row-major contiguity with every stride checked (size-1 axes ignored).
 bool contiguous(const Tensor *t);
 

@@ -164,8 +164,10 @@ bool grad_pair(const Tensor *a, const Tensor *b, const Tensor *g, uint64_t simd)
 
 template <Bin OP>
 void binary_backward(Tensor **in, const Tensor *out, const char *where) {
-  if (!ensure_init()) return;
   const Tensor *a = in[0], *b = in[1];
+  if (!no_half({out->grad, a->requires_grad ? a->grad : nullptr, b->requires_grad ? b->grad : nullptr}, where) ||
+      !ensure_init())
+    return;
   if (!check_f32(a, where) || !check_f32(b, where)) return;
   if (!out->grad) {
     report_error(where, "output has no gradient");
@@ -214,9 +216,9 @@ void unary_forward(const Tensor **in, Tensor *out, KernelParams p, const char *w
 
 template <Un OP>
 void unary_backward(Tensor **in, const Tensor *out, KernelParams p, const char *where) {
-  if (!ensure_init()) return;
   const Tensor *a = in[0];
   if (!a->requires_grad || !a->grad) return;
+  if (!no_half({a->grad, out->grad}, where) || !ensure_init()) return;
   if (!check_f32(a, where)) return;
   if (!out->grad) {
     report_error(where, "output has no gradient");
@@ -272,13 +274,9 @@ void view_like_forward(const Tensor **in, Tensor *out) {
 }
 
 void view_like_backward(Tensor **in, const Tensor *out, const char *where) {
-  if (!ensure_init()) return;
   Tensor *a = in[0];
   if (!a->requires_grad || !out->grad || !a->grad) return;
-  if (is_half(a->grad) || is_half(out->grad)) {
-    report_error(where, "gradients of 16-bit views are not accumulated");
-    return;
-  }
+  if (!no_half({a->grad, out->grad}, where) || !ensure_init()) return;
   reshape_accumulate(static_cast<float *>(a->grad->data),
                      static_cast<const float *>(out->grad->data), numel(a), where);
   finish(where);
@@ -398,10 +396,7 @@ void transpose_hip_forward(const Tensor **inputs, Tensor *output, KernelParams p
 void transpose_hip_backward(Tensor **inputs, const Tensor *output, KernelParams params) {
   Tensor *a = inputs[0];
   if (!a->requires_grad || !output->grad || !a->grad) return;
-  if (is_half(a->grad) || is_half(output->grad)) {
-    report_error("transpose_hip_backward", "gradients of 16-bit views are not accumulated");
-    return;
-  }
+  if (!no_half({a->grad, output->grad}, "transpose_hip_backward")) return;
   transpose_backward_hip(static_cast<float *>(a->grad->data),
                          static_cast<const float *>(output->grad->data), a->shape,
                          a->grad->strides, output->grad->strides, a->ndim, params.dim,

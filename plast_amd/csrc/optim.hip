@@ -166,7 +166,9 @@ __global__ __launch_bounds__(kOptBlock<OPT>) void opt_table_kernel(OptScalars S,
                     E.vec != 0, b - E.first_block);
 }
 
-bool f32_param(const Tensor *t) { return t && t->grad && t->dtype == FLOAT32 && t->grad->data && t->data; }
+bool f32_param(const Tensor *t) {
+  return t && t->grad && t->dtype == FLOAT32 && !is_half(t->grad) && t->grad->data && t->data;
+}
 
 // The device copy of the last table of more than kGroup entries (see OptTableCache).
 std::mutex g_table_mu;
@@ -351,9 +353,9 @@ void adam_like_step(OptT *o, Tensor **params, int count, const char *where) {
   }
   for (int k = 0; k < count; ++k) {
     if (!params[k] || !params[k]->grad) continue;
-    if (!o->m[k] || !o->v[k] || numel(o->m[k]) != numel(params[k]) ||
-        numel(o->v[k]) != numel(params[k])) {
-      report_error(where, "moment tensors of parameter %d are missing or mis-sized", k);
+    if (!o->m[k] || !o->v[k] || numel(o->m[k]) != numel(params[k]) || numel(o->v[k]) != numel(params[k]) ||
+        is_half(o->m[k]) || is_half(o->v[k])) {
+      report_error(where, "moment tensors of parameter %d are missing, mis-sized or of 16 bits", k);
       return;
     }
   }

@@ -55,7 +55,7 @@ bool dims_ok(const Tensor *a, KernelParams p, const char *where) {
 template <class Comb>
 void reduce_forward(const Tensor **in, Tensor *out, KernelParams p, Post post,
                     const char *where) {
-  if (!ensure_init()) return;
+  if (!no_half({out}, where) || !ensure_init()) return;
   const Tensor *a = in[0];
   if (!dims_ok(a, p, where)) return;
   const bool keep = p.keepdim != 0;
@@ -82,9 +82,9 @@ void reduce_forward(const Tensor **in, Tensor *out, KernelParams p, Post post,
 // da += dc (/ n) broadcast back over the reduced axis (reduce_ops.c:89-154).
 void sum_mean_backward(Tensor **in, const Tensor *out, KernelParams p, bool mean,
                        const char *where) {
-  if (!ensure_init()) return;
   Tensor *a = in[0];
   if (!a->requires_grad || !a->grad) return;
+  if (!no_half({out, a->grad, out->grad}, where) || !ensure_init()) return;
   if (!dims_ok(a, p, where)) return;
   if (!out->grad) {
     report_error(where, "output has no gradient");
@@ -273,9 +273,9 @@ bool ext_backward_rows(const Tensor *a, const Tensor *out, uint64_t dim, const i
 
 template <bool IS_MAX>
 void ext_backward(Tensor **in, const Tensor *out, KernelParams p, const char *where) {
-  if (!ensure_init()) return;
   Tensor *a = in[0];
   if (!a->requires_grad || !a->grad) return;
+  if (!no_half({out, a->grad, out->grad}, where) || !ensure_init()) return;
   if (!dims_ok(a, p, where)) return;
   if (!out->grad) {
     report_error(where, "output has no gradient");

@@ -569,7 +569,7 @@ void ones_hip(Tensor *t, u64 num_elements) {
 }
 
 void set_ones_grad_hip(Tensor *t) {
-  if (!t || !t->grad || !ensure_init()) return;
+  if (!t || !t->grad || !no_half({t->grad}, "set_ones_grad_hip") || !ensure_init()) return;
   ones_into(t->grad->data, t->dtype, numel(t), "set_ones_grad_hip");
 }
 

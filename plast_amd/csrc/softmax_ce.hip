@@ -1809,9 +1809,9 @@ void softmax_forward(const Tensor **inputs, Tensor *output, KernelParams params,
 template <bool LOG>
 void softmax_backward(Tensor **inputs, const Tensor *output, KernelParams params,
                       const char *where) {
-  if (!ensure_init()) return;
   Tensor *x = inputs[0];
   if (!x->requires_grad || !x->grad) return;
+  if (!no_half({x->grad, output->grad}, where) || !ensure_init()) return;
   if (!check_softmax(x, output, params, where)) return;
   if (!output->grad || !contiguous(output->grad) || !contiguous(x->grad)) {
     report_error(where, "needs the output gradient and a contiguous input gradient");
@@ -1906,10 +1906,10 @@ void softmax_cross_entropy_hip_forward(const Tensor **inputs, Tensor *output, Ke
 // gradient buffer with no other contribution (saves one HBM read of [N, C]).
 void softmax_cross_entropy_hip_backward(Tensor **inputs, const Tensor *output, KernelParams params) {
   const char *where = "softmax_cross_entropy_hip_backward";
-  if (!ensure_init()) return;
   Tensor *x = inputs[0];
   const Tensor *lab = inputs[1], *st = inputs[2];
   if (!x->requires_grad || !x->grad) return;
+  if (!no_half({x->grad, output->grad}, where) || !ensure_init()) return;
   if (!check_ce(x, lab, st, where)) return;
   if (!output->grad || !contiguous(x->grad)) {
     report_error(where, "needs the loss gradient and a contiguous logits gradient");

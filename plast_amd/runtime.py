@@ -248,6 +248,8 @@ class DeviceTensor:
         return out
 
     def fill_(self, kind: str, seed: int, a: float, b: float) -> "DeviceTensor":
+        if self.itemsize < 4:
+            raise ValueError("only tensors of 32 bits and more are filled with generated values")
         L = lib()
         n = int(np.prod(self.shape))
         if kind == "uniform":
