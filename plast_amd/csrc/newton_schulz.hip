@@ -141,14 +141,14 @@ struct Scales {
 };
 
 // The power of two that one X is kept times: `scale` where |X| = |G| / (|G| + eps) is about 1. A smaller |G|
-// leaves a small X, whose iterates grow by up to `growth` bits in all, a being their largest factor: it is
-// raised by the bits that X lacks, less those that it may still grow by and has no room for.
-__device__ __forceinline__ double scale_of_x(double norm, float eps, int growth, float scale) {
+// leaves a small X, whose iterates grow by up to `growth` bits in all: it is raised by the bits that X lacks, less
+// those that it may still grow by beyond the `room` above the largest iterate at `scale`.
+__device__ __forceinline__ double scale_of_x(double norm, float eps, int growth, int room, float scale) {
   const double x = norm / (norm + double(eps));
   int lacks = x > 0.0 && x < 0.5 ? -ilogb(x) - 1 : 0;
   lacks = lacks > 110 ? 110 : lacks;
   const int grows = lacks < growth ? lacks : growth;
-  return ldexp(double(scale), lacks - (grows > 3 ? grows - 3 : 0));
+  return ldexp(double(scale), lacks - (grows > room ? grows - room : 0));
 }
 
 // A stack of factors in lines: `rows` padded rows of `pitch` bytes.
@@ -183,7 +183,7 @@ __device__ __forceinline__ float get1(const char *at) {
 template <class T, bool MUON>
 __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, const double *part,
                                                          uint32_t parts, float eps, int growth,
-                                                         float base, Lines X, Lines XT, float *xscale) {
+                                                         int room, float base, Lines X, Lines XT, float *xscale) {
   __shared__ float tile[64][65];
   const uint32_t b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of the source
   const bool tall = G.rows > G.cols;
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kNsBlock) void start_kernel(Stack G, MuonSet S, con
       }
     }
   }
-  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth, base);
+  const double norm = norm_of(part, b, parts), sx = scale_of_x(norm, eps, growth, room, base);
   const double scale = sx / (norm + double(eps));
   if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) xscale[b] = float(sx);
 #pragma unroll
@@ -631,6 +631,7 @@ struct Plan {
   Tiling gram, square, update;
   bool pairs;       // steps go by pairs
   Scales scale;
+  int growth, room;  // of X
 };
 
 // The pieces that leave the fewest rounds of `slots` workgroups, each a share of the sum. In lines' time, a round
@@ -663,16 +664,20 @@ Tiling tiling(uint32_t tile, uint32_t rows, uint32_t cols, bool sym, uint64_t co
 uint32_t round_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
 // The rule followed for singular values in [0, 1]: the scales that give each factor room, and whether two steps'
-// factor, P' P - a^2, has room at the scale of S; `most` is the largest singular value met.
+// factor, P' P - a^2, has room at the scale of S; `most` is the largest singular value met, `growth` the bits by
+// which any grows at most, `room` those between `most` at its scale and fp16's range.
 struct RuleRange {
   Scales scale;
   bool pairs;
   double most;
+  int growth, room;
 };
 RuleRange follow(const NewtonSchulz &r) {
-  double x = 1.0, a = 1.0, s = 0.0, q = 0.0;
+  double x = 1.0, a = 1.0, s = 0.0, q = 0.0, ratio = 1.0;
+  for (int i = 1; i <= r.steps; ++i) ratio = std::fmax(ratio, std::pow(std::fabs(double(r.a)), i));  // towards 0
   for (int k = 0; k <= 4096; ++k) {
-    double v = double(k) / 4096.0, before = 0.0;
+    const double from = double(k) / 4096.0;
+    double v = from, before = 0.0;
     for (int i = 0; i < r.steps; ++i) {
       const double l = v * v, p = r.a + r.b * l + r.c * l * l;
       a = std::fmax(a, std::fmax(l, std::fabs(p * l)));
@@ -681,6 +686,7 @@ RuleRange follow(const NewtonSchulz &r) {
       before = p;
       v *= p;
       x = std::fmax(x, std::fabs(v));
+      if (k) ratio = std::fmax(ratio, std::fabs(v) / from);
     }
   }
   const auto fit = [](double most, int bits) {
@@ -688,7 +694,9 @@ RuleRange follow(const NewtonSchulz &r) {
     return float(std::ldexp(1.0, bits));
   };
   const Scales to{fit(x, 12), fit(a, 12), fit(s, 11)};
-  return RuleRange{to, q * to.s <= 32768.0, x};
+  const double growth = std::ceil(std::log2(ratio));
+  const double room = std::floor(std::log2(64000.0 / (x * to.x)));
+  return RuleRange{to, q * to.s <= 32768.0, x, int(growth < 110.0 ? growth : 110.0), int(room > 0.0 ? room : 0.0)};
 }
 // The same, worked out when the rule is another than the last call's (45 us on the host).
 RuleRange range_of(const NewtonSchulz &r) {
@@ -719,6 +727,8 @@ Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz 
   // 1.18; under 2^30 the launch costs more).
   const RuleRange range = range_of(rule);
   p.scale = range.scale;
+  p.growth = range.growth;
+  p.room = range.room;
   p.pairs = range.pairs && rule.steps >= 2 && uint64_t(p.m) * p.m * (p.n - p.m) * count >= uint64_t(1) << 30;
   p.mp = round_up(p.m, tile);
   p.np = round_up(p.n, tile);
@@ -796,11 +806,10 @@ void iterate(const Plan &plan, const Stack &G, const Stack &O, const MuonSet &S,
   const uint32_t np = uint32_t(parts > kNormParts ? kNormParts : parts);
   if constexpr (MUON) momentum_kernel<<<dim3(np, count), kNsBlock, 0, stream()>>>(S, size, norms);
   else norm_kernel<T><<<dim3(np, count), kNsBlock, 0, stream()>>>(G, MagicDiv::make(G.cols), norms);
-  const float most_growth = std::fabs(rule.a) > 1.0f ? std::ceil(std::log2(std::fabs(rule.a)) * float(rule.steps)) : 0.0f;
-  const int growth = int(most_growth < 110.0f ? most_growth : 110.0f);
   const bool tall = G.rows > G.cols;
   const dim3 grid((tall ? plan.mp : plan.np) / 64, (tall ? plan.np : plan.mp) / 64, count);
-  start_kernel<T, MUON><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, growth, plan.scale.x, x, xt, xscale);
+  start_kernel<T, MUON><<<grid, kNsBlock, 0, stream()>>>(G, S, norms, np, rule.eps, plan.growth, plan.room,
+                                                       plan.scale.x, x, xt, xscale);
   const float sa = plan.scale.a, ss = plan.scale.s;
   Product P;
   memset(&P, 0, sizeof P);
