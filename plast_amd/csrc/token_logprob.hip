@@ -491,11 +491,10 @@ __device__ __forceinline__ V get_shared(const V *p) {
 }
 struct Pieces {
   uint32_t n;
-  Piece *found;      // [rows][n]
-  uint32_t *tickets;  // [rows], zero between launches
+  Piece *found;  // [rows][n]
 };
-constexpr uint32_t kTickets = 4096, kMaxPieces = 32;
-__device__ uint32_t g_tickets[kTickets];
+constexpr uint32_t kMaxPieces = 32, kCutBlocks = 512;  // of a row, of a launch
+__device__ uint32_t g_tickets[kCutBlocks / 2];         // of each row, zero between launches
 
 // W waves per row (or piece of one), four rows per workgroup where W is 1. One pass: a lane's units of 16 bytes
 // come four at a time. What bounds it is the read for fp32 and the vector units for the 16-bit types: of a
@@ -652,10 +651,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (gl == 0)
-      is_last = __hip_atomic_fetch_add(&P.tickets[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == P.n - 1;
+      is_last = __hip_atomic_fetch_add(&g_tickets[row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == P.n - 1;
     __syncthreads();
     if (!is_last) return;
-    if (gl == 0) put_shared(&P.tickets[row], 0u);
+    if (gl == 0) put_shared(&g_tickets[row], 0u);
     // a wave's lanes take the pieces; the merged sums are the same whoever comes last
     Running o;
     const uint32_t lane = gl % 64;
@@ -1254,18 +1253,6 @@ bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *t
   return true;
 }
 
-uint32_t *tickets(const char *where) {
-  static uint32_t *at = nullptr;
-  if (at) return at;
-  void *p = nullptr;
-  const hipError_t e = hipGetSymbolAddress(&p, HIP_SYMBOL(g_tickets));
-  if (e != hipSuccess) {
-    report_error(where, "hipGetSymbolAddress: %s", hipGetErrorString(e));
-    return nullptr;
-  }
-  return at = static_cast<uint32_t *>(p);
-}
-
 // launch(args, workgroups) for parts of the rows that one grid of `threads` lanes holds.
 template <class F>
 void by_parts(const TokenArgs &A, uint64_t rows_per_block, uint64_t threads, F &&launch) {
@@ -1286,10 +1273,10 @@ void launch_held(const TokenArgs &A) {
   });
 }
 
-// Workgroups that a row is cut over: few rows, up to 512 workgroups of 1024 units or more.
+// Workgroups that a row is cut over: few rows, up to kCutBlocks workgroups of 1024 units or more.
 uint32_t pieces_of(uint64_t rows, uint64_t vocab, uint64_t bytes) {
   uint64_t cut = vocab * bytes / 16 / 1024;
-  if (cut > 512 / rows) cut = 512 / rows;
+  if (cut > kCutBlocks / rows) cut = kCutBlocks / rows;
   return uint32_t(cut > kMaxPieces ? kMaxPieces : cut < 1 ? 1 : cut);
 }
 uint64_t pieces_bytes(uint64_t rows, uint64_t vocab, uint64_t bytes) {
@@ -1301,7 +1288,7 @@ uint64_t pieces_bytes(uint64_t rows, uint64_t vocab, uint64_t bytes) {
 template <class T, bool TOP>
 bool launch_rows(const TokenArgs &A, void *room, const char *where) {
   const uint64_t unit = 16 / sizeof(T), units = A.vocab / unit;
-  Pieces P{1, nullptr, nullptr};
+  Pieces P{1, nullptr};
   if constexpr (!TOP)
     if (most_units<T>(A.vocab) <= 256) {
       with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto n) {
@@ -1336,8 +1323,7 @@ bool launch_rows(const TokenArgs &A, void *room, const char *where) {
   if (P.n > 1) {
     if (!room) room = partials(pieces_bytes(A.rows, A.vocab, sizeof(T)), where);
     P.found = static_cast<Piece *>(room);
-    P.tickets = tickets(where);
-    if (!P.tickets || !P.found) return false;
+    if (!P.found) return false;
     fwd_kernel<T, 4, TOP, true><<<A.rows * P.n, 256, 0, stream()>>>(A, P);
   } else if (A.rows < 512 && units >= 6000) {
     // sixteen waves a row where a few hundred long ones leave the chip half empty: [300, 131072] in bf16 with 20
