@@ -272,16 +272,17 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
 /* ------------------------------------------------------------------ orthogonalised updates --- */
 
 /* out = the Newton-Schulz iteration of g, a matrix [rows, cols] or a stack [count, rows, cols] of
- * them, each by itself: FLOAT32, FLOAT16 or BFLOAT16, any strides (out's must not overlap); out has
- * g's type and shape and may be g itself. The iteration runs on
+ * them, each by itself, of up to 65535 rows and columns: FLOAT32, FLOAT16 or BFLOAT16, any strides
+ * (out's must not overlap); out has g's type and shape and may be g itself. The iteration runs on
  * float32-grade products: every factor is held as a pair of 16-bit floats, 22 significant bits,
  * summed in 32 bits. A rule that takes a singular value in [0, 1] beyond 4 is refused.
  * No counterpart in the reference. */
 void newton_schulz_hip(const Tensor *g, Tensor *out, const NewtonSchulz *rule);
-/* One Muon step over `num_parameters` contiguous FLOAT32 matrices of any shapes (other ranks are
- * refused; parameters that are NULL or have no grad are skipped). Moments as in adam_step_hip:
- * allocated and zeroed by this library when optimizer->m is NULL (freed by plast_hip_muon_release),
- * else the caller's. Matrices of one shape run through the same launches. */
+/* One Muon step over `num_parameters` contiguous FLOAT32 matrices of any shapes of up to 65535 rows
+ * and columns (other ranks are refused; parameters that are NULL or have no grad are skipped).
+ * Moments as in adam_step_hip: allocated and zeroed by this library when optimizer->m is NULL (an
+ * error while a capture is open; freed by plast_hip_muon_release), else the caller's. Matrices of
+ * one shape run through the same launches. */
 void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters);
 void plast_hip_muon_release(Muon *optimizer, int num_parameters);
 

@@ -1018,6 +1018,10 @@ void muon_step_hip(Muon *optimizer, Tensor **parameters, int num_parameters) {
     }
   }
   if (!ensure_init()) return;
+  if (!optimizer->m && capturing()) {  // a replay would zero them each time
+    report_error(where, "the first step makes the moments: run one before capturing");
+    return;
+  }
   if (!optimizer->m && !alloc_moments(optimizer, parameters, num_parameters, where)) return;
   for (int k = 0; k < num_parameters; ++k)
     if (parameters[k] && parameters[k]->grad && !f32_matrix(optimizer->m[k], parameters[k])) {
