@@ -1,0 +1,75 @@
+"""Newton-Schulz and Muon on each side of the lines between the products' tiles: 128 wide from m n count >= 3 2^20 with
+m > 128, 256 wide from 2^23 with m > 2048 (m the smaller extent), for each type, tall and wide, one step at a time and
+two. Sums of so few tiles are cut in pieces and joined. Bars as in test_gpu_newton_schulz."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from plast_amd import abi
+from test_gpu_newton_schulz import A, B, CC, EPS, _rt, iterate, muon_exact, near, run
+from token_cases import load, store
+
+pytestmark = pytest.mark.gpu
+
+# (shape, tile): squares, whose singular values lie far apart, go one step at a time
+WIDE = [((128, 26000), 64), ((129, 24385), 64), ((129, 24387), 128), ((1100, 2900), 128), ((2048, 4100), 128),
+        ((2049, 4090), 128), ((2049, 4100), 256), ((2300, 5000), 256)]
+
+
+@pytest.mark.parametrize("shape, tile", WIDE + [((1800, 1800), 128), ((2900, 2900), 256)], ids=str)
+@pytest.mark.parametrize("tall", [False, True])
+def test_tiles(shape, tile, tall):
+    if tall:
+        shape = shape[::-1]
+    print(f"newton_schulz tiles {shape} {tile}", flush=True)
+    g = np.random.RandomState(tile).randn(*shape).astype(np.float32)
+    near(run(g, "f32"), iterate(g), 2e-5 if shape[0] != shape[1] else 3.3e-4, "f32", f"{shape}")
+
+
+@pytest.mark.parametrize("shape", [(1100, 2900), (2900, 1100), (2100, 4100), (4100, 2100)], ids=str)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_16_bit_results(shape, kind):
+    print(f"newton_schulz tiles {kind} {shape}", flush=True)
+    g = load(store(np.random.RandomState(3).randn(*shape).astype(np.float32), kind))
+    near(run(g, kind, steps=3), iterate(g, 3), 2e-5, kind, f"{kind} {shape}")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(3, 600, 1800), (3, 1800, 600)], ids=str)
+def test_stacks_and_strong_directions(shape, kind):
+    print(f"newton_schulz tiles {kind} {shape}", flush=True)
+    rng = np.random.RandomState(4)
+    g = rng.randn(*shape)
+    g[1] += 3 * rng.randn(shape[1], 8) @ rng.randn(8, shape[2])
+    g = load(store(g.astype(np.float32), kind))
+    got = run(g, kind)
+    for b in range(3):
+        near(got[b], iterate(g[b]), 3.3e-4 if b == 1 else 2e-5, kind, f"{kind} {shape}[{b}]")
+
+
+def test_muon_of_large_shapes():
+    rt = _rt()
+    rng = np.random.RandomState(5)
+    shapes = [(1100, 2900), (2900, 1100), (2100, 4100), (4100, 2100), (1100, 2900)]
+    lr, mom, decay = 0.02, 0.9, 0.1
+    p0 = [rng.randn(*s).astype(np.float32) for s in shapes]
+    dev = [rt.DeviceTensor.from_numpy(p, requires_grad=True) for p in p0]
+    moments = [rt.DeviceTensor(s) for s in shapes]
+    arr, keep = abi.tensor_array(*[d.t for d in dev])
+    held, keep_m = abi.tensor_array(*[m.t for m in moments])
+    opt = abi.Muon(lr, mom, decay, 1, abi.NewtonSchulz(A, B, CC, EPS, 5), held)
+    grads = [rng.randn(*s).astype(np.float32) for s in shapes]
+    for d, g in zip(dev, grads):
+        rt.lib().arena_memcpy_h2d_hip(d.grad.ptr, g.ctypes.data, g.nbytes)
+    rt.lib().muon_step_hip(C.byref(opt), arr, len(dev))
+    rt.lib().check("muon_step")
+    for k, (d, s) in enumerate(zip(dev, shapes)):
+        print(f"muon {s}", flush=True)
+        p, m = muon_exact(p0[k].astype(np.float64), grads[k], np.zeros(s), lr, mom, decay, 1)
+        # lr times a matrix of singular values below 1.3 that is off by 2e-5; the parameter rounds twice
+        bar = lr * 2e-5 * 1.3 * np.sqrt(min(s) * max(1, s[0] / s[1])) + 2.0 ** -23 * np.linalg.norm(p)
+        assert np.linalg.norm(d.numpy() - p) <= bar, f"parameter {k} {s}"
+        assert np.abs(moments[k].numpy() - m).max() <= 2.0 ** -22 * np.abs(m).max()
