@@ -284,12 +284,12 @@ __device__ __forceinline__ void exact_top(const TokenArgs &A, const T *x, uint32
                                           float l0) {
   constexpr uint32_t NL = 64 * W;
   const uint32_t V = A.vocab, wave = gl / 64;
-  uint64_t last = ~uint64_t(0);
+  uint64_t last = 0;
   for (uint32_t k = 0; k < A.top; ++k) {
     uint64_t best = 0;
     for (uint32_t j = gl; j < V; j += NL) {
       const uint64_t key = order_key(float(x[j]), j);
-      if (key < last && key > best) best = key;
+      if ((k == 0 || key < last) && key > best) best = key;
     }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) {
