@@ -1037,15 +1037,16 @@ __global__ __launch_bounds__(kRowBlock) void tiny_kernel(TokenArgs A) {
 // The step over many long rows: a workgroup of 1024 lanes per CU that goes from row to row, the next one's units on
 // their way into a second set of registers while this one is worked on. Rows are handed out as workgroups
 // become free (in fixed turns the odd XCDs end some 8% after the even ones); a result does not depend on who works it
-// out. [32768, 32000] in fp32: 1436 us, 5.84 TB/s, instead of 1585 with a workgroup per row (two of them fit a CU); 16-bit
-// rows, whose two exponentials a logit leave the memory idle at one workgroup per CU, lose: 455 us and 425 at [16384,
-// 32000] in bf16. Rows are whole units, 16-byte aligned in the gradient (the others' bounds cost registers that the two sets
-// need).
-constexpr uint32_t kStreamLanes = 1024;
+// out. [32768, 32000] in fp32: 1436 us, 5.84 TB/s, instead of 1585 with a workgroup per row (two of them fit a CU). With half
+// the units, where more rows share a CU anyway, it loses: [32768, 8800] 522 us and 443, [32768, 16000] 743 and 709,
+// [2048, 16000] 56 and 50; so do 16-bit rows, whose two exponentials a logit leave the memory idle at one workgroup per
+// CU: 455 us and 425 at [16384, 32000] in bf16. Rows are whole units, 16-byte aligned in the gradient (the others'
+// bounds cost registers that the two sets need).
+constexpr uint32_t kStreamLanes = 1024, kStreamUnits = 8;
 __device__ uint32_t g_stream_rows[2];  // rows handed out, workgroups that are done; zero between launches
-template <class T, int N>
 __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) {
-  constexpr uint32_t E = Unit<T>::E, L = kStreamLanes;
+  typedef float T;
+  constexpr uint32_t E = Unit<T>::E, L = kStreamLanes, N = kStreamUnits;
   __shared__ float lds[2][3][16];
   __shared__ uint32_t drawn[2];
   const uint32_t V = A.vocab, gl = threadIdx.x, grid = gridDim.x;
@@ -1054,7 +1055,7 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
     const RowAt at = row_at(A.map, row);
     const T *x = static_cast<const T *>(A.x) + at.x;
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
+    for (uint32_t u = 0; u < N; ++u) {
       v[u] = T(-kInf);
       if (token >= 0 && (u * L + gl) * E < V) v[u] = load_unit(x + u * L * E + gl * E);
     }
@@ -1073,7 +1074,7 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
     const float x_token = gl == 0 && uint32_t(token) < V ? float((static_cast<const T *>(A.x) + at.x)[token]) : 0.0f;
     float m = -kInf;
 #pragma unroll
-    for (int u = 0; u < N; ++u) m = __builtin_elementwise_maximum(m, unit_max(to_floats<T>(v[u])));
+    for (uint32_t u = 0; u < N; ++u) m = __builtin_elementwise_maximum(m, unit_max(to_floats<T>(v[u])));
     if (gl == 0) drawn[turn] = ticket + 2 * grid;
     m = lanes_max<L>(m, lds[turn][0]);  // its barrier makes drawn[turn] visible too
     const uint32_t after_next = __builtin_amdgcn_readfirstlane(drawn[turn]);
@@ -1082,8 +1083,7 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
     const auto exponent = [&](float x) { return fmaxf((x - m) * A.c, -200.0f); };
     float s = 0.0f, w = 0.0f;
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
-      if constexpr (sizeof(T) == 2) keep_raw(v[u]);
+    for (uint32_t u = 0; u < N; ++u) {
       const auto f = to_floats<T>(v[u]);
       auto terms = f;
 #pragma unroll
@@ -1120,10 +1120,9 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
     RowGrad G(A, row, token, m, l, h < 0.0f ? 0.0f : h);
     if (m == -kInf) G.a = G.b = G.onehot = 0.0f;  // padding too
 #pragma unroll
-    for (int u = 0; u < N; ++u) {
+    for (uint32_t u = 0; u < N; ++u) {
       const uint32_t j = (u * L + gl) * E;
       if (j >= V) continue;
-      if constexpr (sizeof(T) == 2) keep_raw(v[u]);
       auto f = to_floats<T>(v[u]);
 #pragma unroll
       for (uint32_t e = 0; e < E; ++e) {
@@ -1490,9 +1489,9 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
     held = with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto units) {
       constexpr int L = decltype(lanes)::value;
       constexpr int U = decltype(units)::value;
-      if constexpr (L == 1024 && U == 8 && sizeof(T) == 4) {
+      if constexpr (L == kStreamLanes && U == kStreamUnits && sizeof(T) == 4) {
         if (A.rows >= 4 * uint32_t(num_cus()) && whole_rows<T>(A)) {
-          held_stream_kernel<T, U><<<num_cus(), kStreamLanes, 0, stream()>>>(A);
+          held_stream_kernel<<<num_cus(), kStreamLanes, 0, stream()>>>(A);
           return;
         }
       }
