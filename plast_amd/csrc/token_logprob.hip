@@ -220,7 +220,7 @@ struct RowLds {
   float group[64];
   float threshold;
   uint32_t count[2], ties;
-  uint64_t list[2][kList];
+  uint64_t list[2 * kList];  // two lists, or one where pieces are joined
 };
 
 __device__ __forceinline__ void wave_sync() {
@@ -339,7 +339,7 @@ struct Candidates {
       if ((gl & 63) == 0) at = atomicAdd(&L.count[cur], n);
       at = __builtin_amdgcn_readfirstlane(at);
     }
-    if (hot && at + before < kList) L.list[cur][at + before] = order_key(v, number);
+    if (hot && at + before < kList) L.list[cur * kList + at + before] = order_key(v, number);
   }
   __device__ __forceinline__ uint32_t listed() const { return W == 1 ? held : L.count[cur]; }
   __device__ __forceinline__ void relist(uint32_t n, uint32_t list) {
@@ -406,7 +406,7 @@ struct Candidates {
         else if (n < to + tail) v = float(x[uint64_t(to) * E + (n - to)]);
         const uint64_t hit = __ballot(v == bound);
         const uint32_t place = __popcll(hit & ((uint64_t(1) << gl) - 1));
-        if (v == bound && place < want) L.list[0][at + place] = order_key(v, n);
+        if (v == bound && place < want) L.list[at + place] = order_key(v, n);
         const uint32_t got = min(uint32_t(__popcll(hit)), want);
         want -= got;
         at += got;
@@ -422,7 +422,7 @@ struct Candidates {
   __device__ __forceinline__ uint32_t rank(uint64_t key, uint32_t n) const {
     uint32_t r = 0;
 #pragma unroll 4
-    for (uint32_t k = 0; k < n; ++k) r += L.list[cur][k] > key;
+    for (uint32_t k = 0; k < n; ++k) r += L.list[cur * kList + k] > key;
     return r;
   }
   // Drops all but the `top` largest and raises the bound to the last of them.
@@ -435,9 +435,9 @@ struct Candidates {
       return;
     }
     for (uint32_t i = gl; i < n; i += NL) {
-      const uint64_t key = L.list[cur][i];
+      const uint64_t key = L.list[cur * kList + i];
       const uint32_t r = rank(key, n);
-      if (r < top) L.list[1 - cur][r] = key;
+      if (r < top) L.list[(1 - cur) * kList + r] = key;
       if (r == top - 1) L.threshold = key_value(key);
     }
     relist(top, 1 - cur);
@@ -461,7 +461,7 @@ struct Candidates {
       float v = 0.0f;
       uint32_t j = 0;
       if (hot) {
-        const uint32_t number = 0xffffffffu - uint32_t(L.list[old][i / E]), e = i % E;
+        const uint32_t number = 0xffffffffu - uint32_t(L.list[old * kList + i / E]), e = i % E;
         j = number < units ? number * E + e : units * E + (number - units);
         hot = number < units || e == 0;
         v = float(x[j]);
@@ -490,11 +490,31 @@ __device__ __forceinline__ V get_shared(const V *p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 struct Pieces {
-  uint32_t n;
+  uint32_t n, r, q;
   Piece *found;  // [rows][n]
 };
 constexpr uint32_t kMaxPieces = 32, kCutBlocks = 512;  // of a row, of a launch
-__device__ uint32_t g_tickets[kCutBlocks / 2];         // of each row, zero between launches
+// What bounds a row's candidates among its n pieces' keys: the q-th largest of the pieces' r-th keys, q r >= top, which
+// has `top` keys at or above it. Of independent logits some three times `top` are, where the largest of the last keys
+// leaves nearly all of them, more than a list holds ([1, 131072] in fp32 with 20: 1468 us, the row read again for each).
+// In any row the q pieces leave at most `top` each and the others r - 1. Finding it takes a step a piece: where there are
+// as many pieces as keys of each, and few keys in all, the largest of the last ones will do ([1, 131072] in fp32 with 5
+// 11.3 us and 11.8, [64, 50001] in fp16 with 5 12.0 and 12.4; but [64, 131072] in bf16 with 20 20.1 and 19.0, [1, 131072] in
+// fp32 with 10 12.9 and 12.4).
+constexpr uint32_t bound_key(uint32_t top, uint32_t n) {
+  const uint32_t r = (3 * top + n - 1) / n;
+  return r < top && (top > n || top * n > 192) ? r : top;
+}
+constexpr bool joined_keys_fit() {
+  for (uint32_t top = 1; top <= PLAST_TOP_MAX; ++top)
+    for (uint32_t n = 2; n <= kMaxPieces; ++n) {
+      const uint32_t r = bound_key(top, n), q = (top + r - 1) / r;
+      if (q > n || q * top + (n - q) * (r - 1) > 2 * kList) return false;
+    }
+  return true;
+}
+static_assert(joined_keys_fit(), "the pieces' keys that count fit both lists");
+__device__ uint32_t g_tickets[kCutBlocks / 2];  // of each row, zero between launches
 
 // W waves per row (or piece of one), four rows per workgroup where W is 1. One pass: a lane's units of 16 bytes
 // come four at a time. What bounds it is the read for fp32 and the vector units for the 16-bit types: of a
@@ -641,7 +661,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
     }
     if (TOP && !top.lost) {
       for (uint32_t i = gl; i < found; i += NL) {
-        const uint64_t key = L.list[top.cur][i];
+        const uint64_t key = L.list[top.cur * kList + i];
         const uint32_t k = top.rank(key, found);
         if (k < A.top) put_shared(&mine[piece].keys[k], key);
       }
@@ -659,13 +679,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
     Running o;
     const uint32_t lane = gl % 64;
     uint32_t lost = 0;
-    uint64_t least = 0, keys[kMaxPieces * PLAST_TOP_MAX / NL];
+    uint64_t mid = 0, keys[kMaxPieces * PLAST_TOP_MAX / NL];
     if (lane < P.n) {
       o.m = get_shared(&mine[lane].m), o.cm = get_shared(&mine[lane].cm);
       o.s = get_shared(&mine[lane].s), o.w = get_shared(&mine[lane].w);
       if constexpr (TOP) {
         lost = get_shared(&mine[lane].lost);
-        least = get_shared(&mine[lane].keys[A.top - 1]);
+        mid = get_shared(&mine[lane].keys[P.r - 1]);
       }
     }
     if constexpr (TOP) {
@@ -678,24 +698,29 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
     r = wave_join(o);
     top.lost = __any(lost != 0);
     if (TOP && !top.lost) {
-      // no logit below a piece's last candidate can be among the largest
+      uint64_t least = mid;
+      const bool one = P.q == 1;
+      if (!one) {
+        uint32_t before = 0;
+        for (uint32_t k = 0; k < P.n; ++k) {
+          const uint32_t high = __builtin_amdgcn_readlane(uint32_t(mid >> 32), k);
+          before += (uint64_t(high) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(mid), k))) > mid;
+        }
+        if (before >= P.q) least = ~uint64_t(0);
+      }
 #pragma unroll
       for (int d = 32; d >= 1; d >>= 1) {
         const uint64_t k = __shfl_xor((unsigned long long)least, d);
-        least = k > least ? k : least;
+        least = (k > least) == one ? k : least;
       }
       top.cur = 0;
       if (gl == 0) L.count[0] = 0;
       __syncthreads();
 #pragma unroll
       for (uint32_t t = 0; t < kMaxPieces * PLAST_TOP_MAX / NL; ++t)
-        if (keys[t] && keys[t] >= least) {
-          const uint32_t at = atomicAdd(&L.count[0], 1u);
-          if (at < kList) L.list[0][at] = keys[t];
-        }
+        if (keys[t] >= least && keys[t]) L.list[atomicAdd(&L.count[0], 1u)] = keys[t];
       __syncthreads();
       found = L.count[0];
-      if (found > kList) top.give_up();
     }
   }
   float m = r.m, l0;
@@ -712,7 +737,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
       return;
     }
     for (uint32_t i = gl; i < found; i += NL) {
-      const uint64_t key = L.list[top.cur][i];
+      const uint64_t key = L.list[top.cur * kList + i];
       const uint32_t k = top.rank(key, found);
       if (k < A.top) put_top(A, row, k, key, m, l0);
     }
@@ -1287,7 +1312,7 @@ uint64_t pieces_bytes(uint64_t rows, uint64_t vocab, uint64_t bytes) {
 template <class T, bool TOP>
 bool launch_rows(const TokenArgs &A, void *room, const char *where) {
   const uint64_t unit = 16 / sizeof(T), units = A.vocab / unit;
-  Pieces P{1, nullptr};
+  Pieces P{1, 1, 1, nullptr};
   if constexpr (!TOP)
     if (most_units<T>(A.vocab) <= 256) {
       with_held_shape(most_units<T>(A.vocab), [&](auto lanes, auto n) {
@@ -1323,6 +1348,7 @@ bool launch_rows(const TokenArgs &A, void *room, const char *where) {
     if (!room) room = partials(pieces_bytes(A.rows, A.vocab, sizeof(T)), where);
     P.found = static_cast<Piece *>(room);
     if (!P.found) return false;
+    if constexpr (TOP) P.r = bound_key(A.top, P.n), P.q = ceil_div(A.top, P.r);
     fwd_kernel<T, 4, TOP, true><<<A.rows * P.n, 256, 0, stream()>>>(A, P);
   } else if (A.rows < 512 && units >= 6000) {
     // sixteen waves a row where a few hundred long ones leave the chip half empty: [300, 131072] in bf16 with 20
