@@ -1521,7 +1521,13 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
   with_float_type(x->dtype, [&](auto t) {
     typedef decltype(t) T;
     const bool whole = whole_rows<T>(A);
-    held = with_held_shape(grad_units<T>(A, whole), [&](auto lanes, auto units) {
+    const uint32_t in_row = grad_units<T>(A, whole);
+    // Sixteen units a lane spill some 25 registers, and take a workgroup per row: they pay in fp32 where rows fill the
+    // chip ([8192, 65000] 965 us and 1058 in two passes, [400, 65000] 58 and 67; but [64, 65000] 21.6 and 20.3, [4, 65000]
+    // 17.8 and 12.9), not in 16 bits, where a lane has twice the logits ([8192, 65600] in bf16 699 and 503, [8192, 131000]
+    // 1109 and 1069, [4, 131000] 27 and 13).
+    const uint32_t most = sizeof(T) == 4 && A.rows >= uint32_t(num_cus()) ? 16 * 1024 : 8 * 1024;
+    held = in_row <= most && with_held_shape(in_row, [&](auto lanes, auto units) {
       constexpr int L = decltype(lanes)::value;
       constexpr int U = decltype(units)::value;
       if constexpr (L == kStreamLanes && U == kStreamUnits && sizeof(T) == 4) {
@@ -1530,7 +1536,7 @@ void token_logprob_step_hip(const Tensor *x, const Tensor *tokens, const Tensor 
           return;
         }
       }
-      launch_held<T, L, U, true>(A);
+      if constexpr (U < 16 || sizeof(T) == 4) launch_held<T, L, U, true>(A);
     });
   });
   if (held) {

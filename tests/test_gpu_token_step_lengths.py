@@ -1,5 +1,5 @@
-"""The one-pass step over rows on each side of what a workgroup's registers hold, aligned and not: the longest that fit
-(65536 float32 and 131072 16-bit logits or a few less, by alignment), and the powers of two below."""
+"""The one-pass step over rows on each side of what a workgroup's registers hold, aligned and not: 65536 logits or one
+unit less, by alignment (float32 rows of more than 32768 where they fill the chip), and the powers of two below."""
 from __future__ import annotations
 
 import numpy as np
@@ -34,7 +34,13 @@ def test_lengths(kind, vocab):
         _step(kind, 12, vocab, up, offset)
 
 
-@pytest.mark.parametrize("vocab", [16388, 32764])
+@pytest.mark.parametrize("vocab", [32772, 65536, 65535])
+def test_long_rows_that_fill_the_chip(vocab):
+    _step("f32", 260, vocab)
+    _step("f32", 260, vocab, 1, 3)
+
+
+@pytest.mark.parametrize("vocab", [16388, 32764, 32768])
 def test_streaming_rows(vocab):
     """Rows of whole 16-byte units, more than four for each compute unit."""
     _step("f32", 1100, vocab)
