@@ -718,10 +718,13 @@ Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz 
   p.m = rows < cols ? rows : cols;
   p.n = rows < cols ? cols : rows;
   // 256 wide tiles read each factor least often, 128 wide ones leave fewer workgroups without work: 4096 x 4096 4.39
-  // and 4.83 ms, 2048 x 2048 909 and 839 us, 24 x 1024 x 1024 2.31 and 2.25 ms; 64 wide ones go on with that: 1024 x 1024
-  // 262 us (128: 324), 512 x 4096 246 (321), 2048 x 2048 913.
+  // and 4.83 ms, 2304 x 4608 1.45 and 1.49, 2048 x 2048 909 and 839 us, 24 x 1024 x 1024 2.31 and 2.25 ms. They pay where
+  // they pad m by no more than 3% beyond the others (5200 x 5200, 2.4%: 8.37 and 9.19 ms; 2049 x 4200, 5.9%: 1.41 and 1.21,
+  // 3100 x 6200, 4%: 3.68 and 3.27). 64 wide ones go on with that: 1024 x 1024 262 us (128: 324), 512 x 4096 246 (321),
+  // 2048 x 2048 913.
   const uint64_t work = uint64_t(p.m) * p.n * count;
-  const uint32_t tile = p.m > 2048 && work >= uint64_t(1) << 23 ? 256 : p.m > 128 && work >= uint64_t(3) << 20 ? 128 : 64;
+  const bool widest = p.m > 2048 && work >= uint64_t(1) << 23 && round_up(p.m, 256) * 100 <= round_up(p.m, 128) * 103;
+  const uint32_t tile = widest ? 256 : p.m > 128 && work >= uint64_t(3) << 20 ? 128 : 64;
   // Two steps at once cost three more m x m products and one product of X X^T and one update of X less: 1.5 m^2 n
   // multiplications less for 1.5 m^3 more, and one launch more (4096 x 16384: 13.6 -> 10.4 ms, 6 x 2605 x 1001 in fp32 1.34 ->
   // 1.18; under 2^30 the launch costs more).

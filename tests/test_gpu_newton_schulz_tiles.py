@@ -1,6 +1,7 @@
 """Newton-Schulz and Muon on each side of the lines between the products' tiles: 128 wide from m n count >= 3 2^20 with
-m > 128, 256 wide from 2^23 with m > 2048 (m the smaller extent), for each type, tall and wide, one step at a time and
-two. Sums of so few tiles are cut in pieces and joined. Bars as in test_gpu_newton_schulz."""
+m > 128, 256 wide from 2^23 with m > 2048 where they pad m by no more than 3% beyond (m the smaller extent), for each
+type, tall and wide, one step at a time and two. Sums of so few tiles are cut in pieces and joined. Bars as in
+test_gpu_newton_schulz."""
 from __future__ import annotations
 
 import ctypes as C
@@ -14,22 +15,22 @@ from token_cases import load, store
 
 pytestmark = pytest.mark.gpu
 
-# (shape, tile): squares, whose singular values lie far apart, go one step at a time
+# (shape, tile): squares, whose singular values lie far apart, and nearly square ones go one step at a time
 WIDE = [((128, 26000), 64), ((129, 24385), 64), ((129, 24387), 128), ((1100, 2900), 128), ((2048, 4100), 128),
-        ((2049, 4090), 128), ((2049, 4100), 256), ((2300, 5000), 256)]
+        ((2300, 3640), 128), ((2300, 3650), 256), ((2176, 4100), 128), ((2300, 5000), 256)]
 
 
-@pytest.mark.parametrize("shape, tile", WIDE + [((1800, 1800), 128), ((2900, 2900), 256)], ids=str)
+@pytest.mark.parametrize("shape, tile", WIDE + [((1800, 1800), 128), ((2800, 3000), 256)], ids=str)
 @pytest.mark.parametrize("tall", [False, True])
 def test_tiles(shape, tile, tall):
     if tall:
         shape = shape[::-1]
     print(f"newton_schulz tiles {shape} {tile}", flush=True)
     g = np.random.RandomState(tile).randn(*shape).astype(np.float32)
-    near(run(g, "f32"), iterate(g), 2e-5 if shape[0] != shape[1] else 3.3e-4, "f32", f"{shape}")
+    near(run(g, "f32"), iterate(g), 2e-5 if max(shape) > 1.2 * min(shape) else 3.3e-4, "f32", f"{shape}")
 
 
-@pytest.mark.parametrize("shape", [(1100, 2900), (2900, 1100), (2100, 4100), (4100, 2100)], ids=str)
+@pytest.mark.parametrize("shape", [(1100, 2900), (2900, 1100), (2300, 4100), (4100, 2300)], ids=str)
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 def test_16_bit_results(shape, kind):
     print(f"newton_schulz tiles {kind} {shape}", flush=True)
@@ -53,7 +54,7 @@ def test_stacks_and_strong_directions(shape, kind):
 def test_muon_of_large_shapes():
     rt = _rt()
     rng = np.random.RandomState(5)
-    shapes = [(1100, 2900), (2900, 1100), (2100, 4100), (4100, 2100), (1100, 2900)]
+    shapes = [(1100, 2900), (2900, 1100), (2300, 4100), (4100, 2300), (1100, 2900)]
     lr, mom, decay = 0.02, 0.9, 0.1
     p0 = [rng.randn(*s).astype(np.float32) for s in shapes]
     dev = [rt.DeviceTensor.from_numpy(p, requires_grad=True) for p in p0]
