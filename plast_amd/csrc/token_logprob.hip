@@ -1336,8 +1336,10 @@ bool launch_rows(const TokenArgs &A, void *room, const char *where) {
     }
   // A wave a row where rows are many and not long, four where a wave would be alone with its row for long: [4096,
   // 131072] in bf16 with 8 alternatives 224 us with one, 184 with four, [8192, 49999] in fp16 with 20 192 and 169;
-  // [20000, 5000] in bf16 with 5 56 and 117.
-  if (units <= 256 || (A.rows >= 8192 && units < 4096)) {
+  // [20000, 5000] in bf16 with 5 56 and 117. Rows of up to 640 units take one from half as many rows on: [4000, 2000] in fp32
+  // with 5 14.3 and 17.7, [8000, 2600] with 20 36.3 and 40.1, but [1024, 2000] with 20 13.4 and 10.7, [4000, 4000] with 5 20.9
+  // and 20.1. Rows of up to 256, one batch of a wave, always do.
+  if (units <= 256 || (A.rows >= 4000 && units <= 640) || (A.rows >= 8192 && units < 4096)) {
     by_parts(A, 4, 256, [&](const TokenArgs &part, unsigned blocks) {
       fwd_kernel<T, 1, TOP, false><<<blocks, 256, 0, stream()>>>(part, P);
     });
