@@ -698,19 +698,22 @@ RuleRange follow(const NewtonSchulz &r) {
   const double room = std::floor(std::log2(64000.0 / (x * to.x)));
   return RuleRange{to, q * to.s <= 32768.0, x, int(growth < 110.0 ? growth : 110.0), int(room > 0.0 ? room : 0.0)};
 }
-// The same, worked out when the rule is another than the last call's (45 us on the host).
+// The same, worked out once for each of the last eight rules (0.1 ms on the host at 5 steps, 30 ms at 1000).
 RuleRange range_of(const NewtonSchulz &r) {
+  constexpr int kRules = 8;
   static std::mutex mu;
-  static NewtonSchulz last{};
-  static RuleRange range{};
-  static bool any = false;
+  static NewtonSchulz rules[kRules];
+  static RuleRange ranges[kRules];
+  static int known = 0, next = 0;
   std::lock_guard<std::mutex> lk(mu);
-  if (!any || memcmp(&last, &r, sizeof r) != 0) {
-    range = follow(r);
-    last = r;
-    any = true;
-  }
-  return range;
+  for (int k = 0; k < known; ++k)
+    if (memcmp(&rules[k], &r, sizeof r) == 0) return ranges[k];
+  const int at = next;
+  rules[at] = r;
+  ranges[at] = follow(r);
+  next = (next + 1) % kRules;
+  known = known < kRules ? known + 1 : kRules;
+  return ranges[at];
 }
 
 Plan make_plan(uint32_t rows, uint32_t cols, uint64_t count, const NewtonSchulz &rule) {
