@@ -1210,7 +1210,8 @@ bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *t
     return false;
   }
   const uint64_t V = x->shape[x->ndim - 1], n = numel(x);
-  if (V < 1 || V > (uint64_t(1) << 31) - 64) {  // unit numbers times their elements stay within 31 bits
+  // the elements of a row, and of the units that its last workgroup has beyond it, stay within 31 bits
+  if (V < 1 || V > (uint64_t(1) << 31) - 2 * kBwdUnits * kRowBlock * Unit<f16_t>::E) {
     report_error(where, "rows of %llu logits are not supported", (unsigned long long)V);
     return false;
   }

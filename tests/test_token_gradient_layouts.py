@@ -1,5 +1,5 @@
 """Which layouts of the logits' gradient the token log-probability entry points refuse, on the CPU: rows that share
-addresses, along one leading axis or between several."""
+addresses, along one leading axis or between several, and rows that leave their last workgroup no 31-bit numbers."""
 from __future__ import annotations
 
 import ctypes as C
@@ -33,4 +33,16 @@ def test_rows_that_share_addresses(strides):
     step = [x, vec[0], None, None, logp, vec[2], x.grad.contents]
     lib.token_logprob_step_hip(*[C.addressof(t) if t is not None else None for t in step], 1.0)
     with pytest.raises(PlastHipError, match="overlap"):
+        lib.check()
+
+
+@pytest.mark.parametrize("vocab", [2 ** 31 - 64, 2 ** 31 - 8191])
+def test_rows_that_are_too_long(vocab):
+    lib = Library()
+    lib.plast_hip_clear_error()
+    x, vec = T((1, vocab), grad=T((1, vocab))), [T((1,), INT32), T((1, 2)), T((1,))]
+    logp = T((1,))
+    ins = (C.c_void_p * 4)(*[C.addressof(t) for t in [x, *vec]])
+    lib.by_address["backward", "token_logprob"](ins, C.addressof(logp), KernelParams(0, 1, 1.0))
+    with pytest.raises(PlastHipError, match="logits are not supported"):
         lib.check()
