@@ -372,8 +372,9 @@ __device__ __forceinline__ void put_block(const Product &P, const MuonSet &S, fl
 // choosing what each lane reads: unit c lies at c ^ (row / 2 % 8). A 16-byte LDS read is served for lanes 0-3, 12-15,
 // 20-27 of a half wave together, then for the others, from 64 banks: this spreads either set over all of them). A ring of
 // five half-line stages, four of them on their way, measured the same within 2%, with 4096 x 4096 in 4.28 ms and 4.30: the
-// matrix units are at 1.1 PFLOP/s of fp16 in the long sums, what a large library product reaches here, and in the
-// short ones wait for the tiles' ways out, when all workgroups store at once (24 x 1024 x 1024: 35% busy).
+// matrix units are at 1.1 PFLOP/s of fp16 in the long sums, what a large library product reaches here (4096 x 16384:
+// 54-56% busy), and in the short ones wait for the tiles' ways out, when all workgroups store at once (24 x 1024 x
+// 1024: 35% busy).
 template <class T, Mode M, bool MUON, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void product_kernel(Product P, MuonSet S) {
   constexpr int NW = (BM / WM) * (BN / WN), LOADS = (BM + BN) / 8 / NW, FA = WM / 32, FB = WN / 32;

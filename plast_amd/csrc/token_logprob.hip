@@ -313,8 +313,10 @@ __device__ __forceinline__ void exact_top(const TokenArgs &A, const T *x, uint32
 // `top` logits before it, those units' largest). A bound under which no unit counts starts as the top-th
 // largest of 16, 32 or 64 lane groups' maxima over the first logits, twice `top` groups at least, and is raised to
 // the top-th unit whenever as many logits again have been read; only units above it go to the list, some
-// top ln(units) in all, and an ascending row raises it more often. Logits after the last whole unit are units
-// of their own.
+// top ln(units) in all where the logits are in no order. Where they rise, or the first batch is masked and a later one is
+// not, a batch has more units above the bound than the list holds: the row is given up and its alternatives found by
+// a pass each ([4096, 32000] in fp32 with 5 86 us, 656 if a start of each row is masked; [4096, 131072] in bf16 with 8 185
+// and 4680). Logits after the last whole unit are units of their own.
 template <class T, int W>
 struct Candidates {
   static constexpr uint32_t NL = 64 * W, E = Unit<T>::E;
@@ -517,8 +519,9 @@ static_assert(joined_keys_fit(), "the pieces' keys that count fit both lists");
 __device__ uint32_t g_tickets[kCutBlocks / 2];  // of each row, zero between launches
 
 // W waves per row (or piece of one), four rows per workgroup where W is 1. One pass: a lane's units of 16 bytes
-// come four at a time. What bounds it is the read for fp32 and the vector units for the 16-bit types: of a
-// logit's ten issue slots four are the exponential.
+// come four at a time. What bounds it is the read for fp32 ([8184, 32000] 143 us, 6.5 TB/s, vector units 44% busy) and the
+// vector units, with the read close behind, for the 16-bit types, whose logit takes ten issue slots, four of them the
+// exponential's, as fp32's does ([8192, 49999] in bf16 124 us, 78% busy; [4096, 131072] with 8 alternatives 182 us, 83%).
 template <class T, int W, bool TOP, bool CUT>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A, Pieces P) {
   constexpr uint32_t NL = 64 * W, E = Unit<T>::E, U = 4;
