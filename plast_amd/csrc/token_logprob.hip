@@ -277,8 +277,8 @@ __device__ __forceinline__ void exact_sums(const TokenArgs &A, const T *x, uint3
   if (gl == 0) row_out(A, row, token, x_token, m, s, w, ref.shift());
 }
 
-// The alternatives of a row with NaN or infinite logits, or of one that the list could not hold: an argmax each, a
-// pass over the row.
+// The alternatives of a row with NaN or infinite logits, or of one that the list could not hold in the end: an argmax
+// each, a pass over the row.
 template <class T, int W>
 __device__ __forceinline__ void exact_top(const TokenArgs &A, const T *x, uint32_t row, uint32_t gl, RowLds<W> &L, float m,
                                           float l0) {
@@ -314,9 +314,10 @@ __device__ __forceinline__ void exact_top(const TokenArgs &A, const T *x, uint32
 // largest of 16, 32 or 64 lane groups' maxima over the first logits, twice `top` groups at least, and is raised to
 // the top-th unit whenever as many logits again have been read; only units above it go to the list, some
 // top ln(units) in all where the logits are in no order. Where they rise, or the first batch is masked and a later one is
-// not, a batch has more units above the bound than the list holds: the row is given up and its alternatives found by
-// a pass each ([4096, 32000] in fp32 with 5 86 us, 656 if a start of each row is masked; [4096, 131072] in bf16 with 8 185
-// and 4680). Logits after the last whole unit are units of their own.
+// not, a batch has more units above the bound than the list holds: the row is given up, and read twice more when its end
+// is reached ([4096, 32000] in fp32 with 5 86 us, 207 if a start of each row is masked; [4096, 131072] in bf16 with 8 182
+// and 450). Lists of the waves' own, which never overflow as each batch bounds its units first, cost 234 there, but
+// 216 where there is no order. Logits after the last whole unit are units of their own.
 template <class T, int W>
 struct Candidates {
   static constexpr uint32_t NL = 64 * W, E = Unit<T>::E;
@@ -447,10 +448,71 @@ struct Candidates {
     row_sync<W>();
     bound = L.threshold;
   }
+  // Batches of the units from..to, for all lanes: f(unit's number, whether there is one, its largest logit).
+  template <class F>
+  __device__ __forceinline__ void each_unit(uint32_t from, uint32_t to, F &&f) const {
+    constexpr uint32_t U = W == 1 ? 1 : 2;  // more would take more registers than the first pass
+    for (uint32_t q0 = from; q0 < to; q0 += NL * U) {
+      typename Unit<T>::vec v[U];
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t q = q0 + u * NL + gl;
+        if (q < to) v[u] = load_unit(x + uint64_t(q) * E);
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < U; ++u) {
+        const uint32_t q = q0 + u * NL + gl;
+        f(q, q < to, q < to ? unit_max(to_floats<T>(v[u])) : 0.0f);
+      }
+    }
+  }
+  // The list of a row that was given up, by two more passes: the units at or above the top-th largest of 64 groups'
+  // largest keys, which has `top` units at or above it. Neighbours are in different groups, so that of units which stand
+  // together few more than `top` are left. More than the list holds are left where many of the largest are 64 or a
+  // multiple apart: that row stays given up.
+  __device__ __forceinline__ void reread(uint32_t from, uint32_t to, uint32_t tails) {
+    const bool has_tail = gl < tails;
+    const float tail = has_tail ? float(x[units * E + gl]) : 0.0f;
+    const uint64_t tail_key = has_tail ? order_key(tail, units + gl) : 0;
+    uint64_t key = tail_key, *const group = L.list + kList;
+    each_unit(from, to, [&](uint32_t q, bool is, float v) {
+      const uint64_t k = order_key(v, q);
+      if (is && k > key) key = k;
+    });
+    row_sync<W>();
+    if (gl < 64) group[gl] = 0;
+    row_sync<W>();
+    atomicMax(reinterpret_cast<unsigned long long *>(&group[gl % 64]), (unsigned long long)key);
+    row_sync<W>();
+    key = group[gl % 64];
+    uint32_t before = 0;
+#pragma unroll 4
+    for (uint32_t k = 0; k < 64; ++k) before += group[k] > key;
+    const uint64_t last = __ballot(key && before == top - 1);  // none: fewer than `top` units, all of them count
+    uint64_t least = 0;
+    if (last) {
+      const int lane = __ffsll((unsigned long long)last) - 1;
+      least = uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(key >> 32), lane))) << 32 |
+              uint32_t(__builtin_amdgcn_readlane(uint32_t(key), lane));
+    }
+    cur = 0;
+    relist(0, 0);
+    row_sync<W>();
+    each_unit(from, to, [&](uint32_t q, bool is, float v) { push(is && order_key(v, q) >= least, v, q); });
+    push(has_tail && tail_key >= least, tail, units + gl);
+    row_sync<W>();
+    bound = key_value(least);
+    lost = listed() > kList;
+    row_sync<W>();
+  }
   // The units' logits in their place: the list holds logits from here on.
-  __device__ __forceinline__ void open() {
+  __device__ __forceinline__ void open(uint32_t from, uint32_t to, uint32_t tails) {
     raise();
-    if (lost) return;
+    if (lost) {
+      reread(from, to, tails);
+      if (lost) return;
+      raise();
+    }
     const uint32_t n = listed(), old = cur;
     const float least = n == top ? bound : -kInf;  // the top-th logit is no smaller
     row_sync<W>();
@@ -522,8 +584,9 @@ __device__ uint32_t g_tickets[kCutBlocks / 2];  // of each row, zero between lau
 // come four at a time. What bounds it is the read for fp32 ([8184, 32000] 143 us, 6.5 TB/s, vector units 44% busy) and the
 // vector units, with the read close behind, for the 16-bit types, whose logit takes ten issue slots, four of them the
 // exponential's, as fp32's does ([8192, 49999] in bf16 124 us, 78% busy; [4096, 131072] with 8 alternatives 182 us, 83%).
+// With alternatives a lane may have 64 registers, so that eight waves share a SIMD (with 77, 203 us).
 template <class T, int W, bool TOP, bool CUT>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A, Pieces P) {
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W, TOP ? 8 : 1) void fwd_kernel(TokenArgs A, Pieces P) {
   constexpr uint32_t NL = 64 * W, E = Unit<T>::E, U = 4;
   __shared__ RowLds<W> lds[W == 1 ? 4 : 1];
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -649,7 +712,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void fwd_kernel(TokenArgs A,
   }
   uint32_t found = 0;
   if constexpr (TOP) {
-    top.open();
+    top.open(from, to, piece == pieces - 1 ? V - units * E : 0);
     found = top.listed();
   }
   if constexpr (CUT) {
@@ -1358,8 +1421,8 @@ bool launch_rows(const TokenArgs &A, void *room, const char *where) {
     fwd_kernel<T, 4, TOP, true><<<A.rows * P.n, 256, 0, stream()>>>(A, P);
   } else if (A.rows < 512 && units >= 6000) {
     // sixteen waves a row where a few hundred long ones leave the chip half empty: [300, 131072] in bf16 with 20
-    // alternatives 53 us with sixteen, 58 with four, [300, 32000] in fp32 15.8 and 16.7; but [500, 32000] in bf16 13.4 and
-    // 12.3, [500, 16000] with 5 19.9 and 13.0
+    // alternatives 40 us with sixteen, 57 with four, [300, 32000] in fp32 15.8 and 16.6; but [500, 32000] in bf16 13.4 and
+    // 12.3, [500, 16000] with 5 16.0 and 13.1
     fwd_kernel<T, 16, TOP, false><<<A.rows, 1024, 0, stream()>>>(A, P);
   } else {
     by_parts(A, 1, 256, [&](const TokenArgs &part, unsigned blocks) {
