@@ -17,7 +17,7 @@
 #include <cmath>
 #include <type_traits>
 
-#include "half_types.hpp"
+#include "rows.hpp"
 
 namespace plast {
 namespace {
@@ -28,28 +28,6 @@ constexpr int kRowBlock = 256;  // lanes of a workgroup
 // |c m| up to which c m and its rounding are used: a mask of -1e30 that a lane meets first, or that fills a row, has
 // an r of 1e22, and 2^r is no number. 2^27 leaves logits of 20 a temperature of 2.2e-7.
 constexpr float kReach = 0x1p27f;
-
-// Where row `r` of the leading axes starts, in elements, in x and in its gradient.
-struct RowMap {
-  int rank;
-  MagicDiv ext[kMaxRank];
-  int64_t x[kMaxRank], g[kMaxRank];
-};
-struct RowAt {
-  int64_t x, g;
-};
-__device__ __forceinline__ RowAt row_at(const RowMap &M, uint32_t r) {
-  RowAt at{0, 0};
-  for (int d = M.rank - 1; d > 0; --d) {
-    const uint32_t q = M.ext[d].div(r), i = r - q * M.ext[d].d;
-    at.x += int64_t(i) * M.x[d];
-    at.g += int64_t(i) * M.g[d];
-    r = q;
-  }
-  at.x += int64_t(r) * M.x[0];
-  at.g += int64_t(r) * M.g[0];
-  return at;
-}
 
 // What a launch needs of its tensors.
 struct TokenArgs {
@@ -64,7 +42,7 @@ struct TokenArgs {
   uint32_t first_row, rows, vocab;  // first_row: of a launch, where one cannot hold all
   float c;      // log2(e) / T
   float inv_t;  // 1 / T
-  RowMap map;
+  RowMap<2> map;  // of x and of its gradient
 };
 
 // The exponent z of a logit. Where c m is beyond kReach, c (x - m) is taken instead.
@@ -81,31 +59,6 @@ struct RowRef {
   __device__ __forceinline__ float shift() const { return far ? 0.0f : __builtin_fmaf(c, m, -cm); }
 };
 
-// 16 bytes of a row.
-template <class T>
-struct Unit {
-  static constexpr uint32_t E = 16 / sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(E)));
-  typedef vec any __attribute__((aligned(sizeof(T))));  // at any element's address
-  typedef float floats __attribute__((ext_vector_type(E)));
-};
-template <class T>
-__device__ __forceinline__ typename Unit<T>::vec load_unit(const T *p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const typename Unit<T>::any *>(p));
-}
-template <class T>
-__device__ __forceinline__ typename Unit<T>::floats to_floats(typename Unit<T>::vec v) {
-  return __builtin_convertvector(v, typename Unit<T>::floats);
-}
-// Holds a unit as it was read: without it the compiler keeps a 16-bit unit's floats, twice the registers, from
-// one use to the next.
-template <class V>
-__device__ __forceinline__ void keep_raw(V &v) {
-  typedef uint32_t words __attribute__((ext_vector_type(4)));
-  words w = __builtin_bit_cast(words, v);
-  asm volatile("" : "+v"(w));
-  v = __builtin_bit_cast(V, w);
-}
 // A unit's sum by pairs: beside a largest term of 1, the fewer roundings the better.
 template <class F>
 __device__ __forceinline__ float unit_sum(F f) {
@@ -543,16 +496,6 @@ struct Piece {
   uint64_t keys[PLAST_TOP_MAX];
   uint32_t lost;  // the list was too short
 };
-// The XCDs' L2 caches are not coherent: what a workgroup leaves for another goes past them, store by store (a
-// fence would write back and drop the whole cache: 46 us instead of 9 with 384 workgroups).
-template <class V>
-__device__ __forceinline__ void put_shared(V *p, V v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-template <class V>
-__device__ __forceinline__ V get_shared(const V *p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 struct Pieces {
   uint32_t n, r, q;
   Piece *found;  // [rows][n]
@@ -598,7 +541,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W, TOP ? 8 : 1) void fwd_kernel
   if (W == 1 && local >= A.rows) return;
   const int32_t token = A.tokens[row];
   const uint32_t V = A.vocab, units = V / E;
-  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
+  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).at[0];
   const uint32_t from = uint32_t(uint64_t(units) * piece / pieces), to = uint32_t(uint64_t(units) * (piece + 1) / pieces);
   // where rows are few, their first units are on their way before the token is known
   typename Unit<T>::vec v[U];
@@ -888,8 +831,8 @@ __global__ __launch_bounds__(kRowBlock) void bwd_kernel(TokenArgs A, uint32_t ch
   const uint32_t block_row = blockIdx.x / chunks, row = A.first_row + block_row;
   const uint32_t q0 = (blockIdx.x - block_row * chunks) * kBwdUnits * kRowBlock + threadIdx.x;
   const int32_t token = A.tokens[row];
-  const RowAt at = row_at(A.map, row);
-  T *dx = static_cast<T *>(A.dx) + at.g;
+  const RowAt<2> at = row_at(A.map, row);
+  T *dx = static_cast<T *>(A.dx) + at.at[1];
   const RowUnits<T> R(dx, A.vocab);
   const float m = A.stats[2 * row];
   if (token < 0 || m == -kInf) {
@@ -902,7 +845,7 @@ __global__ __launch_bounds__(kRowBlock) void bwd_kernel(TokenArgs A, uint32_t ch
     }
     return;
   }
-  const T *x = static_cast<const T *>(A.x) + at.x;
+  const T *x = static_cast<const T *>(A.x) + at.at[0];
   const RowGrad G(A, row, token, m, A.stats[2 * row + 1] + RowRef(A.c, m).shift(), A.entropy[row]);
 #pragma unroll
   for (uint32_t u = 0; u < kBwdUnits; ++u) {
@@ -918,8 +861,8 @@ __global__ __launch_bounds__(kRowBlock) void bwd_short_kernel(TokenArgs A, Magic
   if (at_unit >= uint64_t(A.rows) * units.d) return;
   const uint32_t row = units.div(uint32_t(at_unit)), q = uint32_t(at_unit) - row * units.d;
   const int32_t token = A.tokens[row];
-  const RowAt at = row_at(A.map, row);
-  T *dx = static_cast<T *>(A.dx) + at.g;
+  const RowAt<2> at = row_at(A.map, row);
+  T *dx = static_cast<T *>(A.dx) + at.at[1];
   const RowUnits<T> R(dx, A.vocab);
   const int32_t j = R.first(q);
   if (j >= int32_t(A.vocab)) return;
@@ -930,7 +873,7 @@ __global__ __launch_bounds__(kRowBlock) void bwd_short_kernel(TokenArgs A, Magic
     return;
   }
   const RowGrad G(A, row, token, m, A.stats[2 * row + 1] + RowRef(A.c, m).shift(), A.entropy[row]);
-  grad_unit<T, ADD>(R, G, static_cast<const T *>(A.x) + at.x, dx, token, j);
+  grad_unit<T, ADD>(R, G, static_cast<const T *>(A.x) + at.at[0], dx, token, j);
 }
 
 // ------------------------------------------------------------------------- rows in registers
@@ -986,9 +929,9 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void held_kernel(Tok
   const bool valid = ROWS == 1 || r < A.rows;
   const uint32_t row = A.first_row + (valid ? r : A.rows - 1);
   const int32_t token = A.tokens[row];
-  const RowAt at = row_at(A.map, row);
-  const T *x = static_cast<const T *>(A.x) + at.x;
-  T *dx = static_cast<T *>(A.dx) + at.g;
+  const RowAt<2> at = row_at(A.map, row);
+  const T *x = static_cast<const T *>(A.x) + at.at[0];
+  T *dx = static_cast<T *>(A.dx) + at.at[1];
   const RowUnits<T> R(GRAD ? dx : x, V);
   typename Unit<T>::vec v[N];
   if (token >= 0) {
@@ -1094,7 +1037,7 @@ __global__ __launch_bounds__(kRowBlock) void tiny_kernel(TokenArgs A) {
   const bool valid = r < A.rows;
   const uint32_t row = A.first_row + (valid ? r : A.rows - 1), V = A.vocab;
   const int32_t token = A.tokens[row];
-  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).x;
+  const T *x = static_cast<const T *>(A.x) + row_at(A.map, row).at[0];
   const bool mine = token >= 0 && gl < V;
   const float v = mine ? float(x[gl]) : -kInf;
   const uint32_t key = mine ? uint32_t(order_key(v, gl) >> 32) : 0;
@@ -1143,8 +1086,8 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
   const uint32_t V = A.vocab, gl = threadIdx.x, grid = gridDim.x;
   typedef typename Unit<T>::vec vec;
   const auto fetch = [&](vec (&v)[N], uint32_t row, int32_t token) {
-    const RowAt at = row_at(A.map, row);
-    const T *x = static_cast<const T *>(A.x) + at.x;
+    const RowAt<2> at = row_at(A.map, row);
+    const T *x = static_cast<const T *>(A.x) + at.at[0];
 #pragma unroll
     for (uint32_t u = 0; u < N; ++u) {
       v[u] = T(-kInf);
@@ -1160,9 +1103,9 @@ __global__ __launch_bounds__(kStreamLanes) void held_stream_kernel(TokenArgs A) 
     uint32_t ticket = 0;  // an increment, not an add: its result is waited for where it is used, below
     if (gl == 0) ticket = atomicInc(&g_stream_rows[0], 0xffffffffu);
     if (next < A.rows) fetch(after, next, next_token);
-    const RowAt at = row_at(A.map, row);
-    T *dx = static_cast<T *>(A.dx) + at.g;
-    const float x_token = gl == 0 && uint32_t(token) < V ? float((static_cast<const T *>(A.x) + at.x)[token]) : 0.0f;
+    const RowAt<2> at = row_at(A.map, row);
+    T *dx = static_cast<T *>(A.dx) + at.at[1];
+    const float x_token = gl == 0 && uint32_t(token) < V ? float((static_cast<const T *>(A.x) + at.at[0])[token]) : 0.0f;
     float m = -kInf;
 #pragma unroll
     for (uint32_t u = 0; u < N; ++u) m = __builtin_elementwise_maximum(m, unit_max(to_floats<T>(v[u])));
@@ -1259,10 +1202,6 @@ bool with_held_shape(uint32_t units, F &&f) {
 
 // ------------------------------------------------------------------------- host
 
-bool f32_vector(const Tensor *t, uint64_t n) {
-  return t && t->device == GPU && t->dtype == FLOAT32 && numel(t) == n && contiguous(t) && (t->data || n == 0);
-}
-
 // Checks x, the tokens and the temperature; fills the row map (of x and, where given, its gradient).
 bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *tokens, float temp,
                 const char *where) {
@@ -1338,8 +1277,8 @@ bool token_args(TokenArgs &A, const Tensor *x, const Tensor *dx, const Tensor *t
   A.map.rank = s.rank;
   for (int d = 0; n && d < s.rank; ++d) {
     A.map.ext[d] = MagicDiv::make(uint32_t(s.shape[d]));
-    A.map.x[d] = s.st[0][d];
-    A.map.g[d] = s.st[1][d];
+    A.map.st[0][d] = s.st[0][d];
+    A.map.st[1][d] = s.st[1][d];
   }
   return true;
 }
@@ -1445,7 +1384,7 @@ template <class T>
 bool whole_rows(const TokenArgs &A) {
   constexpr int64_t E = Unit<T>::E;
   bool whole = A.vocab % E == 0 && aligned16(A.dx);
-  for (int d = 0; d < A.map.rank; ++d) whole = whole && A.map.g[d] % E == 0;
+  for (int d = 0; d < A.map.rank; ++d) whole = whole && A.map.st[1][d] % E == 0;
   return whole;
 }
 
