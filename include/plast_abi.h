@@ -19,8 +19,8 @@
  * Extensions (appended after the reference's last enumerator so every existing numeric value is
  * unchanged): DTYPE gains INT64 (argmax indices) and the 16-bit FLOAT16 and BFLOAT16 (logits and
  * matrices of the operators that say so); OP_TYPE gains ARGMAX, FUSED_ELEMENTWISE,
- * SOFTMAX_CROSS_ENTROPY, SOFTMAX, LOG_SOFTMAX and TOKEN_LOGPROB. NewtonSchulz and Muon have no
- * counterpart in the reference.
+ * SOFTMAX_CROSS_ENTROPY, SOFTMAX, LOG_SOFTMAX, TOKEN_LOGPROB, LAYER_NORM and GATED_RECURRENCE.
+ * NewtonSchulz and Muon have no counterpart in the reference.
  */
 #ifndef PLAST_ABI_H
 #define PLAST_ABI_H
@@ -124,6 +124,8 @@ typedef enum OP_TYPE {
   SOFTMAX,
   LOG_SOFTMAX,
   TOKEN_LOGPROB,
+  LAYER_NORM,
+  GATED_RECURRENCE,
   PLAST_NUM_OP_TYPES
 } OP_TYPE;
 

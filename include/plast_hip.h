@@ -125,6 +125,51 @@ PLAST_HIP_KERNEL_PAIR(log_softmax)
 #define PLAST_TOP_MAX 32
 PLAST_HIP_KERNEL_PAIR(token_logprob)
 
+/* Layer norm over the last axis: no reference op. For each row x of C elements
+ *   y = (x - mean) / sqrt(mean (x - mean)^2 + eps) * weight + bias.
+ * inputs: [0] x, FLOAT32, FLOAT16 or BFLOAT16, any rank and leading strides, the last axis
+ *             contiguous; its N rows are the leading axes in row-major order;
+ *         [1] weight and [2] bias, C FLOAT32 each;
+ *         [3] stats, 2 N FLOAT32 (written by forward: the row's mean and 1 / sqrt(variance + eps);
+ *             read by backward).
+ * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap.
+ * params.fval: eps, finite and above 0; params.keepdim: 1 makes the backward overwrite the gradients,
+ * 0 accumulate into them. Sums are FLOAT32: the squares of a row's differences from its mean must fit.
+ * A NaN or infinity makes its row NaN.
+ * Backward, for the upstream gradient dy of x's type and shape, with n = (x - mean) * stats[1] and
+ * g = dy * weight, each gradient only where its input requires one:
+ *   x->grad (+)= stats[1] * (g - mean g - n mean(g n))   (x's type and shape, the last axis contiguous,
+ *                                                         rows that do not overlap, nor with dy's or x's)
+ *   weight->grad (+)= sum over rows of dy n,  bias->grad (+)= sum over rows of dy   (C FLOAT32 each)
+ * in an order that is the same on every call. */
+PLAST_HIP_KERNEL_PAIR(layer_norm)
+
+/* Gated linear recurrence along a sequence, each channel by itself: no reference op.
+ *   a = sigmoid(f),  h[t] = a[t] h[t-1] + (1 - a[t]) v[t],  h[-1] = initial.
+ * inputs: [0] f and [1] v, [batch B, time T, channels D], of one type, FLOAT32, FLOAT16 or BFLOAT16; any
+ *             strides of batch and time, the last axis contiguous (halves of one projection, say);
+ *         [2] initial, B D FLOAT32; it may be `last` itself (a state updated token by token);
+ *         [3] lengths, B INT32: the steps of each sequence, taken as 0 .. T. Steps behind a sequence's
+ *             end are padding: whatever they hold, h and the gradients are 0 there;
+ *         [4] last, B D FLOAT32 (written by forward: the state after the sequence's last step; its grad
+ *             is the upstream gradient, none counts as zero);
+ *         [5] states, B ceil(T / PLAST_RECURRENCE_CHUNK) D FLOAT32 (written by forward and read by
+ *             backward: the state before each chunk of steps): only where params.dim is 1.
+ * output: h, of f's type and shape, the last axis contiguous, steps that do not overlap (its grad is the
+ * upstream gradient, none counts as zero).
+ * params.dim: 1 keeps the states for a backward pass, 0 does not; params.keepdim: 1 makes the backward
+ * overwrite the gradients, 0 accumulate into them.
+ * A gate so far out that the smaller of a and 1 - a is below FLOAT32's range (infinities, say) selects:
+ * h[t] is h[t-1] or v[t] whatever the other holds, and no gradient passes to the other. Other NaN and
+ * infinities make the states from there on NaN or infinite.
+ * Backward (needs params.dim 1), each gradient only where its input requires one, of its input's type and
+ * shape (f's and v's with a contiguous last axis and steps that do not overlap):
+ *   dh[t] = dy[t] + a[t+1] dh[t+1], the gradient of `last` added at the sequence's last step;
+ *   v->grad (+)= (1 - a) dh,  f->grad (+)= dh (h[t-1] - v) a (1 - a),  initial->grad (+)= a[0] dh[0].
+ * All results are the same bits on every call. */
+#define PLAST_RECURRENCE_CHUNK 128
+PLAST_HIP_KERNEL_PAIR(gated_recurrence)
+
 #undef PLAST_HIP_KERNEL_PAIR
 
 /* ------------------------------------------------------------------ fused-chain tape --------- */
@@ -196,6 +241,17 @@ void zero_grad_hip(Tensor *t);
  * NULL (no effect on caller-provided ones, which the library never owns). */
 void plast_hip_adam_release(Adam *optimizer, int num_parameters);
 void plast_hip_adamw_release(AdamW *optimizer, int num_parameters);
+
+/* The global norm of the parameters' gradients, sqrt of the sum of all their squares, and their clipping
+ * to it: where it is above max_norm, every gradient times max_norm / norm. norm, one FLOAT32 element in
+ * device memory, gets the norm before clipping (NULL: not wanted). To be called between the backward pass
+ * and the optimizer's step; nothing waits for the GPU in between. Parameters that are NULL or have no grad
+ * are skipped, as by the steps; gradients are contiguous GPU tensors of FLOAT32, FLOAT16 or BFLOAT16, of
+ * one type or several, and must not share memory (a parameter listed twice is refused). A norm that is NaN
+ * or infinite leaves the gradients as they are. max_norm: at least 0, infinity computes the norm alone.
+ * Sums are in 64 bits; all results are the same bits on every call. A call over more than 96 gradients
+ * keeps their table in device memory, as the steps do. No counterpart in the reference. */
+void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm, Tensor *norm);
 
 /* ------------------------------------------------------------------ matmul epilogue pieces ---- */
 

@@ -22,7 +22,7 @@ OP_NAMES = [
     "TAN", "VIEW", "TRANSPOSE", "UNSQUEEZE", "SQUEEZE", "EXPAND", "FLATTEN", "BROADCAST", "MEAN",
     "MIN", "MAX", "SUM", "CONV2D", "MATMUL_RELU", "MATMUL_BIAS_RELU", "CONV_RELU",
     "ARGMAX", "FUSED_ELEMENTWISE", "SOFTMAX_CROSS_ENTROPY", "SOFTMAX", "LOG_SOFTMAX",
-    "TOKEN_LOGPROB",
+    "TOKEN_LOGPROB", "LAYER_NORM", "GATED_RECURRENCE",
 ]
 OP = {name: i for i, name in enumerate(OP_NAMES)}
 
@@ -158,6 +158,7 @@ class Muon(C.Structure):
 
 
 TOP_MAX = 32  # alternatives of token_logprob (PLAST_TOP_MAX)
+RECURRENCE_CHUNK = 128  # steps of gated_recurrence for each state that it keeps (PLAST_RECURRENCE_CHUNK)
 
 
 def params(dim: int = 0, keepdim: int = 0, fval: float = 0.0) -> KernelParams:

@@ -1,0 +1,447 @@
+// layer_norm.hip — layer norm over the last axis and its gradients. For a row x of C elements:
+//   mu = sum x / C,  r = 1 / sqrt(sum (x - mu)^2 / C + eps),  n = (x - mu) r,  y = n w + b,
+//   dx = r (g - sum g / C - n sum (g n) / C) with g = dy w,
+//   dw = sum over rows of dy n,  db = sum over rows of dy.
+// The mean of fp32 sums is off by some 1e-7 of the largest |x|: a row far from zero loses digits of x - mu. So mu is
+// corrected by the mean of the differences d = x - mu themselves, which are small, in the pass that sums their squares:
+//   mu' = mu + m, m = sum d / C,  sum (x - mu')^2 = sum d^2 - C m^2.
+#include <cfloat>
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+#include "rows.hpp"
+
+namespace plast {
+namespace {
+
+constexpr int kRowBlock = 256;  // lanes of a workgroup
+constexpr int kFinLanes = 256;
+
+// What a launch needs of its tensors. map: of x, of y or dy, and of dx.
+struct NormArgs {
+  const void *x, *dy;
+  void *y, *dx;
+  const float *w, *b;
+  float *stats;     // [rows][2]: mu, r
+  float *dw, *db;   // either may be null: not wanted
+  uint32_t first_row, rows, width;  // first_row: of a launch, where one cannot hold all
+  float eps;
+  RowMap<3> map;
+};
+
+template <class T>
+__device__ __forceinline__ void store_any(typename Unit<T>::floats f, T *p) {
+  *reinterpret_cast<typename Unit<T>::any *>(p) = __builtin_convertvector(f, typename Unit<T>::vec);
+}
+
+// A unit's elements from column j on, zeros behind the row's end.
+template <class T>
+__device__ __forceinline__ typename Unit<T>::floats load_cols(const T *row, uint32_t j, uint32_t width) {
+  constexpr uint32_t E = Unit<T>::E;
+  if (j + E <= width) return to_floats<T>(load_unit(row + j));
+  typename Unit<T>::floats f = 0.0f;
+#pragma unroll
+  for (uint32_t e = 0; e < E; ++e)
+    if (j + e < width) f[e] = float(row[j + e]);
+  return f;
+}
+template <class T>
+__device__ __forceinline__ void store_cols(typename Unit<T>::floats f, T *row, uint32_t j, uint32_t width) {
+  constexpr uint32_t E = Unit<T>::E;
+  if (j + E <= width) {
+    store_any<T>(f, row + j);
+    return;
+  }
+#pragma unroll
+  for (uint32_t e = 0; e < E; ++e)
+    if (j + e < width) row[j + e] = T(f[e]);
+}
+// E columns of a weight or bias.
+template <int E>
+struct Cols {
+  typedef float floats __attribute__((ext_vector_type(E)));
+};
+template <int E>
+__device__ __forceinline__ typename Cols<E>::floats load_w(const float *w, uint32_t j, uint32_t width) {
+  typename Cols<E>::floats f = 0.0f;
+  if (j + E <= width) {
+#pragma unroll
+    for (int q = 0; q < E; q += 4) {
+      const f4 v = *reinterpret_cast<const f4u *>(w + j + q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[q + e] = v[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (j + e < width) f[e] = w[j + e];
+  }
+  return f;
+}
+
+// The sums of a and b over a workgroup of W waves, in every lane. `lds` holds 2 W floats that the call before did not use.
+template <int W>
+__device__ __forceinline__ void block_sums(float &a, float &b, float *lds) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    a += __shfl_xor(a, d);
+    b += __shfl_xor(b, d);
+  }
+  if constexpr (W > 1) {
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) lds[2 * wave] = a, lds[2 * wave + 1] = b;
+    __syncthreads();
+    a = lds[0], b = lds[1];
+#pragma unroll
+    for (int w = 1; w < W; ++w) a += lds[2 * w], b += lds[2 * w + 1];
+  }
+}
+
+// ------------------------------------------------------------------------- rows of any length
+
+// A workgroup a row, read three times.
+template <class T>
+__global__ __launch_bounds__(kRowBlock) void fwd_long_kernel(NormArgs A) {
+  typedef typename Unit<T>::floats F;
+  constexpr uint32_t E = Unit<T>::E;
+  __shared__ float lds[2][2 * kRowBlock / 64];
+  const uint32_t row = A.first_row + blockIdx.x, C = A.width;
+  const RowAt<3> at = row_at(A.map, row);
+  const T *x = static_cast<const T *>(A.x) + at.at[0];
+  T *y = static_cast<T *>(A.y) + at.at[1];
+  const uint32_t step = kRowBlock * E, first = threadIdx.x * E;
+  float s = 0.0f, q = 0.0f;
+  for (uint32_t j = first; j < C; j += step) {
+    const F f = load_cols<T>(x, j, C);
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) s += f[e];
+  }
+  block_sums<kRowBlock / 64>(s, q, lds[0]);
+  float mu = s / float(C);
+  s = q = 0.0f;
+  for (uint32_t j = first; j < C; j += step) {
+    const F f = load_cols<T>(x, j, C);
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+      const float d = j + e < C ? f[e] - mu : 0.0f;
+      s += d;
+      q = __builtin_fmaf(d, d, q);
+    }
+  }
+  block_sums<kRowBlock / 64>(s, q, lds[1]);
+  const float m = s / float(C);
+  const float var = __builtin_elementwise_maximum(q / float(C) - m * m, 0.0f);  // NaN stays
+  mu += m;
+  const float r = 1.0f / sqrtf(var + A.eps);
+  if (threadIdx.x == 0) {
+    A.stats[2 * uint64_t(row)] = mu;
+    A.stats[2 * uint64_t(row) + 1] = r;
+  }
+  for (uint32_t j = first; j < C; j += step) {
+    F f = load_cols<T>(x, j, C);
+    const typename Cols<E>::floats w = load_w<E>(A.w, j, C), b = load_w<E>(A.b, j, C);
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) f[e] = __builtin_fmaf((f[e] - mu) * r, w[e], b[e]);
+    store_cols<T>(f, y, j, C);
+  }
+}
+
+// The means of g and of g n of a row, [rows][2]: a workgroup a row.
+template <class T>
+__global__ __launch_bounds__(kRowBlock) void row_means_kernel(NormArgs A, float *means) {
+  typedef typename Unit<T>::floats F;
+  constexpr uint32_t E = Unit<T>::E;
+  __shared__ float lds[2 * kRowBlock / 64];
+  const uint32_t row = A.first_row + blockIdx.x, C = A.width;
+  const RowAt<3> at = row_at(A.map, row);
+  const T *x = static_cast<const T *>(A.x) + at.at[0], *dy = static_cast<const T *>(A.dy) + at.at[1];
+  const float mu = A.stats[2 * uint64_t(row)], r = A.stats[2 * uint64_t(row) + 1];
+  float s = 0.0f, q = 0.0f;
+  for (uint32_t j = threadIdx.x * E; j < C; j += kRowBlock * E) {
+    const F f = load_cols<T>(x, j, C), u = load_cols<T>(dy, j, C);
+    const typename Cols<E>::floats w = load_w<E>(A.w, j, C);
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+      const float g = u[e] * w[e];  // 0 behind the end
+      s += g;
+      if (j + e < C) q = __builtin_fmaf(g, (f[e] - mu) * r, q);
+    }
+  }
+  block_sums<kRowBlock / 64>(s, q, lds);
+  if (threadIdx.x == 0) {
+    means[2 * uint64_t(row)] = s / float(C);
+    means[2 * uint64_t(row) + 1] = q / float(C);
+  }
+}
+
+// Columns of some rows: a workgroup's lanes hold E columns each and go from row to row; blockIdx.x counts the blocks of columns
+// of each piece of `per` rows. dx from the rows' means (null: not wanted), and the piece's share of dw and db to part[piece][2][C].
+template <class T, bool ADD>
+__global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const float *means, float *part, uint32_t blocks,
+                                                            uint32_t per) {
+  typedef typename Unit<T>::floats F;
+  constexpr uint32_t E = Unit<T>::E;
+  typedef typename Cols<E>::floats W;
+  const uint32_t piece = blockIdx.x / blocks, C = A.width;
+  const uint32_t j = ((blockIdx.x - piece * blocks) * kRowBlock + threadIdx.x) * E;
+  if (j >= C) return;
+  const W w = load_w<E>(A.w, j, C);
+  W dw = 0.0f, db = 0.0f;
+  const uint32_t r0 = piece * per, r1 = r0 + per < A.rows ? r0 + per : A.rows;
+  for (uint32_t row = r0; row < r1; ++row) {
+    const RowAt<3> at = row_at(A.map, row);
+    const F f = load_cols<T>(static_cast<const T *>(A.x) + at.at[0], j, C);
+    const F u = load_cols<T>(static_cast<const T *>(A.dy) + at.at[1], j, C);
+    const float mu = A.stats[2 * uint64_t(row)], r = A.stats[2 * uint64_t(row) + 1];
+    F n;
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) {
+      n[e] = (f[e] - mu) * r;
+      dw[e] = __builtin_fmaf(u[e], n[e], dw[e]);
+      db[e] += u[e];
+    }
+    if (means) {
+      T *dx = static_cast<T *>(A.dx) + at.at[2];
+      const float mg = means[2 * uint64_t(row)], mgn = means[2 * uint64_t(row) + 1];
+      F d = 0.0f;
+      if constexpr (ADD) d = load_cols<T>(dx, j, C);
+#pragma unroll
+      for (uint32_t e = 0; e < E; ++e) d[e] += r * (__builtin_fmaf(u[e], w[e], -mg) - n[e] * mgn);
+      store_cols<T>(d, dx, j, C);
+    }
+  }
+  if (part) {
+    float *p = part + uint64_t(piece) * 2 * C;
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e)
+      if (j + e < C) {
+        p[j + e] = dw[e];
+        p[C + j + e] = db[e];
+      }
+  }
+}
+
+// dw and db from the pieces' shares, in the order of the pieces.
+template <bool ADD>
+__global__ __launch_bounds__(kFinLanes) void join_kernel(const float *part, uint32_t pieces, uint32_t width, float *dw,
+                                                         float *db) {
+  const uint64_t i = uint64_t(blockIdx.x) * kFinLanes + threadIdx.x;
+  if (i >= 2 * uint64_t(width)) return;
+  float *to = i < width ? dw : db;
+  if (!to) return;
+  const uint64_t j = i < width ? i : i - width;
+  float s = 0.0f;
+  for (uint32_t p = 0; p < pieces; ++p) s += part[uint64_t(p) * 2 * width + i];
+  to[j] = ADD ? to[j] + s : s;
+}
+
+// ------------------------------------------------------------------------- host
+
+// Whether t lies like x: x's type and shape, a contiguous last axis.
+bool like(const Tensor *t, const Tensor *x, uint64_t n) {
+  const uint64_t last = x->ndim - 1;
+  return t && t->device == GPU && t->dtype == x->dtype && same_shape(t, x) && (n == 0 || t->data) &&
+         (x->shape[last] <= 1 || t->strides[last] == 1);
+}
+
+// Checks x, the weight, the bias, the statistics and eps; fills the row maps (of x, `second` and, where given, dx).
+bool norm_args(NormArgs &A, const Tensor *const *inputs, const Tensor *second, const Tensor *dx, float eps,
+               const char *where) {
+  memset(&A, 0, sizeof A);
+  const Tensor *x = inputs[0], *w = inputs[1], *b = inputs[2], *stats = inputs[3];
+  if (!x || !w || !b || !stats || !second) {
+    report_error(where, "a tensor is NULL");
+    return false;
+  }
+  if (x->device != GPU || !is_float(x) || x->ndim < 1 || x->ndim > PLAST_MAX_NDIM) {
+    report_error(where, "x must be a GPU tensor of FLOAT32, FLOAT16 or BFLOAT16 with a last axis");
+    return false;
+  }
+  const uint64_t C = x->shape[x->ndim - 1], n = numel(x);
+  // the elements of a row, and of the units that its last workgroup has beyond it, stay within 31 bits
+  if (C < 1 || C > (uint64_t(1) << 31) - 65536) {
+    report_error(where, "rows of %llu elements are not supported", (unsigned long long)C);
+    return false;
+  }
+  const uint64_t N = n / C;
+  if (N >= uint64_t(1) << 31) {
+    report_error(where, "%llu rows are not supported", (unsigned long long)N);
+    return false;
+  }
+  if (C > 1 && x->strides[x->ndim - 1] != 1) {
+    report_error(where, "the last axis of x must be contiguous, not strided by %llu",
+                 (unsigned long long)x->strides[x->ndim - 1]);
+    return false;
+  }
+  if (n && !x->data) {
+    report_error(where, "x has no data");
+    return false;
+  }
+  if (!f32_vector(w, C) || !f32_vector(b, C)) {
+    report_error(where, "weight and bias must be contiguous FLOAT32 GPU tensors of %llu elements", (unsigned long long)C);
+    return false;
+  }
+  if (!f32_vector(stats, 2 * N)) {
+    report_error(where, "stats must be a contiguous FLOAT32 GPU tensor of 2 N elements, N = %llu", (unsigned long long)N);
+    return false;
+  }
+  if (!(eps > 0.0f && eps <= FLT_MAX)) {
+    report_error(where, "eps must be finite and above 0, not %g", double(eps));
+    return false;
+  }
+  A.x = x->data;
+  A.w = static_cast<const float *>(w->data);
+  A.b = static_cast<const float *>(b->data);
+  A.stats = static_cast<float *>(stats->data);
+  A.rows = uint32_t(N);
+  A.width = uint32_t(C);
+  A.eps = eps;
+  Space s;
+  s.rank = int(x->ndim) - 1;
+  s.nops = 3;
+  for (int d = 0; d < s.rank; ++d) {
+    s.shape[d] = x->shape[d];
+    s.st[0][d] = int64_t(x->strides[d]);
+    s.st[1][d] = int64_t(second->strides[d]);
+    s.st[2][d] = dx ? int64_t(dx->strides[d]) : 0;
+  }
+  if (!n) return true;
+  collapse(s);
+  A.map.rank = s.rank;
+  for (int d = 0; d < s.rank; ++d) {
+    A.map.ext[d] = MagicDiv::make(uint32_t(s.shape[d]));
+    for (int k = 0; k < 3; ++k) A.map.st[k][d] = s.st[k][d];
+  }
+  return true;
+}
+
+// launch(args, workgroups) for parts of the rows that one grid holds, a workgroup of `threads` lanes for `per` rows.
+template <class F>
+void by_parts(const NormArgs &A, uint64_t per, uint64_t threads, F &&launch) {
+  const uint64_t most = max_blocks(threads) * per;
+  NormArgs part = A;
+  for (uint64_t r = 0; r < A.rows; r += most) {
+    part.first_row = uint32_t(r);
+    part.rows = uint32_t(A.rows - r < most ? A.rows - r : most);
+    launch(part, ceil_div(part.rows, per));
+  }
+}
+
+template <class T>
+void launch_forward(const NormArgs &A) {
+  by_parts(A, 1, kRowBlock, [](const NormArgs &part, unsigned blocks) {
+    fwd_long_kernel<T><<<blocks, kRowBlock, 0, stream()>>>(part);
+  });
+}
+
+// Rows of any length: their means, then columns of pieces of rows, then the pieces' sums.
+template <class T, bool ADD>
+bool launch_long_backward(const NormArgs &A, const char *where) {
+  constexpr uint32_t E = Unit<T>::E;
+  const uint32_t blocks = ceil_div(A.width, kRowBlock * E);
+  // some 2048 workgroups, pieces of 16 rows or more
+  uint64_t pieces = 2048 / blocks;
+  if (pieces < 1) pieces = 1;
+  if (pieces > ceil_div(A.rows, 16)) pieces = ceil_div(A.rows, 16);
+  const uint32_t per = ceil_div(A.rows, pieces);
+  pieces = ceil_div(A.rows, per);
+  const bool sums = A.dw || A.db;
+  const uint64_t means_bytes = A.dx ? (8 * uint64_t(A.rows) + 255) / 256 * 256 : 0;
+  const uint64_t part_bytes = sums ? pieces * 2 * A.width * sizeof(float) : 0;
+  char *work = static_cast<char *>(partials(means_bytes + part_bytes, where));
+  if (!work) return false;
+  float *means = A.dx ? reinterpret_cast<float *>(work) : nullptr;
+  float *part = sums ? reinterpret_cast<float *>(work + means_bytes) : nullptr;
+  if (means)
+    by_parts(A, 1, kRowBlock, [&](const NormArgs &p, unsigned n) {
+      row_means_kernel<T><<<n, kRowBlock, 0, stream()>>>(p, means);
+    });
+  columns_kernel<T, ADD><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
+  if (sums)
+    join_kernel<ADD><<<ceil_div(2 * uint64_t(A.width), kFinLanes), kFinLanes, 0, stream()>>>(part, uint32_t(pieces), A.width,
+                                                                                           A.dw, A.db);
+  return true;
+}
+
+// A gradient that is wanted: null where it is not, reported where it does not fit.
+bool vector_gradient(const Tensor *t, uint64_t n, float **out, const char *where) {
+  *out = nullptr;
+  if (!t->requires_grad) return true;
+  if (!f32_vector(t->grad, n)) {
+    report_error(where, "the gradients of weight and bias must be contiguous FLOAT32 GPU tensors of %llu elements",
+                 (unsigned long long)n);
+    return false;
+  }
+  *out = static_cast<float *>(t->grad->data);
+  return true;
+}
+
+}  // namespace
+}  // namespace plast
+
+using namespace plast;
+
+extern "C" {
+
+void layer_norm_hip_forward(const Tensor **inputs, Tensor *output, KernelParams params) {
+  const char *where = "layer_norm_hip_forward";
+  NormArgs A;
+  if (!norm_args(A, inputs, output, nullptr, params.fval, where)) return;
+  if (!like(output, inputs[0], A.rows) || (numel(output) && overlapping(output))) {
+    report_error(where, "the output must have x's type and shape, a contiguous last axis and rows that do not overlap");
+    return;
+  }
+  if (A.rows == 0 || !ensure_init()) return;
+  A.y = output->data;
+  with_float_type(inputs[0]->dtype, [&](auto t) { launch_forward<decltype(t)>(A); });
+  finish(where);
+}
+
+void layer_norm_hip_backward(Tensor **inputs, const Tensor *output, KernelParams params) {
+  const char *where = "layer_norm_hip_backward";
+  const Tensor *x = inputs[0], *dy = output ? output->grad : nullptr, *dx = x && x->requires_grad ? x->grad : nullptr;
+  if (x && x->requires_grad && !dx) {
+    report_error(where, "x requires a gradient but has none");
+    return;
+  }
+  if (!dy) {
+    report_error(where, "the output has no gradient");
+    return;
+  }
+  NormArgs A;
+  if (!norm_args(A, inputs, dy, dx, params.fval, where)) return;
+  if (!like(dy, x, A.rows)) {
+    report_error(where, "the output's gradient must have x's type and shape and a contiguous last axis");
+    return;
+  }
+  if (dx && (!like(dx, x, A.rows) || (numel(dx) && overlapping(dx)))) {
+    report_error(where, "the gradient of x must have x's type and shape, a contiguous last axis and rows that do not overlap");
+    return;
+  }
+  if (!vector_gradient(inputs[1], A.width, &A.dw, where) || !vector_gradient(inputs[2], A.width, &A.db, where)) return;
+  if (A.dw && A.dw == A.db) {
+    report_error(where, "weight and bias have one gradient");
+    return;
+  }
+  if (!dx && !A.dw && !A.db) return;
+  const bool add = params.keepdim != 1;
+  if (!ensure_init()) return;
+  A.dy = dy->data;
+  A.dx = dx ? dx->data : nullptr;
+  if (A.rows == 0) {  // sums over no rows
+    if (!add) {
+      if (A.dw) zeros_hip(inputs[1]->grad, A.width);
+      if (A.db) zeros_hip(inputs[2]->grad, A.width);
+    }
+    return;
+  }
+  bool ok = false;
+  with_float_type(x->dtype, [&](auto t) {
+    typedef decltype(t) T;
+    ok = add ? launch_long_backward<T, true>(A, where) : launch_long_backward<T, false>(A, where);
+  });
+  if (ok) finish(where);
+}
+
+}  // extern "C"

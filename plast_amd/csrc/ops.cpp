@@ -48,6 +48,8 @@ Op make_op(OP_TYPE t) {
     SLOT(SOFTMAX, softmax)
     SLOT(LOG_SOFTMAX, log_softmax)
     SLOT(TOKEN_LOGPROB, token_logprob)
+    SLOT(LAYER_NORM, layer_norm)
+    SLOT(GATED_RECURRENCE, gated_recurrence)
 #undef SLOT
   default:
     break;  // MATMUL, CONV2D and their fused epilogues have no GPU slot here

@@ -15,7 +15,7 @@ from .abi import KernelParams
 from .runtime import DeviceTensor, lib
 
 # the first of an op's inputs that its forward writes: results beside the output, which later nodes may read
-WRITES_FROM = {"token_logprob": 2}
+WRITES_FROM = {"token_logprob": 2, "layer_norm": 3, "gated_recurrence": 4}
 
 
 class Graph:

@@ -132,6 +132,48 @@ def token_logprob(x: DeviceTensor, tokens: DeviceTensor, temperature: float = 1.
     return inputs, logp, p
 
 
+def layer_norm(x: DeviceTensor, weight: DeviceTensor, bias: DeviceTensor, eps: float = 1e-5,
+               requires_grad: bool = False):
+    """Layer norm over the last axis. Returns (inputs, y, params): `inputs` are [x, weight, bias, stats];
+    backward("layer_norm", inputs, y, params) accumulates into the gradients of x, weight and bias from y's."""
+    shape = abi.shape_of(x.t)
+    stats = DeviceTensor(shape[:-1] + (2,), FLOAT32, zero=False)
+    y = DeviceTensor(shape, x.dtype, requires_grad, zero=False)
+    inputs, p = [x, weight, bias, stats], KernelParams(0, 0, eps)
+    forward("layer_norm", inputs, y, p)
+    return inputs, y, p
+
+
+def gated_recurrence(f: DeviceTensor, v: DeviceTensor, initial: DeviceTensor | None = None,
+                     lengths: DeviceTensor | None = None, requires_grad: bool = False):
+    """h[t] = a[t] h[t-1] + (1 - a[t]) v[t] with a = sigmoid(f), from `initial` (zeros where none is given)
+    over the first `lengths` steps of each sequence (all of them where none are given). Returns
+    (inputs, h, params): `inputs` are [f, v, initial, lengths, last] and, with requires_grad, the states that
+    backward("gated_recurrence", inputs, h, params) starts from; `last` is each sequence's last state."""
+    batch, length, width = abi.shape_of(f.t)
+    if initial is None:
+        initial = DeviceTensor((batch, width))
+    if lengths is None:
+        lengths = DeviceTensor.from_numpy(np.full(batch, length, np.int32))
+    inputs = [f, v, initial, lengths, DeviceTensor((batch, width), FLOAT32, requires_grad, zero=False)]
+    if requires_grad:
+        inputs.append(DeviceTensor((batch, -(-length // abi.RECURRENCE_CHUNK), width), zero=False))
+    h = DeviceTensor((batch, length, width), f.dtype, requires_grad, zero=False)
+    p = KernelParams(int(requires_grad), 0, 0.0)
+    forward("gated_recurrence", inputs, h, p)
+    return inputs, h, p
+
+
+def clip_grad_norm(parameters, max_norm: float) -> DeviceTensor:
+    """Scales the gradients of the parameters to a global norm of at most max_norm (clip_grad_norm_hip);
+    the norm that they had, a tensor of one element."""
+    norm = DeviceTensor((1,), FLOAT32, zero=False)
+    ptrs, keep = abi.tensor_array(*[p.t for p in parameters])
+    lib().clip_grad_norm_hip(ptrs, len(parameters), max_norm, C.byref(norm.t))
+    lib().check("clip_grad_norm")
+    return norm
+
+
 def newton_schulz(g: DeviceTensor, steps: int = 5, a: float = 3.4445, b: float = -4.7750,
                   c: float = 2.0315, eps: float = 1e-7) -> DeviceTensor:
     """The orthogonalised g, a matrix or a stack of matrices (newton_schulz_hip)."""
@@ -160,5 +202,5 @@ def fused(tape: abi.FusedTape, inputs, shape) -> DeviceTensor:
 
 
 __all__ = ["binary", "unary", "reduce", "transpose", "permute", "expand", "softmax_cross_entropy",
-           "token_logprob", "newton_schulz", "bfloat16_bits", "bfloat16_values", "BFLOAT16", "make_tape", "fused", "broadcast_shape", "reduced_shape", "backward", "forward", "lib",
+           "token_logprob", "layer_norm", "gated_recurrence", "clip_grad_norm", "newton_schulz", "bfloat16_bits", "bfloat16_values", "BFLOAT16", "make_tape", "fused", "broadcast_shape", "reduced_shape", "backward", "forward", "lib",
            "DeviceTensor", "np", "INT32"]

@@ -28,7 +28,8 @@ _DT_OF_NP = {np.dtype(np.float32): FLOAT32, np.dtype(np.int32): INT32, np.dtype(
 OP_NAMES = ["add", "sub", "mul", "div", "exp", "log", "neg", "abs", "sin", "cos", "tan",
             "leaky_relu", "sum", "mean", "max", "min", "argmax", "view", "flatten", "squeeze",
             "unsqueeze", "expand", "broadcast", "transpose", "fused_elementwise",
-            "softmax_cross_entropy", "softmax", "log_softmax", "token_logprob"]
+            "softmax_cross_entropy", "softmax", "log_softmax", "token_logprob", "layer_norm",
+            "gated_recurrence"]
 
 
 class PlastHipError(RuntimeError):
@@ -87,6 +88,7 @@ class Library:
             "adam_step_hip": ([C.POINTER(abi.Adam), TensorPP, C.c_int], None),
             "adamw_step_hip": ([C.POINTER(abi.AdamW), TensorPP, C.c_int], None),
             "zero_grad_hip": ([TensorP], None),
+            "clip_grad_norm_hip": ([C.c_void_p, C.c_int, C.c_float, C.c_void_p], None),
             "token_logprob_step_hip": ([C.c_void_p] * 7 + [C.c_float], None),
             "newton_schulz_hip": ([C.c_void_p] * 3, None),
             "muon_step_hip": ([C.c_void_p, C.c_void_p, C.c_int], None),
