@@ -279,10 +279,17 @@ def test_one_sequence_read_as_gate_and_value():
 def test_no_steps():
     from plast_amd import ops
     initial = np.random.RandomState(1).randn(3, 5).astype(np.float32)
-    from plast_amd.runtime import DeviceTensor
+    from plast_amd.runtime import DeviceTensor, backward
     empty = DeviceTensor((3, 0, 5))
     inputs, h, p = ops.gated_recurrence(empty, DeviceTensor((3, 0, 5)), device(initial, "f32"))
     assert np.array_equal(inputs[4].numpy(), initial)
+    for old in (0.0, 3.0):  # what comes for the last state goes to the initial one
+        g, ini = device(np.full((3, 5), old), "f32"), np.ones((3, 5), np.float32)
+        states, lengths = DeviceTensor((3, 0, 5)), DeviceTensor((3,), abi.INT32)
+        ins = [empty, empty, device(ini, "f32", grad=g), lengths, device(ini, "f32", grad=device(initial, "f32")), states]
+        h = DeviceTensor((3, 0, 5), requires_grad=True)
+        backward("gated_recurrence", ins, h, KernelParams(1, 0 if old else 1, 0.0))
+        assert np.array_equal(values(g), initial + np.float32(old))
     for shape in ((0, 4, 5), (3, 4, 0)):
         ops.gated_recurrence(DeviceTensor(shape), DeviceTensor(shape))
 
