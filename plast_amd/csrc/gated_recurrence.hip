@@ -2,11 +2,12 @@
 //   a = sigmoid(f),  z = 1 - a,  h[t] = a[t] h[t-1] + z[t] v[t],
 //   dh[t] = dy[t] + a[t+1] dh[t+1],  dv = z dh,  df = dh (h[t-1] - v) a z,  dh[-1] = a[0] dh[0].
 //
-// A gate that remembers for long has an a next to 1, whose fp32 value has lost the digits of z that say for how long. So a
-// gate is held as its smaller side, s = min(a, z) = e / (1 + e) with e = exp(-|f|), which is exact to some 1e-7 of itself at
-// either end, and as which side that is:
-//   h' = f > 0 ? h + s (v - h) : v + s (h - v).
-// A gate so far out that s is 0 selects: h' is h or v whatever the other holds, NaN too.
+// With e = exp(-|f|), the larger of a and z is 1 / (1 + e) and the smaller e / (1 + e), each to some 1e-7 of itself: next to 1
+// the larger has lost what the smaller holds. A step multiplies the state by a, whose rounding would add up over a long memory
+// if steps were all there is: so runs of eight steps are short cuts of their own, which take what they do to a state from the
+// smaller sides where those count (Share), and every run starts from there.
+// A product with a factor of 0 is 0 whatever the other factor is (v_mul_legacy_f32): a gate so far out that one side is 0
+// selects, and lets no NaN through.
 #include <cfloat>
 #include <cmath>
 #include <cstring>
@@ -34,34 +35,20 @@ struct ScanArgs {
   uint32_t batch, length, width, chunks;
 };
 
-// A gate as its smaller side, with the sign bit set where the value is what the state mostly becomes.
-__device__ __forceinline__ float gate_of(float f) {
-  const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(f));
-  const float s = e * __builtin_amdgcn_rcpf(1.0f + e);
-  return f > 0.0f ? s : -s;
-}
-constexpr float kHold = 0.0f;  // the gate that leaves a state as it is
+extern "C" __device__ float mul_legacy(float, float) __asm("llvm.amdgcn.fmul.legacy");
+
+// Both sides of a gate.
 struct Gate {
-  float s;
-  bool keep;
-  __device__ __forceinline__ explicit Gate(float g) : s(fabsf(g)), keep(!__builtin_signbit(g)) {}
-  // the state after a step
-  __device__ __forceinline__ float next(float h, float v) const {
-    const float base = keep ? h : v, other = keep ? v : h;
-    return s == 0.0f ? base : __builtin_fmaf(s, other, __builtin_fmaf(-s, base, base));
-  }
-  // z x and a x
-  __device__ __forceinline__ float take(float x) const { return side(x, !keep); }
-  __device__ __forceinline__ float hold(float x) const { return side(x, keep); }
-  __device__ __forceinline__ float side(float x, bool larger) const {
-    if (s == 0.0f) return larger ? x : 0.0f;
-    return larger ? __builtin_fmaf(-s, x, x) : s * x;
-  }
-  // d next / d f for upstream dh
-  __device__ __forceinline__ float slope(float dh, float h, float v) const {
-    return s == 0.0f ? 0.0f : dh * (h - v) * __builtin_fmaf(-s, s, s);
+  float a, z;
+  __device__ __forceinline__ explicit Gate(float f) {
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(f));
+    const float large = __builtin_amdgcn_rcpf(1.0f + e), small = e * large;
+    const bool keep = f > 0.0f;
+    a = keep ? large : small;
+    z = keep ? small : large;
   }
 };
+constexpr float kHold = __builtin_huge_valf();  // the gate that leaves a state as it is: a is 1, z is 0
 
 // What a run of steps does to the state x before it: x keeps a share and something is added. Of the share both are kept, A and
 // its complement C: a long memory's A next to 1 has lost the digits of C that count, a short one's C those of A. `code` is the one
@@ -70,12 +57,10 @@ struct Gate {
 struct Share {
   float a = 1.0f, c = 0.0f;
   bool shut = false;
-  __device__ __forceinline__ void step(float g) {
-    const float s = fabsf(g), r = 1.0f - s;
-    const bool keep = !__builtin_signbit(g);
-    c = __builtin_fmaf(keep ? s : r, 1.0f - c, c);
-    a *= keep ? r : s;
-    shut = shut || (s == 0.0f && !keep);
+  __device__ __forceinline__ void step(float ga, float gz) {
+    c = __builtin_fmaf(ga, c, gz);
+    a *= ga;
+    shut = shut || ga == 0.0f;
   }
   __device__ __forceinline__ float code() const {
     return shut ? -0.0f : c < 0.9375f ? c : -fmaxf(a, FLT_MIN);
@@ -106,9 +91,9 @@ struct Quad {
   typedef vec any __attribute__((aligned(sizeof(T))));
 };
 template <class T>
-__device__ __forceinline__ typename Quad<T>::vec load_quad(const T *p, int n) {
+__device__ __forceinline__ typename Quad<T>::vec load_quad(const T *p, int n, float otherwise = 0.0f) {
   if (n >= 4) return *reinterpret_cast<const typename Quad<T>::any *>(p);
-  typename Quad<T>::vec v = T(0.0f);
+  typename Quad<T>::vec v = T(otherwise);
 #pragma unroll
   for (int e = 0; e < 3; ++e)
     if (e < n) v[e] = p[e];
@@ -127,8 +112,8 @@ __device__ __forceinline__ void store_quad(T *p, f4 f, int n) {
 }
 // The same at a lane's offset in bytes from a step's address, which is the same for all lanes.
 template <class T>
-__device__ __forceinline__ typename Quad<T>::vec load_at(const void *step, uint32_t offset, int n) {
-  return load_quad(reinterpret_cast<const T *>(static_cast<const char *>(step) + offset), n);
+__device__ __forceinline__ typename Quad<T>::vec load_at(const void *step, uint32_t offset, int n, float otherwise = 0.0f) {
+  return load_quad(reinterpret_cast<const T *>(static_cast<const char *>(step) + offset), n, otherwise);
 }
 template <class T>
 __device__ __forceinline__ void store_at(void *step, uint32_t offset, f4 f, int n) {
@@ -139,33 +124,27 @@ __device__ __forceinline__ f4 to_f4(typename Quad<T>::vec v) {
   return __builtin_convertvector(v, f4);
 }
 
-// Holds a lane's gates and values as they are from one pass to the next: without it the compiler keeps what it worked out of
-// them, the comparisons' masks above all, in twice the registers.
+// Holds quads as they were read from one pass to the next: without it the compiler keeps their floats, and what was worked out
+// of them, beside them.
 template <class V, uint32_t N>
-__device__ __forceinline__ void keep_as_is(f4 (&g)[N], V (&v)[N]) {
+__device__ __forceinline__ void keep_raw(V (&v)[N]) {
+  typedef uint32_t words __attribute__((ext_vector_type(sizeof(V) / 4)));
 #pragma unroll
   for (uint32_t k = 0; k < N; ++k) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(g[k][e]));
-    if constexpr (sizeof(V) == 16) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) asm volatile("" : "+v"(v[k][e]));
-    } else {
-      typedef uint32_t words __attribute__((ext_vector_type(2)));
-      words w = __builtin_bit_cast(words, v[k]);
-      asm volatile("" : "+v"(w));
-      v[k] = __builtin_bit_cast(V, w);
-    }
+    words w = __builtin_bit_cast(words, v[k]);
+    asm volatile("" : "+v"(w));
+    v[k] = __builtin_bit_cast(V, w);
   }
 }
 
 // ------------------------------------------------------------------------- tiles
 
-// A tile is a chunk of kChunk steps of 64 channels: 16 lanes across, four channels each, and 16 slices of kSteps steps,
-// a slice a lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and
-// each lane goes through its steps again from the state that its slice starts with.
-constexpr uint32_t kLanes = 256, kAcross = 16, kSlices = 16, kSteps = kChunk / kSlices, kTileWidth = 4 * kAcross;
-static_assert(kSteps * kSlices == kChunk, "chunks are whole slices");
+// A tile is a chunk of kChunk steps of 64 channels: 16 lanes across, four channels each, and slices of some steps, a slice a
+// lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and each lane goes
+// through its steps again from the state that its slice starts with. The forward pass has 16 slices of eight steps; the
+// backward pass, which holds twice as much of a step, 32 of four.
+constexpr uint32_t kLanes = 256, kAcross = 16, kTileWidth = 4 * kAcross;
+constexpr uint32_t kFwdSlices = 16, kBwdSlices = 32;
 
 // What tiles of one column of tiles leave for those behind them: `plus` and `code` of the chunk alone, and the state after it.
 // A word's upper half says that it is there, so each word counts by itself.
@@ -243,16 +222,17 @@ __device__ __forceinline__ float look_back(Record *mine, int64_t step, uint32_t 
 struct TileAt {
   uint32_t chunk, b, column;
 };
-// Where a tile lies in a sequence operand: the address of its first slices' step k, and a lane's offset from there.
+// Where a tile lies in a sequence operand: the address of its step k, and the offset from there of a lane whose slice starts
+// `first` steps into the tile.
 template <class T, class P>
 struct TileSeq {
   P p;
   int64_t step;
   uint32_t offset;
-  __device__ __forceinline__ TileSeq(const Seq<P> &s, const TileAt &at, uint32_t slice, uint32_t across) {
+  __device__ __forceinline__ TileSeq(const Seq<P> &s, const TileAt &at, uint32_t first, uint32_t across) {
     p = s.p + (int64_t(at.b) * s.b + int64_t(at.chunk * kChunk) * s.t + at.column * kTileWidth) * int64_t(sizeof(T));
     step = s.t * int64_t(sizeof(T));
-    offset = (slice * kSteps * uint32_t(s.t) + 4 * across) * uint32_t(sizeof(T));
+    offset = (first * uint32_t(s.t) + 4 * across) * uint32_t(sizeof(T));
   }
   __device__ __forceinline__ P at(uint32_t k) const { return p + step * k; }
 };
@@ -262,33 +242,44 @@ __device__ __forceinline__ TileAt tile_at(const ScanArgs &A, uint32_t i, uint32_
 }
 
 template <class T, bool MANY>
-__global__ __launch_bounds__(kLanes, sizeof(T) == 4 ? 3 : 4) void fwd_kernel(ScanArgs A, Look K, uint32_t columns) {
+__global__ __launch_bounds__(kAcross * kFwdSlices, 3) void fwd_kernel(ScanArgs A, Look K, uint32_t columns) {
+  constexpr uint32_t kSlices = kFwdSlices, kSteps = kChunk / kSlices;
   __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth];
   __shared__ uint32_t taken;
   uint32_t tile = blockIdx.x;
   if constexpr (MANY) {
     if (threadIdx.x == 0) taken = atomicAdd(K.ticket, 1u);
     __syncthreads();
-    tile = taken;
+    tile = __builtin_amdgcn_readfirstlane(taken);
   }
   const TileAt at = tile_at(A, tile, columns);
   const uint32_t end = live_steps(A, at.b), across = threadIdx.x & (kAcross - 1), slice = threadIdx.x / kAcross;
   const uint32_t c = at.column * kTileWidth + 4 * across, t0 = at.chunk * kChunk + slice * kSteps;
   const int n = int(A.width) - int(c);
-  const TileSeq<T, char *> y(A.h, at, slice, across);
+  const TileSeq<T, char *> y(A.h, at, slice * kSteps, across);
   if (at.chunk > 0 && at.chunk * kChunk >= end) {  // padding alone
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k)
       if (t0 + k < A.length) store_at<T>(y.at(k), y.offset, f4(0.0f), n);
     return;
   }
-  const TileSeq<T, const char *> f(A.f, at, slice, across), v(A.v, at, slice, across);
+  const TileSeq<T, const char *> f(A.f, at, slice * kSteps, across), v(A.v, at, slice * kSteps, across);
   typename Quad<T>::vec gates[kSteps], val[kSteps];
+  // a tile of channels and steps that are all there takes no bounds
+  const bool whole = (at.column + 1) * kTileWidth <= A.width && (at.chunk + 1) * kChunk <= end;
+  if (whole) {
 #pragma unroll
-  for (uint32_t k = 0; k < kSteps; ++k) {
-    const int m = t0 + k < end ? n : 0;
-    gates[k] = load_at<T>(f.at(k), f.offset, m);
-    val[k] = load_at<T>(v.at(k), v.offset, m);
+    for (uint32_t k = 0; k < kSteps; ++k) {
+      gates[k] = load_at<T>(f.at(k), f.offset, 4);
+      val[k] = load_at<T>(v.at(k), v.offset, 4);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t k = 0; k < kSteps; ++k) {
+      const int m = t0 + k < end ? n : 0;
+      gates[k] = load_at<T>(f.at(k), f.offset, m, kHold);
+      val[k] = load_at<T>(v.at(k), v.offset, m);
+    }
   }
   // wave 0's lanes are the tile's channels while the slices are joined
   const uint32_t lane = threadIdx.x, channel = at.column * kTileWidth + lane;
@@ -305,17 +296,18 @@ __global__ __launch_bounds__(kLanes, sizeof(T) == 4 ? 3 : 4) void fwd_kernel(Sca
       start = A.initial[uint64_t(at.b) * A.width + channel];
     }
   }
-  f4 g[kSteps];
+  f4 keep[kSteps], add[kSteps], sum = 0.0f;
   Share share[4];
-  f4 sum = 0.0f;
 #pragma unroll
   for (uint32_t k = 0; k < kSteps; ++k) {
     const f4 x = to_f4<T>(gates[k]), u = to_f4<T>(val[k]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      g[k][e] = t0 + k < end ? gate_of(x[e]) : kHold;
-      share[e].step(g[k][e]);
-      sum[e] = Gate(g[k][e]).next(sum[e], u[e]);
+      const Gate g(x[e]);
+      keep[k][e] = g.a;
+      add[k][e] = mul_legacy(g.z, u[e]);
+      share[e].step(g.a, g.z);
+      sum[e] = mul_legacy(g.a, sum[e]) + add[k][e];
     }
   }
   f4 code;
@@ -324,18 +316,17 @@ __global__ __launch_bounds__(kLanes, sizeof(T) == 4 ? 3 : 4) void fwd_kernel(Sca
   *reinterpret_cast<f4 *>(&codes[slice][4 * across]) = code;
   *reinterpret_cast<f4 *>(&plus[slice][4 * across]) = sum;
   __syncthreads();
-  keep_as_is(g, val);
   if (joins) {
     float cs[kSlices], ps[kSlices];
 #pragma unroll
     for (uint32_t i = 0; i < kSlices; ++i) cs[i] = codes[i][lane], ps[i] = plus[i][lane];
     if constexpr (MANY) {
-      Share whole;
-      float add = 0.0f;
+      Share joined;
+      float all = 0.0f;
 #pragma unroll
-      for (uint32_t i = 0; i < kSlices; ++i) whole.join(cs[i]), add = apply(cs[i], ps[i], add);
-      if (at.chunk > 0) start = look_back(mine, int64_t(A.batch) * columns, at.chunk, lane, ready, whole.code(), add);
-      put_word(&(K.records + tile)->state[lane], apply(whole.code(), add, start));
+      for (uint32_t i = 0; i < kSlices; ++i) joined.join(cs[i]), all = apply(cs[i], ps[i], all);
+      if (at.chunk > 0) start = look_back(mine, int64_t(A.batch) * columns, at.chunk, lane, ready, joined.code(), all);
+      put_word(&(K.records + tile)->state[lane], apply(joined.code(), all, start));
     }
     if (A.states && inside) A.states[(uint64_t(at.b) * A.chunks + at.chunk) * A.width + channel] = start;
     if (end == 0 && inside) A.last[uint64_t(at.b) * A.width + channel] = start;
@@ -346,13 +337,21 @@ __global__ __launch_bounds__(kLanes, sizeof(T) == 4 ? 3 : 4) void fwd_kernel(Sca
     }
   }
   __syncthreads();
-  keep_as_is(g, val);
   f4 h = *reinterpret_cast<const f4 *>(&plus[slice][4 * across]);
+  if (whole) {
+#pragma unroll
+    for (uint32_t k = 0; k < kSteps; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = mul_legacy(keep[k][e], h[e]) + add[k][e];
+      store_at<T>(y.at(k), y.offset, h, 4);
+    }
+    if (t0 + kSteps == end) store_quad<float>(A.last + uint64_t(at.b) * A.width + c, h, 4);
+    return;
+  }
 #pragma unroll
   for (uint32_t k = 0; k < kSteps; ++k) {
-    const f4 u = to_f4<T>(val[k]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = Gate(g[k][e]).next(h[e], u[e]);
+    for (int e = 0; e < 4; ++e) h[e] = mul_legacy(keep[k][e], h[e]) + add[k][e];
     if (t0 + k < A.length) store_at<T>(y.at(k), y.offset, t0 + k < end ? h : f4(0.0f), n);
     if (t0 + k + 1 == end) store_quad<float>(A.last + uint64_t(at.b) * A.width + c, h, n);
   }
@@ -365,21 +364,22 @@ __device__ __forceinline__ void put_at(char *step, uint32_t offset, f4 f, int n)
 }
 
 template <class T, bool ADD, bool MANY>
-__global__ __launch_bounds__(kLanes, 2) void bwd_kernel(ScanArgs A, Look K, uint32_t columns) {
+__global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A, Look K, uint32_t columns) {
+  constexpr uint32_t kSlices = kBwdSlices, kSteps = kChunk / kSlices;
   __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth], back[kSlices][kTileWidth];
   __shared__ uint32_t taken;
   uint32_t tile = blockIdx.x;
   if constexpr (MANY) {
     if (threadIdx.x == 0) taken = atomicAdd(K.ticket, 1u);
     __syncthreads();
-    tile = taken;
+    tile = __builtin_amdgcn_readfirstlane(taken);
   }
   TileAt at = tile_at(A, tile, columns);
   at.chunk = A.chunks - 1 - at.chunk;
   const uint32_t end = live_steps(A, at.b), across = threadIdx.x & (kAcross - 1), slice = threadIdx.x / kAcross;
   const uint32_t c = at.column * kTileWidth + 4 * across, t0 = at.chunk * kChunk + slice * kSteps;
   const int n = int(A.width) - int(c);
-  const TileSeq<T, char *> df(A.df, at, slice, across), dv(A.dv, at, slice, across);
+  const TileSeq<T, char *> df(A.df, at, slice * kSteps, across), dv(A.dv, at, slice * kSteps, across);
   if (at.chunk > 0 && at.chunk * kChunk >= end) {  // padding alone
     if (!ADD)
 #pragma unroll
@@ -390,14 +390,24 @@ __global__ __launch_bounds__(kLanes, 2) void bwd_kernel(ScanArgs A, Look K, uint
         }
     return;
   }
-  const TileSeq<T, const char *> f(A.f, at, slice, across), v(A.v, at, slice, across), dy(A.dy, at, slice, across);
+  const TileSeq<T, const char *> f(A.f, at, slice * kSteps, across), v(A.v, at, slice * kSteps, across), dy(A.dy, at, slice * kSteps, across);
   typename Quad<T>::vec gates[kSteps], val[kSteps], up[kSteps];
+  const bool whole = (at.column + 1) * kTileWidth <= A.width && (at.chunk + 1) * kChunk <= end && A.dy.p && A.df.p && A.dv.p;
+  if (whole) {
 #pragma unroll
-  for (uint32_t k = 0; k < kSteps; ++k) {
-    const int m = t0 + k < end ? n : 0;
-    gates[k] = load_at<T>(f.at(k), f.offset, m);
-    val[k] = load_at<T>(v.at(k), v.offset, m);
-    up[k] = load_at<T>(dy.at(k), dy.offset, A.dy.p ? m : 0);
+    for (uint32_t k = 0; k < kSteps; ++k) {
+      gates[k] = load_at<T>(f.at(k), f.offset, 4);
+      val[k] = load_at<T>(v.at(k), v.offset, 4);
+      up[k] = load_at<T>(dy.at(k), dy.offset, 4);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t k = 0; k < kSteps; ++k) {
+      const int m = t0 + k < end ? n : 0;
+      gates[k] = load_at<T>(f.at(k), f.offset, m, kHold);
+      val[k] = load_at<T>(v.at(k), v.offset, m);
+      up[k] = load_at<T>(dy.at(k), dy.offset, A.dy.p ? m : 0);
+    }
   }
   // waves 0 and 1 join the slices, one forward and one from the end
   const uint32_t lane = threadIdx.x & 63, channel = at.column * kTileWidth + lane, wave = threadIdx.x / 64;
@@ -407,27 +417,28 @@ __global__ __launch_bounds__(kLanes, 2) void bwd_kernel(ScanArgs A, Look K, uint
   uint64_t ready = 0;
   if (wave == 0 && inside && end) start = A.states[(uint64_t(at.b) * A.chunks + at.chunk) * A.width + channel];
   if (MANY && wave == 1 && !last) ready = get_shared(&(K.records + tile - A.batch * columns)->state[lane]);
-  f4 g[kSteps], sum = 0.0f, rev = 0.0f;
   f4 dlast = 0.0f;
   if (A.dlast && end && t0 < end && end <= t0 + kSteps) dlast = load_quad<float>(A.dlast + uint64_t(at.b) * A.width + c, n);
+  f4 keep[kSteps], into[kSteps], sum = 0.0f, rev = 0.0f;
   Share share[4];
 #pragma unroll
   for (uint32_t k = 0; k < kSteps; ++k) {
     const f4 x = to_f4<T>(gates[k]), u = to_f4<T>(val[k]);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      g[k][e] = t0 + k < end ? gate_of(x[e]) : kHold;
-      share[e].step(g[k][e]);
-      sum[e] = Gate(g[k][e]).next(sum[e], u[e]);
+      const Gate g(x[e]);
+      keep[k][e] = g.a;
+      into[k][e] = g.z;
+      share[e].step(g.a, g.z);
+      sum[e] = mul_legacy(g.a, sum[e]) + mul_legacy(g.z, u[e]);
     }
   }
-  keep_as_is(g, up);
 #pragma unroll
   for (uint32_t k = kSteps; k-- > 0;) {
     f4 d = to_f4<T>(up[k]);
     if (t0 + k + 1 == end) d += dlast;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) rev[e] = Gate(g[k][e]).hold(rev[e] + d[e]);
+    for (int e = 0; e < 4; ++e) rev[e] = mul_legacy(keep[k][e], rev[e] + d[e]);
   }
   f4 code;
 #pragma unroll
@@ -436,33 +447,31 @@ __global__ __launch_bounds__(kLanes, 2) void bwd_kernel(ScanArgs A, Look K, uint
   *reinterpret_cast<f4 *>(&plus[slice][4 * across]) = sum;
   *reinterpret_cast<f4 *>(&back[slice][4 * across]) = rev;
   __syncthreads();
-  keep_as_is(g, val);
+  keep_raw(val);
+  keep_raw(up);
   if (wave == 0) {
-    float cs[kSlices], ps[kSlices];
-#pragma unroll
-    for (uint32_t i = 0; i < kSlices; ++i) cs[i] = codes[i][lane], ps[i] = plus[i][lane];
-#pragma unroll
+#pragma unroll 8
     for (uint32_t i = 0; i < kSlices; ++i) {
+      const float after = apply(codes[i][lane], plus[i][lane], start);
       plus[i][lane] = start;
-      start = apply(cs[i], ps[i], start);
+      start = after;
     }
   } else if (wave == 1) {
-    float cs[kSlices], ps[kSlices];
-#pragma unroll
-    for (uint32_t i = 0; i < kSlices; ++i) cs[i] = codes[i][lane], ps[i] = back[i][lane];
     float from = 0.0f;  // a dh of the step behind the tile
     if constexpr (MANY) {
-      Share whole;
-      float add = 0.0f;
-#pragma unroll
-      for (uint32_t i = kSlices; i-- > 0;) whole.join(cs[i]), add = apply(cs[i], ps[i], add);
-      if (!last) from = look_back(K.records + tile, int64_t(A.batch) * columns, A.chunks - 1 - at.chunk, lane, ready, whole.code(), add);
-      put_word(&(K.records + tile)->state[lane], apply(whole.code(), add, from));
+      Share joined;
+      float all = 0.0f;
+#pragma unroll 8
+      for (uint32_t i = kSlices; i-- > 0;) joined.join(codes[i][lane]), all = apply(codes[i][lane], back[i][lane], all);
+      if (!last)
+        from = look_back(K.records + tile, int64_t(A.batch) * columns, A.chunks - 1 - at.chunk, lane, ready, joined.code(), all);
+      put_word(&(K.records + tile)->state[lane], apply(joined.code(), all, from));
     }
-#pragma unroll
+#pragma unroll 8
     for (uint32_t i = kSlices; i-- > 0;) {
+      const float after = apply(codes[i][lane], back[i][lane], from);
       back[i][lane] = from;
-      from = apply(cs[i], ps[i], from);
+      from = after;
     }
     if (at.chunk == 0 && A.dinitial && inside) {
       if (end == 0 && A.dlast) from = A.dlast[state_at];
@@ -470,35 +479,43 @@ __global__ __launch_bounds__(kLanes, 2) void bwd_kernel(ScanArgs A, Look K, uint
     }
   }
   __syncthreads();
-  keep_as_is(g, val);
   f4 h = *reinterpret_cast<const f4 *>(&plus[slice][4 * across]);
   f4 d = *reinterpret_cast<const f4 *>(&back[slice][4 * across]);
-  f4 before[kSteps];
-#pragma unroll
-  for (uint32_t k = 0; k < kSteps; ++k) {
-    const f4 u = to_f4<T>(val[k]);
-    before[k] = h;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = Gate(g[k][e]).next(h[e], u[e]);
-  }
-  keep_as_is(g, val);
+  f4 dh[kSteps];
+  keep_raw(up);
+  keep_raw(val);
 #pragma unroll
   for (uint32_t k = kSteps; k-- > 0;) {
-    const uint32_t t = t0 + k;
-    const f4 u = to_f4<T>(val[k]);
-    f4 to_f = 0.0f, to_v = 0.0f;
-    if (t < end) {
-      d += to_f4<T>(up[k]);
-      if (t + 1 == end) d += dlast;
+    dh[k] = d + to_f4<T>(up[k]);
+    if (t0 + k + 1 == end) dh[k] += dlast;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const Gate gate(g[k][e]);
-        to_v[e] = gate.take(d[e]);
-        to_f[e] = gate.slope(d[e], before[k][e], u[e]);
-        d[e] = gate.hold(d[e]);
-      }
+    for (int e = 0; e < 4; ++e) d[e] = mul_legacy(keep[k][e], dh[k][e]);
+  }
+  const auto gradients = [&](uint32_t k, f4 &to_f, f4 &to_v) {
+    const f4 u = to_f4<T>(val[k]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      to_v[e] = mul_legacy(into[k][e], dh[k][e]);
+      to_f[e] = mul_legacy(keep[k][e] * into[k][e], dh[k][e] * (h[e] - u[e]));
+      h[e] = mul_legacy(keep[k][e], h[e]) + mul_legacy(into[k][e], u[e]);
     }
-    if (t < (ADD ? end : A.length)) {
+  };
+  if (whole) {
+#pragma unroll
+    for (uint32_t k = 0; k < kSteps; ++k) {
+      f4 to_f, to_v;
+      gradients(k, to_f, to_v);
+      put_at<T, ADD>(df.at(k), df.offset, to_f, 4);
+      put_at<T, ADD>(dv.at(k), dv.offset, to_v, 4);
+    }
+    return;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < kSteps; ++k) {
+    f4 to_f, to_v;
+    gradients(k, to_f, to_v);
+    if (t0 + k >= end) to_f = to_v = f4(0.0f);
+    if (t0 + k < (ADD ? end : A.length)) {
       if (A.df.p) put_at<T, ADD>(df.at(k), df.offset, to_f, n);
       if (A.dv.p) put_at<T, ADD>(dv.at(k), dv.offset, to_v, n);
     }
@@ -523,7 +540,10 @@ __global__ __launch_bounds__(kLanes) void few_kernel(ScanArgs A, uint32_t quads)
       const f4 x = to_f4<T>(load_quad<T>(reinterpret_cast<const T *>(A.f.p) + int64_t(b) * A.f.b + int64_t(t) * A.f.t + c, n));
       const f4 u = to_f4<T>(load_quad<T>(reinterpret_cast<const T *>(A.v.p) + int64_t(b) * A.v.b + int64_t(t) * A.v.t + c, n));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = Gate(gate_of(x[e])).next(h[e], u[e]);
+      for (int e = 0; e < 4; ++e) {
+        const Gate g(x[e]);
+        h[e] = mul_legacy(g.a, h[e]) + mul_legacy(g.z, u[e]);
+      }
     }
     store_quad<T>(reinterpret_cast<T *>(A.h.p) + int64_t(b) * A.h.b + int64_t(t) * A.h.t + c, t < end ? h : f4(0.0f), n);
   }
@@ -610,7 +630,7 @@ template <class F>
 bool by_tiles(const ScanArgs &A, const char *where, F &&launch) {
   const uint32_t columns = ceil_div(A.width, kTileWidth);
   const uint64_t tiles = uint64_t(A.batch) * columns * A.chunks;
-  if (tiles > max_blocks(kLanes)) {
+  if (tiles > max_blocks(kAcross * kBwdSlices)) {
     report_error(where, "%llu chunks of 64 channels are not supported", (unsigned long long)tiles);
     return false;
   }
@@ -628,16 +648,16 @@ bool launch_forward(const ScanArgs &A, const char *where) {
     return true;
   }
   return by_tiles(A, where, [&](uint32_t columns, unsigned tiles, const Look &K, bool many) {
-    if (many) fwd_kernel<T, true><<<tiles, kLanes, 0, stream()>>>(A, K, columns);
-    else fwd_kernel<T, false><<<tiles, kLanes, 0, stream()>>>(A, K, columns);
+    if (many) fwd_kernel<T, true><<<tiles, kAcross * kFwdSlices, 0, stream()>>>(A, K, columns);
+    else fwd_kernel<T, false><<<tiles, kAcross * kFwdSlices, 0, stream()>>>(A, K, columns);
   });
 }
 template <class T, bool ADD>
 bool launch_backward(ScanArgs A, const char *where) {
   if (A.length == 0) A.chunks = 1;  // what comes for the last state is the initial one's
   return by_tiles(A, where, [&](uint32_t columns, unsigned tiles, const Look &K, bool many) {
-    if (many) bwd_kernel<T, ADD, true><<<tiles, kLanes, 0, stream()>>>(A, K, columns);
-    else bwd_kernel<T, ADD, false><<<tiles, kLanes, 0, stream()>>>(A, K, columns);
+    if (many) bwd_kernel<T, ADD, true><<<tiles, kAcross * kBwdSlices, 0, stream()>>>(A, K, columns);
+    else bwd_kernel<T, ADD, false><<<tiles, kAcross * kBwdSlices, 0, stream()>>>(A, K, columns);
   });
 }
 
