@@ -447,6 +447,10 @@ void plast_hip_set_sync(int sync);
  * whose CPU bias gradient accumulates with omp atomics (kernel_macros.h:292-297). */
 void plast_hip_set_deterministic(int on);
 int plast_hip_deterministic(void);
+/* How often a workgroup of the gated recurrence looks for what the chunk of steps before its own leaves before
+ * it works that chunk out itself (default 4096, some milliseconds; 0: at once). Results are the same bits
+ * with every value. No counterpart in the reference. */
+void plast_hip_set_recurrence_looks(int looks);
 /* Wait for all work queued on the library stream. Returns 0 on success. */
 int plast_hip_synchronize(void);
 /* Graph capture of launch-bound work. Between plast_hip_capture_begin() and

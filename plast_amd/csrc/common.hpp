@@ -338,8 +338,11 @@ bool capturing();
 bool ensure_init();
 // Device scratch of at least `bytes`, owned by the library and reused across calls. Slot 0 holds
 // the reduction engine's partial summaries; slot 1 an op's own temporaries (tie counts, extremes);
-// slot 2 the staging buffer of host transfers of strided tensors.
+// slot 2 the staging buffer of host transfers of strided tensors; kRecordSlot, filled with zeros when it is made, the records of
+// chunks that no other call writes.
+constexpr int kRecordSlot = 3;
 void *workspace(size_t bytes, int slot = 0);
+size_t workspace_bytes(int slot);
 // A fixed device array of kScratchFloats floats (32 MiB: the column sums of 256 workgroups over rows
 // of up to 32768 floats), each GPU's own until the process ends: its address on the library's device
 // (null, after reporting, when the lookup fails).

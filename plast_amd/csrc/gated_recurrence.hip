@@ -63,7 +63,7 @@ struct Share {
     shut = shut || ga == 0.0f;
   }
   __device__ __forceinline__ float code() const {
-    return shut ? -0.0f : c < 0.9375f ? c : -fmaxf(a, FLT_MIN);
+    return shut ? -0.0f : c < 0.9375f ? c : -fmaxf(a, 0x1p-149f);
   }
   // the share of this run and one behind it
   __device__ __forceinline__ void join(float code) {
@@ -92,7 +92,7 @@ struct Quad {
 };
 template <class T>
 __device__ __forceinline__ typename Quad<T>::vec load_quad(const T *p, int n, float otherwise = 0.0f) {
-  if (n >= 4) return *reinterpret_cast<const typename Quad<T>::any *>(p);
+  if (n >= 4) return __builtin_nontemporal_load(reinterpret_cast<const typename Quad<T>::any *>(p));
   typename Quad<T>::vec v = T(otherwise);
 #pragma unroll
   for (int e = 0; e < 3; ++e)
@@ -103,7 +103,7 @@ template <class T>
 __device__ __forceinline__ void store_quad(T *p, f4 f, int n) {
   const typename Quad<T>::vec v = __builtin_convertvector(f, typename Quad<T>::vec);
   if (n >= 4) {
-    *reinterpret_cast<typename Quad<T>::any *>(p) = v;
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Quad<T>::any *>(p));
     return;
   }
 #pragma unroll
@@ -139,135 +139,204 @@ __device__ __forceinline__ void keep_raw(V (&v)[N]) {
 
 // ------------------------------------------------------------------------- tiles
 
-// A tile is a chunk of kChunk steps of 64 channels: 16 lanes across, four channels each, and slices of some steps, a slice a
+// A tile is a chunk of kChunk steps of some channels: lanes across, four channels each, and slices of a few steps, a slice a
 // lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and each lane goes
-// through its steps again from the state that its slice starts with. The forward pass has 16 slices of eight steps; the
-// backward pass, which holds twice as much of a step, 32 of four.
-constexpr uint32_t kLanes = 256, kAcross = 16, kTileWidth = 4 * kAcross;
-constexpr uint32_t kFwdSlices = 16, kBwdSlices = 32;
+// through its steps again from the state that its slice starts with.
+template <uint32_t ACROSS, uint32_t STEPS>
+struct Shape {
+  static constexpr uint32_t kAcross = ACROSS, kSteps = STEPS, kWidth = 4 * ACROSS, kSlices = kChunk / STEPS, kLanes = ACROSS * kSlices;
+  static_assert(kSteps * kSlices == kChunk && kWidth % 64 == 0, "chunks are whole slices, channels whole waves");
+};
+typedef Shape<32, 8> Fwd;
+typedef Shape<16, 4> Bwd;  // holds twice as much of a step
 
-// What tiles of one column of tiles leave for those behind them: `plus` and `code` of the chunk alone, and the state after it.
-// A word's upper half says that it is there, so each word counts by itself.
+// What a chunk leaves of 64 channels for those behind it: `plus` and `code` of the chunk alone, and the state after it. A word's
+// upper half is the launch's tag where the word is there, so each word counts by itself.
 struct Record {
-  uint64_t code[kTileWidth], plus[kTileWidth], state[kTileWidth];
+  uint64_t code[64], plus[64], state[64];
 };
 struct Look {
-  uint32_t *ticket;
-  Record *records;  // [chunks][batch, columns]
+  Record *records;  // [chunks][64 channels of the columns of tiles]
+  uint32_t tag, most;
+  __device__ __forceinline__ void put(uint64_t *p, float v) const { put_shared(p, uint64_t(tag) << 32 | __float_as_uint(v)); }
+  __device__ __forceinline__ bool there(uint64_t w) const { return uint32_t(w >> 32) == tag; }
+  // a word that has been sent, and may be under way
+  __device__ __forceinline__ float get(const uint64_t *p) const {
+    uint64_t w = get_shared(p);
+    while (!there(w)) w = get_shared(p);
+    return __uint_as_float(uint32_t(w));
+  }
 };
-__device__ __forceinline__ void put_word(uint64_t *p, float v) { put_shared(p, uint64_t(1) << 32 | __float_as_uint(v)); }
-__device__ __forceinline__ bool is_there(uint64_t w) { return (w >> 32) != 0; }
-__device__ __forceinline__ float word_value(uint64_t w) { return __uint_as_float(uint32_t(w)); }
 
-__global__ __launch_bounds__(kLanes) void clear_kernel(uint64_t *p, uint64_t n) {
-  const uint64_t i = uint64_t(blockIdx.x) * kLanes + threadIdx.x;
+__global__ __launch_bounds__(256) void clear_kernel(uint64_t *p, uint64_t n) {
+  const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i < n) p[i] = 0;
 }
 
-// The state that a tile starts with, by one wave, a lane a channel: of the `n` tiles before it (`step` records apart) the
-// nearest whose state is there is found, and the shares of those between are applied to it one after the other, as they
-// themselves do: the bits do not depend on which it was.
-// Tiles take tickets in the order of their chunks, so those before are at work or done, and each leaves its own share before it
-// waits for anything: every wait ends. kMostLooks, some seconds, bounds it all the same; the state is NaN then.
-constexpr uint32_t kMostLooks = 1u << 22, kWindow = 4;
-__device__ __forceinline__ float look_back(Record *mine, int64_t step, uint32_t n, uint32_t lane, uint64_t ready, float code,
-                                           float plus) {
-  if (__all(is_there(ready))) return word_value(ready);
-  put_word(&mine->code[lane], code);
-  put_word(&mine->plus[lane], plus);
-  uint32_t d0 = 1, looks = 0;  // the nearest tile of a window is d0 before this one
-  for (;;) {
-    uint64_t s[kWindow], c[kWindow], p[kWindow];
-#pragma unroll
-    for (uint32_t w = 0; w < kWindow; ++w) {
-      const Record *r = mine - step * int64_t(d0 + w < n ? d0 + w : n);
-      s[w] = get_shared(&r->state[lane]);
-      c[w] = get_shared(&r->code[lane]);
-      p[w] = get_shared(&r->plus[lane]);
-    }
-    uint32_t at = 0;  // tiles of the window whose shares are there and states are not
-    bool found = false, whole = true;
-    float x = 0.0f;
-#pragma unroll
-    for (uint32_t w = 0; w < kWindow; ++w)
-      if (!found && whole) {
-        found = __all(is_there(s[w]));
-        if (found) x = word_value(s[w]);
-        else if (__all(is_there(c[w]) && is_there(p[w]))) ++at;
-        else whole = false;
-      }
-    if (found) {
-#pragma unroll
-      for (uint32_t w = kWindow; w-- > 0;)
-        if (w < at) x = apply(word_value(c[w]), word_value(p[w]), x);
-      for (uint32_t d = d0; d > 1;) {  // the windows before, which are there
-        d -= kWindow;
-#pragma unroll
-        for (uint32_t w = 0; w < kWindow; ++w) {
-          const Record *r = mine - step * int64_t(d + w);
-          c[w] = get_shared(&r->code[lane]);
-          p[w] = get_shared(&r->plus[lane]);
-        }
-#pragma unroll
-        for (uint32_t w = kWindow; w-- > 0;) x = apply(word_value(c[w]), word_value(p[w]), x);
-      }
-      return x;
-    }
-    if (whole) d0 += kWindow;
-    else if (++looks == kMostLooks) return __builtin_nanf("");
-    else __builtin_amdgcn_s_sleep(1);
-  }
-}
-
-struct TileAt {
-  uint32_t chunk, b, column;
+// Which tile a workgroup works on. Workgroups are dispatched in their order, round robin over the eight XCDs: an XCD's take
+// columns of its own (`each`; 0: all take all), chunk by chunk, so that what lies side by side is read side by side.
+struct Tile {
+  uint32_t chunk, column, b, c0, end;  // c0: first channel; end: steps of the sequence that are there
+  bool none, dead, whole;  // no tile; padding alone; all of its steps and channels there, so that it needs no bounds
 };
+template <class S, bool BACK>
+__device__ __forceinline__ Tile tile_at(const ScanArgs &A, uint32_t across, uint32_t each) {
+  const uint32_t columns = A.batch * across, i = blockIdx.x;
+  Tile t;
+  if (each) {
+    t.chunk = i / 8 / each;
+    t.column = i % 8 * each + i / 8 % each;
+  } else {
+    t.chunk = i / columns;
+    t.column = i - t.chunk * columns;
+  }
+  t.none = t.column >= columns;
+  if (t.none) return t;
+  if (BACK) t.chunk = A.chunks - 1 - t.chunk;
+  t.b = t.column / across;
+  t.c0 = (t.column - t.b * across) * S::kWidth;
+  t.end = live_steps(A, t.b);
+  t.dead = t.chunk > 0 && t.chunk * kChunk >= t.end;
+  t.whole = t.c0 + S::kWidth <= A.width && (t.chunk + 1) * kChunk <= t.end;
+  return t;
+}
 // Where a tile lies in a sequence operand: the address of its step k, and the offset from there of a lane whose slice starts
-// `first` steps into the tile.
+// `first` steps into the tile and whose channels are `c` into it.
 template <class T, class P>
 struct TileSeq {
   P p;
   int64_t step;
   uint32_t offset;
-  __device__ __forceinline__ TileSeq(const Seq<P> &s, const TileAt &at, uint32_t first, uint32_t across) {
-    p = s.p + (int64_t(at.b) * s.b + int64_t(at.chunk * kChunk) * s.t + at.column * kTileWidth) * int64_t(sizeof(T));
+  __device__ __forceinline__ TileSeq(const Seq<P> &s, const Tile &t, uint32_t first, uint32_t c) {
+    p = s.p + (int64_t(t.b) * s.b + int64_t(t.chunk * kChunk) * s.t + t.c0) * int64_t(sizeof(T));
     step = s.t * int64_t(sizeof(T));
-    offset = (first * uint32_t(s.t) + 4 * across) * uint32_t(sizeof(T));
+    offset = (first * uint32_t(s.t) + c) * uint32_t(sizeof(T));
   }
   __device__ __forceinline__ P at(uint32_t k) const { return p + step * k; }
 };
-__device__ __forceinline__ TileAt tile_at(const ScanArgs &A, uint32_t i, uint32_t columns) {
-  const uint32_t row = A.batch * columns, chunk = i / row, rest = i - chunk * row, b = rest / columns;
-  return {chunk, b, rest - b * columns};
+
+// A channel's chunk worked out by one lane, bit for bit as the chunk's own tile does.
+template <class T, class S, bool BACK>
+__device__ __forceinline__ void chunk_share(const ScanArgs &A, const Tile &t, uint32_t chunk, uint32_t channel, float &code, float &plus) {
+  constexpr uint32_t kSlices = S::kSlices, kSteps = S::kSteps;
+  Share joined;
+  float all = 0.0f;
+  const uint64_t at = uint64_t(t.b) * A.width + channel;
+#pragma unroll 1
+  for (uint32_t i = 0; i < kSlices; ++i) {
+    const uint32_t t0 = chunk * kChunk + (BACK ? kSlices - 1 - i : i) * kSteps;
+    float keep[kSteps], sum = 0.0f;
+    Share share;
+#pragma unroll
+    for (uint32_t k = 0; k < kSteps; ++k) {
+      const bool live = t0 + k < t.end && channel < A.width;
+      const T *f = reinterpret_cast<const T *>(A.f.p) + int64_t(t.b) * A.f.b + int64_t(t0 + k) * A.f.t + channel;
+      const T *v = reinterpret_cast<const T *>(A.v.p) + int64_t(t.b) * A.v.b + int64_t(t0 + k) * A.v.t + channel;
+      const Gate g(live ? float(*f) : kHold);
+      keep[k] = g.a;
+      share.step(g.a, g.z);
+      if (!BACK) sum = mul_legacy(g.a, sum) + mul_legacy(g.z, live ? float(*v) : 0.0f);
+    }
+    if (BACK)
+#pragma unroll
+      for (uint32_t k = kSteps; k-- > 0;) {
+        const bool live = t0 + k < t.end && channel < A.width;
+        const T *dy = reinterpret_cast<const T *>(A.dy.p) + int64_t(t.b) * A.dy.b + int64_t(t0 + k) * A.dy.t + channel;
+        float d = live && A.dy.p ? float(*dy) : 0.0f;
+        if (t0 + k + 1 == t.end && A.dlast && channel < A.width) d += A.dlast[at];
+        sum = mul_legacy(keep[k], sum + d);
+      }
+    const float c = share.code();
+    joined.join(c);
+    all = apply(c, sum, all);
+  }
+  code = joined.code();
+  plus = all;
+}
+
+// The state that a tile starts with, a lane a channel of a wave's 64: of the `n` chunks before it (`step` records apart) the
+// nearest whose state is there is found, and the shares of those between are applied to it one after the other, as they
+// themselves do: the bits do not depend on which it was. One load looks at 32 chunks, a word of each: looking at all of what a
+// few of them leave, again and again, took half of the memory's rate.
+// Workgroups start in the order of their chunks, so those before are at work, and each leaves its own share before it waits for
+// anything. Should one not come, as nothing promises that order, its share is worked out here after L.most looks: every wait ends.
+template <class T, class S, bool BACK>
+__device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, const Tile &t, uint32_t channel, Record *mine,
+                                           int64_t step, uint32_t n, uint32_t lane, uint64_t ready, float code, float plus) {
+  if (__all(L.there(ready))) return __uint_as_float(uint32_t(ready));
+  L.put(&mine->code[lane], code);
+  L.put(&mine->plus[lane], plus);
+  uint32_t d0 = 1, looks = 0;  // the nearest chunk of a look is d0 before this one
+  for (;;) {
+    const uint32_t at = d0 + (lane & 31);
+    const Record *r = mine - step * int64_t(at < n ? at : n);
+    const uint64_t seen = __ballot(L.there(get_shared(lane < 32 ? &r->code[0] : &r->state[0])));
+    const uint32_t shares = uint32_t(seen), states = uint32_t(seen >> 32);
+    const uint32_t known = __builtin_ctzll(~uint64_t(shares));  // chunks whose shares are there, up to the first that is not
+    if (states && uint32_t(__builtin_ctz(states)) <= known) {
+      d0 += __builtin_ctz(states);
+      break;
+    }
+    if (known == 32) {
+      d0 += 32;
+    } else if (++looks < L.most) {
+      __builtin_amdgcn_s_sleep(1);
+    } else {  // the first chunk has a state alone
+      const uint32_t d = d0 + known;
+      Record *late = mine - step * int64_t(d);
+      float own_code, own_plus;
+      chunk_share<T, S, BACK>(A, t, BACK ? t.chunk + d : t.chunk - d, channel, own_code, own_plus);
+      if (BACK ? (t.chunk + d + 1) * kChunk >= t.end : t.chunk == d) {
+        const float from = !BACK && channel < A.width ? A.initial[uint64_t(t.b) * A.width + channel] : 0.0f;
+        L.put(&late->state[lane], apply(own_code, own_plus, from));
+      } else {
+        L.put(&late->code[lane], own_code);
+        L.put(&late->plus[lane], own_plus);
+      }
+    }
+  }
+  float x = L.get(&(mine - step * int64_t(d0))->state[lane]);
+  constexpr uint32_t W = 4;
+  for (uint32_t d = d0 - 1; d > 0;) {
+    uint64_t c[W], p[W];
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+      const Record *r = mine - step * int64_t(d > w ? d - w : 1);
+      c[w] = get_shared(&r->code[lane]);
+      p[w] = get_shared(&r->plus[lane]);
+    }
+    uint32_t done = 0;
+    bool there = true;
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+      there = there && w < d && __all(L.there(c[w]) && L.there(p[w]));
+      if (there) x = apply(__uint_as_float(uint32_t(c[w])), __uint_as_float(uint32_t(p[w])), x), ++done;
+    }
+    d -= done;
+  }
+  return x;
 }
 
 template <class T, bool MANY>
-__global__ __launch_bounds__(kAcross * kFwdSlices, 3) void fwd_kernel(ScanArgs A, Look K, uint32_t columns) {
-  constexpr uint32_t kSlices = kFwdSlices, kSteps = kChunk / kSlices;
+__global__ __launch_bounds__(Fwd::kLanes, 4) void fwd_kernel(ScanArgs A, Look L, uint32_t tiles_across, uint32_t each) {
+  typedef Fwd S;
+  constexpr uint32_t kAcross = S::kAcross, kSteps = S::kSteps, kSlices = S::kSlices, kTileWidth = S::kWidth;
   __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth];
-  __shared__ uint32_t taken;
-  uint32_t tile = blockIdx.x;
-  if constexpr (MANY) {
-    if (threadIdx.x == 0) taken = atomicAdd(K.ticket, 1u);
-    __syncthreads();
-    tile = __builtin_amdgcn_readfirstlane(taken);
-  }
-  const TileAt at = tile_at(A, tile, columns);
-  const uint32_t end = live_steps(A, at.b), across = threadIdx.x & (kAcross - 1), slice = threadIdx.x / kAcross;
-  const uint32_t c = at.column * kTileWidth + 4 * across, t0 = at.chunk * kChunk + slice * kSteps;
+  const Tile t = tile_at<S, false>(A, tiles_across, each);
+  if (t.none) return;
+  const uint32_t across = 4 * (threadIdx.x & (kAcross - 1)), slice = threadIdx.x / kAcross;
+  const uint32_t c = t.c0 + across, t0 = t.chunk * kChunk + slice * kSteps;
   const int n = int(A.width) - int(c);
-  const TileSeq<T, char *> y(A.h, at, slice * kSteps, across);
-  if (at.chunk > 0 && at.chunk * kChunk >= end) {  // padding alone
+  const TileSeq<T, char *> y(A.h, t, slice * kSteps, across);
+  if (t.dead) {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k)
       if (t0 + k < A.length) store_at<T>(y.at(k), y.offset, f4(0.0f), n);
     return;
   }
-  const TileSeq<T, const char *> f(A.f, at, slice * kSteps, across), v(A.v, at, slice * kSteps, across);
+  const TileSeq<T, const char *> f(A.f, t, slice * kSteps, across), v(A.v, t, slice * kSteps, across);
   typename Quad<T>::vec gates[kSteps], val[kSteps];
-  // a tile of channels and steps that are all there takes no bounds
-  const bool whole = (at.column + 1) * kTileWidth <= A.width && (at.chunk + 1) * kChunk <= end;
-  if (whole) {
+  if (t.whole) {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k) {
       gates[k] = load_at<T>(f.at(k), f.offset, 4);
@@ -276,25 +345,21 @@ __global__ __launch_bounds__(kAcross * kFwdSlices, 3) void fwd_kernel(ScanArgs A
   } else {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k) {
-      const int m = t0 + k < end ? n : 0;
+      const int m = t0 + k < t.end ? n : 0;
       gates[k] = load_at<T>(f.at(k), f.offset, m, kHold);
       val[k] = load_at<T>(v.at(k), v.offset, m);
     }
   }
-  // wave 0's lanes are the tile's channels while the slices are joined
-  const uint32_t lane = threadIdx.x, channel = at.column * kTileWidth + lane;
-  const bool joins = threadIdx.x < 64, inside = channel < A.width;
-  Record *mine = nullptr;
+  // the first waves' lanes are the tile's channels while the slices are joined
+  const uint32_t lane = threadIdx.x, channel = t.c0 + lane;
+  const bool joins = lane < kTileWidth, inside = channel < A.width;
+  const int64_t columns = int64_t(A.batch) * tiles_across * (kTileWidth / 64);
+  Record *mine = MANY ? L.records + t.chunk * columns + t.column * (kTileWidth / 64) + lane / 64 : nullptr;
   uint64_t ready = 0;
   float start = 0.0f;
   if (joins) {
-    if (MANY && at.chunk > 0) {
-      mine = K.records + tile;
-      ready = get_shared(&(mine - A.batch * columns)->state[lane]);
-    } else if (inside) {
-      if constexpr (MANY) mine = K.records + tile;
-      start = A.initial[uint64_t(at.b) * A.width + channel];
-    }
+    if (MANY && t.chunk > 0) ready = get_shared(&(mine - columns)->state[lane & 63]);
+    else if (inside) start = A.initial[uint64_t(t.b) * A.width + channel];
   }
   f4 keep[kSteps], add[kSteps], sum = 0.0f;
   Share share[4];
@@ -313,47 +378,46 @@ __global__ __launch_bounds__(kAcross * kFwdSlices, 3) void fwd_kernel(ScanArgs A
   f4 code;
 #pragma unroll
   for (int e = 0; e < 4; ++e) code[e] = share[e].code();
-  *reinterpret_cast<f4 *>(&codes[slice][4 * across]) = code;
-  *reinterpret_cast<f4 *>(&plus[slice][4 * across]) = sum;
+  *reinterpret_cast<f4 *>(&codes[slice][across]) = code;
+  *reinterpret_cast<f4 *>(&plus[slice][across]) = sum;
   __syncthreads();
   if (joins) {
-    float cs[kSlices], ps[kSlices];
-#pragma unroll
-    for (uint32_t i = 0; i < kSlices; ++i) cs[i] = codes[i][lane], ps[i] = plus[i][lane];
     if constexpr (MANY) {
       Share joined;
       float all = 0.0f;
-#pragma unroll
-      for (uint32_t i = 0; i < kSlices; ++i) joined.join(cs[i]), all = apply(cs[i], ps[i], all);
-      if (at.chunk > 0) start = look_back(mine, int64_t(A.batch) * columns, at.chunk, lane, ready, joined.code(), all);
-      put_word(&(K.records + tile)->state[lane], apply(joined.code(), all, start));
+#pragma unroll 8
+      for (uint32_t i = 0; i < kSlices; ++i) joined.join(codes[i][lane]), all = apply(codes[i][lane], plus[i][lane], all);
+      if (t.chunk > 0)
+        start = look_back<T, S, false>(A, L, t, channel, mine, columns, t.chunk, lane & 63, ready, joined.code(), all);
+      L.put(&mine->state[lane & 63], apply(joined.code(), all, start));
     }
-    if (A.states && inside) A.states[(uint64_t(at.b) * A.chunks + at.chunk) * A.width + channel] = start;
-    if (end == 0 && inside) A.last[uint64_t(at.b) * A.width + channel] = start;
-#pragma unroll
+    if (A.states && inside) A.states[(uint64_t(t.b) * A.chunks + t.chunk) * A.width + channel] = start;
+    if (t.end == 0 && inside) A.last[uint64_t(t.b) * A.width + channel] = start;
+#pragma unroll 8
     for (uint32_t i = 0; i < kSlices; ++i) {
+      const float after = apply(codes[i][lane], plus[i][lane], start);
       plus[i][lane] = start;
-      start = apply(cs[i], ps[i], start);
+      start = after;
     }
   }
   __syncthreads();
-  f4 h = *reinterpret_cast<const f4 *>(&plus[slice][4 * across]);
-  if (whole) {
+  f4 h = *reinterpret_cast<const f4 *>(&plus[slice][across]);
+  if (t.whole) {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) h[e] = mul_legacy(keep[k][e], h[e]) + add[k][e];
       store_at<T>(y.at(k), y.offset, h, 4);
     }
-    if (t0 + kSteps == end) store_quad<float>(A.last + uint64_t(at.b) * A.width + c, h, 4);
+    if (t0 + kSteps == t.end) store_quad<float>(A.last + uint64_t(t.b) * A.width + c, h, 4);
     return;
   }
 #pragma unroll
   for (uint32_t k = 0; k < kSteps; ++k) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) h[e] = mul_legacy(keep[k][e], h[e]) + add[k][e];
-    if (t0 + k < A.length) store_at<T>(y.at(k), y.offset, t0 + k < end ? h : f4(0.0f), n);
-    if (t0 + k + 1 == end) store_quad<float>(A.last + uint64_t(at.b) * A.width + c, h, n);
+    if (t0 + k < A.length) store_at<T>(y.at(k), y.offset, t0 + k < t.end ? h : f4(0.0f), n);
+    if (t0 + k + 1 == t.end) store_quad<float>(A.last + uint64_t(t.b) * A.width + c, h, n);
   }
 }
 
@@ -364,23 +428,17 @@ __device__ __forceinline__ void put_at(char *step, uint32_t offset, f4 f, int n)
 }
 
 template <class T, bool ADD, bool MANY>
-__global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A, Look K, uint32_t columns) {
-  constexpr uint32_t kSlices = kBwdSlices, kSteps = kChunk / kSlices;
+__global__ __launch_bounds__(Bwd::kLanes, 4) void bwd_kernel(ScanArgs A, Look L, uint32_t tiles_across, uint32_t each) {
+  typedef Bwd S;
+  constexpr uint32_t kAcross = S::kAcross, kSteps = S::kSteps, kSlices = S::kSlices, kTileWidth = S::kWidth;
   __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth], back[kSlices][kTileWidth];
-  __shared__ uint32_t taken;
-  uint32_t tile = blockIdx.x;
-  if constexpr (MANY) {
-    if (threadIdx.x == 0) taken = atomicAdd(K.ticket, 1u);
-    __syncthreads();
-    tile = __builtin_amdgcn_readfirstlane(taken);
-  }
-  TileAt at = tile_at(A, tile, columns);
-  at.chunk = A.chunks - 1 - at.chunk;
-  const uint32_t end = live_steps(A, at.b), across = threadIdx.x & (kAcross - 1), slice = threadIdx.x / kAcross;
-  const uint32_t c = at.column * kTileWidth + 4 * across, t0 = at.chunk * kChunk + slice * kSteps;
+  const Tile t = tile_at<S, true>(A, tiles_across, each);
+  if (t.none) return;
+  const uint32_t across = 4 * (threadIdx.x & (kAcross - 1)), slice = threadIdx.x / kAcross;
+  const uint32_t c = t.c0 + across, t0 = t.chunk * kChunk + slice * kSteps;
   const int n = int(A.width) - int(c);
-  const TileSeq<T, char *> df(A.df, at, slice * kSteps, across), dv(A.dv, at, slice * kSteps, across);
-  if (at.chunk > 0 && at.chunk * kChunk >= end) {  // padding alone
+  const TileSeq<T, char *> df(A.df, t, slice * kSteps, across), dv(A.dv, t, slice * kSteps, across);
+  if (t.dead) {
     if (!ADD)
 #pragma unroll
       for (uint32_t k = 0; k < kSteps; ++k)
@@ -390,9 +448,10 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
         }
     return;
   }
-  const TileSeq<T, const char *> f(A.f, at, slice * kSteps, across), v(A.v, at, slice * kSteps, across), dy(A.dy, at, slice * kSteps, across);
+  const TileSeq<T, const char *> f(A.f, t, slice * kSteps, across), v(A.v, t, slice * kSteps, across),
+      dy(A.dy, t, slice * kSteps, across);
   typename Quad<T>::vec gates[kSteps], val[kSteps], up[kSteps];
-  const bool whole = (at.column + 1) * kTileWidth <= A.width && (at.chunk + 1) * kChunk <= end && A.dy.p && A.df.p && A.dv.p;
+  const bool whole = t.whole && A.dy.p && A.df.p && A.dv.p;
   if (whole) {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k) {
@@ -403,22 +462,24 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
   } else {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k) {
-      const int m = t0 + k < end ? n : 0;
+      const int m = t0 + k < t.end ? n : 0;
       gates[k] = load_at<T>(f.at(k), f.offset, m, kHold);
       val[k] = load_at<T>(v.at(k), v.offset, m);
       up[k] = load_at<T>(dy.at(k), dy.offset, A.dy.p ? m : 0);
     }
   }
-  // waves 0 and 1 join the slices, one forward and one from the end
-  const uint32_t lane = threadIdx.x & 63, channel = at.column * kTileWidth + lane, wave = threadIdx.x / 64;
-  const bool inside = channel < A.width, last = at.chunk * kChunk + kChunk >= end;  // last: nothing comes from behind
-  const uint64_t state_at = uint64_t(at.b) * A.width + channel;
+  // the first waves join the slices forward, the next ones from the end
+  const uint32_t lane = threadIdx.x & (kTileWidth - 1), channel = t.c0 + lane, role = threadIdx.x / kTileWidth;
+  const bool inside = channel < A.width, last = t.chunk * kChunk + kChunk >= t.end;  // last: nothing comes from behind
+  const int64_t columns = int64_t(A.batch) * tiles_across * (kTileWidth / 64);
+  Record *mine = MANY ? L.records + (A.chunks - 1 - t.chunk) * columns + t.column * (kTileWidth / 64) + lane / 64 : nullptr;
+  const uint64_t state_at = uint64_t(t.b) * A.width + channel;
   float start = 0.0f;
   uint64_t ready = 0;
-  if (wave == 0 && inside && end) start = A.states[(uint64_t(at.b) * A.chunks + at.chunk) * A.width + channel];
-  if (MANY && wave == 1 && !last) ready = get_shared(&(K.records + tile - A.batch * columns)->state[lane]);
+  if (role == 0 && inside && t.end) start = A.states[(uint64_t(t.b) * A.chunks + t.chunk) * A.width + channel];
+  if (MANY && role == 1 && !last) ready = get_shared(&(mine - columns)->state[lane & 63]);
   f4 dlast = 0.0f;
-  if (A.dlast && end && t0 < end && end <= t0 + kSteps) dlast = load_quad<float>(A.dlast + uint64_t(at.b) * A.width + c, n);
+  if (A.dlast && t.end && t0 < t.end && t.end <= t0 + kSteps) dlast = load_quad<float>(A.dlast + uint64_t(t.b) * A.width + c, n);
   f4 keep[kSteps], into[kSteps], sum = 0.0f, rev = 0.0f;
   Share share[4];
 #pragma unroll
@@ -436,27 +497,27 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
 #pragma unroll
   for (uint32_t k = kSteps; k-- > 0;) {
     f4 d = to_f4<T>(up[k]);
-    if (t0 + k + 1 == end) d += dlast;
+    if (t0 + k + 1 == t.end) d += dlast;
 #pragma unroll
     for (int e = 0; e < 4; ++e) rev[e] = mul_legacy(keep[k][e], rev[e] + d[e]);
   }
   f4 code;
 #pragma unroll
   for (int e = 0; e < 4; ++e) code[e] = share[e].code();
-  *reinterpret_cast<f4 *>(&codes[slice][4 * across]) = code;
-  *reinterpret_cast<f4 *>(&plus[slice][4 * across]) = sum;
-  *reinterpret_cast<f4 *>(&back[slice][4 * across]) = rev;
+  *reinterpret_cast<f4 *>(&codes[slice][across]) = code;
+  *reinterpret_cast<f4 *>(&plus[slice][across]) = sum;
+  *reinterpret_cast<f4 *>(&back[slice][across]) = rev;
   __syncthreads();
   keep_raw(val);
   keep_raw(up);
-  if (wave == 0) {
+  if (role == 0) {
 #pragma unroll 8
     for (uint32_t i = 0; i < kSlices; ++i) {
       const float after = apply(codes[i][lane], plus[i][lane], start);
       plus[i][lane] = start;
       start = after;
     }
-  } else if (wave == 1) {
+  } else if (role == 1) {
     float from = 0.0f;  // a dh of the step behind the tile
     if constexpr (MANY) {
       Share joined;
@@ -464,8 +525,8 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
 #pragma unroll 8
       for (uint32_t i = kSlices; i-- > 0;) joined.join(codes[i][lane]), all = apply(codes[i][lane], back[i][lane], all);
       if (!last)
-        from = look_back(K.records + tile, int64_t(A.batch) * columns, A.chunks - 1 - at.chunk, lane, ready, joined.code(), all);
-      put_word(&(K.records + tile)->state[lane], apply(joined.code(), all, from));
+        from = look_back<T, S, true>(A, L, t, channel, mine, columns, A.chunks - 1 - t.chunk, lane & 63, ready, joined.code(), all);
+      L.put(&mine->state[lane & 63], apply(joined.code(), all, from));
     }
 #pragma unroll 8
     for (uint32_t i = kSlices; i-- > 0;) {
@@ -473,21 +534,22 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
       back[i][lane] = from;
       from = after;
     }
-    if (at.chunk == 0 && A.dinitial && inside) {
-      if (end == 0 && A.dlast) from = A.dlast[state_at];
+    if (t.chunk == 0 && A.dinitial && inside) {
+      if (t.end == 0 && A.dlast) from = A.dlast[state_at];
       A.dinitial[state_at] = ADD ? A.dinitial[state_at] + from : from;
     }
   }
   __syncthreads();
-  f4 h = *reinterpret_cast<const f4 *>(&plus[slice][4 * across]);
-  f4 d = *reinterpret_cast<const f4 *>(&back[slice][4 * across]);
+  f4 h = *reinterpret_cast<const f4 *>(&plus[slice][across]);
+  f4 d = *reinterpret_cast<const f4 *>(&back[slice][across]);
   f4 dh[kSteps];
   keep_raw(up);
   keep_raw(val);
 #pragma unroll
   for (uint32_t k = kSteps; k-- > 0;) {
-    dh[k] = d + to_f4<T>(up[k]);
-    if (t0 + k + 1 == end) dh[k] += dlast;
+    f4 u = to_f4<T>(up[k]);
+    if (t0 + k + 1 == t.end) u += dlast;
+    dh[k] = d + u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) d[e] = mul_legacy(keep[k][e], dh[k][e]);
   }
@@ -514,8 +576,8 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
   for (uint32_t k = 0; k < kSteps; ++k) {
     f4 to_f, to_v;
     gradients(k, to_f, to_v);
-    if (t0 + k >= end) to_f = to_v = f4(0.0f);
-    if (t0 + k < (ADD ? end : A.length)) {
+    if (t0 + k >= t.end) to_f = to_v = f4(0.0f);
+    if (t0 + k < (ADD ? t.end : A.length)) {
       if (A.df.p) put_at<T, ADD>(df.at(k), df.offset, to_f, n);
       if (A.dv.p) put_at<T, ADD>(dv.at(k), dv.offset, to_v, n);
     }
@@ -525,10 +587,10 @@ __global__ __launch_bounds__(kAcross * kBwdSlices, 4) void bwd_kernel(ScanArgs A
 // ------------------------------------------------------------------------- few steps
 
 // A lane four channels, step by step: tokens of a decode batch.
-constexpr uint32_t kFewSteps = 16;
+constexpr uint32_t kFewSteps = 16, kFewLanes = 256;
 template <class T>
-__global__ __launch_bounds__(kLanes) void few_kernel(ScanArgs A, uint32_t quads) {
-  const uint64_t i = uint64_t(blockIdx.x) * kLanes + threadIdx.x;
+__global__ __launch_bounds__(kFewLanes) void few_kernel(ScanArgs A, uint32_t quads) {
+  const uint64_t i = uint64_t(blockIdx.x) * kFewLanes + threadIdx.x;
   if (i >= uint64_t(A.batch) * quads) return;
   const uint32_t b = uint32_t(i / quads), c = 4 * (uint32_t(i) - b * quads), end = live_steps(A, b);
   const int n = int(A.width) - int(c);
@@ -615,28 +677,42 @@ bool scan_args(ScanArgs &A, const Tensor *const *in, bool states, const char *wh
   return true;
 }
 
-// Clears the records and the ticket of a launch over several chunks.
-bool look_at(Look &K, uint64_t tiles, const char *where) {
-  const uint64_t words = 32 + tiles * sizeof(Record) / 8;  // the ticket has 256 bytes
-  uint64_t *p = static_cast<uint64_t *>(partials(words * 8, where));
-  if (!p) return false;
-  K.ticket = reinterpret_cast<uint32_t *>(p);
-  K.records = reinterpret_cast<Record *>(p + 32);
-  clear_kernel<<<ceil_div(words, kLanes), kLanes, 0, stream()>>>(p, words);
-  return true;
+// How often a workgroup looks for a chunk before it works the chunk out itself: some milliseconds.
+uint32_t g_most_looks = 4096;
+uint32_t g_tag = 0;  // of the last launch over the workspace's records
+
+// The records of a launch over several chunks. Eager launches tag theirs with a number of their own, so that no record of
+// another one counts; the slot's records are zeros at first. A graph's replays all have one tag, and clear theirs.
+bool look_at(Look &L, uint64_t records, const char *where) {
+  L.most = g_most_looks;
+  const uint64_t bytes = records * sizeof(Record);
+  if (capturing()) {
+    L.tag = 1;
+    L.records = static_cast<Record *>(bytes <= workspace_bytes(kRecordSlot) ? workspace(bytes, kRecordSlot) : partials(bytes, where));
+    const uint64_t words = bytes / 8;
+    if (L.records) clear_kernel<<<ceil_div(words, 256), 256, 0, stream()>>>(reinterpret_cast<uint64_t *>(L.records), words);
+  } else {
+    L.records = static_cast<Record *>(workspace(bytes, kRecordSlot));
+    if (++g_tag < 2) g_tag = 2;  // past zero and the graphs' tag
+    L.tag = g_tag;
+  }
+  return L.records != nullptr;
 }
-// launch(columns, tiles, records, whether there are several chunks)
-template <class F>
+// launch(workgroups, records, tiles across a sequence, columns of an XCD, whether there are several chunks)
+template <class S, class F>
 bool by_tiles(const ScanArgs &A, const char *where, F &&launch) {
-  const uint32_t columns = ceil_div(A.width, kTileWidth);
-  const uint64_t tiles = uint64_t(A.batch) * columns * A.chunks;
-  if (tiles > max_blocks(kAcross * kBwdSlices)) {
-    report_error(where, "%llu chunks of 64 channels are not supported", (unsigned long long)tiles);
+  const uint32_t across = ceil_div(A.width, S::kWidth);
+  const uint64_t columns = uint64_t(A.batch) * across;
+  // columns that an XCD has more of than another cost time
+  const uint64_t each = columns % 8 == 0 || columns >= 128 ? (columns + 7) / 8 : 0;
+  const uint64_t blocks = (each ? 8 * each : columns) * A.chunks;
+  if (blocks > max_blocks(S::kLanes)) {
+    report_error(where, "%llu chunks of %u channels are not supported", (unsigned long long)blocks, S::kWidth);
     return false;
   }
-  Look K{nullptr, nullptr};
-  if (A.chunks > 1 && !look_at(K, tiles, where)) return false;
-  launch(columns, unsigned(tiles), K, A.chunks > 1);
+  Look L{nullptr, 0, 0};
+  if (A.chunks > 1 && !look_at(L, columns * (S::kWidth / 64) * A.chunks, where)) return false;
+  launch(unsigned(blocks), L, across, uint32_t(each), A.chunks > 1);
   return true;
 }
 
@@ -644,20 +720,20 @@ template <class T>
 bool launch_forward(const ScanArgs &A, const char *where) {
   if (A.length <= kFewSteps) {
     const uint32_t quads = ceil_div(A.width, 4);
-    few_kernel<T><<<ceil_div(uint64_t(A.batch) * quads, kLanes), kLanes, 0, stream()>>>(A, quads);
+    few_kernel<T><<<ceil_div(uint64_t(A.batch) * quads, kFewLanes), kFewLanes, 0, stream()>>>(A, quads);
     return true;
   }
-  return by_tiles(A, where, [&](uint32_t columns, unsigned tiles, const Look &K, bool many) {
-    if (many) fwd_kernel<T, true><<<tiles, kAcross * kFwdSlices, 0, stream()>>>(A, K, columns);
-    else fwd_kernel<T, false><<<tiles, kAcross * kFwdSlices, 0, stream()>>>(A, K, columns);
+  return by_tiles<Fwd>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each, bool many) {
+    if (many) fwd_kernel<T, true><<<blocks, Fwd::kLanes, 0, stream()>>>(A, L, across, each);
+    else fwd_kernel<T, false><<<blocks, Fwd::kLanes, 0, stream()>>>(A, L, across, each);
   });
 }
 template <class T, bool ADD>
 bool launch_backward(ScanArgs A, const char *where) {
   if (A.length == 0) A.chunks = 1;  // what comes for the last state is the initial one's
-  return by_tiles(A, where, [&](uint32_t columns, unsigned tiles, const Look &K, bool many) {
-    if (many) bwd_kernel<T, ADD, true><<<tiles, kAcross * kBwdSlices, 0, stream()>>>(A, K, columns);
-    else bwd_kernel<T, ADD, false><<<tiles, kAcross * kBwdSlices, 0, stream()>>>(A, K, columns);
+  return by_tiles<Bwd>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each, bool many) {
+    if (many) bwd_kernel<T, ADD, true><<<blocks, Bwd::kLanes, 0, stream()>>>(A, L, across, each);
+    else bwd_kernel<T, ADD, false><<<blocks, Bwd::kLanes, 0, stream()>>>(A, L, across, each);
   });
 }
 
@@ -667,6 +743,8 @@ bool launch_backward(ScanArgs A, const char *where) {
 using namespace plast;
 
 extern "C" {
+
+void plast_hip_set_recurrence_looks(int looks) { g_most_looks = looks > 0 ? uint32_t(looks) : 0; }
 
 void gated_recurrence_hip_forward(const Tensor **inputs, Tensor *output, KernelParams params) {
   const char *where = "gated_recurrence_hip_forward";

@@ -23,7 +23,7 @@ bool g_deterministic = false;  // results must not depend on timing (plast_hip_s
 hipStream_t g_stream = nullptr;
 int g_err_count = 0;
 char g_err_msg[512] = "";
-constexpr int kSlots = 3;
+constexpr int kSlots = 4, kPublicSlots = 3;  // the record slot is the library's own
 WorkspaceLedger<kSlots> g_ws;  // workspace slots, and the graphs captured over them
 std::vector<void *> g_deferred_frees;  // arena_free_hip calls made while capturing
 hipEvent_t g_t0 = nullptr, g_t1 = nullptr;
@@ -94,6 +94,9 @@ static void release_deferred_frees() {
   g_deferred_frees.clear();
 }
 
+size_t workspace_bytes(int slot) { return g_ws.bytes(slot); }
+static void fill_bytes(void *p, size_t n);
+
 void *workspace(size_t bytes, int slot) {
   if (slot < 0 || slot >= kSlots) return nullptr;
   if (bytes <= g_ws.bytes(slot)) return g_ws.buffer(slot);
@@ -103,7 +106,7 @@ void *workspace(size_t bytes, int slot) {
     return nullptr;
   }
   const size_t want = bytes < (size_t(1) << 20) ? (size_t(1) << 20) : bytes;
-  return g_ws.grow(
+  void *const fresh = g_ws.grow(
       slot, bytes, want,
       [](size_t n) -> void * {
         void *p = nullptr;
@@ -115,6 +118,8 @@ void *workspace(size_t bytes, int slot) {
         return p;
       },
       release_workspace);
+  if (slot == kRecordSlot && fresh) fill_bytes(fresh, want);
+  return fresh;
 }
 
 static_assert(sizeof(scratch) == kScratchFloats * sizeof(float), "scratch size");
@@ -338,6 +343,10 @@ __global__ void copy_tail_kernel(float *dst, const float *src, uint64_t from, ui
 }
 
 }  // namespace
+
+static void fill_bytes(void *p, size_t n) {
+  fill_bytes_kernel<<<gen_blocks(n), kBlock, 0, stream()>>>(static_cast<unsigned char *>(p), n, 0);
+}
 }  // namespace plast
 
 using namespace plast;
@@ -427,15 +436,15 @@ void plast_hip_graph_destroy(void *graph) {
 
 int plast_hip_workspace_reserve(int slot, uint64_t bytes) {
   if (!ensure_init()) return -1;
-  if (slot < 0 || slot >= kSlots) {
-    report_error("plast_hip_workspace_reserve", "slot %d is not one of 0..%d", slot, kSlots - 1);
+  if (slot < 0 || slot >= kPublicSlots) {
+    report_error("plast_hip_workspace_reserve", "slot %d is not one of 0..%d", slot, kPublicSlots - 1);
     return -1;
   }
   return bytes == 0 || workspace(size_t(bytes), slot) ? 0 : -1;
 }
 
 uint64_t plast_hip_workspace_bytes(int slot) {
-  return slot >= 0 && slot < kSlots ? uint64_t(g_ws.bytes(slot)) : 0;
+  return slot >= 0 && slot < kPublicSlots ? uint64_t(g_ws.bytes(slot)) : 0;
 }
 
 int plast_hip_graphs_alive(void) { return int(g_ws.live_graphs()); }

@@ -11,6 +11,9 @@ from plast_amd.abi import BFLOAT16, FLOAT16, FLOAT32
 from token_cases import HALF_STEP, load, store
 
 U = 2.0 ** -24
+# a product below 2^-126 is off by up to half of 2^-149, whatever its size; a step takes up to four, of the step itself and of
+# the states that a run of steps is joined from, and the next steps pass it on times a
+TINY = 4 * 2.0 ** -150
 DTYPE = {"f32": FLOAT32, "f16": FLOAT16, "bf16": BFLOAT16}
 
 
@@ -149,7 +152,7 @@ def scan_exact(f, v, initial, lengths, dy=None, dlast=None):
         new_size = mix(size, np.abs(v[:, t]), a[:, t], z[:, t])
         with np.errstate(invalid="ignore"):
             new_err = mix(err, 0.0, a[:, t], 0.0 * z[:, t]) + np.where(
-                s[:, t] == 0, 0.0, rel[:, t] * s[:, t] * np.abs(v[:, t] - state) + 8 * U * (new_size + s[:, t] * np.abs(state)))
+                s[:, t] == 0, 0.0, rel[:, t] * s[:, t] * np.abs(v[:, t] - state) + 8 * U * (new_size + s[:, t] * np.abs(state)) + TINY)
         state, err, size = (np.where(live, p, q) for p, q in ((new, state), (new_err, err), (new_size, size)))
         h[:, t], E[:, t], M[:, t] = np.where(live, state, 0.0), np.where(live, err, 0.0), size
     out = {"h": h, "h_tol": E, "last": state, "last_tol": err}
@@ -175,7 +178,7 @@ def scan_exact(f, v, initial, lengths, dy=None, dlast=None):
                                + at * zt * dh_size * (E_before[:, t] + 2 * U * (np.abs(before[:, t]) + np.abs(v[:, t]))))
             ng = np.where(at == 0, 0.0, at * dh)
             nsize = np.where(at == 0, 0.0, at * dh_size)
-            nerr = np.where(at == 0, 0.0, at * dh_err + np.where(shut, 0.0, rt * st * dh_size + 8 * U * dh_size))
+            nerr = np.where(at == 0, 0.0, at * dh_err + np.where(shut, 0.0, rt * st * dh_size + 8 * U * dh_size + TINY))
         for to, x in ((df, dft), (dv, dvt), (df_tol, dft_tol), (dv_tol, dvt_tol)):
             to[:, t] = np.where(live, x, 0.0)
         g, err, size = (np.where(live, p, q) for p, q in ((ng, g), (nerr, err), (nsize, size)))

@@ -74,7 +74,7 @@ def test_layer_norm_backward_with_gradients_that_are_missing(L):  # noqa: F811
 def scan_call(L, kind="forward", dim=1, out=True, **kw):  # noqa: F811
     B, N, D = 3, 200, 5
     ins = [kw.get("f", T((B, N, D))), kw.get("v", T((B, N, D))), kw.get("initial", T((B, D))), kw.get("lengths", T((B,), INT32)),
-           kw.get("last", T((B, D))), kw.get("states", T((B, 2, D)))]
+           kw.get("last", T((B, D))), kw.get("states", T((B, -(-N // abi.RECURRENCE_CHUNK), D)))]
     _call(L, kind, "gated_recurrence", ins, T((B, N, D), grad=T((B, N, D))) if out is True else out, KernelParams(dim, 0, 0.0))
 
 
@@ -89,7 +89,7 @@ def scan_call(L, kind="forward", dim=1, out=True, **kw):  # noqa: F811
     (dict(initial=T((3, 6))), "initial and the last"), (dict(last=T((3, 5), BFLOAT16)), "initial and the last"),
     (dict(last=T((3, 5), strides=(10, 1))), "initial and the last"),
     (dict(lengths=T((3,), INT64)), "lengths"), (dict(lengths=T((4,), INT32)), "lengths"), (dict(lengths=T((3,), INT32, data=0)), "lengths"),
-    (dict(states=T((3, 1, 5))), "states"), (dict(states=None), "states"), (dict(states=T((3, 2, 5), FLOAT16)), "states"),
+    (dict(states=T((3, 1, 5))), "states"), (dict(states=None), "states"), (dict(states=T((3, -(-200 // abi.RECURRENCE_CHUNK), 5), FLOAT16)), "states"),
     (dict(dim=2), "params.dim|params.dim 1"),
 ])
 def test_recurrence_refuses(L, kind, kw, match):  # noqa: F811

@@ -15,7 +15,8 @@ CHUNK = abi.RECURRENCE_CHUNK
 # one step, a few, around a chunk, several chunks; one channel, around a workgroup's columns, odd ones
 SHAPES = [(1, 1, 1), (3, 1, 5), (2, 1, 64), (300, 1, 7), (5, 2, 33), (2, 7, 65), (3, 16, 4), (2, 17, 130), (1, 40, 1003), (2, 100, 66),
           (1, 127, 3), (2, 128, 64), (3, 129, 5), (70, 130, 6), (1, 256, 128), (2, 257, 63), (1, 500, 515), (3, 1000, 20),
-          (1, 3001, 2), (2, 2050, 70), (33, 300, 1)]
+          (1, 3001, 2), (2, 2050, 70), (33, 300, 1), (1, 63, 127), (2, 64, 128),
+          (2, 65, 129), (8, 192, 130), (130, 140, 5), (1, 6400, 3)]
 
 
 class Scan:
@@ -329,6 +330,23 @@ def test_same_bits_every_time():
         for other in runs[1:]:
             for a, b in zip(runs[0], other):
                 assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("looks", [0, 1])
+def test_chunks_that_do_not_come_in_time(looks):
+    """A workgroup that does not wait for the chunk before its own works it out itself: the same bits."""
+    from plast_amd.runtime import lib
+    for shape, kind in (((2, 1000, 200), "f32"), ((1, 3000, 40), "bf16"), ((8, 500, 128), "f16")):
+        runs = []
+        for most in (4096, looks):
+            lib().plast_hip_set_recurrence_looks(most)
+            try:
+                s = _check(shape, kind, ragged=shape[0] > 1, seed=16)
+            finally:
+                lib().plast_hip_set_recurrence_looks(4096)
+            runs.append([values(t) for t in (s.h, s.last, s.f.kept_grad, s.v.kept_grad, s.initial.kept_grad)])
+        for a, b in zip(*runs):
+            assert np.array_equal(a, b)
 
 
 def test_replayed_with_other_work_between():
