@@ -167,7 +167,7 @@ PLAST_HIP_KERNEL_PAIR(layer_norm)
  *   dh[t] = dy[t] + a[t+1] dh[t+1], the gradient of `last` added at the sequence's last step;
  *   v->grad (+)= (1 - a) dh,  f->grad (+)= dh (h[t-1] - v) a (1 - a),  initial->grad (+)= a[0] dh[0].
  * All results are the same bits on every call. */
-#define PLAST_RECURRENCE_CHUNK 128
+#define PLAST_RECURRENCE_CHUNK 64
 PLAST_HIP_KERNEL_PAIR(gated_recurrence)
 
 #undef PLAST_HIP_KERNEL_PAIR

@@ -158,7 +158,7 @@ class Muon(C.Structure):
 
 
 TOP_MAX = 32  # alternatives of token_logprob (PLAST_TOP_MAX)
-RECURRENCE_CHUNK = 128  # steps of gated_recurrence for each state that it keeps (PLAST_RECURRENCE_CHUNK)
+RECURRENCE_CHUNK = 64  # steps of gated_recurrence for each state that it keeps (PLAST_RECURRENCE_CHUNK)
 
 
 def params(dim: int = 0, keepdim: int = 0, fval: float = 0.0) -> KernelParams:

@@ -79,6 +79,13 @@ __device__ __forceinline__ float apply(float code, float plus, float x) {
   return code == 0.0f ? plus : __builtin_fmaf(-code, x, plus);
 }
 
+__device__ __forceinline__ f4 apply(f4 code, f4 plus, f4 x) {
+  f4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = apply(code[e], plus[e], x[e]);
+  return y;
+}
+
 __device__ __forceinline__ uint32_t live_steps(const ScanArgs &A, uint32_t b) {
   const int32_t n = A.lengths[b];
   return n < 0 ? 0 : uint32_t(n) < A.length ? uint32_t(n) : A.length;
@@ -139,25 +146,25 @@ __device__ __forceinline__ void keep_raw(V (&v)[N]) {
 
 // ------------------------------------------------------------------------- tiles
 
-// A tile is a chunk of kChunk steps of some channels: lanes across, four channels each, and slices of a few steps, a slice a
-// lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and each lane goes
+// A tile is TILE steps (one of kChunk or several) of some channels: lanes across, four channels each, and slices of a few steps,
+// a slice a lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and each lane goes
 // through its steps again from the state that its slice starts with.
-template <uint32_t ACROSS, uint32_t STEPS>
+template <uint32_t ACROSS, uint32_t STEPS, uint32_t TILE, uint32_t WAVES>
 struct Shape {
-  static constexpr uint32_t kAcross = ACROSS, kSteps = STEPS, kWidth = 4 * ACROSS, kSlices = kChunk / STEPS, kLanes = ACROSS * kSlices;
-  static_assert(kSteps * kSlices == kChunk && kWidth % 64 == 0, "chunks are whole slices, channels whole waves");
+  static constexpr uint32_t kAcross = ACROSS, kSteps = STEPS, kTile = TILE, kWidth = 4 * ACROSS, kSlices = TILE / STEPS;
+  static constexpr uint32_t kLanes = ACROSS * kSlices, kWaves = WAVES;  // waves that share a SIMD
+  static constexpr uint32_t kChunkSlices = kChunk / STEPS;
+  static_assert(kTile % kChunk == 0 && kChunk % kSteps == 0 && kWidth % 64 == 0, "whole chunks, slices and waves");
 };
-typedef Shape<32, 8> Fwd;
-typedef Shape<16, 4> Bwd;  // holds twice as much of a step
 
-// What a chunk leaves of 64 channels for those behind it: `plus` and `code` of the chunk alone, and the state after it. A word's
+// What a tile leaves of 64 channels for those behind it: `plus` and `code` of the tile alone, and the state after it. A word's
 // upper half is the launch's tag where the word is there, so each word counts by itself.
 struct Record {
   uint64_t code[64], plus[64], state[64];
 };
 struct Look {
-  Record *records;  // [chunks][64 channels of the columns of tiles]
-  uint32_t tag, most;
+  Record *records;  // [tiles of a sequence][64 channels of the columns of tiles]
+  uint32_t tiles, tag, most;
   __device__ __forceinline__ void put(uint64_t *p, float v) const { put_shared(p, uint64_t(tag) << 32 | __float_as_uint(v)); }
   __device__ __forceinline__ bool there(uint64_t w) const { return uint32_t(w >> 32) == tag; }
   // a word that has been sent, and may be under way
@@ -174,30 +181,31 @@ __global__ __launch_bounds__(256) void clear_kernel(uint64_t *p, uint64_t n) {
 }
 
 // Which tile a workgroup works on. Workgroups are dispatched in their order, round robin over the eight XCDs: an XCD's take
-// columns of its own (`each`; 0: all take all), chunk by chunk, so that what lies side by side is read side by side.
+// columns of its own (`each`; 0: all take all), tile by tile, so that what lies side by side is read side by side.
 struct Tile {
-  uint32_t chunk, column, b, c0, end;  // c0: first channel; end: steps of the sequence that are there
+  uint32_t i, column, b, c0, t0, end;  // i: its number in the sequence; c0, t0: first channel and step; end: steps that are there
   bool none, dead, whole;  // no tile; padding alone; all of its steps and channels there, so that it needs no bounds
 };
 template <class S, bool BACK>
-__device__ __forceinline__ Tile tile_at(const ScanArgs &A, uint32_t across, uint32_t each) {
+__device__ __forceinline__ Tile tile_at(const ScanArgs &A, const Look &L, uint32_t across, uint32_t each) {
   const uint32_t columns = A.batch * across, i = blockIdx.x;
   Tile t;
   if (each) {
-    t.chunk = i / 8 / each;
+    t.i = i / 8 / each;
     t.column = i % 8 * each + i / 8 % each;
   } else {
-    t.chunk = i / columns;
-    t.column = i - t.chunk * columns;
+    t.i = i / columns;
+    t.column = i - t.i * columns;
   }
   t.none = t.column >= columns;
   if (t.none) return t;
-  if (BACK) t.chunk = A.chunks - 1 - t.chunk;
+  if (BACK) t.i = L.tiles - 1 - t.i;
   t.b = t.column / across;
   t.c0 = (t.column - t.b * across) * S::kWidth;
+  t.t0 = t.i * S::kTile;
   t.end = live_steps(A, t.b);
-  t.dead = t.chunk > 0 && t.chunk * kChunk >= t.end;
-  t.whole = t.c0 + S::kWidth <= A.width && (t.chunk + 1) * kChunk <= t.end;
+  t.dead = t.i > 0 && t.t0 >= t.end;
+  t.whole = t.c0 + S::kWidth <= A.width && t.t0 + S::kTile <= t.end;
   return t;
 }
 // Where a tile lies in a sequence operand: the address of its step k, and the offset from there of a lane whose slice starts
@@ -208,23 +216,23 @@ struct TileSeq {
   int64_t step;
   uint32_t offset;
   __device__ __forceinline__ TileSeq(const Seq<P> &s, const Tile &t, uint32_t first, uint32_t c) {
-    p = s.p + (int64_t(t.b) * s.b + int64_t(t.chunk * kChunk) * s.t + t.c0) * int64_t(sizeof(T));
+    p = s.p + (int64_t(t.b) * s.b + int64_t(t.t0) * s.t + t.c0) * int64_t(sizeof(T));
     step = s.t * int64_t(sizeof(T));
     offset = (first * uint32_t(s.t) + c) * uint32_t(sizeof(T));
   }
   __device__ __forceinline__ P at(uint32_t k) const { return p + step * k; }
 };
 
-// A channel's chunk worked out by one lane, bit for bit as the chunk's own tile does.
+// A channel's tile `i` worked out by one lane, bit for bit as its own workgroup does.
 template <class T, class S, bool BACK>
-__device__ __forceinline__ void chunk_share(const ScanArgs &A, const Tile &t, uint32_t chunk, uint32_t channel, float &code, float &plus) {
+__device__ __forceinline__ void tile_share(const ScanArgs &A, const Tile &t, uint32_t tile, uint32_t channel, float &code, float &plus) {
   constexpr uint32_t kSlices = S::kSlices, kSteps = S::kSteps;
   Share joined;
   float all = 0.0f;
   const uint64_t at = uint64_t(t.b) * A.width + channel;
 #pragma unroll 1
   for (uint32_t i = 0; i < kSlices; ++i) {
-    const uint32_t t0 = chunk * kChunk + (BACK ? kSlices - 1 - i : i) * kSteps;
+    const uint32_t t0 = tile * S::kTile + (BACK ? kSlices - 1 - i : i) * kSteps;
     float keep[kSteps], sum = 0.0f;
     Share share;
 #pragma unroll
@@ -254,11 +262,11 @@ __device__ __forceinline__ void chunk_share(const ScanArgs &A, const Tile &t, ui
   plus = all;
 }
 
-// The state that a tile starts with, a lane a channel of a wave's 64: of the `n` chunks before it (`step` records apart) the
+// The state that a tile starts with, a lane a channel of a wave's 64: of the `n` tiles before it (`step` records apart) the
 // nearest whose state is there is found, and the shares of those between are applied to it one after the other, as they
-// themselves do: the bits do not depend on which it was. One load looks at 32 chunks, a word of each: looking at all of what a
+// themselves do: the bits do not depend on which it was. One load looks at 32 tiles, a word of each: looking at all of what a
 // few of them leave, again and again, took half of the memory's rate.
-// Workgroups start in the order of their chunks, so those before are at work, and each leaves its own share before it waits for
+// Workgroups start in the order of their tiles, so those before are at work, and each leaves its own share before it waits for
 // anything. Should one not come, as nothing promises that order, its share is worked out here after L.most looks: every wait ends.
 template <class T, class S, bool BACK>
 __device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, const Tile &t, uint32_t channel, Record *mine,
@@ -266,13 +274,13 @@ __device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, con
   if (__all(L.there(ready))) return __uint_as_float(uint32_t(ready));
   L.put(&mine->code[lane], code);
   L.put(&mine->plus[lane], plus);
-  uint32_t d0 = 1, looks = 0;  // the nearest chunk of a look is d0 before this one
+  uint32_t d0 = 1, looks = 0;  // the nearest tile of a look is d0 before this one
   for (;;) {
     const uint32_t at = d0 + (lane & 31);
     const Record *r = mine - step * int64_t(at < n ? at : n);
     const uint64_t seen = __ballot(L.there(get_shared(lane < 32 ? &r->code[0] : &r->state[0])));
     const uint32_t shares = uint32_t(seen), states = uint32_t(seen >> 32);
-    const uint32_t known = __builtin_ctzll(~uint64_t(shares));  // chunks whose shares are there, up to the first that is not
+    const uint32_t known = __builtin_ctzll(~uint64_t(shares));  // tiles whose shares are there, up to the first that is not
     if (states && uint32_t(__builtin_ctz(states)) <= known) {
       d0 += __builtin_ctz(states);
       break;
@@ -281,12 +289,12 @@ __device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, con
       d0 += 32;
     } else if (++looks < L.most) {
       __builtin_amdgcn_s_sleep(1);
-    } else {  // the first chunk has a state alone
+    } else {  // the first tile has a state alone
       const uint32_t d = d0 + known;
       Record *late = mine - step * int64_t(d);
       float own_code, own_plus;
-      chunk_share<T, S, BACK>(A, t, BACK ? t.chunk + d : t.chunk - d, channel, own_code, own_plus);
-      if (BACK ? (t.chunk + d + 1) * kChunk >= t.end : t.chunk == d) {
+      tile_share<T, S, BACK>(A, t, BACK ? t.i + d : t.i - d, channel, own_code, own_plus);
+      if (BACK ? (t.i + d + 1) * S::kTile >= t.end : t.i == d) {
         const float from = !BACK && channel < A.width ? A.initial[uint64_t(t.b) * A.width + channel] : 0.0f;
         L.put(&late->state[lane], apply(own_code, own_plus, from));
       } else {
@@ -317,15 +325,14 @@ __device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, con
   return x;
 }
 
-template <class T, bool MANY>
-__global__ __launch_bounds__(Fwd::kLanes, 4) void fwd_kernel(ScanArgs A, Look L, uint32_t tiles_across, uint32_t each) {
-  typedef Fwd S;
+template <class T, class S, bool MANY>
+__global__ __launch_bounds__(S::kLanes, S::kWaves) void fwd_kernel(ScanArgs A, Look L, uint32_t tiles_across, uint32_t each) {
   constexpr uint32_t kAcross = S::kAcross, kSteps = S::kSteps, kSlices = S::kSlices, kTileWidth = S::kWidth;
-  __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth];
-  const Tile t = tile_at<S, false>(A, tiles_across, each);
+  __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth], starts[kTileWidth];
+  const Tile t = tile_at<S, false>(A, L, tiles_across, each);
   if (t.none) return;
   const uint32_t across = 4 * (threadIdx.x & (kAcross - 1)), slice = threadIdx.x / kAcross;
-  const uint32_t c = t.c0 + across, t0 = t.chunk * kChunk + slice * kSteps;
+  const uint32_t c = t.c0 + across, t0 = t.t0 + slice * kSteps;
   const int n = int(A.width) - int(c);
   const TileSeq<T, char *> y(A.h, t, slice * kSteps, across);
   if (t.dead) {
@@ -354,11 +361,11 @@ __global__ __launch_bounds__(Fwd::kLanes, 4) void fwd_kernel(ScanArgs A, Look L,
   const uint32_t lane = threadIdx.x, channel = t.c0 + lane;
   const bool joins = lane < kTileWidth, inside = channel < A.width;
   const int64_t columns = int64_t(A.batch) * tiles_across * (kTileWidth / 64);
-  Record *mine = MANY ? L.records + t.chunk * columns + t.column * (kTileWidth / 64) + lane / 64 : nullptr;
+  Record *mine = MANY ? L.records + t.i * columns + t.column * (kTileWidth / 64) + lane / 64 : nullptr;
   uint64_t ready = 0;
   float start = 0.0f;
   if (joins) {
-    if (MANY && t.chunk > 0) ready = get_shared(&(mine - columns)->state[lane & 63]);
+    if (MANY && t.i > 0) ready = get_shared(&(mine - columns)->state[lane & 63]);
     else if (inside) start = A.initial[uint64_t(t.b) * A.width + channel];
   }
   f4 keep[kSteps], add[kSteps], sum = 0.0f;
@@ -381,27 +388,29 @@ __global__ __launch_bounds__(Fwd::kLanes, 4) void fwd_kernel(ScanArgs A, Look L,
   *reinterpret_cast<f4 *>(&codes[slice][across]) = code;
   *reinterpret_cast<f4 *>(&plus[slice][across]) = sum;
   __syncthreads();
-  if (joins) {
-    if constexpr (MANY) {
-      Share joined;
-      float all = 0.0f;
-#pragma unroll 8
-      for (uint32_t i = 0; i < kSlices; ++i) joined.join(codes[i][lane]), all = apply(codes[i][lane], plus[i][lane], all);
-      if (t.chunk > 0)
-        start = look_back<T, S, false>(A, L, t, channel, mine, columns, t.chunk, lane & 63, ready, joined.code(), all);
-      L.put(&mine->state[lane & 63], apply(joined.code(), all, start));
-    }
-    if (A.states && inside) A.states[(uint64_t(t.b) * A.chunks + t.chunk) * A.width + channel] = start;
-    if (t.end == 0 && inside) A.last[uint64_t(t.b) * A.width + channel] = start;
+  if (joins) {  // before each slice: the share of those before it and what they add
+    Share joined;
+    float all = 0.0f;
 #pragma unroll 8
     for (uint32_t i = 0; i < kSlices; ++i) {
-      const float after = apply(codes[i][lane], plus[i][lane], start);
-      plus[i][lane] = start;
-      start = after;
+      const float one = codes[i][lane], more = plus[i][lane];
+      codes[i][lane] = joined.code();
+      plus[i][lane] = all;
+      joined.join(one);
+      all = apply(one, more, all);
     }
+    if constexpr (MANY) {
+      if (t.i > 0) start = look_back<T, S, false>(A, L, t, channel, mine, columns, t.i, lane & 63, ready, joined.code(), all);
+      L.put(&mine->state[lane & 63], apply(joined.code(), all, start));
+    }
+    if (t.end == 0 && inside) A.last[uint64_t(t.b) * A.width + channel] = start;
+    starts[lane] = start;
   }
   __syncthreads();
-  f4 h = *reinterpret_cast<const f4 *>(&plus[slice][across]);
+  f4 h = apply(*reinterpret_cast<const f4 *>(&codes[slice][across]), *reinterpret_cast<const f4 *>(&plus[slice][across]),
+               *reinterpret_cast<const f4 *>(&starts[across]));
+  if (A.states && slice % S::kChunkSlices == 0 && t0 < A.length)
+    store_quad<float>(A.states + (uint64_t(t.b) * A.chunks + t0 / kChunk) * A.width + c, h, n);
   if (t.whole) {
 #pragma unroll
     for (uint32_t k = 0; k < kSteps; ++k) {
@@ -427,15 +436,15 @@ __device__ __forceinline__ void put_at(char *step, uint32_t offset, f4 f, int n)
   store_at<T>(step, offset, f, n);
 }
 
-template <class T, bool ADD, bool MANY>
-__global__ __launch_bounds__(Bwd::kLanes, 4) void bwd_kernel(ScanArgs A, Look L, uint32_t tiles_across, uint32_t each) {
-  typedef Bwd S;
+template <class T, class S, bool ADD, bool MANY>
+__global__ __launch_bounds__(S::kLanes, S::kWaves) void bwd_kernel(ScanArgs A, Look L, uint32_t tiles_across, uint32_t each) {
   constexpr uint32_t kAcross = S::kAcross, kSteps = S::kSteps, kSlices = S::kSlices, kTileWidth = S::kWidth;
   __shared__ __align__(16) float codes[kSlices][kTileWidth], plus[kSlices][kTileWidth], back[kSlices][kTileWidth];
-  const Tile t = tile_at<S, true>(A, tiles_across, each);
+  __shared__ __align__(16) float after[kSlices][kTileWidth], starts[kTileWidth];
+  const Tile t = tile_at<S, true>(A, L, tiles_across, each);
   if (t.none) return;
   const uint32_t across = 4 * (threadIdx.x & (kAcross - 1)), slice = threadIdx.x / kAcross;
-  const uint32_t c = t.c0 + across, t0 = t.chunk * kChunk + slice * kSteps;
+  const uint32_t c = t.c0 + across, t0 = t.t0 + slice * kSteps;
   const int n = int(A.width) - int(c);
   const TileSeq<T, char *> df(A.df, t, slice * kSteps, across), dv(A.dv, t, slice * kSteps, across);
   if (t.dead) {
@@ -470,13 +479,13 @@ __global__ __launch_bounds__(Bwd::kLanes, 4) void bwd_kernel(ScanArgs A, Look L,
   }
   // the first waves join the slices forward, the next ones from the end
   const uint32_t lane = threadIdx.x & (kTileWidth - 1), channel = t.c0 + lane, role = threadIdx.x / kTileWidth;
-  const bool inside = channel < A.width, last = t.chunk * kChunk + kChunk >= t.end;  // last: nothing comes from behind
+  const bool inside = channel < A.width, last = t.t0 + S::kTile >= t.end;  // last: nothing comes from behind
   const int64_t columns = int64_t(A.batch) * tiles_across * (kTileWidth / 64);
-  Record *mine = MANY ? L.records + (A.chunks - 1 - t.chunk) * columns + t.column * (kTileWidth / 64) + lane / 64 : nullptr;
+  Record *mine = MANY ? L.records + (L.tiles - 1 - t.i) * columns + t.column * (kTileWidth / 64) + lane / 64 : nullptr;
   const uint64_t state_at = uint64_t(t.b) * A.width + channel;
   float start = 0.0f;
   uint64_t ready = 0;
-  if (role == 0 && inside && t.end) start = A.states[(uint64_t(t.b) * A.chunks + t.chunk) * A.width + channel];
+  if (role == 0 && inside && t.end) start = A.states[(uint64_t(t.b) * A.chunks + t.t0 / kChunk) * A.width + channel];
   if (MANY && role == 1 && !last) ready = get_shared(&(mine - columns)->state[lane & 63]);
   f4 dlast = 0.0f;
   if (A.dlast && t.end && t0 < t.end && t.end <= t0 + kSteps) dlast = load_quad<float>(A.dlast + uint64_t(t.b) * A.width + c, n);
@@ -517,31 +526,33 @@ __global__ __launch_bounds__(Bwd::kLanes, 4) void bwd_kernel(ScanArgs A, Look L,
       plus[i][lane] = start;
       start = after;
     }
-  } else if (role == 1) {
+  } else if (role == 1) {  // behind each slice: the share of those behind it and what they add
     float from = 0.0f;  // a dh of the step behind the tile
-    if constexpr (MANY) {
-      Share joined;
-      float all = 0.0f;
-#pragma unroll 8
-      for (uint32_t i = kSlices; i-- > 0;) joined.join(codes[i][lane]), all = apply(codes[i][lane], back[i][lane], all);
-      if (!last)
-        from = look_back<T, S, true>(A, L, t, channel, mine, columns, A.chunks - 1 - t.chunk, lane & 63, ready, joined.code(), all);
-      L.put(&mine->state[lane & 63], apply(joined.code(), all, from));
-    }
+    Share joined;
+    float all = 0.0f;
 #pragma unroll 8
     for (uint32_t i = kSlices; i-- > 0;) {
-      const float after = apply(codes[i][lane], back[i][lane], from);
-      back[i][lane] = from;
-      from = after;
+      const float one = codes[i][lane], more = back[i][lane];
+      after[i][lane] = joined.code();
+      back[i][lane] = all;
+      joined.join(one);
+      all = apply(one, more, all);
     }
-    if (t.chunk == 0 && A.dinitial && inside) {
-      if (t.end == 0 && A.dlast) from = A.dlast[state_at];
+    if constexpr (MANY) {
+      if (!last)
+        from = look_back<T, S, true>(A, L, t, channel, mine, columns, L.tiles - 1 - t.i, lane & 63, ready, joined.code(), all);
+      L.put(&mine->state[lane & 63], apply(joined.code(), all, from));
+    }
+    starts[lane] = from;
+    if (t.i == 0 && A.dinitial && inside) {
+      from = t.end ? apply(joined.code(), all, from) : A.dlast ? A.dlast[state_at] : 0.0f;
       A.dinitial[state_at] = ADD ? A.dinitial[state_at] + from : from;
     }
   }
   __syncthreads();
   f4 h = *reinterpret_cast<const f4 *>(&plus[slice][across]);
-  f4 d = *reinterpret_cast<const f4 *>(&back[slice][across]);
+  f4 d = apply(*reinterpret_cast<const f4 *>(&after[slice][across]), *reinterpret_cast<const f4 *>(&back[slice][across]),
+               *reinterpret_cast<const f4 *>(&starts[across]));
   f4 dh[kSteps];
   keep_raw(up);
   keep_raw(val);
@@ -698,23 +709,63 @@ bool look_at(Look &L, uint64_t records, const char *where) {
   }
   return L.records != nullptr;
 }
-// launch(workgroups, records, tiles across a sequence, columns of an XCD, whether there are several chunks)
+// launch(workgroups, records, tiles across a sequence, columns of an XCD)
 template <class S, class F>
 bool by_tiles(const ScanArgs &A, const char *where, F &&launch) {
   const uint32_t across = ceil_div(A.width, S::kWidth);
   const uint64_t columns = uint64_t(A.batch) * across;
   // columns that an XCD has more of than another cost time
   const uint64_t each = columns % 8 == 0 || columns >= 128 ? (columns + 7) / 8 : 0;
-  const uint64_t blocks = (each ? 8 * each : columns) * A.chunks;
+  Look L{nullptr, A.length > S::kTile ? ceil_div(A.length, S::kTile) : 1, 0, 0};
+  const uint64_t blocks = (each ? 8 * each : columns) * L.tiles;
   if (blocks > max_blocks(S::kLanes)) {
-    report_error(where, "%llu chunks of %u channels are not supported", (unsigned long long)blocks, S::kWidth);
+    report_error(where, "%llu tiles of %u steps and %u channels are not supported", (unsigned long long)blocks, S::kTile, S::kWidth);
     return false;
   }
-  Look L{nullptr, 0, 0};
-  if (A.chunks > 1 && !look_at(L, columns * (S::kWidth / 64) * A.chunks, where)) return false;
-  launch(unsigned(blocks), L, across, uint32_t(each), A.chunks > 1);
+  if (L.tiles > 1 && !look_at(L, columns * (S::kWidth / 64) * L.tiles, where)) return false;
+  launch(unsigned(blocks), L, across, uint32_t(each));
   return true;
 }
+
+template <class T, class S>
+bool launch_fwd(const ScanArgs &A, const char *where) {
+  return by_tiles<S>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
+    if constexpr (S::kTile < 256)  // the longest have several
+      if (L.tiles == 1) {
+        fwd_kernel<T, S, false><<<blocks, S::kLanes, 0, stream()>>>(A, L, across, each);
+        return;
+      }
+    fwd_kernel<T, S, true><<<blocks, S::kLanes, 0, stream()>>>(A, L, across, each);
+  });
+}
+template <class T, class S, bool ADD>
+bool launch_bwd(const ScanArgs &A, const char *where) {
+  return by_tiles<S>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
+    if constexpr (S::kTile < 256)
+      if (L.tiles == 1) {
+        bwd_kernel<T, S, ADD, false><<<blocks, S::kLanes, 0, stream()>>>(A, L, across, each);
+        return;
+      }
+    bwd_kernel<T, S, ADD, true><<<blocks, S::kLanes, 0, stream()>>>(A, L, across, each);
+  });
+}
+// Columns of 64 channels that a launch has, and the shapes of their tiles. A tile's lanes hold eight steps of four channels, so that
+// a workgroup of 256 lanes takes 128 steps of 64 channels: with shorter tiles the slices are joined in less time and with longer
+// ones states pass from tile to tile less often, which bounds a few long sequences. us, forward and backward of [batch, steps,
+// channels], tiles of 64, 128 and 256 steps:
+//   bf16 [1, 65536, 1024] 203 125 103, 251 200 207; [1, 65536, 256] 169 83 52, 175 90 65; [1, 32768, 2048] 135 100 97,
+//   188 185 205; [1, 16384, 4096] 101 90 92, 164 170 201; [8, 4096, 1024] 52 48 53, 85 89 104; [32, 512, 2048] 47 49 49, 73 79 102
+//   fp32 [1, 65536, 1024] 235 167 147, 326 268 287; [1, 16384, 4096] 153 142 143, 260 246 291; [8, 4096, 1024] 78 78 80,
+//   139 138 151; [32, 512, 2048] 76 86 82, 140 153 152.
+// The forward pass of fp32 over many columns is faster with twice the width, four steps a lane: [32, 512, 2048] 72,
+// [8, 4096, 1024] 74, [5, 3001, 1003] 44 instead of 52, but [1, 16384, 4096] 151.
+typedef Shape<16, 8, 64, 2> Short;
+typedef Shape<16, 8, 128, 4> Middle;
+typedef Shape<16, 8, 128, 2> MiddleBack;
+typedef Shape<16, 8, 256, 4> Long;
+typedef Shape<16, 8, 256, 2> LongBack;
+typedef Shape<32, 4, 64, 5> Wide;
+uint64_t columns_of(const ScanArgs &A) { return uint64_t(A.batch) * ceil_div(A.width, 64); }
 
 template <class T>
 bool launch_forward(const ScanArgs &A, const char *where) {
@@ -723,18 +774,18 @@ bool launch_forward(const ScanArgs &A, const char *where) {
     few_kernel<T><<<ceil_div(uint64_t(A.batch) * quads, kFewLanes), kFewLanes, 0, stream()>>>(A, quads);
     return true;
   }
-  return by_tiles<Fwd>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each, bool many) {
-    if (many) fwd_kernel<T, true><<<blocks, Fwd::kLanes, 0, stream()>>>(A, L, across, each);
-    else fwd_kernel<T, false><<<blocks, Fwd::kLanes, 0, stream()>>>(A, L, across, each);
-  });
+  const uint64_t columns = columns_of(A);
+  if (columns <= 32 && A.length >= 8192) return launch_fwd<T, Long>(A, where);
+  if constexpr (sizeof(T) == 4)
+    if (A.length <= 64 * columns) return launch_fwd<T, Wide>(A, where);
+  return launch_fwd<T, Middle>(A, where);
 }
 template <class T, bool ADD>
-bool launch_backward(ScanArgs A, const char *where) {
-  if (A.length == 0) A.chunks = 1;  // what comes for the last state is the initial one's
-  return by_tiles<Bwd>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each, bool many) {
-    if (many) bwd_kernel<T, ADD, true><<<blocks, Bwd::kLanes, 0, stream()>>>(A, L, across, each);
-    else bwd_kernel<T, ADD, false><<<blocks, Bwd::kLanes, 0, stream()>>>(A, L, across, each);
-  });
+bool launch_backward(const ScanArgs &A, const char *where) {
+  const uint64_t columns = columns_of(A);
+  if (columns <= 8 && A.length >= 8192) return launch_bwd<T, LongBack, ADD>(A, where);
+  if (columns >= (sizeof(T) == 2 ? 64 : 512)) return launch_bwd<T, Short, ADD>(A, where);
+  return launch_bwd<T, MiddleBack, ADD>(A, where);
 }
 
 }  // namespace

@@ -5,6 +5,7 @@
 // The mean of fp32 sums is off by some 1e-7 of the largest |x|: a row far from zero loses digits of x - mu. So mu is
 // corrected by the mean of the differences d = x - mu themselves, which are small, in the pass that sums their squares:
 //   mu' = mu + m, m = sum d / C,  sum (x - mu')^2 = sum d^2 - C m^2.
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstring>
@@ -16,7 +17,6 @@ namespace plast {
 namespace {
 
 constexpr int kRowBlock = 256;  // lanes of a workgroup
-constexpr int kFinLanes = 256;
 
 // What a launch needs of its tensors. map: of x, of y or dy, and of dx.
 struct NormArgs {
@@ -41,6 +41,7 @@ __device__ __forceinline__ typename Unit<T>::floats load_cols(const T *row, uint
   constexpr uint32_t E = Unit<T>::E;
   if (j + E <= width) return to_floats<T>(load_unit(row + j));
   typename Unit<T>::floats f = 0.0f;
+  if (j >= width) return f;
 #pragma unroll
   for (uint32_t e = 0; e < E; ++e)
     if (j + e < width) f[e] = float(row[j + e]);
@@ -53,6 +54,7 @@ __device__ __forceinline__ void store_cols(typename Unit<T>::floats f, T *row, u
     store_any<T>(f, row + j);
     return;
   }
+  if (j >= width) return;
 #pragma unroll
   for (uint32_t e = 0; e < E; ++e)
     if (j + e < width) row[j + e] = T(f[e]);
@@ -95,6 +97,191 @@ __device__ __forceinline__ void block_sums(float &a, float &b, float *lds) {
     a = lds[0], b = lds[1];
 #pragma unroll
     for (int w = 1; w < W; ++w) a += lds[2 * w], b += lds[2 * w + 1];
+  }
+}
+
+// The sums of a and b over the L lanes that share a row, in each of them. `lds` holds two floats a wave that the call before did
+// not use.
+template <int L>
+__device__ __forceinline__ void row_sums(float &a, float &b, float *lds) {
+#pragma unroll
+  for (int d = (L < 64 ? L : 64) / 2; d >= 1; d >>= 1) {
+    a += __shfl_xor(a, d);
+    b += __shfl_xor(b, d);
+  }
+  if constexpr (L > 64) {
+    constexpr int W = L / 64;
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
+    if ((threadIdx.x & 63) == 0) lds[2 * wave] = a, lds[2 * wave + 1] = b;
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) a += lds[2 * (first + w)], b += lds[2 * (first + w) + 1];
+  }
+}
+template <class F>
+__device__ __forceinline__ float unit_sum(F f) {
+  if constexpr (sizeof(F) == 32) return ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+  else return (f[0] + f[1]) + (f[2] + f[3]);
+}
+
+// ------------------------------------------------------------------------- rows in registers
+
+// A row in U units of each of L lanes: read once, written once.
+template <class T, int L, int U>
+__global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel(NormArgs A) {
+  typedef typename Unit<T>::floats F;
+  constexpr int E = Unit<T>::E, B = L > kRowBlock ? L : kRowBlock;
+  __shared__ float lds[2][2 * B / 64];
+  const uint32_t at_row = blockIdx.x * (B / L) + threadIdx.x / L, lane = threadIdx.x % L, C = A.width;
+  if (at_row >= A.rows) return;  // L lanes together, and all of them where they meet
+  const uint32_t row = A.first_row + at_row;
+  const RowAt<3> at = row_at(A.map, row);
+  const T *x = static_cast<const T *>(A.x) + at.at[0];
+  T *y = static_cast<T *>(A.y) + at.at[1];
+  F f[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) f[u] = load_cols<T>(x, (u * L + lane) * E, C);
+  float s = 0.0f, q = 0.0f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) s += unit_sum(f[u]);
+  row_sums<L>(s, q, lds[0]);
+  const float inv = 1.0f / float(C);
+  float mu = s * inv;
+  s = q = 0.0f;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t j = (u * L + lane) * E;
+    F d = f[u] - mu;
+    if (j + E > C) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (j + e >= C) d[e] = 0.0f;
+    }
+    s += unit_sum(d);
+    q += unit_sum(d * d);
+  }
+  row_sums<L>(s, q, lds[1]);
+  const float m = s * inv, var = __builtin_elementwise_maximum(q * inv - m * m, 0.0f);  // NaN stays
+  mu += m;
+  const float r = 1.0f / sqrtf(var + A.eps);
+  if (lane == 0) {
+    A.stats[2 * uint64_t(row)] = mu;
+    A.stats[2 * uint64_t(row) + 1] = r;
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t j = (u * L + lane) * E;
+    if (j >= C) break;
+    const typename Cols<E>::floats w = load_w<E>(A.w, j, C), b = load_w<E>(A.b, j, C);
+    F o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf((f[u][e] - mu) * r, w[e], b[e]);
+    store_cols<T>(o, y, j, C);
+  }
+}
+
+// The gradients of rows held as above, by workgroups that go from row to row: a lane keeps the shares of dw and db of its columns
+// in registers, the workgroup's rows are joined at the end, and its share goes to part[workgroup][2][C]. x and dy are read once.
+template <int L>
+constexpr int kBwdBlock = L > 512 ? L : 512;
+template <class T, int L, int U, bool ADD>
+__global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, float *part) {
+  typedef typename Unit<T>::floats F;
+  constexpr int E = Unit<T>::E, R = kBwdBlock<L> / L;  // rows at a time
+  typedef typename Cols<E>::floats W;
+  __shared__ float lds[2][2 * kBwdBlock<L> / 64];
+  const uint32_t group = threadIdx.x / L, lane = threadIdx.x % L, C = A.width;
+  W w[U], dw[U], db[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    w[u] = load_w<E>(A.w, (u * L + lane) * E, C);
+    dw[u] = db[u] = 0.0f;
+  }
+  const float inv = 1.0f / float(C);
+  int turn = 0;
+  // all of a workgroup's lanes take as many turns
+  for (uint32_t first = blockIdx.x * R; first < A.rows; first += gridDim.x * R, turn ^= 1) {
+    const uint32_t row = first + group;
+    const bool live = R == 1 || row < A.rows;
+    RowAt<3> at{};
+    float mu = 0.0f, r = 0.0f;
+    F f[U], g[U];
+    if (live) {
+      at = row_at(A.map, row);
+      const T *x = static_cast<const T *>(A.x) + at.at[0], *dy = static_cast<const T *>(A.dy) + at.at[1];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        f[u] = load_cols<T>(x, (u * L + lane) * E, C);
+        g[u] = load_cols<T>(dy, (u * L + lane) * E, C);
+      }
+      mu = A.stats[2 * uint64_t(row)], r = A.stats[2 * uint64_t(row) + 1];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) f[u] = g[u] = 0.0f;
+    }
+    float s = 0.0f, q = 0.0f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      f[u] = (f[u] - mu) * r;
+      const uint32_t j = (u * L + lane) * E;
+      if (j + E > C) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (j + e >= C) f[u][e] = 0.0f;
+      }
+      dw[u] = __builtin_elementwise_fma(g[u], f[u], dw[u]);
+      db[u] += g[u];
+      g[u] *= w[u];
+      s += unit_sum(g[u]);
+      q += unit_sum(g[u] * f[u]);
+    }
+    if (!A.dx) continue;
+    row_sums<L>(s, q, lds[turn]);
+    s *= inv, q *= inv;
+    if (!live) continue;
+    T *dx = static_cast<T *>(A.dx) + at.at[2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t j = (u * L + lane) * E;
+      F d = r * ((g[u] - s) - f[u] * q);
+      if constexpr (ADD) d += load_cols<T>(dx, j, C);
+      store_cols<T>(d, dx, j, C);
+    }
+  }
+  if (!part) return;
+  // the groups' shares, halves onto halves
+  __shared__ float other[R > 1 ? (R / 2) * L * U * E : 1];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    W *mine = k ? db : dw;
+#pragma unroll
+    for (int h = R / 2; h >= 1; h /= 2) {
+      __syncthreads();
+      if (group >= uint32_t(h) && group < 2 * uint32_t(h)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) other[(((group - h) * U + u) * E + e) * L + lane] = mine[u][e];
+      }
+      __syncthreads();
+      if (group < uint32_t(h)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int e = 0; e < E; ++e) mine[u][e] += other[((group * U + u) * E + e) * L + lane];
+      }
+    }
+    if (group == 0) {
+      float *p = part + (uint64_t(blockIdx.x) * 2 + k) * C;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t j = (u * L + lane) * E + e;
+          if (j < C) p[j] = mine[u][e];
+        }
+    }
   }
 }
 
@@ -222,17 +409,25 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
   }
 }
 
-// dw and db from the pieces' shares, in the order of the pieces.
+// dw and db from the pieces' shares: 32 columns a workgroup, eight lanes a column, each every eighth piece.
+constexpr uint32_t kFinCols = 32, kFinParts = 8;
 template <bool ADD>
-__global__ __launch_bounds__(kFinLanes) void join_kernel(const float *part, uint32_t pieces, uint32_t width, float *dw,
-                                                         float *db) {
-  const uint64_t i = uint64_t(blockIdx.x) * kFinLanes + threadIdx.x;
-  if (i >= 2 * uint64_t(width)) return;
+__global__ __launch_bounds__(kFinCols * kFinParts) void join_kernel(const float *part, uint32_t pieces, uint32_t width, float *dw,
+                                                                    float *db) {
+  __shared__ float sums[kFinParts][kFinCols];
+  const uint32_t col = threadIdx.x % kFinCols, k = threadIdx.x / kFinCols;
+  const uint64_t i = uint64_t(blockIdx.x) * kFinCols + col, n = 2 * uint64_t(width);
   float *to = i < width ? dw : db;
-  if (!to) return;
-  const uint64_t j = i < width ? i : i - width;
   float s = 0.0f;
-  for (uint32_t p = 0; p < pieces; ++p) s += part[uint64_t(p) * 2 * width + i];
+  if (i < n && to)
+#pragma unroll 8
+    for (uint32_t p = k; p < pieces; p += kFinParts) s += part[p * n + i];
+  sums[k][col] = s;
+  __syncthreads();
+  if (k || i >= n || !to) return;
+#pragma unroll
+  for (uint32_t q = 1; q < kFinParts; ++q) s += sums[q][col];
+  const uint64_t j = i < width ? i : i - width;
   to[j] = ADD ? to[j] + s : s;
 }
 
@@ -328,11 +523,57 @@ void by_parts(const NormArgs &A, uint64_t per, uint64_t threads, F &&launch) {
   }
 }
 
+// f(lanes, units) for rows of `units` units that registers hold; false for longer ones.
+template <int MOST, class F>
+bool with_held(uint32_t units, F &&f) {
+  using std::integral_constant;
+#define HELD(l, n) \
+  if constexpr (n <= MOST) \
+    if (units <= l * n) { f(integral_constant<int, l>{}, integral_constant<int, n>{}); return true; }
+  HELD(16, 1) HELD(16, 2) HELD(16, 4) HELD(64, 2) HELD(64, 4) HELD(256, 1) HELD(256, 2) HELD(256, 4) HELD(1024, 1) HELD(1024, 2)
+  HELD(1024, 4) HELD(1024, 8)
+#undef HELD
+  return false;
+}
+
 template <class T>
 void launch_forward(const NormArgs &A) {
-  by_parts(A, 1, kRowBlock, [](const NormArgs &part, unsigned blocks) {
-    fwd_long_kernel<T><<<blocks, kRowBlock, 0, stream()>>>(part);
+  const bool held = with_held<8>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
+    constexpr int L = decltype(lanes)::value, U = decltype(units)::value, B = L > kRowBlock ? L : kRowBlock;
+    by_parts(A, B / L, B, [](const NormArgs &part, unsigned blocks) {
+      fwd_held_kernel<T, L, U><<<blocks, B, 0, stream()>>>(part);
+    });
   });
+  if (!held)
+    by_parts(A, 1, kRowBlock, [](const NormArgs &part, unsigned blocks) {
+      fwd_long_kernel<T><<<blocks, kRowBlock, 0, stream()>>>(part);
+    });
+}
+
+template <bool ADD>
+void launch_join(const NormArgs &A, const float *part, uint64_t pieces) {
+  join_kernel<ADD><<<ceil_div(2 * uint64_t(A.width), kFinCols), kFinCols * kFinParts, 0, stream()>>>(part, uint32_t(pieces),
+                                                                                                   A.width, A.dw, A.db);
+}
+
+// Rows that registers hold, 16 columns a lane: two workgroups a CU.
+template <class T, bool ADD>
+bool launch_held_backward(const NormArgs &A, bool &held, const char *where) {
+  bool ok = false;
+  held = with_held<16 / int(Unit<T>::E)>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
+    constexpr int L = decltype(lanes)::value, U = decltype(units)::value, R = kBwdBlock<L> / L;
+    const uint64_t most = uint64_t(num_cus()) * (L > 512 ? 1 : 2);
+    const uint64_t blocks = std::min<uint64_t>(most, ceil_div(A.rows, R));
+    float *part = nullptr;
+    if (A.dw || A.db) {
+      part = static_cast<float *>(partials(blocks * 2 * A.width * sizeof(float), where));
+      if (!part) return;
+    }
+    bwd_held_kernel<T, L, U, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
+    if (part) launch_join<ADD>(A, part, blocks);
+    ok = true;
+  });
+  return ok;
 }
 
 // Rows of any length: their means, then columns of pieces of rows, then the pieces' sums.
@@ -358,9 +599,7 @@ bool launch_long_backward(const NormArgs &A, const char *where) {
       row_means_kernel<T><<<n, kRowBlock, 0, stream()>>>(p, means);
     });
   columns_kernel<T, ADD><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
-  if (sums)
-    join_kernel<ADD><<<ceil_div(2 * uint64_t(A.width), kFinLanes), kFinLanes, 0, stream()>>>(part, uint32_t(pieces), A.width,
-                                                                                           A.dw, A.db);
+  if (sums) launch_join<ADD>(A, part, pieces);
   return true;
 }
 
@@ -439,7 +678,9 @@ void layer_norm_hip_backward(Tensor **inputs, const Tensor *output, KernelParams
   bool ok = false;
   with_float_type(x->dtype, [&](auto t) {
     typedef decltype(t) T;
-    ok = add ? launch_long_backward<T, true>(A, where) : launch_long_backward<T, false>(A, where);
+    bool held = false;
+    ok = add ? launch_held_backward<T, true>(A, held, where) : launch_held_backward<T, false>(A, held, where);
+    if (!held) ok = add ? launch_long_backward<T, true>(A, where) : launch_long_backward<T, false>(A, where);
   });
   if (ok) finish(where);
 }

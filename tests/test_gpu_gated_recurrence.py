@@ -16,7 +16,7 @@ CHUNK = abi.RECURRENCE_CHUNK
 SHAPES = [(1, 1, 1), (3, 1, 5), (2, 1, 64), (300, 1, 7), (5, 2, 33), (2, 7, 65), (3, 16, 4), (2, 17, 130), (1, 40, 1003), (2, 100, 66),
           (1, 127, 3), (2, 128, 64), (3, 129, 5), (70, 130, 6), (1, 256, 128), (2, 257, 63), (1, 500, 515), (3, 1000, 20),
           (1, 3001, 2), (2, 2050, 70), (33, 300, 1), (1, 63, 127), (2, 64, 128),
-          (2, 65, 129), (8, 192, 130), (130, 140, 5), (1, 6400, 3)]
+          (2, 65, 129), (8, 192, 130), (130, 140, 5), (1, 6400, 3), (1, 8300, 130), (2, 9001, 33), (600, 70, 3)]
 
 
 class Scan:
