@@ -30,22 +30,36 @@ struct NormArgs {
   RowMap<3> map;
 };
 
+// Results are stored past the caches and operands read through them: what fits the last-level cache is there for the backward pass.
+// us, both ways / operands past the caches too: forward [30011, 333] in fp32 19.7 / 24.0, [16384, 4096] 100 / 98, backward
+// [512, 20000] in fp16 42 / 56, [30011, 333] in fp32 34 / 38; results through them: forward [16384, 4096] 103.
 template <class T>
 __device__ __forceinline__ void store_any(typename Unit<T>::floats f, T *p) {
-  *reinterpret_cast<typename Unit<T>::any *>(p) = __builtin_convertvector(f, typename Unit<T>::vec);
+  __builtin_nontemporal_store(__builtin_convertvector(f, typename Unit<T>::vec), reinterpret_cast<typename Unit<T>::any *>(p));
 }
 
 // A unit's elements from column j on, zeros behind the row's end.
 template <class T>
-__device__ __forceinline__ typename Unit<T>::floats load_cols(const T *row, uint32_t j, uint32_t width) {
+__device__ __forceinline__ typename Unit<T>::vec load_raw(const T *row, uint32_t j, uint32_t width) {
   constexpr uint32_t E = Unit<T>::E;
-  if (j + E <= width) return to_floats<T>(load_unit(row + j));
-  typename Unit<T>::floats f = 0.0f;
-  if (j >= width) return f;
+  if (j + E <= width) return *reinterpret_cast<const typename Unit<T>::any *>(row + j);
+  typename Unit<T>::vec v = T(0.0f);
+  if (j >= width) return v;
 #pragma unroll
   for (uint32_t e = 0; e < E; ++e)
-    if (j + e < width) f[e] = float(row[j + e]);
-  return f;
+    if (j + e < width) v[e] = row[j + e];
+  return v;
+}
+// The same where WHOLE says that a row's units are whole and as many as its lanes hold: no branch, so that the loads of several
+// rows are told apart while they are on their way.
+template <bool WHOLE, class T>
+__device__ __forceinline__ typename Unit<T>::vec load_held(const T *row, uint32_t j, uint32_t width) {
+  if constexpr (WHOLE) return *reinterpret_cast<const typename Unit<T>::any *>(row + j);
+  else return load_raw(row, j, width);
+}
+template <class T>
+__device__ __forceinline__ typename Unit<T>::floats load_cols(const T *row, uint32_t j, uint32_t width) {
+  return to_floats<T>(load_raw(row, j, width));
 }
 template <class T>
 __device__ __forceinline__ void store_cols(typename Unit<T>::floats f, T *row, uint32_t j, uint32_t width) {
@@ -58,6 +72,11 @@ __device__ __forceinline__ void store_cols(typename Unit<T>::floats f, T *row, u
 #pragma unroll
   for (uint32_t e = 0; e < E; ++e)
     if (j + e < width) row[j + e] = T(f[e]);
+}
+template <bool WHOLE, class T>
+__device__ __forceinline__ void store_held(typename Unit<T>::floats f, T *row, uint32_t j, uint32_t width) {
+  if constexpr (WHOLE) store_any<T>(f, row + j);
+  else store_cols<T>(f, row, j, width);
 }
 // E columns of a weight or bias.
 template <int E>
@@ -127,127 +146,185 @@ __device__ __forceinline__ float unit_sum(F f) {
 
 // ------------------------------------------------------------------------- rows in registers
 
-// A row in U units of each of L lanes: read once, written once.
-template <class T, int L, int U>
+// A row in U units of each of L lanes: read once, written once. Workgroups go from row to row (B / L of them at a time), the units of
+// the next two on their way, the weight and the bias in registers where there are few.
+template <class T, int L, int U, bool WHOLE>
 __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel(NormArgs A) {
   typedef typename Unit<T>::floats F;
+  typedef typename Unit<T>::vec V;
   constexpr int E = Unit<T>::E, B = L > kRowBlock ? L : kRowBlock;
+  constexpr bool HOLD = U * E <= 16;
+  typedef typename Cols<E>::floats W;
   __shared__ float lds[2][2 * B / 64];
-  const uint32_t at_row = blockIdx.x * (B / L) + threadIdx.x / L, lane = threadIdx.x % L, C = A.width;
-  if (at_row >= A.rows) return;  // L lanes together, and all of them where they meet
-  const uint32_t row = A.first_row + at_row;
-  const RowAt<3> at = row_at(A.map, row);
-  const T *x = static_cast<const T *>(A.x) + at.at[0];
-  T *y = static_cast<T *>(A.y) + at.at[1];
-  F f[U];
+  const uint32_t lane = threadIdx.x % L, C = A.width, step = gridDim.x * (B / L);
+  const uint64_t row0 = blockIdx.x * (B / L) + threadIdx.x / L;
+  if (row0 >= A.rows) return;  // L lanes together, and all of them where they meet
+  struct Row {
+    int64_t y;
+    V v[U];
+  };
+  const auto load = [&](Row &o, uint64_t row) {
+    if (WHOLE) row = row < A.rows ? row : A.rows - 1;
+    else if (row >= A.rows) return;
+    const RowAt<3> at = row_at(A.map, uint32_t(row));
+    o.y = at.at[1];
 #pragma unroll
-  for (int u = 0; u < U; ++u) f[u] = load_cols<T>(x, (u * L + lane) * E, C);
-  float s = 0.0f, q = 0.0f;
-#pragma unroll
-  for (int u = 0; u < U; ++u) s += unit_sum(f[u]);
-  row_sums<L>(s, q, lds[0]);
+    for (int u = 0; u < U; ++u) o.v[u] = load_held<WHOLE>(static_cast<const T *>(A.x) + at.at[0], (u * L + lane) * E, C);
+  };
+  W w[HOLD ? U : 1], b[HOLD ? U : 1];
   const float inv = 1.0f / float(C);
-  float mu = s * inv;
-  s = q = 0.0f;
+  const auto turn = [&](Row &o, uint64_t row) {
+    F f[U];
+    float s = 0.0f, q = 0.0f;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t j = (u * L + lane) * E;
-    F d = f[u] - mu;
-    if (j + E > C) {
+    for (int u = 0; u < U; ++u) f[u] = to_floats<T>(o.v[u]), s += unit_sum(f[u]);
+    T *y = static_cast<T *>(A.y) + o.y;
+    if constexpr (HOLD) load(o, row + 2 * uint64_t(step));
+    row_sums<L>(s, q, lds[0]);
+    float mu = s * inv;
+    s = q = 0.0f;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (j + e >= C) d[e] = 0.0f;
+    for (int u = 0; u < U; ++u) {
+      const uint32_t j = (u * L + lane) * E;
+      F d = f[u] - mu;
+      if (!WHOLE && j + E > C) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (j + e >= C) d[e] = 0.0f;
+      }
+      s += unit_sum(d);
+      q += unit_sum(d * d);
     }
-    s += unit_sum(d);
-    q += unit_sum(d * d);
-  }
-  row_sums<L>(s, q, lds[1]);
-  const float m = s * inv, var = __builtin_elementwise_maximum(q * inv - m * m, 0.0f);  // NaN stays
-  mu += m;
-  const float r = 1.0f / sqrtf(var + A.eps);
-  if (lane == 0) {
-    A.stats[2 * uint64_t(row)] = mu;
-    A.stats[2 * uint64_t(row) + 1] = r;
-  }
+    row_sums<L>(s, q, lds[1]);
+    const float m = s * inv, var = __builtin_elementwise_maximum(q * inv - m * m, 0.0f);  // NaN stays
+    mu += m;
+    const float r = 1.0f / sqrtf(var + A.eps);
+    if (lane == 0) {
+      A.stats[2 * row] = mu;
+      A.stats[2 * row + 1] = r;
+    }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t j = (u * L + lane) * E;
-    if (j >= C) break;
-    const typename Cols<E>::floats w = load_w<E>(A.w, j, C), b = load_w<E>(A.b, j, C);
-    F o;
+    for (int u = 0; u < U; ++u) {
+      const uint32_t j = (u * L + lane) * E;
+      if constexpr (HOLD) store_held<WHOLE, T>(__builtin_elementwise_fma((f[u] - mu) * r, w[u], b[u]), y, j, C);
+      else store_held<WHOLE, T>(__builtin_elementwise_fma((f[u] - mu) * r, load_w<E>(A.w, j, C), load_w<E>(A.b, j, C)), y, j, C);
+    }
+  };
+  Row one, two;
+  load(one, row0);
+  if constexpr (!HOLD) {  // a row each
+    turn(one, row0);
+    return;
+  }
+  load(two, row0 + step);
+  if constexpr (HOLD) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf((f[u][e] - mu) * r, w[e], b[e]);
-    store_cols<T>(o, y, j, C);
+    for (int u = 0; u < U; ++u) {
+      w[u] = load_w<E>(A.w, (u * L + lane) * E, C);
+      b[u] = load_w<E>(A.b, (u * L + lane) * E, C);
+    }
+  }
+  for (uint64_t row = row0;; row += 2 * uint64_t(step)) {
+    turn(one, row);
+    if (row + step >= A.rows) return;
+    turn(two, row + step);
+    if (row + 2 * uint64_t(step) >= A.rows) return;
   }
 }
 
-// The gradients of rows held as above, by workgroups that go from row to row: a lane keeps the shares of dw and db of its columns
-// in registers, the workgroup's rows are joined at the end, and its share goes to part[workgroup][2][C]. x and dy are read once.
+// The gradients of rows held as above: a lane keeps the shares of dw and db of its columns in registers, the workgroup's rows are
+// joined at the end, and its share goes to part[workgroup][2][C]. x and dy are read once.
 template <int L>
 constexpr int kBwdBlock = L > 512 ? L : 512;
-template <class T, int L, int U, bool ADD>
+template <class T, int L, int U, bool WHOLE, bool ADD>
 __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, float *part) {
   typedef typename Unit<T>::floats F;
+  typedef typename Unit<T>::vec V;
   constexpr int E = Unit<T>::E, R = kBwdBlock<L> / L;  // rows at a time
   typedef typename Cols<E>::floats W;
   __shared__ float lds[2][2 * kBwdBlock<L> / 64];
-  const uint32_t group = threadIdx.x / L, lane = threadIdx.x % L, C = A.width;
-  W w[U], dw[U], db[U];
+  const uint32_t group = threadIdx.x / L, lane = threadIdx.x % L, C = A.width, step = gridDim.x * R;
+  const T *x = static_cast<const T *>(A.x), *dy = static_cast<const T *>(A.dy);
+  struct Row {
+    int64_t dx;
+    float mu, r;
+    V f[U], g[U];
+  };
+  const auto load = [&](Row &o, uint64_t row) {
+    if (WHOLE) {
+      row = row < A.rows ? row : A.rows - 1;
+    } else if (row >= A.rows) {
+      o.mu = o.r = 0.0f;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    w[u] = load_w<E>(A.w, (u * L + lane) * E, C);
-    dw[u] = db[u] = 0.0f;
-  }
-  const float inv = 1.0f / float(C);
-  int turn = 0;
-  // all of a workgroup's lanes take as many turns
-  for (uint32_t first = blockIdx.x * R; first < A.rows; first += gridDim.x * R, turn ^= 1) {
-    const uint32_t row = first + group;
-    const bool live = R == 1 || row < A.rows;
-    RowAt<3> at{};
-    float mu = 0.0f, r = 0.0f;
-    F f[U], g[U];
-    if (live) {
-      at = row_at(A.map, row);
-      const T *x = static_cast<const T *>(A.x) + at.at[0], *dy = static_cast<const T *>(A.dy) + at.at[1];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        f[u] = load_cols<T>(x, (u * L + lane) * E, C);
-        g[u] = load_cols<T>(dy, (u * L + lane) * E, C);
-      }
-      mu = A.stats[2 * uint64_t(row)], r = A.stats[2 * uint64_t(row) + 1];
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) f[u] = g[u] = 0.0f;
+      for (int u = 0; u < U; ++u) o.f[u] = o.g[u] = T(0.0f);
+      return;
     }
-    float s = 0.0f, q = 0.0f;
+    const RowAt<3> at = row_at(A.map, uint32_t(row));
+    o.dx = at.at[2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      f[u] = (f[u] - mu) * r;
+      o.f[u] = load_held<WHOLE>(x + at.at[0], (u * L + lane) * E, C);
+      o.g[u] = load_held<WHOLE>(dy + at.at[1], (u * L + lane) * E, C);
+    }
+    o.mu = A.stats[2 * row], o.r = A.stats[2 * row + 1];
+  };
+  W w[U], dw[U], db[U];
+  const float inv = 1.0f / float(C);
+  int buffer = 0;
+  const auto turn = [&](Row &o, uint64_t row) {
+    float s = 0.0f, q = 0.0f;
+    F f[U], g[U];
+    const float r = o.r;
+    T *dx = static_cast<T *>(A.dx) + o.dx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      f[u] = (to_floats<T>(o.f[u]) - o.mu) * r;
+      g[u] = to_floats<T>(o.g[u]);
       const uint32_t j = (u * L + lane) * E;
-      if (j + E > C) {
+      if (!WHOLE && j + E > C) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (j + e >= C) f[u][e] = 0.0f;
       }
+    }
+    load(o, row + 2 * uint64_t(step));
+    if (WHOLE && R > 1 && row >= A.rows) {  // a row behind the last
+#pragma unroll
+      for (int u = 0; u < U; ++u) g[u] = 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       dw[u] = __builtin_elementwise_fma(g[u], f[u], dw[u]);
       db[u] += g[u];
       g[u] *= w[u];
       s += unit_sum(g[u]);
       q += unit_sum(g[u] * f[u]);
     }
-    if (!A.dx) continue;
-    row_sums<L>(s, q, lds[turn]);
+    if (!A.dx) return;
+    row_sums<L>(s, q, lds[buffer]);
+    buffer ^= 1;
     s *= inv, q *= inv;
-    if (!live) continue;
-    T *dx = static_cast<T *>(A.dx) + at.at[2];
+    if (R > 1 && row >= A.rows) return;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t j = (u * L + lane) * E;
-      F d = r * ((g[u] - s) - f[u] * q);
-      if constexpr (ADD) d += load_cols<T>(dx, j, C);
-      store_cols<T>(d, dx, j, C);
+      F d = r * __builtin_elementwise_fma(f[u], F(-q), g[u] - s);
+      if constexpr (ADD) d += to_floats<T>(load_held<WHOLE>(dx, j, C));
+      store_held<WHOLE, T>(d, dx, j, C);
     }
+  };
+  Row one, two;
+  load(one, blockIdx.x * R + group);
+  load(two, blockIdx.x * R + step + group);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    w[u] = load_w<E>(A.w, (u * L + lane) * E, C);
+    dw[u] = db[u] = 0.0f;
+  }
+  // all of a workgroup's lanes take as many turns
+  for (uint64_t first = blockIdx.x * R; first < A.rows; first += 2 * uint64_t(step)) {
+    turn(one, first + group);
+    if (first + step < A.rows) turn(two, first + step + group);
   }
   if (!part) return;
   // the groups' shares, halves onto halves
@@ -376,6 +453,7 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
   const W w = load_w<E>(A.w, j, C);
   W dw = 0.0f, db = 0.0f;
   const uint32_t r0 = piece * per, r1 = r0 + per < A.rows ? r0 + per : A.rows;
+#pragma unroll 4
   for (uint32_t row = r0; row < r1; ++row) {
     const RowAt<3> at = row_at(A.map, row);
     const F f = load_cols<T>(static_cast<const T *>(A.x) + at.at[0], j, C);
@@ -523,26 +601,31 @@ void by_parts(const NormArgs &A, uint64_t per, uint64_t threads, F &&launch) {
   }
 }
 
-// f(lanes, units) for rows of `units` units that registers hold; false for longer ones.
-template <int MOST, class F>
+// f(lanes, units) for rows of `units` units that registers hold, MOST units a lane and MOST1024 of 1024 lanes; false for longer ones.
+template <int MOST, int MOST1024, class F>
 bool with_held(uint32_t units, F &&f) {
   using std::integral_constant;
 #define HELD(l, n) \
-  if constexpr (n <= MOST) \
+  if constexpr (n <= (l == 1024 ? MOST1024 : MOST)) \
     if (units <= l * n) { f(integral_constant<int, l>{}, integral_constant<int, n>{}); return true; }
-  HELD(16, 1) HELD(16, 2) HELD(16, 4) HELD(64, 2) HELD(64, 4) HELD(256, 1) HELD(256, 2) HELD(256, 4) HELD(1024, 1) HELD(1024, 2)
+  HELD(16, 1) HELD(16, 2) HELD(16, 4) HELD(64, 2) HELD(64, 4) HELD(256, 1) HELD(256, 2) HELD(256, 4) HELD(512, 1) HELD(512, 2) HELD(1024, 1) HELD(1024, 2)
   HELD(1024, 4) HELD(1024, 8)
 #undef HELD
   return false;
 }
 
+// Workgroups of 256 lanes that go from row to row, for each CU: [30011, 333] in fp32 17.4 us with four, 18.8 with eight, a row each
+// 24; [16384, 4096] in bf16 51, 52, 62.
+constexpr uint64_t kFwdPerCu = 4;
 template <class T>
 void launch_forward(const NormArgs &A) {
-  const bool held = with_held<8>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
+  const bool held = with_held<16 / int(Unit<T>::E), 8>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
     constexpr int L = decltype(lanes)::value, U = decltype(units)::value, B = L > kRowBlock ? L : kRowBlock;
-    by_parts(A, B / L, B, [](const NormArgs &part, unsigned blocks) {
-      fwd_held_kernel<T, L, U><<<blocks, B, 0, stream()>>>(part);
-    });
+    constexpr bool loops = U * Unit<T>::E <= 16;
+    const uint64_t all = ceil_div(A.rows, B / L), most = uint64_t(num_cus()) * kFwdPerCu * kRowBlock / B;
+    const unsigned blocks = unsigned(loops ? std::min(all, most) : all);
+    if (A.width == L * U * Unit<T>::E) fwd_held_kernel<T, L, U, true><<<blocks, B, 0, stream()>>>(A);
+    else fwd_held_kernel<T, L, U, false><<<blocks, B, 0, stream()>>>(A);
   });
   if (!held)
     by_parts(A, 1, kRowBlock, [](const NormArgs &part, unsigned blocks) {
@@ -556,11 +639,11 @@ void launch_join(const NormArgs &A, const float *part, uint64_t pieces) {
                                                                                                    A.width, A.dw, A.db);
 }
 
-// Rows that registers hold, 16 columns a lane: two workgroups a CU.
+// Rows that registers hold, eight columns a lane (16 in the longest rows): two workgroups of 512 lanes a CU.
 template <class T, bool ADD>
 bool launch_held_backward(const NormArgs &A, bool &held, const char *where) {
   bool ok = false;
-  held = with_held<16 / int(Unit<T>::E)>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
+  held = with_held<8 / int(Unit<T>::E), 16 / int(Unit<T>::E)>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
     constexpr int L = decltype(lanes)::value, U = decltype(units)::value, R = kBwdBlock<L> / L;
     const uint64_t most = uint64_t(num_cus()) * (L > 512 ? 1 : 2);
     const uint64_t blocks = std::min<uint64_t>(most, ceil_div(A.rows, R));
@@ -569,7 +652,8 @@ bool launch_held_backward(const NormArgs &A, bool &held, const char *where) {
       part = static_cast<float *>(partials(blocks * 2 * A.width * sizeof(float), where));
       if (!part) return;
     }
-    bwd_held_kernel<T, L, U, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
+    if (A.width == L * U * Unit<T>::E) bwd_held_kernel<T, L, U, true, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
+    else bwd_held_kernel<T, L, U, false, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
     if (part) launch_join<ADD>(A, part, blocks);
     ok = true;
   });
@@ -581,10 +665,10 @@ template <class T, bool ADD>
 bool launch_long_backward(const NormArgs &A, const char *where) {
   constexpr uint32_t E = Unit<T>::E;
   const uint32_t blocks = ceil_div(A.width, kRowBlock * E);
-  // some 2048 workgroups, pieces of 16 rows or more
+  // some 2048 workgroups, pieces of eight rows or more
   uint64_t pieces = 2048 / blocks;
   if (pieces < 1) pieces = 1;
-  if (pieces > ceil_div(A.rows, 16)) pieces = ceil_div(A.rows, 16);
+  if (pieces > ceil_div(A.rows, 8)) pieces = ceil_div(A.rows, 8);
   const uint32_t per = ceil_div(A.rows, pieces);
   pieces = ceil_div(A.rows, per);
   const bool sums = A.dw || A.db;
