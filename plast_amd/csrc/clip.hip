@@ -3,8 +3,8 @@
 // Squares are summed and gradients scaled in 64 bits: no gradient's square, and no factor, leaves their range, and the sum
 // has fp32's digits whatever its order (a conversion and a multiply-add an element, far below the read's time).
 //
-// Two launches: a launch's workgroups take equal runs of the gradients' pieces and leave a sum each; those of the second add
-// all sums up, each for itself and in one order, and scale the pieces they had, the last read first.
+// Two launches: the first one's workgroups take equal runs of the gradients' pieces and leave a sum each; those of the second add
+// all sums up, each for itself and in one order, and scale.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -21,42 +21,61 @@ constexpr int kGroup = 96;      // tensors of a launch whose table is in the ker
 constexpr int kLanes = 256;
 constexpr uint32_t kUnits = 4;  // of 16 bytes, of a lane in a piece
 constexpr uint64_t kPiece = uint64_t(kLanes) * kUnits * 16;  // bytes
-constexpr uint32_t kMostBlocks = 2048;  // of all launches together, eight to a CU
+constexpr uint64_t kCached = uint64_t(256) << 20;  // bytes of the last-level cache
+// Workgroups of all of a call's launches: up to kFewPieces pieces have one each in either launch, so that each XCD scales what its
+// own cache has read ([4, 1024, 1024] in fp32 15 us, 21 otherwise). More are summed by kSumBlocks in one run each (1.07 GB 163 us,
+// 6.6 TB/s; 172 with 2048) and scaled by kScaleBlocks in turns of kRun (150 gradients of 1.2 MB 135 us, 172 piece by piece, whose
+// table is looked up for each; one run each 148; 1.07 GB 593, 558 and 685 in all).
+constexpr uint32_t kFewPieces = 2048, kSumBlocks = 1024, kScaleBlocks = 2048, kRun = 2;
 
-// A gradient: p, n, the number of its first piece; its type in vec.
-struct ClipTable {
+// Gradients: p, n, the number of the first piece, the type in vec; in the kernel's arguments or in device memory. of(): the one that
+// piece p is of, the last whose first piece is at or before it.
+struct InArguments {
   OptEntry e[kGroup];
-};
-
-// f(entry, piece of the entry) for pieces [first, end) of the table's, in order or from the last.
-template <bool BACK, class F>
-__device__ __forceinline__ void for_pieces(const OptEntry *T, int count, uint32_t first, uint32_t end, F &&f) {
-  if (first >= end) return;
-  const uint32_t at = BACK ? end - 1 : first;
-  int i = 0, hi = count - 1;
-  while (i < hi) {
-    const int mid = (i + hi + 1) >> 1;
-    if (T[mid].first_block <= at) i = mid;
-    else hi = mid - 1;
+  __device__ __forceinline__ const OptEntry &operator[](int i) const { return e[i]; }
+  __device__ __forceinline__ int of(int count, uint32_t p) const {
+    int i = 0, hi = count - 1;
+    while (i < hi) {
+      const int mid = (i + hi + 1) >> 1;
+      if (e[mid].first_block <= p) i = mid;
+      else hi = mid - 1;
+    }
+    return i;
   }
-  if (BACK) {
-    for (uint32_t p = end; p-- > first;) {
-      while (T[i].first_block > p) --i;
-      f(T[i], p - T[i].first_block);
+};
+struct InMemory {
+  const OptEntry *e;
+  __device__ __forceinline__ const OptEntry &operator[](int i) const { return e[i]; }
+  // by a wave, 64 at a time: two looks for up to 4096 gradients
+  __device__ __forceinline__ int of(int count, uint32_t p) const {
+    int at = 0, span = count;
+    while (span > 1) {
+      const int step = (span + 63) / 64, i = int(threadIdx.x & 63) * step;
+      const bool before = i < span && e[at + (i < span ? i : 0)].first_block <= p;
+      const int last = (__popcll(__ballot(before)) - 1) * step;
+      at += last;
+      span = span - last < step ? span - last : step;
     }
-  } else {
-    for (uint32_t p = first; p < end; ++p) {
-      while (i + 1 < count && T[i + 1].first_block <= p) ++i;
-      f(T[i], p - T[i].first_block);
-    }
+    return __builtin_amdgcn_readfirstlane(at);
+  }
+};
+// f(entry, first, end) for the pieces [first, end) of the table's that each entry has, pieces of the entry.
+template <class Table, class F>
+__device__ __forceinline__ void for_entries(const Table &T, int count, uint32_t first, uint32_t end, F &&f) {
+  if (first >= end) return;
+  for (int i = T.of(count, first); i < count; ++i) {
+    const OptEntry E = T[i];
+    const uint32_t behind = i + 1 < count ? T[i + 1].first_block : 0xffffffffu;
+    const uint32_t p0 = E.first_block > first ? E.first_block : first, p1 = behind < end ? behind : end;
+    f(E, p0 - E.first_block, p1 - E.first_block);
+    if (behind >= end) return;
   }
 }
 
 // Every launch's share of the work.
 struct ClipRun {
-  const OptEntry *table;  // null: in the arguments
   int count;
-  uint32_t pieces, per;   // per: of a workgroup
+  uint32_t pieces, per, run;  // per: of a workgroup that sums; run: of one that scales, in each of its turns
 };
 
 __device__ __forceinline__ double block_sum(double s, double *lds) {
@@ -71,88 +90,119 @@ __device__ __forceinline__ double block_sum(double s, double *lds) {
 }
 
 template <class T>
-__device__ __forceinline__ double piece_squares(const OptEntry &E, uint32_t piece) {
-  constexpr uint32_t W = Unit<T>::E;
+constexpr uint32_t kPieceOf = kPiece / sizeof(T);  // elements
+
+// A lane's units of a whole piece.
+template <class T, bool NT>
+struct Units {
+  typename Unit<T>::vec v[kUnits];
+  __device__ __forceinline__ void load(const T *g, uint32_t piece) {
+    const T *p = g + uint64_t(piece) * kPieceOf<T> + threadIdx.x * Unit<T>::E;
+#pragma unroll
+    for (uint32_t u = 0; u < kUnits; ++u) {
+      const auto *q = reinterpret_cast<const typename Unit<T>::any *>(p + u * kLanes * Unit<T>::E);
+      if constexpr (NT) v[u] = __builtin_nontemporal_load(q);
+      else v[u] = *q;
+    }
+  }
+};
+// f(element) for a lane's elements of a last piece, which is not whole.
+template <class T, class F>
+__device__ __forceinline__ void for_rest(T *g, uint64_t n, uint32_t piece, F &&f) {
+  for (uint64_t j = uint64_t(piece) * kPieceOf<T> + threadIdx.x; j < n; j += kLanes) f(g[j]);
+}
+
+// The sum of the squares of pieces [p, end) of a gradient: the next piece's units on their way, a sum for each unit.
+template <class T, bool NT>
+__device__ __forceinline__ double squares(const OptEntry &E, uint32_t p, uint32_t end) {
   const T *g = reinterpret_cast<const T *>(E.p);
-  const uint64_t at = uint64_t(piece) * (kPiece / sizeof(T)) + threadIdx.x * W;
-  double s = 0.0;
-  if (uint64_t(piece + 1) * (kPiece / sizeof(T)) <= E.n) {
-    typename Unit<T>::vec v[kUnits];
+  const uint32_t whole = uint32_t(E.n / kPieceOf<T>), stop = end < whole ? end : whole;
+  double s[kUnits] = {};
+  if (p < stop) {
+    Units<T, NT> now, next;
+    now.load(g, p);
+    for (;;) {
+      const bool more = ++p < stop;
+      if (more) next.load(g, p);
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) v[u] = *reinterpret_cast<const typename Unit<T>::any *>(g + at + u * kLanes * W);
+      for (uint32_t u = 0; u < kUnits; ++u) {
+        const typename Unit<T>::floats f = to_floats<T>(now.v[u]);
 #pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) {
-      const typename Unit<T>::floats f = to_floats<T>(v[u]);
-#pragma unroll
-      for (uint32_t e = 0; e < W; ++e) s = __builtin_fma(double(f[e]), double(f[e]), s);
-    }
-    return s;
-  }
-  for (uint32_t u = 0; u < kUnits; ++u)
-    for (uint32_t e = 0; e < W; ++e) {
-      const uint64_t j = at + u * kLanes * W + e;
-      if (j < E.n) {
-        const double f = double(float(g[j]));
-        s = __builtin_fma(f, f, s);
+        for (uint32_t e = 0; e < Unit<T>::E; ++e) s[u] = __builtin_fma(double(f[e]), double(f[e]), s[u]);
       }
+      if (!more) break;
+      now = next;
     }
-  return s;
-}
-
-template <class T>
-__device__ __forceinline__ void scale_piece(const OptEntry &E, uint32_t piece, double scale) {
-  constexpr uint32_t W = Unit<T>::E;
-  T *g = reinterpret_cast<T *>(E.p);
-  const uint64_t at = uint64_t(piece) * (kPiece / sizeof(T)) + threadIdx.x * W;
-  if (uint64_t(piece + 1) * (kPiece / sizeof(T)) <= E.n) {
-    typename Unit<T>::vec v[kUnits];
-#pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) v[u] = *reinterpret_cast<const typename Unit<T>::any *>(g + at + u * kLanes * W);
-#pragma unroll
-    for (uint32_t u = 0; u < kUnits; ++u) {
-      typename Unit<T>::floats f = to_floats<T>(v[u]);
-#pragma unroll
-      for (uint32_t e = 0; e < W; ++e) f[e] = float(double(f[e]) * scale);
-      *reinterpret_cast<typename Unit<T>::any *>(g + at + u * kLanes * W) =
-          __builtin_convertvector(f, typename Unit<T>::vec);
-    }
-    return;
   }
-  for (uint32_t u = 0; u < kUnits; ++u)
-    for (uint32_t e = 0; e < W; ++e) {
-      const uint64_t j = at + u * kLanes * W + e;
-      if (j < E.n) g[j] = T(float(double(float(g[j])) * scale));
+  if (end > whole)
+    for_rest(const_cast<T *>(g), E.n, whole, [&](T &v) {
+      const double f = double(float(v));
+      s[0] = __builtin_fma(f, f, s[0]);
+    });
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+static_assert(kUnits == 4, "four sums");
+
+// Pieces [p, end) times scale, the next one's units on their way.
+template <class T>
+__device__ __forceinline__ void scale_pieces(const OptEntry &E, uint32_t p, uint32_t end, double scale) {
+  T *g = reinterpret_cast<T *>(E.p);
+  const uint32_t whole = uint32_t(E.n / kPieceOf<T>), stop = end < whole ? end : whole;
+  if (p < stop) {
+    Units<T, false> now, next;
+    now.load(g, p);
+    for (;;) {
+      T *to = g + uint64_t(p) * kPieceOf<T> + threadIdx.x * Unit<T>::E;
+      const bool more = ++p < stop;
+      if (more) next.load(g, p);
+#pragma unroll
+      for (uint32_t u = 0; u < kUnits; ++u) {
+        typename Unit<T>::floats f = to_floats<T>(now.v[u]);
+#pragma unroll
+        for (uint32_t e = 0; e < Unit<T>::E; ++e) f[e] = float(double(f[e]) * scale);
+        __builtin_nontemporal_store(__builtin_convertvector(f, typename Unit<T>::vec),
+                                    reinterpret_cast<typename Unit<T>::any *>(to + u * kLanes * Unit<T>::E));
+      }
+      if (!more) break;
+      now = next;
     }
+  }
+  if (end > whole) for_rest(g, E.n, whole, [&](T &v) { v = T(float(double(float(v)) * scale)); });
 }
 
-__global__ __launch_bounds__(kLanes) void squares_kernel(ClipTable A, ClipRun R, double *sums) {
+template <class Table, bool NT>
+__global__ __launch_bounds__(kLanes) void squares_kernel(Table A, ClipRun R, double *sums) {
   __shared__ double lds[kLanes / 64];
   const uint32_t first = blockIdx.x * R.per, end = first + R.per < R.pieces ? first + R.per : R.pieces;
   double s = 0.0;
-  for_pieces<false>(R.table ? R.table : A.e, R.count, first, end, [&](const OptEntry &E, uint32_t piece) {
-    if (E.vec == FLOAT32) s += piece_squares<float>(E, piece);
-    else if (E.vec == FLOAT16) s += piece_squares<f16_t>(E, piece);
-    else s += piece_squares<bf16_t>(E, piece);
+  for_entries(A, R.count, first, end, [&](const OptEntry &E, uint32_t p, uint32_t to) {
+    if (E.vec == FLOAT32) s += squares<float, NT>(E, p, to);
+    else if (E.vec == FLOAT16) s += squares<f16_t, NT>(E, p, to);
+    else s += squares<bf16_t, NT>(E, p, to);
   });
   s = block_sum(s, lds);
   if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(kLanes) void scale_kernel(ClipTable A, ClipRun R, const double *sums, uint32_t n, float bound,
+template <class Table>
+__global__ __launch_bounds__(kLanes) void scale_kernel(Table A, ClipRun R, const double *sums, uint32_t n, float bound,
                                                        float *norm_out) {
   __shared__ double lds[kLanes / 64];
   double s = 0.0;
+#pragma unroll 8
   for (uint32_t i = threadIdx.x; i < n; i += kLanes) s += sums[i];
   const double norm = sqrt(block_sum(s, lds));
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = float(norm);
   if (!(norm > double(bound)) || norm == __builtin_huge_val()) return;  // within the bound, or not finite
   const double scale = double(bound) / norm;
-  const uint32_t first = blockIdx.x * R.per, end = first + R.per < R.pieces ? first + R.per : R.pieces;
-  for_pieces<true>(R.table ? R.table : A.e, R.count, first, end, [&](const OptEntry &E, uint32_t piece) {
-    if (E.vec == FLOAT32) scale_piece<float>(E, piece, scale);
-    else if (E.vec == FLOAT16) scale_piece<f16_t>(E, piece, scale);
-    else scale_piece<bf16_t>(E, piece, scale);
-  });
+  for (uint64_t p = uint64_t(blockIdx.x) * R.run; p < R.pieces; p += uint64_t(gridDim.x) * R.run) {
+    const uint32_t first = uint32_t(p), end = R.pieces - first < R.run ? R.pieces : first + R.run;
+    for_entries(A, R.count, first, end, [&](const OptEntry &E, uint32_t q, uint32_t to) {
+      if (E.vec == FLOAT32) scale_pieces<float>(E, q, to, scale);
+      else if (E.vec == FLOAT16) scale_pieces<f16_t>(E, q, to, scale);
+      else scale_pieces<bf16_t>(E, q, to, scale);
+    });
+  }
 }
 
 // ------------------------------------------------------------------------- host
@@ -216,6 +266,7 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
   std::vector<OptEntry> entries;
   std::vector<std::pair<uint64_t, uint64_t>> spans;
   uint64_t pieces = 0;
+  if (parameters && num_parameters > 0) entries.reserve(size_t(num_parameters)), spans.reserve(size_t(num_parameters));
   for (int k = 0; parameters && k < num_parameters; ++k) {
     const Tensor *t = parameters[k];
     if (!t || !t->grad) continue;
@@ -252,40 +303,55 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
   const bool table = entries.size() > size_t(kGroup) && !capturing();
   const size_t group = table ? entries.size() : size_t(kGroup);
   const size_t launches = entries.empty() ? 1 : (entries.size() + group - 1) / group;
-  const uint32_t most = uint32_t(std::max<size_t>(1, kMostBlocks / launches));
+  const auto share = [&](uint32_t blocks) { return uint32_t(std::max<size_t>(1, blocks / launches)); };
   std::lock_guard<std::mutex> lk(g_table_mu);
   const OptEntry *T = table ? device_table(entries, where) : nullptr;
   if (table && !T) return;
   struct Launch {
     ClipRun run;
-    uint32_t blocks, first_sum;
+    uint32_t blocks, scale_blocks, first_sum;
   };
   std::vector<Launch> plan;
   uint32_t sums = 0;
   for (size_t i = 0; i < launches; ++i) {
     const size_t a = i * group, b = std::min(entries.size(), a + group);
     const uint64_t p0 = a < b ? entries[a].first_block : 0, p1 = b < entries.size() ? entries[b].first_block : pieces;
-    const uint32_t n = uint32_t(p1 - p0), per = n ? ceil_div(n, most) : 1, blocks = n ? ceil_div(n, per) : 1;
-    plan.push_back({{T, int(b - a), n, per}, blocks, sums});
+    const uint32_t n = uint32_t(p1 - p0);
+    const bool few = n <= share(kFewPieces);
+    const uint32_t per = few ? 1 : ceil_div(n, share(kSumBlocks)), blocks = n ? ceil_div(n, per) : 1;
+    const uint32_t run = few ? 1 : kRun, scale = few ? blocks : std::min(ceil_div(n, run), share(kScaleBlocks));
+    plan.push_back({{int(b - a), n, per, run}, blocks, scale, sums});
     sums += blocks;
   }
   double *room = static_cast<double *>(partials(sums * sizeof(double), where));
   if (!room) return;
-  const auto arguments = [&](size_t i) {
-    ClipTable A;
-    memset(&A, 0, sizeof A);
-    if (!T)
+  const bool past = pieces * kPiece > kCached;
+  float *const out = norm ? static_cast<float *>(norm->data) : nullptr;
+  // both launches of each group, all sums before the first scaling
+  const auto launch = [&](auto tables) {
+    typedef decltype(tables(0)) Table;
+    for (size_t i = 0; i < launches; ++i) {
+      double *to = room + plan[i].first_sum;
+      if (past) squares_kernel<Table, true><<<plan[i].blocks, kLanes, 0, stream()>>>(tables(i), plan[i].run, to);
+      else squares_kernel<Table, false><<<plan[i].blocks, kLanes, 0, stream()>>>(tables(i), plan[i].run, to);
+    }
+    for (size_t i = 0; i < launches; ++i)
+      scale_kernel<Table><<<plan[i].scale_blocks, kLanes, 0, stream()>>>(tables(i), plan[i].run, room, sums, max_norm,
+                                                                         i == 0 ? out : nullptr);
+  };
+  if (T) {
+    launch([&](size_t) { return InMemory{T}; });
+  } else {
+    launch([&](size_t i) {
+      InArguments A;
+      memset(&A, 0, sizeof A);
       for (int k = 0; k < plan[i].run.count; ++k) {
         A.e[k] = entries[i * group + k];
         A.e[k].first_block -= entries[i * group].first_block;
       }
-    return A;
-  };
-  for (size_t i = 0; i < launches; ++i)
-    squares_kernel<<<plan[i].blocks, kLanes, 0, stream()>>>(arguments(i), plan[i].run, room + plan[i].first_sum);
-  for (size_t i = 0; i < launches; ++i)
-    scale_kernel<<<plan[i].blocks, kLanes, 0, stream()>>>(arguments(i), plan[i].run, room, sums, max_norm,
-                                                          i == 0 && norm ? static_cast<float *>(norm->data) : nullptr);
+      return A;
+    });
+  }
   finish(where);
 }
 
