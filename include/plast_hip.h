@@ -132,7 +132,7 @@ PLAST_HIP_KERNEL_PAIR(token_logprob)
  *         [1] weight and [2] bias, C FLOAT32 each;
  *         [3] stats, 2 N FLOAT32 (written by forward: the row's mean and 1 / sqrt(variance + eps);
  *             read by backward).
- * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap.
+ * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap; it may be x itself.
  * params.fval: eps, finite and above 0; params.keepdim: 1 makes the backward overwrite the gradients,
  * 0 accumulate into them. Sums are FLOAT32: the squares of a row's differences from its mean must fit.
  * A NaN or infinity makes its row NaN.
@@ -148,25 +148,27 @@ PLAST_HIP_KERNEL_PAIR(layer_norm)
  *   a = sigmoid(f),  h[t] = a[t] h[t-1] + (1 - a[t]) v[t],  h[-1] = initial.
  * inputs: [0] f and [1] v, [batch B, time T, channels D], of one type, FLOAT32, FLOAT16 or BFLOAT16; any
  *             strides of batch and time, the last axis contiguous (halves of one projection, say);
- *         [2] initial, B D FLOAT32; it may be `last` itself (a state updated token by token);
+ *         [2] initial, B D FLOAT32; it may be `last` itself (a state that is updated in place);
  *         [3] lengths, B INT32: the steps of each sequence, taken as 0 .. T. Steps behind a sequence's
  *             end are padding: whatever they hold, h and the gradients are 0 there;
  *         [4] last, B D FLOAT32 (written by forward: the state after the sequence's last step; its grad
  *             is the upstream gradient, none counts as zero);
  *         [5] states, B ceil(T / PLAST_RECURRENCE_CHUNK) D FLOAT32 (written by forward and read by
  *             backward: the state before each chunk of steps): only where params.dim is 1.
- * output: h, of f's type and shape, the last axis contiguous, steps that do not overlap (its grad is the
- * upstream gradient, none counts as zero).
+ * output: h, of f's type and shape, the last axis contiguous, steps that do not overlap, in a place of its
+ * own (its grad is the upstream gradient, none counts as zero). Steps of an operand are at most 2^22 elements
+ * apart.
  * params.dim: 1 keeps the states for a backward pass, 0 does not; params.keepdim: 1 makes the backward
  * overwrite the gradients, 0 accumulate into them.
  * A gate so far out that the smaller of a and 1 - a is below FLOAT32's range (infinities, say) selects:
  * h[t] is h[t-1] or v[t] whatever the other holds, and no gradient passes to the other. Other NaN and
  * infinities make the states from there on NaN or infinite.
  * Backward (needs params.dim 1), each gradient only where its input requires one, of its input's type and
- * shape (f's and v's with a contiguous last axis and steps that do not overlap):
+ * shape (f's and v's with a contiguous last axis and steps that do not overlap, each in a place of its own):
  *   dh[t] = dy[t] + a[t+1] dh[t+1], the gradient of `last` added at the sequence's last step;
  *   v->grad (+)= (1 - a) dh,  f->grad (+)= dh (h[t-1] - v) a (1 - a),  initial->grad (+)= a[0] dh[0].
- * All results are the same bits on every call. */
+ * All results are the same bits on every call. Calls over several chunks leave what passes from one to the next
+ * in records of the library: replays of captured calls on another stream than the library's race on them. */
 #define PLAST_RECURRENCE_CHUNK 64
 PLAST_HIP_KERNEL_PAIR(gated_recurrence)
 

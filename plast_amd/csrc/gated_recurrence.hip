@@ -8,7 +8,7 @@
 // smaller sides where those count (Share), and every run starts from there.
 // A product with a factor of 0 is 0 whatever the other factor is (v_mul_legacy_f32): a gate so far out that one side is 0
 // selects, and lets no NaN through.
-#include <cfloat>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <type_traits>
@@ -168,22 +168,30 @@ struct Shape {
 struct Record {
   uint64_t code[64], plus[64], state[64];
 };
+constexpr uint32_t kMostGets = 1u << 20;
 struct Look {
   Record *records;  // [tiles of a sequence][64 channels of the columns of tiles]
   uint32_t tiles, tag, most;
   __device__ __forceinline__ void put(uint64_t *p, float v) const { put_shared(p, uint64_t(tag) << 32 | __float_as_uint(v)); }
   __device__ __forceinline__ bool there(uint64_t w) const { return uint32_t(w >> 32) == tag; }
-  // a word that has been sent, and may be under way
+  // A word that has been sent, and may be under way. It comes, but where a launch on another stream writes the same records: NaN.
   __device__ __forceinline__ float get(const uint64_t *p) const {
-    uint64_t w = get_shared(p);
-    while (!there(w)) w = get_shared(p);
-    return __uint_as_float(uint32_t(w));
+    for (uint32_t i = 0; i < kMostGets; ++i) {
+      const uint64_t w = get_shared(p);
+      if (there(w)) return __uint_as_float(uint32_t(w));
+    }
+    return __builtin_nanf("");
   }
 };
 
 __global__ __launch_bounds__(256) void clear_kernel(uint64_t *p, uint64_t n) {
   const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i < n) p[i] = 0;
+}
+
+__global__ __launch_bounds__(256) void copy_kernel(float *to, const float *from, uint64_t n) {
+  const uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) to[i] = from[i];
 }
 
 // Which tile a workgroup works on. Workgroups are dispatched in their order, round robin over the eight XCDs: an XCD's take
@@ -311,7 +319,9 @@ __device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, con
   }
   float x = L.get(&(mine - step * int64_t(d0))->state[lane]);
   constexpr uint32_t W = 4;
+  uint32_t turns = 0;
   for (uint32_t d = d0 - 1; d > 0;) {
+    if (++turns == kMostGets) return __builtin_nanf("");  // as above
     uint64_t c[W], p[W];
 #pragma unroll
     for (uint32_t w = 0; w < W; ++w) {
@@ -709,22 +719,27 @@ bool scan_args(ScanArgs &A, const Tensor *const *in, bool states, const char *wh
 
 // How often a workgroup looks for a chunk before it works the chunk out itself: some milliseconds.
 uint32_t g_most_looks = 4096;
-uint32_t g_tag = 0;  // of the last launch over the workspace's records
+std::atomic<uint32_t> g_tag{1};  // of the last launch over the workspace's records; the graphs' is 1
 
 // The records of a launch over several chunks. Eager launches tag theirs with a number of their own, so that no record of
 // another one counts; the slot's records are zeros at first. A graph's replays all have one tag, and clear theirs.
 bool look_at(Look &L, uint64_t records, const char *where) {
   L.most = g_most_looks;
   const uint64_t bytes = records * sizeof(Record);
+  const auto clear = [](void *p, uint64_t n) {
+    clear_kernel<<<ceil_div(n / 8, 256), 256, 0, stream()>>>(static_cast<uint64_t *>(p), n / 8);
+  };
   if (capturing()) {
     L.tag = 1;
     L.records = static_cast<Record *>(bytes <= workspace_bytes(kRecordSlot) ? workspace(bytes, kRecordSlot) : partials(bytes, where));
-    const uint64_t words = bytes / 8;
-    if (L.records) clear_kernel<<<ceil_div(words, 256), 256, 0, stream()>>>(reinterpret_cast<uint64_t *>(L.records), words);
+    if (L.records) clear(L.records, bytes);
   } else {
     L.records = static_cast<Record *>(workspace(bytes, kRecordSlot));
-    if (++g_tag < 2) g_tag = 2;  // past zero and the graphs' tag
-    L.tag = g_tag;
+    L.tag = ++g_tag;
+    if (L.tag < 2) {  // all numbers have been used
+      if (L.records) clear(L.records, workspace_bytes(kRecordSlot));
+      g_tag = L.tag = 2;
+    }
   }
   return L.records != nullptr;
 }
@@ -747,7 +762,15 @@ bool by_tiles(const ScanArgs &A, const char *where, F &&launch) {
 }
 
 template <class T, class S>
-bool launch_fwd(const ScanArgs &A, const char *where) {
+bool launch_fwd(ScanArgs A, const char *where) {
+  if (A.initial == A.last && A.length > S::kTile) {
+    // a tile that is worked out by another one's workgroup reads the initial state, whenever that is
+    const uint64_t n = uint64_t(A.batch) * A.width;
+    float *const kept = static_cast<float *>(partials(n * sizeof(float), where));
+    if (!kept) return false;
+    copy_kernel<<<ceil_div(n, 256), 256, 0, stream()>>>(kept, A.initial, n);
+    A.initial = kept;
+  }
   return by_tiles<S>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
     if constexpr (S::kTile < 256)  // the longest have several
       if (L.tiles == 1) {
@@ -840,8 +863,13 @@ void gated_recurrence_hip_forward(const Tensor **inputs, Tensor *output, KernelP
     report_error(where, "the output must have f's type and shape, a contiguous last axis and steps that do not overlap");
     return;
   }
-  if (!A.batch || !A.width || !ensure_init()) return;
+  if (!A.batch || !A.width) return;
   A.h = seq<char *>(output);
+  if (A.length && (A.h.p == A.f.p || A.h.p == A.v.p)) {
+    report_error(where, "the output lies in the place of f or v");
+    return;
+  }
+  if (!ensure_init()) return;
   bool ok = false;
   with_float_type(inputs[0]->dtype, [&](auto t) { ok = launch_forward<decltype(t)>(A, where); });
   if (ok) finish(where);
@@ -885,12 +913,21 @@ void gated_recurrence_hip_backward(Tensor **inputs, const Tensor *output, Kernel
     report_error(where, "f and v have one gradient");
     return;
   }
+  for (const char *g : {A.df.p, A.dv.p})
+    if (g && A.length && (g == A.f.p || g == A.v.p || g == A.dy.p)) {
+      report_error(where, "a gradient lies in the place of f, v or the output's gradient");
+      return;
+    }
   if (inputs[2]->requires_grad) {
     if (!f32_vector(inputs[2]->grad, uint64_t(A.batch) * A.width)) {
       report_error(where, "the initial state's gradient must be a contiguous FLOAT32 GPU tensor of its elements");
       return;
     }
     A.dinitial = static_cast<float *>(inputs[2]->grad->data);
+    if (A.dinitial && A.dinitial == A.dlast) {
+      report_error(where, "the initial and the last state have one gradient");
+      return;
+    }
   }
   if ((!A.df.p && !A.dv.p && !A.dinitial) || !A.batch || !A.width || !ensure_init()) return;
   bool ok = false;

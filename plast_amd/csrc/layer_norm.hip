@@ -157,15 +157,15 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
   typedef typename Cols<E>::floats W;
   __shared__ float lds[2][2 * B / 64];
   const uint32_t lane = threadIdx.x % L, C = A.width, step = gridDim.x * (B / L);
-  const uint64_t row0 = blockIdx.x * (B / L) + threadIdx.x / L;
-  if (row0 >= A.rows) return;  // L lanes together, and all of them where they meet
+  const uint64_t row0 = A.first_row + uint64_t(blockIdx.x) * (B / L) + threadIdx.x / L, end = uint64_t(A.first_row) + A.rows;
+  if (row0 >= end) return;  // L lanes together, and all of them where they meet
   struct Row {
     int64_t y;
     V v[U];
   };
   const auto load = [&](Row &o, uint64_t row) {
-    if (WHOLE) row = row < A.rows ? row : A.rows - 1;
-    else if (row >= A.rows) return;
+    if (WHOLE) row = row < end ? row : end - 1;
+    else if (row >= end) return;
     const RowAt<3> at = row_at(A.map, uint32_t(row));
     o.y = at.at[1];
 #pragma unroll
@@ -226,9 +226,9 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
   }
   for (uint64_t row = row0;; row += 2 * uint64_t(step)) {
     turn(one, row);
-    if (row + step >= A.rows) return;
+    if (row + step >= end) return;
     turn(two, row + step);
-    if (row + 2 * uint64_t(step) >= A.rows) return;
+    if (row + 2 * uint64_t(step) >= end) return;
   }
 }
 
@@ -621,11 +621,13 @@ template <class T>
 void launch_forward(const NormArgs &A) {
   const bool held = with_held<16 / int(Unit<T>::E), 8>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
     constexpr int L = decltype(lanes)::value, U = decltype(units)::value, B = L > kRowBlock ? L : kRowBlock;
-    constexpr bool loops = U * Unit<T>::E <= 16;
-    const uint64_t all = ceil_div(A.rows, B / L), most = uint64_t(num_cus()) * kFwdPerCu * kRowBlock / B;
-    const unsigned blocks = unsigned(loops ? std::min(all, most) : all);
-    if (A.width == L * U * Unit<T>::E) fwd_held_kernel<T, L, U, true><<<blocks, B, 0, stream()>>>(A);
-    else fwd_held_kernel<T, L, U, false><<<blocks, B, 0, stream()>>>(A);
+    const auto launch = [](const NormArgs &part, unsigned blocks) {
+      if (part.width == L * U * Unit<T>::E) fwd_held_kernel<T, L, U, true><<<blocks, B, 0, stream()>>>(part);
+      else fwd_held_kernel<T, L, U, false><<<blocks, B, 0, stream()>>>(part);
+    };
+    if constexpr (U * int(Unit<T>::E) <= 16)  // goes from row to row
+      launch(A, unsigned(std::min<uint64_t>(ceil_div(A.rows, B / L), uint64_t(num_cus()) * kFwdPerCu * kRowBlock / B)));
+    else by_parts(A, B / L, B, launch);
   });
   if (!held)
     by_parts(A, 1, kRowBlock, [](const NormArgs &part, unsigned blocks) {
@@ -740,6 +742,10 @@ void layer_norm_hip_backward(Tensor **inputs, const Tensor *output, KernelParams
   }
   if (dx && (!like(dx, x, A.rows) || (numel(dx) && overlapping(dx)))) {
     report_error(where, "the gradient of x must have x's type and shape, a contiguous last axis and rows that do not overlap");
+    return;
+  }
+  if (dx && (dx->data == dy->data || dx->data == x->data) && A.rows) {
+    report_error(where, "the gradient of x lies in the place of x or of the output's gradient");
     return;
   }
   if (!vector_gradient(inputs[1], A.width, &A.dw, where) || !vector_gradient(inputs[2], A.width, &A.db, where)) return;

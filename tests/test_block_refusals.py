@@ -55,6 +55,7 @@ def test_layer_norm_refuses(L, kw, match):  # noqa: F811
     (dict(x=T((6, 10), grad=T((6, 10), data=0))), "gradient of x"),
     (dict(w=T((10,), grad=T((9,)))), "weight and bias"), (dict(b=T((10,), grad=T((10,), FLOAT16))), "weight and bias"),
     (dict(w=T((10,), grad=T((10,))), b=T((10,), grad=T((10,)))), "one gradient"),
+    (dict(x=T((6, 10), grad=T((6, 10)))), "in the place of"), (dict(x=T((6, 10), data=AT + 4096, grad=T((6, 10)))), "in the place of"),
 ])
 def test_layer_norm_backward_refuses(L, kw, match):  # noqa: F811
     norm_call(L, "backward", **kw)
@@ -104,6 +105,16 @@ def test_recurrence_refuses_outputs(L, out):  # noqa: F811
     refused(L, "the output must have")
 
 
+def test_recurrence_refuses_its_operands_places(L):  # noqa: F811
+    scan_call(L, out=T((3, 200, 5)), f=T((3, 200, 5), data=AT + 65536))
+    refused(L, "in the place of")
+    scan_call(L, out=T((3, 200, 5)), v=T((3, 200, 5), data=AT + 65536))
+    refused(L, "in the place of")
+    for steps in ((1 << 22) + 1, 2 ** 64 - 5):
+        scan_call(L, f=T((3, 200, 5), strides=(5, steps, 1)))
+        refused(L, "f and v")
+
+
 def G(grad, shape=(3, 200, 5)):
     return T(shape, grad=grad)
 
@@ -114,8 +125,10 @@ def G(grad, shape=(3, 200, 5)):
     (dict(last=G(T((3, 4)), (3, 5))), "last state's gradient"), (dict(last=G(T((3, 5), FLOAT16), (3, 5))), "last state's gradient"),
     (dict(f=G(T((3, 200, 5), BFLOAT16))), "gradients of f and v"), (dict(v=G(T((3, 200, 5), strides=(0, 5, 1)))), "gradients of f and v"),
     (dict(v=G(T((3, 200, 5), data=0))), "gradients of f and v"),
-    (dict(f=G(T((3, 200, 5))), v=G(T((3, 200, 5)))), "one gradient"),
+    (dict(f=G(T((3, 200, 5), data=AT + 4096)), v=G(T((3, 200, 5), data=AT + 4096))), "one gradient"),
     (dict(initial=G(T((3, 4)), (3, 5))), "initial state's gradient"),
+    (dict(f=G(T((3, 200, 5), data=AT))), "in the place of"), (dict(out=G(T((3, 200, 5), data=AT + 4096)), v=G(T((3, 200, 5), data=AT + 4096))), "in the place of"),
+    (dict(initial=G(T((3, 5), data=AT + 64), (3, 5)), last=G(T((3, 5), data=AT + 64), (3, 5))), "have one gradient"),
 ])
 def test_recurrence_backward_refuses(L, kw, match):  # noqa: F811
     scan_call(L, "backward", **kw)

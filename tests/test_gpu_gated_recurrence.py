@@ -218,15 +218,21 @@ def test_only_what_is_wanted(wanted):
         s.check_backward(want, f"{wanted} {add}", add)
 
 
+@pytest.mark.parametrize("looks", [0, 4096])
 @pytest.mark.parametrize("length", [1, 5, 300, 1000])
-def test_the_state_in_place(length):
+def test_the_state_in_place(length, looks):
     """The initial state's buffer is the last state's: a decoder that goes on from where it is."""
+    from plast_amd.runtime import lib
     f, v, initial, lengths, _, _ = _data((4, length, 70), "f32", 9)
     lengths[:] = [length, length // 2, 0, length]
     want = scan_exact(f, v, initial, lengths)
     s = Scan(f, v, initial, lengths, "f32")
     s.ins[4] = s.initial
-    s.forward(keep=False)
+    lib().plast_hip_set_recurrence_looks(looks)
+    try:
+        s.forward(keep=False)
+    finally:
+        lib().plast_hip_set_recurrence_looks(4096)
     close(values(s.initial), want["last"], want["last_tol"] + stored(want["last"], "f32"), "state")
     close(values(s.h), want["h"], want["h_tol"] + stored(want["h"], "f32"), "h")
 

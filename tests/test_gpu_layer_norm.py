@@ -96,6 +96,17 @@ def test_values_that_are_no_numbers_stay_in_their_rows():
         assert bad[[1, 3, 5]].all() and not bad[[0, 2, 4, 6]].any(), width
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(3000, 100), (40, 333), (700, 4096), (9, 20000), (3, 140000)])
+def test_in_place(shape, kind):
+    from plast_amd.runtime import DeviceTensor, forward
+    x, w, b, _ = _case(shape, kind, 11)
+    X, S = device(x, kind), DeviceTensor((shape[0], 2))
+    forward("layer_norm", [X, device(w, "f32"), device(b, "f32"), S], X, KernelParams(0, 0, EPS))
+    want = norm_exact(x, w, b, np.float32(EPS))
+    close(values(X), want["y"], want["y_tol"] + stored(want["y"], kind), "in place")
+
+
 def test_equal_values():
     """Rows of one value: the differences are exactly 0 where the mean of equal values is exact, the bias is left."""
     from plast_amd.runtime import DeviceTensor, backward, forward
