@@ -132,7 +132,8 @@ PLAST_HIP_KERNEL_PAIR(token_logprob)
  *         [1] weight and [2] bias, C FLOAT32 each;
  *         [3] stats, 2 N FLOAT32 (written by forward: the row's mean and 1 / sqrt(variance + eps);
  *             read by backward).
- * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap; it may be x itself.
+ * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap; it may be x itself,
+ *         with its strides.
  * params.fval: eps, finite and above 0; params.keepdim: 1 makes the backward overwrite the gradients,
  * 0 accumulate into them. Sums are FLOAT32: the squares of a row's differences from its mean must fit.
  * A NaN or infinity makes its row NaN.
@@ -154,7 +155,8 @@ PLAST_HIP_KERNEL_PAIR(layer_norm)
  *         [4] last, B D FLOAT32 (written by forward: the state after the sequence's last step; its grad
  *             is the upstream gradient, none counts as zero);
  *         [5] states, B ceil(T / PLAST_RECURRENCE_CHUNK) D FLOAT32 (written by forward and read by
- *             backward: the state before each chunk of steps): only where params.dim is 1.
+ *             backward: the state before each chunk of steps that a sequence has): only where params.dim
+ *             is 1.
  * output: h, of f's type and shape, the last axis contiguous, steps that do not overlap, in a place of its
  * own (its grad is the upstream gradient, none counts as zero). Steps of an operand are at most 2^22 elements
  * apart.
@@ -162,7 +164,7 @@ PLAST_HIP_KERNEL_PAIR(layer_norm)
  * overwrite the gradients, 0 accumulate into them.
  * A gate so far out that the smaller of a and 1 - a is below FLOAT32's range (infinities, say) selects:
  * h[t] is h[t-1] or v[t] whatever the other holds, and no gradient passes to the other. Other NaN and
- * infinities make the states from there on NaN or infinite.
+ * infinities make the states from there on NaN or infinite (0 times a gate that is NaN may be 0).
  * Backward (needs params.dim 1), each gradient only where its input requires one, of its input's type and
  * shape (f's and v's with a contiguous last axis and steps that do not overlap, each in a place of its own):
  *   dh[t] = dy[t] + a[t+1] dh[t+1], the gradient of `last` added at the sequence's last step;
@@ -249,10 +251,11 @@ void plast_hip_adamw_release(AdamW *optimizer, int num_parameters);
  * device memory, gets the norm before clipping (NULL: not wanted). To be called between the backward pass
  * and the optimizer's step; nothing waits for the GPU in between. Parameters that are NULL or have no grad
  * are skipped, as by the steps; gradients are contiguous GPU tensors of FLOAT32, FLOAT16 or BFLOAT16, of
- * one type or several, and must not share memory (a parameter listed twice is refused). A norm that is NaN
+ * one type or several, and must not share memory, nor with norm (a parameter listed twice is refused). A norm that is NaN
  * or infinite leaves the gradients as they are. max_norm: at least 0, infinity computes the norm alone.
  * Sums are in 64 bits; all results are the same bits on every call. A call over more than 96 gradients
- * keeps their table in device memory, as the steps do. No counterpart in the reference. */
+ * keeps their table in device memory, as the steps do; a captured one adds its sums in groups of 96, in an
+ * order of its own. No counterpart in the reference. */
 void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm, Tensor *norm);
 
 /* ------------------------------------------------------------------ matmul epilogue pieces ---- */

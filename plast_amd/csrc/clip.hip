@@ -1,6 +1,6 @@
 // clip.hip — the global norm of the gradients of a list of parameters, and their scaling to a bound on it:
 //   norm = sqrt(sum over all elements of all gradients of g^2);  where norm > bound: g = g bound / norm.
-// Squares are summed and gradients scaled in 64 bits: no gradient's square, and no factor, leaves their range, and the sum
+// Squares are summed and gradients scaled in 64 bits, and rounded to fp32 and from there to their type: no gradient's square, and no factor, leaves their range, and the sum
 // has fp32's digits whatever its order (a conversion and a multiply-add an element, far below the read's time).
 //
 // Two launches: the first one's workgroups take equal runs of the gradients' pieces and leave a sum each; those of the second add
@@ -9,6 +9,7 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "opt_plan.hpp"
@@ -207,10 +208,11 @@ __global__ __launch_bounds__(kLanes) void scale_kernel(Table A, ClipRun R, const
 
 // ------------------------------------------------------------------------- host
 
+const char *const where = "clip_grad_norm_hip";
 std::mutex g_table_mu;
 OptTableCache g_table;  // of the last call with more than kGroup gradients
 
-const OptEntry *device_table(const std::vector<OptEntry> &e, const char *where) {
+const OptEntry *device_table(const std::vector<OptEntry> &e) {
   return g_table.get(
       e,
       [&]() {
@@ -253,8 +255,7 @@ using namespace plast;
 
 extern "C" {
 
-void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm, Tensor *norm) {
-  const char *where = "clip_grad_norm_hip";
+void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm, Tensor *norm) try {
   if (!(max_norm >= 0.0f)) {
     report_error(where, "max_norm must be at least 0, not %g", double(max_norm));
     return;
@@ -293,8 +294,9 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
     report_error(where, "gradients of more than 2^46 bytes");
     return;
   }
+  if (norm) spans.emplace_back(reinterpret_cast<uint64_t>(norm->data), reinterpret_cast<uint64_t>(norm->data) + sizeof(float));
   if (share_memory(spans)) {
-    report_error(where, "two gradients share memory, or a parameter is listed twice");
+    report_error(where, "two gradients, or the norm and one of them, share memory, or a parameter is listed twice");
     return;
   }
   if ((entries.empty() && !norm) || !ensure_init()) return;
@@ -305,7 +307,7 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
   const size_t launches = entries.empty() ? 1 : (entries.size() + group - 1) / group;
   const auto share = [&](uint32_t blocks) { return uint32_t(std::max<size_t>(1, blocks / launches)); };
   std::lock_guard<std::mutex> lk(g_table_mu);
-  const OptEntry *T = table ? device_table(entries, where) : nullptr;
+  const OptEntry *T = table ? device_table(entries) : nullptr;
   if (table && !T) return;
   struct Launch {
     ClipRun run;
@@ -353,6 +355,8 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
     });
   }
   finish(where);
+} catch (const std::bad_alloc &) {
+  report_error(where, "no host memory for the tables of %d gradients", num_parameters);
 }
 
 }  // extern "C"

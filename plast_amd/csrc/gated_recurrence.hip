@@ -64,7 +64,7 @@ struct Share {
     shut = shut || ga == 0.0f;
   }
   __device__ __forceinline__ float code() const {
-    return shut ? -0.0f : c < 0.9375f ? c : -fmaxf(a, 0x1p-149f);
+    return shut ? -0.0f : c < 0.9375f ? c : -__builtin_elementwise_maximum(a, 0x1p-149f);  // NaN stays
   }
   // the share of this run and one behind it
   __device__ __forceinline__ void join(float code) {
@@ -299,12 +299,12 @@ __device__ __forceinline__ float look_back(const ScanArgs &A, const Look &L, con
       d0 += __builtin_ctz(states);
       break;
     }
-    if (known == 32) {
+    if (known == 32 && d0 + 32 <= n) {
       d0 += 32;
     } else if (++looks < L.most) {
       __builtin_amdgcn_s_sleep(1);
     } else {  // the first tile has a state alone
-      const uint32_t d = d0 + known;
+      const uint32_t d = d0 + known < n ? d0 + known : n;
       Record *late = mine - step * int64_t(d);
       float own_code, own_plus;
       tile_share<T, S, BACK>(A, t, BACK ? t.i + d : t.i - d, channel, own_code, own_plus);
@@ -657,8 +657,8 @@ __global__ __launch_bounds__(kFewLanes) void few_kernel(ScanArgs A, uint32_t qua
 // A lane's offset in a tile has 32 bits.
 constexpr uint64_t kMostStep = uint64_t(1) << 22;
 bool sequence(const Tensor *t, const Tensor *f) {
-  return t && (t->ndim != 3 || t->shape[1] <= 1 || t->strides[1] <= kMostStep) && t->device == GPU && t->dtype == f->dtype && same_shape(t, f) && (numel(f) == 0 || t->data) &&
-         (f->shape[2] <= 1 || t->strides[2] == 1);
+  return t && t->device == GPU && t->dtype == f->dtype && same_shape(t, f) && (numel(f) == 0 || t->data) &&
+         (f->shape[2] <= 1 || t->strides[2] == 1) && (f->shape[1] <= 1 || t->strides[1] <= kMostStep);
 }
 template <class P>
 Seq<P> seq(const Tensor *t) {
@@ -722,16 +722,24 @@ uint32_t g_most_looks = 4096;
 std::atomic<uint32_t> g_tag{1};  // of the last launch over the workspace's records; the graphs' is 1
 
 // The records of a launch over several chunks. Eager launches tag theirs with a number of their own, so that no record of
-// another one counts; the slot's records are zeros at first. A graph's replays all have one tag, and clear theirs.
-bool look_at(Look &L, uint64_t records, const char *where) {
+// another one counts; the slot's records are zeros at first. A graph's replays all have one tag, and clear theirs. `kept` gets room
+// for `more` floats beside them.
+bool look_at(Look &L, uint64_t records, uint64_t more, float *&kept, const char *where) {
   L.most = g_most_looks;
-  const uint64_t bytes = records * sizeof(Record);
+  const uint64_t bytes = records * sizeof(Record), beside = more * sizeof(float);
   const auto clear = [](void *p, uint64_t n) {
     clear_kernel<<<ceil_div(n / 8, 256), 256, 0, stream()>>>(static_cast<uint64_t *>(p), n / 8);
   };
+  if (capturing() && bytes > workspace_bytes(kRecordSlot)) {
+    L.records = static_cast<Record *>(partials(bytes + beside, where));
+    if (more && L.records) kept = reinterpret_cast<float *>(L.records + records);
+  } else if (more) {
+    kept = static_cast<float *>(partials(beside, where));
+    if (!kept) return false;
+  }
   if (capturing()) {
     L.tag = 1;
-    L.records = static_cast<Record *>(bytes <= workspace_bytes(kRecordSlot) ? workspace(bytes, kRecordSlot) : partials(bytes, where));
+    if (!L.records) L.records = static_cast<Record *>(workspace(bytes, kRecordSlot));
     if (L.records) clear(L.records, bytes);
   } else {
     L.records = static_cast<Record *>(workspace(bytes, kRecordSlot));
@@ -743,9 +751,9 @@ bool look_at(Look &L, uint64_t records, const char *where) {
   }
   return L.records != nullptr;
 }
-// launch(workgroups, records, tiles across a sequence, columns of an XCD)
+// launch(args, workgroups, records, tiles across a sequence, columns of an XCD)
 template <class S, class F>
-bool by_tiles(const ScanArgs &A, const char *where, F &&launch) {
+bool by_tiles(ScanArgs A, const char *where, F &&launch) {
   const uint32_t across = ceil_div(A.width, S::kWidth);
   const uint64_t columns = uint64_t(A.batch) * across;
   // columns that an XCD has more of than another cost time
@@ -756,22 +764,23 @@ bool by_tiles(const ScanArgs &A, const char *where, F &&launch) {
     report_error(where, "%llu tiles of %u steps and %u channels are not supported", (unsigned long long)blocks, S::kTile, S::kWidth);
     return false;
   }
-  if (L.tiles > 1 && !look_at(L, columns * (S::kWidth / 64) * L.tiles, where)) return false;
-  launch(unsigned(blocks), L, across, uint32_t(each));
+  if (L.tiles > 1) {
+    // a tile that is worked out by another one's workgroup reads the initial state, whenever that is
+    const uint64_t states = A.h.p && A.initial == A.last ? uint64_t(A.batch) * A.width : 0;
+    float *kept = nullptr;
+    if (!look_at(L, columns * (S::kWidth / 64) * L.tiles, states, kept, where)) return false;
+    if (states) {
+      copy_kernel<<<ceil_div(states, 256), 256, 0, stream()>>>(kept, A.initial, states);
+      A.initial = kept;
+    }
+  }
+  launch(A, unsigned(blocks), L, across, uint32_t(each));
   return true;
 }
 
 template <class T, class S>
-bool launch_fwd(ScanArgs A, const char *where) {
-  if (A.initial == A.last && A.length > S::kTile) {
-    // a tile that is worked out by another one's workgroup reads the initial state, whenever that is
-    const uint64_t n = uint64_t(A.batch) * A.width;
-    float *const kept = static_cast<float *>(partials(n * sizeof(float), where));
-    if (!kept) return false;
-    copy_kernel<<<ceil_div(n, 256), 256, 0, stream()>>>(kept, A.initial, n);
-    A.initial = kept;
-  }
-  return by_tiles<S>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
+bool launch_fwd(const ScanArgs &A, const char *where) {
+  return by_tiles<S>(A, where, [](const ScanArgs &A, unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
     if constexpr (S::kTile < 256)  // the longest have several
       if (L.tiles == 1) {
         fwd_kernel<T, S, false><<<blocks, S::kLanes, 0, stream()>>>(A, L, across, each);
@@ -782,7 +791,7 @@ bool launch_fwd(ScanArgs A, const char *where) {
 }
 template <class T, class S, bool ADD>
 bool launch_bwd(const ScanArgs &A, const char *where) {
-  return by_tiles<S>(A, where, [&](unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
+  return by_tiles<S>(A, where, [](const ScanArgs &A, unsigned blocks, const Look &L, uint32_t across, uint32_t each) {
     if constexpr (S::kTile < 256)
       if (L.tiles == 1) {
         bwd_kernel<T, S, ADD, false><<<blocks, S::kLanes, 0, stream()>>>(A, L, across, each);

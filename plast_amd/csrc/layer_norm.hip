@@ -717,6 +717,12 @@ void layer_norm_hip_forward(const Tensor **inputs, Tensor *output, KernelParams 
     report_error(where, "the output must have x's type and shape, a contiguous last axis and rows that do not overlap");
     return;
   }
+  const Tensor *x = inputs[0];
+  for (uint64_t d = 0; A.rows && output->data == x->data && d + 1 < x->ndim; ++d)
+    if (x->shape[d] > 1 && output->strides[d] != x->strides[d]) {
+      report_error(where, "the output lies in the place of x with other strides");
+      return;
+    }
   if (A.rows == 0 || !ensure_init()) return;
   A.y = output->data;
   with_float_type(inputs[0]->dtype, [&](auto t) { launch_forward<decltype(t)>(A); });

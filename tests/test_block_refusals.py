@@ -40,7 +40,8 @@ def norm_call(L, kind="forward", eps=1e-5, out=True, **kw):  # noqa: F811
     (dict(eps=0.0), "eps"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"),
     (dict(out=T((6, 10), FLOAT16)), "output must have"), (dict(out=T((6, 11))), "output must have"),
     (dict(out=T((6, 10), strides=(0, 1))), "do not overlap"), (dict(out=T((6, 10), strides=(20, 2))), "contiguous last axis"),
-    (dict(out=T((6, 10), data=0)), "output must have"),
+    (dict(out=T((6, 10), data=0)), "output must have"), (dict(out=T((6, 10), strides=(20, 1), data=AT)), "other strides"),
+    (dict(x=T((6, 10), strides=(0, 1)), out=T((6, 10), data=AT)), "other strides"),
 ])
 def test_layer_norm_refuses(L, kw, match):  # noqa: F811
     norm_call(L, **kw)
@@ -159,6 +160,7 @@ def clip_call(L, grads, bound=1.0, norm=None):  # noqa: F811
     ([T((8,), INT32)], {}, "parameter 0"), ([T((8,)), T((8, 8), device=CPU, data=AT + 4096)], {}, "parameter 1"),
     ([T((8, 8), strides=(1, 8))], {}, "parameter 0"), ([T((8,), data=0)], {}, "parameter 0"), ([((9,), T((8,)))], {}, "parameter 0"),
     ([T((8,)), T((8,))], {}, "share memory"), ([T((8,)), T((8,), data=AT + 28)], {}, "share memory"),
+    ([T((8,)), T((8,), data=AT + 32)], dict(norm=T((1,), data=AT + 60)), "share memory"), ([T((8,))], dict(norm=T((1,), data=AT)), "share memory"),
     ([T((4,), data=AT + 32), T((8,), data=AT + 64), T((4,), BFLOAT16, data=AT + 40)], {}, "share memory"),
 ])
 def test_clip_refuses(L, grads, kw, match):  # noqa: F811

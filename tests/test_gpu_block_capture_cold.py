@@ -54,6 +54,23 @@ def test_gated_recurrence(cold, shape):  # noqa: F811
     s.check_backward(want, "cold")
 
 
+@pytest.mark.parametrize("shape", [(4, 300, 70), (1, 9000, 40)])
+def test_a_state_in_place(cold, shape):  # noqa: F811
+    """The last state takes the place of the initial one, of which several tiles need a copy beside what they leave each other."""
+    print(f"cold capture of a state in place {shape}", flush=True)
+    f, v, initial, lengths, _, _ = _data(shape, "f32", 18)
+    s = Scan(f, v, initial, lengths, "f32")
+    fresh, s.ins[4] = device(initial, "f32"), s.initial
+
+    def call():
+        cold.arena_memcpy_d2d_hip(s.initial.ptr, fresh.ptr, initial.nbytes)
+        s.forward(keep=False)
+    _replayed(cold, call, [s.initial, s.h])
+    want = scan_exact(f, v, initial, lengths)
+    close(values(s.initial), want["last"], want["last_tol"] + stored(want["last"], "f32"), "state")
+    close(values(s.h), want["h"], want["h_tol"] + stored(want["h"], "f32"), "h")
+
+
 def test_clipping(cold):  # noqa: F811
     """The gradients are scaled in place, so each replay starts from fresh ones."""
     from plast_amd import runtime as rt

@@ -205,6 +205,29 @@ def test_not_a_number_spreads_along_its_channel_only():
     assert np.array_equal(np.argwhere(np.isnan(values(s.last))), [[0, 2], [1, 33]])
 
 
+@pytest.mark.parametrize("length", [20, 400, 9000])
+def test_a_gate_that_is_not_a_number_is_not_lost(length):
+    """With a value of 0 nothing but the state itself is NaN, and without gradients behind it but the last state's: what passes on
+    from there is NaN in every step, up to a gate that selects."""
+    shape = (1, length, 70)
+    f, v, initial, lengths, _, dlast = _data(shape, "f32", 19)
+    at, shut = length // 2, length * 3 // 4
+    f[0, at, ::3], v[0, at:, ::3], f[0, shut, 6] = np.nan, 0.0, -np.inf
+    s = Scan(f, v, initial, lengths, "f32", np.zeros(shape, np.float32), dlast)
+    s.forward()
+    bad = np.zeros(shape, bool)
+    bad[0, at:, ::3] = True
+    bad[0, shut:, 6] = False
+    assert np.array_equal(np.isnan(values(s.h)), bad)
+    assert np.array_equal(np.isnan(values(s.last)), bad[:, -1])
+    s.backward()
+    lost = np.zeros(70, bool)
+    lost[::3] = True
+    lost[6] = False  # a gradient of 0 times a gate that is NaN: 0 or NaN
+    got = np.isnan(values(s.initial.kept_grad)[0])
+    assert got[lost].all() and not got[np.arange(70) % 3 != 0].any()
+
+
 @pytest.mark.parametrize("wanted", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 0, 0)])
 def test_only_what_is_wanted(wanted):
     f, v, initial, lengths, dy, dlast = _data((3, 300, 50), "f32", 8, ragged=True)
