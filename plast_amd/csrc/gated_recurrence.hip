@@ -8,6 +8,12 @@
 // smaller sides where those count (Share), and every run starts from there.
 // A product with a factor of 0 is 0 whatever the other factor is (v_mul_legacy_f32): a gate so far out that one side is 0
 // selects, and lets no NaN through.
+//
+// A sequence is cut into tiles of steps, a workgroup each, so that a few long ones fill the card, and read once: a tile's share and
+// what it adds are left for those behind it, and the state that it starts with comes from those before it within the same launch.
+// That wait, a tile's loads, its two passes and its stores follow one another, and the tiles that a CU holds hide it in part: forward
+// [1, 65536, 1024] in bf16 99 us, 4.1 TB/s, vector units 43% busy; [8, 4096, 2048] 90 us, 4.7 TB/s, 48%; backward 151 us, 4.6 TB/s, 53%.
+// States from two launches more (shares alone, then all again) would read f and v twice.
 #include <atomic>
 #include <cmath>
 #include <cstring>
@@ -152,8 +158,8 @@ __device__ __forceinline__ void keep_raw(V (&v)[N]) {
 
 // ------------------------------------------------------------------------- tiles
 
-// A tile is TILE steps (one of kChunk or several) of some channels: lanes across, four channels each, and slices of a few steps,
-// a slice a lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and each lane goes
+// A tile is TILE steps (one kChunk or several) of some channels: lanes across, four channels each, and slices of a few steps, a slice
+// a lane's. Every lane finds its slice's share and what it adds from a state of 0, the slices' are joined in LDS, and each lane goes
 // through its steps again from the state that its slice starts with.
 template <uint32_t ACROSS, uint32_t STEPS, uint32_t TILE, uint32_t WAVES>
 struct Shape {

@@ -5,6 +5,14 @@
 // The mean of fp32 sums is off by some 1e-7 of the largest |x|: a row far from zero loses digits of x - mu. So mu is
 // corrected by the mean of the differences d = x - mu themselves, which are small, in the pass that sums their squares:
 //   mu' = mu + m, m = sum d / C,  sum (x - mu')^2 = sum d^2 - C m^2.
+//
+// The memory bounds it: x read and y written, x and dy read and dx written. So rows are held in registers between their sums and
+// their results, up to 32768 elements of fp32 and 65536 of 16 bits forward and 16384 backward, and workgroups go from row to row
+// with the next rows on their way, as one row's reads, sums and stores one after the other leave the memory idle. A lane keeps its
+// columns' sums for dw and db over all of its rows. us, and TB/s of what passes the L2 caches: forward [16384, 4096] in fp32 86, 6.3;
+// in bf16 46, 5.9; backward in bf16 71, 5.9, and 5 to join the workgroups' sums; [30011, 333] in fp32 18.5, 4.5 and 28, 4.4, its
+// rows off the 16-byte addresses and 84 of 128 units there. Longer rows are read by a workgroup each (three times; backward once for
+// the means and once by columns): backward [512, 20000] in fp16 9 + 18, and 4 to join.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -147,7 +155,7 @@ __device__ __forceinline__ float unit_sum(F f) {
 // ------------------------------------------------------------------------- rows in registers
 
 // A row in U units of each of L lanes: read once, written once. Workgroups go from row to row (B / L of them at a time), the units of
-// the next two on their way, the weight and the bias in registers where there are few.
+// the next two on their way, the weight and the bias in registers; with more than 16 columns a lane a row each.
 template <class T, int L, int U, bool WHOLE>
 __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel(NormArgs A) {
   typedef typename Unit<T>::floats F;
@@ -439,9 +447,12 @@ __global__ __launch_bounds__(kRowBlock) void row_means_kernel(NormArgs A, float 
   }
 }
 
-// Columns of some rows: a workgroup's lanes hold E columns each and go from row to row; blockIdx.x counts the blocks of columns
-// of each piece of `per` rows. dx from the rows' means (null: not wanted), and the piece's share of dw and db to part[piece][2][C].
-template <class T, bool ADD>
+// Columns of some rows: a workgroup's lanes hold E columns each; blockIdx.x counts the blocks of columns of each piece of `per`
+// rows. dx from the rows' means (null: not wanted), and the piece's share of dw and db to part[piece][2][C]. WHOLE: rows of whole
+// units. kColRows rows are read before the first of them is stored, as no load passes a store: backward of [512, 20000] in fp16 in all
+// 32.4 us row by row, 30.4 with four, 29.9 with eight; with pieces of four rows 35.9.
+constexpr uint32_t kColRows = 8;
+template <class T, bool ADD, bool WHOLE>
 __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const float *means, float *part, uint32_t blocks,
                                                             uint32_t per) {
   typedef typename Unit<T>::floats F;
@@ -453,27 +464,34 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
   const W w = load_w<E>(A.w, j, C);
   W dw = 0.0f, db = 0.0f;
   const uint32_t r0 = piece * per, r1 = r0 + per < A.rows ? r0 + per : A.rows;
-#pragma unroll 4
-  for (uint32_t row = r0; row < r1; ++row) {
-    const RowAt<3> at = row_at(A.map, row);
-    const F f = load_cols<T>(static_cast<const T *>(A.x) + at.at[0], j, C);
-    const F u = load_cols<T>(static_cast<const T *>(A.dy) + at.at[1], j, C);
-    const float mu = A.stats[2 * uint64_t(row)], r = A.stats[2 * uint64_t(row) + 1];
-    F n;
+  struct Row {
+    int64_t dx;
+    float mu, r, mg, mgn;
+    typename Unit<T>::vec f, u;
+  } o[kColRows];
+  for (uint32_t row0 = r0; row0 < r1; row0 += kColRows) {
 #pragma unroll
-    for (uint32_t e = 0; e < E; ++e) {
-      n[e] = (f[e] - mu) * r;
-      dw[e] = __builtin_fmaf(u[e], n[e], dw[e]);
-      db[e] += u[e];
+    for (uint32_t k = 0; k < kColRows; ++k) {
+      const uint32_t row = row0 + k < r1 ? row0 + k : r1 - 1;
+      const RowAt<3> at = row_at(A.map, row);
+      o[k].dx = at.at[2];
+      o[k].f = load_held<WHOLE>(static_cast<const T *>(A.x) + at.at[0], j, C);
+      o[k].u = load_held<WHOLE>(static_cast<const T *>(A.dy) + at.at[1], j, C);
+      o[k].mu = A.stats[2 * uint64_t(row)], o[k].r = A.stats[2 * uint64_t(row) + 1];
+      if (means) o[k].mg = means[2 * uint64_t(row)], o[k].mgn = means[2 * uint64_t(row) + 1];
     }
-    if (means) {
-      T *dx = static_cast<T *>(A.dx) + at.at[2];
-      const float mg = means[2 * uint64_t(row)], mgn = means[2 * uint64_t(row) + 1];
-      F d = 0.0f;
-      if constexpr (ADD) d = load_cols<T>(dx, j, C);
 #pragma unroll
-      for (uint32_t e = 0; e < E; ++e) d[e] += r * (__builtin_fmaf(u[e], w[e], -mg) - n[e] * mgn);
-      store_cols<T>(d, dx, j, C);
+    for (uint32_t k = 0; k < kColRows; ++k) {
+      if (row0 + k >= r1) break;
+      const F n = (to_floats<T>(o[k].f) - o[k].mu) * o[k].r, u = to_floats<T>(o[k].u);
+      dw = __builtin_elementwise_fma(u, n, dw);
+      db += u;
+      if (means) {
+        T *dx = static_cast<T *>(A.dx) + o[k].dx;
+        F d = o[k].r * (__builtin_elementwise_fma(u, w, F(-o[k].mg)) - n * o[k].mgn);
+        if constexpr (ADD) d += to_floats<T>(load_held<WHOLE>(dx, j, C));
+        store_held<WHOLE, T>(d, dx, j, C);
+      }
     }
   }
   if (part) {
@@ -608,8 +626,8 @@ bool with_held(uint32_t units, F &&f) {
 #define HELD(l, n) \
   if constexpr (n <= (l == 1024 ? MOST1024 : MOST)) \
     if (units <= l * n) { f(integral_constant<int, l>{}, integral_constant<int, n>{}); return true; }
-  HELD(16, 1) HELD(16, 2) HELD(16, 4) HELD(64, 2) HELD(64, 4) HELD(256, 1) HELD(256, 2) HELD(256, 4) HELD(512, 1) HELD(512, 2) HELD(1024, 1) HELD(1024, 2)
-  HELD(1024, 4) HELD(1024, 8)
+  HELD(16, 1) HELD(16, 2) HELD(16, 4) HELD(64, 2) HELD(64, 4) HELD(256, 1) HELD(256, 2) HELD(256, 4) HELD(512, 1) HELD(512, 2) HELD(1024, 1)
+  HELD(1024, 2) HELD(1024, 4) HELD(1024, 8)
 #undef HELD
   return false;
 }
@@ -684,7 +702,8 @@ bool launch_long_backward(const NormArgs &A, const char *where) {
     by_parts(A, 1, kRowBlock, [&](const NormArgs &p, unsigned n) {
       row_means_kernel<T><<<n, kRowBlock, 0, stream()>>>(p, means);
     });
-  columns_kernel<T, ADD><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
+  if (A.width % E == 0) columns_kernel<T, ADD, true><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
+  else columns_kernel<T, ADD, false><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
   if (sums) launch_join<ADD>(A, part, pieces);
   return true;
 }
