@@ -17,8 +17,8 @@
  * headers and static_asserts equal sizeof/offsetof for every field.
  *
  * Extensions (appended after the reference's last enumerator so every existing numeric value is
- * unchanged): DTYPE gains INT64 (argmax indices) and the 16-bit FLOAT16 and BFLOAT16 (logits and
- * matrices of the operators that say so); OP_TYPE gains ARGMAX, FUSED_ELEMENTWISE,
+ * unchanged): DTYPE gains INT64 (argmax indices) and the 16-bit FLOAT16 and BFLOAT16 (logits,
+ * matrices, rows and sequences of the operators that say so); OP_TYPE gains ARGMAX, FUSED_ELEMENTWISE,
  * SOFTMAX_CROSS_ENTROPY, SOFTMAX, LOG_SOFTMAX, TOKEN_LOGPROB, LAYER_NORM and GATED_RECURRENCE.
  * NewtonSchulz and Muon have no counterpart in the reference.
  */

@@ -12,7 +12,7 @@
 // A sequence is cut into tiles of steps, a workgroup each, so that a few long ones fill the card, and read once: a tile's share and
 // what it adds are left for those behind it, and the state that it starts with comes from those before it within the same launch.
 // That wait, a tile's loads, its two passes and its stores follow one another, and the tiles that a CU holds hide it in part: forward
-// [1, 65536, 1024] in bf16 99 us, 4.1 TB/s, vector units 43% busy; [8, 4096, 2048] 90 us, 4.7 TB/s, 48%; backward 151 us, 4.6 TB/s, 53%.
+// [1, 65536, 1024] in bf16 99 us, 4.2 TB/s, vector units 42% busy; [8, 4096, 2048] 90 us, 4.8 TB/s, 50%; backward 150 us, 4.8 TB/s, 53%.
 // States from two launches more (shares alone, then all again) would read f and v twice.
 #include <atomic>
 #include <cmath>
