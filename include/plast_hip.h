@@ -253,9 +253,7 @@ void plast_hip_adamw_release(AdamW *optimizer, int num_parameters);
  * are skipped, as by the steps; gradients are contiguous GPU tensors of FLOAT32, FLOAT16 or BFLOAT16, of
  * one type or several, and must not share memory, nor with norm (a parameter listed twice is refused). A norm that is NaN
  * or infinite leaves the gradients as they are. max_norm: at least 0, infinity computes the norm alone.
- * Sums are in 64 bits; all results are the same bits on every call. A call over more than 96 gradients
- * keeps their table in device memory, as the steps do; a captured one adds its sums in groups of 96, in an
- * order of its own. No counterpart in the reference. */
+ * Sums are in 64 bits; all results are the same bits on every call. No counterpart in the reference. */
 void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm, Tensor *norm);
 
 /* ------------------------------------------------------------------ matmul epilogue pieces ---- */

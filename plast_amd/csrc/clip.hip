@@ -11,51 +11,55 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <mutex>
 #include <new>
+#include <type_traits>
 #include <vector>
 
-#include "opt_plan.hpp"
 #include "rows.hpp"
 
 namespace plast {
 namespace {
 
-constexpr int kGroup = 96;      // tensors of a launch whose table is in the kernel's arguments
+constexpr int kGroup = 160;     // gradients whose table fits a kernel's arguments
 constexpr int kLanes = 256;
 constexpr uint32_t kUnits = 4;  // of 16 bytes, of a lane in a piece
 constexpr uint64_t kPiece = uint64_t(kLanes) * kUnits * 16;  // bytes
 constexpr uint64_t kCached = uint64_t(256) << 20;  // bytes of the last-level cache
-// Workgroups of all of a call's launches: up to kFewPieces pieces have one each in either launch, so that each XCD scales what its
+// A launch's workgroups: up to kFewPieces pieces have one each in either launch, so that each XCD scales what its
 // own cache has read ([4, 1024, 1024] in fp32 15 us, 21 otherwise). More are summed by kSumBlocks in one run each (1.07 GB 163 us,
 // 6.6 TB/s; 172 with 2048) and scaled by kScaleBlocks in turns of kRun (150 gradients of 1.2 MB 135 us, 172 piece by piece, whose
 // table is looked up for each; one run each 148; 1.07 GB 593, 558 and 685 in all).
 constexpr uint32_t kFewPieces = 2048, kSumBlocks = 1024, kScaleBlocks = 2048, kRun = 2;
 
-// Gradients: p, n, the number of the first piece, the type in vec; in the kernel's arguments or in device memory. of(): the one that
-// piece p is of, the last whose first piece is at or before it.
+struct Entry {
+  char *p;
+  uint64_t n;            // elements
+  uint32_t first, type;  // first: the number of its first piece
+};
+// Gradients, in the kernel's arguments or in device memory. of(): the one that piece p is of, the last whose first piece is at or
+// before it.
 struct InArguments {
-  OptEntry e[kGroup];
-  __device__ __forceinline__ const OptEntry &operator[](int i) const { return e[i]; }
+  Entry e[kGroup];
+  __device__ __forceinline__ const Entry &operator[](int i) const { return e[i]; }
   __device__ __forceinline__ int of(int count, uint32_t p) const {
     int i = 0, hi = count - 1;
     while (i < hi) {
       const int mid = (i + hi + 1) >> 1;
-      if (e[mid].first_block <= p) i = mid;
+      if (e[mid].first <= p) i = mid;
       else hi = mid - 1;
     }
     return i;
   }
 };
 struct InMemory {
-  const OptEntry *e;
-  __device__ __forceinline__ const OptEntry &operator[](int i) const { return e[i]; }
+  const Entry *e;
+  __device__ __forceinline__ const Entry &operator[](int i) const { return e[i]; }
   // by a wave, 64 at a time: two looks for up to 4096 gradients
   __device__ __forceinline__ int of(int count, uint32_t p) const {
     int at = 0, span = count;
     while (span > 1) {
       const int step = (span + 63) / 64, i = int(threadIdx.x & 63) * step;
-      const bool before = i < span && e[at + (i < span ? i : 0)].first_block <= p;
+      const bool before = i < span && e[at + (i < span ? i : 0)].first <= p;
       const int last = (__popcll(__ballot(before)) - 1) * step;
       at += last;
       span = span - last < step ? span - last : step;
@@ -68,15 +72,14 @@ template <class Table, class F>
 __device__ __forceinline__ void for_entries(const Table &T, int count, uint32_t first, uint32_t end, F &&f) {
   if (first >= end) return;
   for (int i = T.of(count, first); i < count; ++i) {
-    const OptEntry E = T[i];
-    const uint32_t behind = i + 1 < count ? T[i + 1].first_block : 0xffffffffu;
-    const uint32_t p0 = E.first_block > first ? E.first_block : first, p1 = behind < end ? behind : end;
-    f(E, p0 - E.first_block, p1 - E.first_block);
+    const Entry E = T[i];
+    const uint32_t behind = i + 1 < count ? T[i + 1].first : 0xffffffffu;
+    const uint32_t p0 = E.first > first ? E.first : first, p1 = behind < end ? behind : end;
+    f(E, p0 - E.first, p1 - E.first);
     if (behind >= end) return;
   }
 }
 
-// Every launch's share of the work.
 struct ClipRun {
   int count;
   uint32_t pieces, per, run;  // per: of a workgroup that sums; run: of one that scales, in each of its turns
@@ -118,7 +121,7 @@ __device__ __forceinline__ void for_rest(T *g, uint64_t n, uint32_t piece, F &&f
 
 // The sum of the squares of pieces [p, end) of a gradient: the next piece's units on their way, a sum for each unit.
 template <class T, bool NT>
-__device__ __forceinline__ double squares(const OptEntry &E, uint32_t p, uint32_t end) {
+__device__ __forceinline__ double squares(const Entry &E, uint32_t p, uint32_t end) {
   const T *g = reinterpret_cast<const T *>(E.p);
   const uint32_t whole = uint32_t(E.n / kPieceOf<T>), stop = end < whole ? end : whole;
   double s[kUnits] = {};
@@ -149,7 +152,7 @@ static_assert(kUnits == 4, "four sums");
 
 // Pieces [p, end) times scale, the next one's units on their way.
 template <class T>
-__device__ __forceinline__ void scale_pieces(const OptEntry &E, uint32_t p, uint32_t end, double scale) {
+__device__ __forceinline__ void scale_pieces(const Entry &E, uint32_t p, uint32_t end, double scale) {
   T *g = reinterpret_cast<T *>(E.p);
   const uint32_t whole = uint32_t(E.n / kPieceOf<T>), stop = end < whole ? end : whole;
   if (p < stop) {
@@ -179,9 +182,9 @@ __global__ __launch_bounds__(kLanes) void squares_kernel(Table A, ClipRun R, dou
   __shared__ double lds[kLanes / 64];
   const uint32_t first = blockIdx.x * R.per, end = first + R.per < R.pieces ? first + R.per : R.pieces;
   double s = 0.0;
-  for_entries(A, R.count, first, end, [&](const OptEntry &E, uint32_t p, uint32_t to) {
-    if (E.vec == FLOAT32) s += squares<float, NT>(E, p, to);
-    else if (E.vec == FLOAT16) s += squares<f16_t, NT>(E, p, to);
+  for_entries(A, R.count, first, end, [&](const Entry &E, uint32_t p, uint32_t to) {
+    if (E.type == FLOAT32) s += squares<float, NT>(E, p, to);
+    else if (E.type == FLOAT16) s += squares<f16_t, NT>(E, p, to);
     else s += squares<bf16_t, NT>(E, p, to);
   });
   s = block_sum(s, lds);
@@ -201,43 +204,25 @@ __global__ __launch_bounds__(kLanes) void scale_kernel(Table A, ClipRun R, const
   const double scale = double(bound) / norm;
   for (uint64_t p = uint64_t(blockIdx.x) * R.run; p < R.pieces; p += uint64_t(gridDim.x) * R.run) {
     const uint32_t first = uint32_t(p), end = R.pieces - first < R.run ? R.pieces : first + R.run;
-    for_entries(A, R.count, first, end, [&](const OptEntry &E, uint32_t q, uint32_t to) {
-      if (E.vec == FLOAT32) scale_pieces<float>(E, q, to, scale);
-      else if (E.vec == FLOAT16) scale_pieces<f16_t>(E, q, to, scale);
+    for_entries(A, R.count, first, end, [&](const Entry &E, uint32_t q, uint32_t to) {
+      if (E.type == FLOAT32) scale_pieces<float>(E, q, to, scale);
+      else if (E.type == FLOAT16) scale_pieces<f16_t>(E, q, to, scale);
       else scale_pieces<bf16_t>(E, q, to, scale);
     });
   }
 }
 
+// Part of a longer table to device memory, from the arguments: a copy from the host would have to keep its source until it is done, or be
+// waited for. us, this / a table copied and kept for as long as the calls' gradients are the same: 400 gradients of 3 KB 20 / 11, of
+// other addresses in each call 21 / 31; 400 of 0.8 MB 161 / 155 and 209 / 226.
+__global__ __launch_bounds__(kLanes) void table_kernel(InArguments A, int count, Entry *to) {
+  if (int(threadIdx.x) < count) to[threadIdx.x] = A.e[threadIdx.x];
+}
+static_assert(kGroup <= kLanes, "a lane an entry");
+
 // ------------------------------------------------------------------------- host
 
 const char *const where = "clip_grad_norm_hip";
-std::mutex g_table_mu;
-OptTableCache g_table;  // of the last call with more than kGroup gradients
-
-const OptEntry *device_table(const std::vector<OptEntry> &e) {
-  return g_table.get(
-      e,
-      [&]() {
-        if (hipStreamSynchronize(stream()) == hipSuccess) return true;
-        report_error(where, "waiting for the library stream failed");
-        return false;
-      },
-      [&](size_t n) -> OptEntry * {
-        OptEntry *p = nullptr;
-        if (hipMalloc(&p, n * sizeof(OptEntry)) == hipSuccess) return p;
-        report_error(where, "allocation of the tensor table (%zu entries) failed", n);
-        return nullptr;
-      },
-      [](OptEntry *p) { (void)hipFree(p); },
-      [&](OptEntry *dst, const std::vector<OptEntry> &src) {
-        if (hipMemcpyAsync(dst, src.data(), src.size() * sizeof(OptEntry), hipMemcpyHostToDevice, stream()) == hipSuccess &&
-            hipStreamSynchronize(stream()) == hipSuccess)
-          return true;
-        report_error(where, "upload of the tensor table failed");
-        return false;
-      });
-}
 
 // Whether two of the gradients share memory: one scaled by two workgroups at once would be scaled twice, or once.
 bool share_memory(std::vector<std::pair<uint64_t, uint64_t>> &spans) {
@@ -267,7 +252,7 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
     report_error(where, "norm must be a FLOAT32 GPU tensor of one element");
     return;
   }
-  std::vector<OptEntry> entries;
+  std::vector<Entry> entries;
   std::vector<std::pair<uint64_t, uint64_t>> spans;
   uint64_t pieces = 0;
   if (parameters && num_parameters > 0) entries.reserve(size_t(num_parameters)), spans.reserve(size_t(num_parameters));
@@ -282,15 +267,9 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
                    "size", k);
       return;
     }
-    OptEntry e;
-    memset(&e, 0, sizeof e);
-    e.p = static_cast<float *>(g->data);
-    e.n = n;
-    e.first_block = uint32_t(pieces);
-    e.vec = uint32_t(g->dtype);
     const uint64_t bytes = n * float_bytes(g), at = reinterpret_cast<uint64_t>(g->data);
+    entries.push_back({static_cast<char *>(g->data), n, uint32_t(pieces), uint32_t(g->dtype)});
     pieces += (bytes + kPiece - 1) / kPiece;
-    entries.push_back(e);
     spans.emplace_back(at, at + bytes);
   }
   if (pieces >= uint64_t(1) << 32) {
@@ -304,58 +283,33 @@ void clip_grad_norm_hip(Tensor **parameters, int num_parameters, float max_norm,
   }
   if ((entries.empty() && !norm) || !ensure_init()) return;
 
-  // the launches: one over a table in device memory, or, in a capture, one for each kGroup gradients
-  const bool table = entries.size() > size_t(kGroup) && !capturing();
-  const size_t group = table ? entries.size() : size_t(kGroup);
-  const size_t launches = entries.empty() ? 1 : (entries.size() + group - 1) / group;
-  const auto share = [&](uint32_t blocks) { return uint32_t(std::max<size_t>(1, blocks / launches)); };
-  std::lock_guard<std::mutex> lk(g_table_mu);
-  const OptEntry *T = table ? device_table(entries) : nullptr;
-  if (table && !T) return;
-  struct Launch {
-    ClipRun run;
-    uint32_t blocks, scale_blocks, first_sum;
-  };
-  std::vector<Launch> plan;
-  uint32_t sums = 0;
-  for (size_t i = 0; i < launches; ++i) {
-    const size_t a = i * group, b = std::min(entries.size(), a + group);
-    const uint64_t p0 = a < b ? entries[a].first_block : 0, p1 = b < entries.size() ? entries[b].first_block : pieces;
-    const uint32_t n = uint32_t(p1 - p0);
-    const bool few = n <= share(kFewPieces);
-    const uint32_t per = few ? 1 : ceil_div(n, share(kSumBlocks)), blocks = n ? ceil_div(n, per) : 1;
-    const uint32_t run = few ? 1 : kRun, scale = few ? blocks : std::min(ceil_div(n, run), share(kScaleBlocks));
-    plan.push_back({{int(b - a), n, per, run}, blocks, scale, sums});
-    sums += blocks;
-  }
-  double *room = static_cast<double *>(partials(sums * sizeof(double), where));
+  const uint32_t n = uint32_t(pieces), per = n <= kFewPieces ? 1 : ceil_div(n, kSumBlocks), sums = n ? ceil_div(n, per) : 1;
+  const uint32_t run = n <= kFewPieces ? 1 : kRun, blocks = n <= kFewPieces ? sums : std::min(ceil_div(n, run), kScaleBlocks);
+  const bool many = entries.size() > size_t(kGroup);
+  char *room = static_cast<char *>(partials(sums * sizeof(double) + (many ? entries.size() * sizeof(Entry) : 0), where));
   if (!room) return;
-  const bool past = pieces * kPiece > kCached;
+  double *const to = reinterpret_cast<double *>(room);
   float *const out = norm ? static_cast<float *>(norm->data) : nullptr;
-  // both launches of each group, all sums before the first scaling
-  const auto launch = [&](auto tables) {
-    typedef decltype(tables(0)) Table;
-    for (size_t i = 0; i < launches; ++i) {
-      double *to = room + plan[i].first_sum;
-      if (past) squares_kernel<Table, true><<<plan[i].blocks, kLanes, 0, stream()>>>(tables(i), plan[i].run, to);
-      else squares_kernel<Table, false><<<plan[i].blocks, kLanes, 0, stream()>>>(tables(i), plan[i].run, to);
-    }
-    for (size_t i = 0; i < launches; ++i)
-      scale_kernel<Table><<<plan[i].scale_blocks, kLanes, 0, stream()>>>(tables(i), plan[i].run, room, sums, max_norm,
-                                                                         i == 0 ? out : nullptr);
+  const ClipRun R{int(entries.size()), n, per, run};
+  const auto launch = [&](const auto &table) {
+    typedef std::decay_t<decltype(table)> Table;
+    if (pieces * kPiece > kCached) squares_kernel<Table, true><<<sums, kLanes, 0, stream()>>>(table, R, to);
+    else squares_kernel<Table, false><<<sums, kLanes, 0, stream()>>>(table, R, to);
+    scale_kernel<Table><<<blocks, kLanes, 0, stream()>>>(table, R, to, sums, max_norm, out);
   };
-  if (T) {
-    launch([&](size_t) { return InMemory{T}; });
+  InArguments A;
+  memset(&A, 0, sizeof A);
+  if (!many) {
+    std::copy(entries.begin(), entries.end(), A.e);
+    launch(A);
   } else {
-    launch([&](size_t i) {
-      InArguments A;
-      memset(&A, 0, sizeof A);
-      for (int k = 0; k < plan[i].run.count; ++k) {
-        A.e[k] = entries[i * group + k];
-        A.e[k].first_block -= entries[i * group].first_block;
-      }
-      return A;
-    });
+    Entry *const table = reinterpret_cast<Entry *>(to + sums);
+    for (size_t i = 0; i < entries.size(); i += kGroup) {
+      const size_t m = std::min(entries.size() - i, size_t(kGroup));
+      std::copy_n(entries.begin() + i, m, A.e);
+      table_kernel<<<1, kLanes, 0, stream()>>>(A, int(m), table + i);
+    }
+    launch(InMemory{table});
   }
   finish(where);
 } catch (const std::bad_alloc &) {

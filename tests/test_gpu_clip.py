@@ -50,7 +50,7 @@ def _check(arrays, kinds, ratio, leads=None):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("sizes", [[1], [2, 3], [255, 256, 257], [4096], [16384, 16383, 5], [100003], [7] * 90, [1000] * 97, [33] * 300,
+@pytest.mark.parametrize("sizes", [[1], [2, 3], [255, 256, 257], [4096], [16384, 16383, 5], [100003], [7] * 90, [1000] * 97, [33] * 300, [5] * 160, [9] * 161, [70] * 330,
                                    [3000001, 1, 65536]])
 def test_sizes(sizes, kind):
     rng = np.random.RandomState(len(sizes))
