@@ -10,7 +10,7 @@
 // their results, up to 32768 elements of fp32 and 65536 of 16 bits forward and 16384 backward, and workgroups go from row to row
 // with the next rows on their way, as one row's reads, sums and stores one after the other leave the memory idle. A lane keeps its
 // columns' sums for dw and db over all of its rows. us, and TB/s of what passes the L2 caches: forward [16384, 4096] in fp32 86, 6.3;
-// in bf16 46, 5.9; backward in bf16 71, 5.9, and 5 to join the workgroups' sums; [30011, 333] in fp32 18.5, 4.5 and 28, 4.4, its
+// in bf16 46, 5.9; backward in bf16 66, 6.4, and 5 to join the workgroups' sums; [30011, 333] in fp32 15, 5.5 and 30, 4.1, its
 // rows off the 16-byte addresses and 84 of 128 units there. Longer rows are read by a workgroup each (three times; backward once for
 // the means and once by columns): backward [512, 20000] in fp16 9 + 18, and 4 to join.
 #include <algorithm>
@@ -39,8 +39,8 @@ struct NormArgs {
 };
 
 // Results are stored past the caches and operands read through them: what fits the last-level cache is there for the backward pass.
-// us, both ways / operands past the caches too: forward [30011, 333] in fp32 19.7 / 24.0, [16384, 4096] 100 / 98, backward
-// [512, 20000] in fp16 42 / 56, [30011, 333] in fp32 34 / 38; results through them: forward [16384, 4096] 103.
+// us, that / operands past the caches too, before units were read without branches: forward [30011, 333] in fp32 19.7 / 24.0,
+// [16384, 4096] 100 / 98, backward [512, 20000] in fp16 42 / 56; results through the caches: forward [16384, 4096] 103.
 template <class T>
 __device__ __forceinline__ void store_any(typename Unit<T>::floats f, T *p) {
   __builtin_nontemporal_store(__builtin_convertvector(f, typename Unit<T>::vec), reinterpret_cast<typename Unit<T>::any *>(p));
@@ -58,12 +58,31 @@ __device__ __forceinline__ typename Unit<T>::vec load_raw(const T *row, uint32_t
     if (j + e < width) v[e] = row[j + e];
   return v;
 }
-// The same where WHOLE says that a row's units are whole and as many as its lanes hold: no branch, so that the loads of several
-// rows are told apart while they are on their way.
-template <bool WHOLE, class T>
+// How a row's units lie that its lanes hold: kWhole, all of them whole; kInside, those that reach beyond the row's end moved back to
+// lie before it, where their first elements are other units' too; kAny, for rows shorter than a unit. The first two read without
+// branches, so that the loads of several rows are told apart while they are on their way: us, rows as in kAny / kInside, forward
+// [8192, 5000] in fp32 100 / 79, backward [60000, 100] in fp16 37 / 18, [8192, 5001] in bf16 129 / 80.
+enum Fit { kWhole, kInside, kAny };
+template <Fit FIT, class T>
+__device__ __forceinline__ uint32_t place(uint32_t j, uint32_t width) {
+  return FIT == kInside && j + Unit<T>::E > width ? width - Unit<T>::E : j;
+}
+template <Fit FIT, class T>
 __device__ __forceinline__ typename Unit<T>::vec load_held(const T *row, uint32_t j, uint32_t width) {
-  if constexpr (WHOLE) return *reinterpret_cast<const typename Unit<T>::any *>(row + j);
-  else return load_raw(row, j, width);
+  if constexpr (FIT == kAny) return load_raw(row, j, width);
+  else return *reinterpret_cast<const typename Unit<T>::any *>(row + place<FIT, T>(j, width));
+}
+// Whether element e of the unit at column j is in the row and no other unit's.
+template <Fit FIT, class T>
+__device__ __forceinline__ bool owns(uint32_t e, uint32_t j, uint32_t width) {
+  return FIT == kWhole || (FIT == kAny ? j + e < width : place<FIT, T>(j, width) + e >= j);
+}
+// A unit's own elements, zeros for others.
+template <Fit FIT, class T>
+__device__ __forceinline__ typename Unit<T>::floats own(typename Unit<T>::floats f, uint32_t j, uint32_t width) {
+#pragma unroll
+  for (uint32_t e = 0; e < Unit<T>::E; ++e) f[e] = owns<FIT, T>(e, j, width) ? f[e] : 0.0f;
+  return f;
 }
 template <class T>
 __device__ __forceinline__ typename Unit<T>::floats load_cols(const T *row, uint32_t j, uint32_t width) {
@@ -81,10 +100,18 @@ __device__ __forceinline__ void store_cols(typename Unit<T>::floats f, T *row, u
   for (uint32_t e = 0; e < E; ++e)
     if (j + e < width) row[j + e] = T(f[e]);
 }
-template <bool WHOLE, class T>
+template <Fit FIT, class T>
 __device__ __forceinline__ void store_held(typename Unit<T>::floats f, T *row, uint32_t j, uint32_t width) {
-  if constexpr (WHOLE) store_any<T>(f, row + j);
-  else store_cols<T>(f, row, j, width);
+  if constexpr (FIT == kAny) {
+    store_cols<T>(f, row, j, width);
+  } else if (FIT == kWhole || j + Unit<T>::E <= width) {
+    store_any<T>(f, row + j);
+  } else if (j < width) {
+    const uint32_t at = place<FIT, T>(j, width);
+#pragma unroll
+    for (uint32_t e = 0; e < Unit<T>::E; ++e)
+      if (at + e >= j) row[at + e] = T(f[e]);
+  }
 }
 // E columns of a weight or bias.
 template <int E>
@@ -156,7 +183,7 @@ __device__ __forceinline__ float unit_sum(F f) {
 
 // A row in U units of each of L lanes: read once, written once. Workgroups go from row to row (B / L of them at a time), the units of
 // the next two on their way, the weight and the bias in registers; with more than 16 columns a lane a row each.
-template <class T, int L, int U, bool WHOLE>
+template <class T, int L, int U, Fit FIT>
 __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel(NormArgs A) {
   typedef typename Unit<T>::floats F;
   typedef typename Unit<T>::vec V;
@@ -172,12 +199,12 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
     V v[U];
   };
   const auto load = [&](Row &o, uint64_t row) {
-    if (WHOLE) row = row < end ? row : end - 1;
+    if (FIT != kAny) row = row < end ? row : end - 1;
     else if (row >= end) return;
     const RowAt<3> at = row_at(A.map, uint32_t(row));
     o.y = at.at[1];
 #pragma unroll
-    for (int u = 0; u < U; ++u) o.v[u] = load_held<WHOLE>(static_cast<const T *>(A.x) + at.at[0], (u * L + lane) * E, C);
+    for (int u = 0; u < U; ++u) o.v[u] = load_held<FIT>(static_cast<const T *>(A.x) + at.at[0], (u * L + lane) * E, C);
   };
   W w[HOLD ? U : 1], b[HOLD ? U : 1];
   const float inv = 1.0f / float(C);
@@ -185,7 +212,7 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
     F f[U];
     float s = 0.0f, q = 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) f[u] = to_floats<T>(o.v[u]), s += unit_sum(f[u]);
+    for (int u = 0; u < U; ++u) f[u] = own<FIT, T>(to_floats<T>(o.v[u]), (u * L + lane) * E, C), s += unit_sum(f[u]);
     T *y = static_cast<T *>(A.y) + o.y;
     if constexpr (HOLD) load(o, row + 2 * uint64_t(step));
     row_sums<L>(s, q, lds[0]);
@@ -193,13 +220,7 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
     s = q = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t j = (u * L + lane) * E;
-      F d = f[u] - mu;
-      if (!WHOLE && j + E > C) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (j + e >= C) d[e] = 0.0f;
-      }
+      const F d = own<FIT, T>(f[u] - mu, (u * L + lane) * E, C);
       s += unit_sum(d);
       q += unit_sum(d * d);
     }
@@ -214,8 +235,10 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint32_t j = (u * L + lane) * E;
-      if constexpr (HOLD) store_held<WHOLE, T>(__builtin_elementwise_fma((f[u] - mu) * r, w[u], b[u]), y, j, C);
-      else store_held<WHOLE, T>(__builtin_elementwise_fma((f[u] - mu) * r, load_w<E>(A.w, j, C), load_w<E>(A.b, j, C)), y, j, C);
+      W a, c;
+      if constexpr (HOLD) a = w[u], c = b[u];
+      else a = load_w<E>(A.w, place<FIT, T>(j, C), C), c = load_w<E>(A.b, place<FIT, T>(j, C), C);
+      store_held<FIT, T>(__builtin_elementwise_fma((f[u] - mu) * r, a, c), y, j, C);
     }
   };
   Row one, two;
@@ -228,8 +251,9 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
   if constexpr (HOLD) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      w[u] = load_w<E>(A.w, (u * L + lane) * E, C);
-      b[u] = load_w<E>(A.b, (u * L + lane) * E, C);
+      const uint32_t j = place<FIT, T>((u * L + lane) * E, C);
+      w[u] = load_w<E>(A.w, j, C);
+      b[u] = load_w<E>(A.b, j, C);
     }
   }
   for (uint64_t row = row0;; row += 2 * uint64_t(step)) {
@@ -240,15 +264,17 @@ __global__ __launch_bounds__(L > kRowBlock ? L : kRowBlock) void fwd_held_kernel
   }
 }
 
-// The gradients of rows held as above: a lane keeps the shares of dw and db of its columns in registers, the workgroup's rows are
+// The gradients of rows held as above, but one or two on their way: a lane keeps the shares of dw and db of its columns in registers, the workgroup's rows are
 // joined at the end, and its share goes to part[workgroup][2][C]. x and dy are read once.
 template <int L>
 constexpr int kBwdBlock = L > 512 ? L : 512;
-template <class T, int L, int U, bool WHOLE, bool ADD>
+template <class T, int L, int U, Fit FIT, bool ADD>
 __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, float *part) {
   typedef typename Unit<T>::floats F;
   typedef typename Unit<T>::vec V;
   constexpr int E = Unit<T>::E, R = kBwdBlock<L> / L;  // rows at a time
+  // rows on their way, as many as registers hold: with 16 columns a lane [4096, 16384] in bf16 104 us with one, 153 with two
+  constexpr uint32_t AHEAD = U * E > 8 ? 1 : 2;
   typedef typename Cols<E>::floats W;
   __shared__ float lds[2][2 * kBwdBlock<L> / 64];
   const uint32_t group = threadIdx.x / L, lane = threadIdx.x % L, C = A.width, step = gridDim.x * R;
@@ -259,7 +285,7 @@ __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, floa
     V f[U], g[U];
   };
   const auto load = [&](Row &o, uint64_t row) {
-    if (WHOLE) {
+    if (FIT != kAny) {
       row = row < A.rows ? row : A.rows - 1;
     } else if (row >= A.rows) {
       o.mu = o.r = 0.0f;
@@ -271,8 +297,8 @@ __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, floa
     o.dx = at.at[2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      o.f[u] = load_held<WHOLE>(x + at.at[0], (u * L + lane) * E, C);
-      o.g[u] = load_held<WHOLE>(dy + at.at[1], (u * L + lane) * E, C);
+      o.f[u] = load_held<FIT>(x + at.at[0], (u * L + lane) * E, C);
+      o.g[u] = load_held<FIT>(dy + at.at[1], (u * L + lane) * E, C);
     }
     o.mu = A.stats[2 * row], o.r = A.stats[2 * row + 1];
   };
@@ -286,17 +312,12 @@ __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, floa
     T *dx = static_cast<T *>(A.dx) + o.dx;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      f[u] = (to_floats<T>(o.f[u]) - o.mu) * r;
-      g[u] = to_floats<T>(o.g[u]);
       const uint32_t j = (u * L + lane) * E;
-      if (!WHOLE && j + E > C) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (j + e >= C) f[u][e] = 0.0f;
-      }
+      f[u] = own<FIT, T>((to_floats<T>(o.f[u]) - o.mu) * r, j, C);
+      g[u] = own<FIT, T>(to_floats<T>(o.g[u]), j, C);
     }
-    load(o, row + 2 * uint64_t(step));
-    if (WHOLE && R > 1 && row >= A.rows) {  // a row behind the last
+    load(o, row + AHEAD * uint64_t(step));
+    if (FIT != kAny && R > 1 && row >= A.rows) {  // a row behind the last
 #pragma unroll
       for (int u = 0; u < U; ++u) g[u] = 0.0f;
     }
@@ -317,22 +338,23 @@ __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, floa
     for (int u = 0; u < U; ++u) {
       const uint32_t j = (u * L + lane) * E;
       F d = r * __builtin_elementwise_fma(f[u], F(-q), g[u] - s);
-      if constexpr (ADD) d += to_floats<T>(load_held<WHOLE>(dx, j, C));
-      store_held<WHOLE, T>(d, dx, j, C);
+      if constexpr (ADD) d += to_floats<T>(load_held<FIT>(dx, j, C));
+      store_held<FIT, T>(d, dx, j, C);
     }
   };
   Row one, two;
   load(one, blockIdx.x * R + group);
-  load(two, blockIdx.x * R + step + group);
+  if constexpr (AHEAD == 2) load(two, blockIdx.x * R + step + group);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    w[u] = load_w<E>(A.w, (u * L + lane) * E, C);
+    w[u] = load_w<E>(A.w, place<FIT, T>((u * L + lane) * E, C), C);
     dw[u] = db[u] = 0.0f;
   }
   // all of a workgroup's lanes take as many turns
-  for (uint64_t first = blockIdx.x * R; first < A.rows; first += 2 * uint64_t(step)) {
+  for (uint64_t first = blockIdx.x * R; first < A.rows; first += AHEAD * uint64_t(step)) {
     turn(one, first + group);
-    if (first + step < A.rows) turn(two, first + step + group);
+    if constexpr (AHEAD == 2)
+      if (first + step < A.rows) turn(two, first + step + group);
   }
   if (!part) return;
   // the groups' shares, halves onto halves
@@ -363,8 +385,8 @@ __global__ __launch_bounds__(kBwdBlock<L>) void bwd_held_kernel(NormArgs A, floa
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const uint32_t j = (u * L + lane) * E + e;
-          if (j < C) p[j] = mine[u][e];
+          const uint32_t j = (u * L + lane) * E;
+          if (owns<FIT, T>(e, j, C)) p[place<FIT, T>(j, C) + e] = mine[u][e];
         }
     }
   }
@@ -448,11 +470,10 @@ __global__ __launch_bounds__(kRowBlock) void row_means_kernel(NormArgs A, float 
 }
 
 // Columns of some rows: a workgroup's lanes hold E columns each; blockIdx.x counts the blocks of columns of each piece of `per`
-// rows. dx from the rows' means (null: not wanted), and the piece's share of dw and db to part[piece][2][C]. WHOLE: rows of whole
-// units. kColRows rows are read before the first of them is stored, as no load passes a store: backward of [512, 20000] in fp16 in all
+// rows. dx from the rows' means (null: not wanted), and the piece's share of dw and db to part[piece][2][C]. kColRows rows are read before the first of them is stored, as no load passes a store: backward of [512, 20000] in fp16 in all
 // 32.4 us row by row, 30.4 with four, 29.9 with eight; with pieces of four rows 35.9.
 constexpr uint32_t kColRows = 8;
-template <class T, bool ADD, bool WHOLE>
+template <class T, bool ADD, Fit FIT>
 __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const float *means, float *part, uint32_t blocks,
                                                             uint32_t per) {
   typedef typename Unit<T>::floats F;
@@ -461,7 +482,7 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
   const uint32_t piece = blockIdx.x / blocks, C = A.width;
   const uint32_t j = ((blockIdx.x - piece * blocks) * kRowBlock + threadIdx.x) * E;
   if (j >= C) return;
-  const W w = load_w<E>(A.w, j, C);
+  const W w = load_w<E>(A.w, place<FIT, T>(j, C), C);
   W dw = 0.0f, db = 0.0f;
   const uint32_t r0 = piece * per, r1 = r0 + per < A.rows ? r0 + per : A.rows;
   struct Row {
@@ -475,8 +496,8 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
       const uint32_t row = row0 + k < r1 ? row0 + k : r1 - 1;
       const RowAt<3> at = row_at(A.map, row);
       o[k].dx = at.at[2];
-      o[k].f = load_held<WHOLE>(static_cast<const T *>(A.x) + at.at[0], j, C);
-      o[k].u = load_held<WHOLE>(static_cast<const T *>(A.dy) + at.at[1], j, C);
+      o[k].f = load_held<FIT>(static_cast<const T *>(A.x) + at.at[0], j, C);
+      o[k].u = load_held<FIT>(static_cast<const T *>(A.dy) + at.at[1], j, C);
       o[k].mu = A.stats[2 * uint64_t(row)], o[k].r = A.stats[2 * uint64_t(row) + 1];
       if (means) o[k].mg = means[2 * uint64_t(row)], o[k].mgn = means[2 * uint64_t(row) + 1];
     }
@@ -489,18 +510,18 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
       if (means) {
         T *dx = static_cast<T *>(A.dx) + o[k].dx;
         F d = o[k].r * (__builtin_elementwise_fma(u, w, F(-o[k].mg)) - n * o[k].mgn);
-        if constexpr (ADD) d += to_floats<T>(load_held<WHOLE>(dx, j, C));
-        store_held<WHOLE, T>(d, dx, j, C);
+        if constexpr (ADD) d += to_floats<T>(load_held<FIT>(dx, j, C));
+        store_held<FIT, T>(d, dx, j, C);
       }
     }
   }
   if (part) {
-    float *p = part + uint64_t(piece) * 2 * C;
+    float *p = part + uint64_t(piece) * 2 * C + place<FIT, T>(j, C);
 #pragma unroll
     for (uint32_t e = 0; e < E; ++e)
-      if (j + e < C) {
-        p[j + e] = dw[e];
-        p[C + j + e] = db[e];
+      if (owns<FIT, T>(e, j, C)) {
+        p[e] = dw[e];
+        p[C + e] = db[e];
       }
   }
 }
@@ -632,16 +653,25 @@ bool with_held(uint32_t units, F &&f) {
   return false;
 }
 
-// Workgroups of 256 lanes that go from row to row, for each CU: [30011, 333] in fp32 17.4 us with four, 18.8 with eight, a row each
-// 24; [16384, 4096] in bf16 51, 52, 62.
+// f(how a row's units lie that lanes hold in `UNITS` units).
+template <class T, int UNITS, class F>
+void with_fit(uint32_t width, F &&f) {
+  using std::integral_constant;
+  if (width == UNITS * Unit<T>::E) return f(integral_constant<Fit, kWhole>{});
+  if constexpr (UNITS == 16)
+    if (width < Unit<T>::E) return f(integral_constant<Fit, kAny>{});
+  f(integral_constant<Fit, kInside>{});
+}
+
+// Workgroups of 256 lanes that go from row to row, for each CU: [16384, 4096] in bf16 51 us with four, 52 with eight, a row
+// each 62.
 constexpr uint64_t kFwdPerCu = 4;
 template <class T>
 void launch_forward(const NormArgs &A) {
   const bool held = with_held<16 / int(Unit<T>::E), 8>(ceil_div(A.width, Unit<T>::E), [&](auto lanes, auto units) {
     constexpr int L = decltype(lanes)::value, U = decltype(units)::value, B = L > kRowBlock ? L : kRowBlock;
     const auto launch = [](const NormArgs &part, unsigned blocks) {
-      if (part.width == L * U * Unit<T>::E) fwd_held_kernel<T, L, U, true><<<blocks, B, 0, stream()>>>(part);
-      else fwd_held_kernel<T, L, U, false><<<blocks, B, 0, stream()>>>(part);
+      with_fit<T, L * U>(part.width, [&](auto fit) { fwd_held_kernel<T, L, U, decltype(fit)::value><<<blocks, B, 0, stream()>>>(part); });
     };
     if constexpr (U * int(Unit<T>::E) <= 16)  // goes from row to row
       launch(A, unsigned(std::min<uint64_t>(ceil_div(A.rows, B / L), uint64_t(num_cus()) * kFwdPerCu * kRowBlock / B)));
@@ -672,8 +702,9 @@ bool launch_held_backward(const NormArgs &A, bool &held, const char *where) {
       part = static_cast<float *>(partials(blocks * 2 * A.width * sizeof(float), where));
       if (!part) return;
     }
-    if (A.width == L * U * Unit<T>::E) bwd_held_kernel<T, L, U, true, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
-    else bwd_held_kernel<T, L, U, false, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
+    with_fit<T, L * U>(A.width, [&](auto fit) {
+      bwd_held_kernel<T, L, U, decltype(fit)::value, ADD><<<unsigned(blocks), kBwdBlock<L>, 0, stream()>>>(A, part);
+    });
     if (part) launch_join<ADD>(A, part, blocks);
     ok = true;
   });
@@ -702,8 +733,8 @@ bool launch_long_backward(const NormArgs &A, const char *where) {
     by_parts(A, 1, kRowBlock, [&](const NormArgs &p, unsigned n) {
       row_means_kernel<T><<<n, kRowBlock, 0, stream()>>>(p, means);
     });
-  if (A.width % E == 0) columns_kernel<T, ADD, true><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
-  else columns_kernel<T, ADD, false><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
+  if (A.width % E == 0) columns_kernel<T, ADD, kWhole><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
+  else columns_kernel<T, ADD, kInside><<<unsigned(pieces * blocks), kRowBlock, 0, stream()>>>(A, means, part, blocks, per);
   if (sums) launch_join<ADD>(A, part, pieces);
   return true;
 }
