@@ -104,6 +104,33 @@ def test_shapes(shape, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("width", [3, 4, 5, 6, 7, 63, 65, 66, 67, 68, 69, 129, 131, 133, 191, 193])
+def test_ends_of_rows(width, kind):
+    """Whole tiles of steps whose channels end inside a tile, or a few channels into one."""
+    _check((2, 520, width), kind, lead=1, pitch=width + 3)
+    _check((2, 520, width), kind, add=True, seed=3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("width", [6, 69, 131])
+@pytest.mark.parametrize("channel", [-1, -3, -5])
+def test_what_is_not_finite_near_the_end_of_rows_stays_in_its_channel(channel, width, kind):
+    f, v, initial, lengths, dy, dlast = _data((2, 520, width), kind, 4)
+    results = []
+    for bad in (False, True):
+        if bad:
+            f, v, dy = f.copy(), v.copy(), dy.copy()
+            f[:, 7, channel], v[:, 9, channel], dy[:, 11, channel] = np.nan, np.inf, -np.inf
+        s = Scan(f, v, initial, lengths, kind, dy, dlast)
+        s.forward()
+        s.backward()
+        results.append([np.delete(values(t), width + channel, axis=-1) for t in (s.h, s.last, s.f.kept_grad, s.v.kept_grad,
+                                                                                 s.initial.kept_grad)])
+    for clean, beside in zip(*results):
+        assert np.isfinite(clean).all() and (clean == beside).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("shape", [(5, 1, 70), (6, 9, 40), (7, 200, 65), (20, 400, 12), (4, 1500, 130)])
 def test_ragged(shape, kind):
     _check(shape, kind, ragged=True)
