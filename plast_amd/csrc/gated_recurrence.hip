@@ -869,9 +869,9 @@ typedef Shape<16, 8, 256, 2> LongBack;
 typedef Shape<32, 4, 64, 5> Wide;
 uint64_t columns_of(const ScanArgs &A) { return uint64_t(A.batch) * ceil_div(A.width, 64); }
 
-// Operands that the last-level cache takes are read through it, others past the caches. Through / past, us: forward and backward of
-// [5, 3001, 1003] in fp32 120 / 135, forward of [32, 512, 2048] in bf16 43 / 50; forward of [1, 65536, 1024] 103 / 98, both of
-// [8, 4096, 2048] 243 / 239.
+// Operands that the last-level cache takes are read through it, others past the caches. Through / past, us: of the operands
+// of the call before, forward and backward of [5, 3001, 1003] in fp32 106 / 134, forward of [32, 512, 2048] in bf16 37 / 43; forward of
+// [1, 65536, 1024] 103 / 98, both of [8, 4096, 2048] 243 / 239.
 constexpr uint64_t kCached = uint64_t(192) << 20;
 template <class T>
 bool past_caches(const ScanArgs &A, uint64_t operands) {
