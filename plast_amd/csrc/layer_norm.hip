@@ -529,11 +529,11 @@ __global__ __launch_bounds__(kRowBlock) void columns_kernel(NormArgs A, const fl
 // dw and db from the pieces' shares: 32 columns a workgroup, eight lanes a column, each every eighth piece.
 constexpr uint32_t kFinCols = 32, kFinParts = 8;
 template <bool ADD>
-__global__ __launch_bounds__(kFinCols * kFinParts) void join_kernel(const float *part, uint32_t pieces, uint32_t width, float *dw,
-                                                                    float *db) {
+__global__ __launch_bounds__(kFinCols * kFinParts) void join_kernel(const float *part, uint32_t pieces, uint32_t width, uint64_t first,
+                                                                    float *dw, float *db) {
   __shared__ float sums[kFinParts][kFinCols];
   const uint32_t col = threadIdx.x % kFinCols, k = threadIdx.x / kFinCols;
-  const uint64_t i = uint64_t(blockIdx.x) * kFinCols + col, n = 2 * uint64_t(width);
+  const uint64_t i = first + uint64_t(blockIdx.x) * kFinCols + col, n = 2 * uint64_t(width);
   float *to = i < width ? dw : db;
   float s = 0.0f;
   if (i < n && to)
@@ -685,8 +685,11 @@ void launch_forward(const NormArgs &A) {
 
 template <bool ADD>
 void launch_join(const NormArgs &A, const float *part, uint64_t pieces) {
-  join_kernel<ADD><<<ceil_div(2 * uint64_t(A.width), kFinCols), kFinCols * kFinParts, 0, stream()>>>(part, uint32_t(pieces),
-                                                                                                   A.width, A.dw, A.db);
+  // eight lanes a column: rows of 2^28 elements and more take several grids
+  const uint64_t n = 2 * uint64_t(A.width), most = max_blocks(kFinCols * kFinParts) * kFinCols;
+  for (uint64_t first = 0; first < n; first += most)
+    join_kernel<ADD><<<ceil_div(std::min(n - first, most), kFinCols), kFinCols * kFinParts, 0, stream()>>>(
+        part, uint32_t(pieces), A.width, first, A.dw, A.db);
 }
 
 // Rows that registers hold, eight columns a lane (16 in the longest rows): two workgroups of 512 lanes a CU.
