@@ -133,16 +133,16 @@ PLAST_HIP_KERNEL_PAIR(token_logprob)
  *         [3] stats, 2 N FLOAT32 (written by forward: the row's mean and 1 / sqrt(variance + eps);
  *             read by backward).
  * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap; it may be x itself,
- *         with its strides.
+ *         with its strides. Otherwise y and stats share no memory with the inputs or each other.
  * params.fval: eps, finite and above 0; params.keepdim: 1 makes the backward overwrite the gradients,
  * 0 accumulate into them. Sums are FLOAT32: the squares of a row's differences from its mean must fit.
  * A NaN or infinity makes its row NaN.
  * Backward, for the upstream gradient dy of x's type and shape, with n = (x - mean) * stats[1] and
  * g = dy * weight, each gradient only where its input requires one:
  *   x->grad (+)= stats[1] * (g - mean g - n mean(g n))   (x's type and shape, the last axis contiguous,
- *                                                         rows that do not overlap, nor with dy's or x's)
+ *                                                         rows that do not overlap, nor with what is read)
  *   weight->grad (+)= sum over rows of dy n,  bias->grad (+)= sum over rows of dy   (C FLOAT32 each)
- * in an order that is the same on every call. */
+ * in an order that is the same on every call; no two gradients share memory. */
 PLAST_HIP_KERNEL_PAIR(layer_norm)
 
 /* Gated linear recurrence along a sequence, each channel by itself: no reference op.

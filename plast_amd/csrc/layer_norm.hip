@@ -776,6 +776,9 @@ void layer_norm_hip_forward(const Tensor **inputs, Tensor *output, KernelParams 
       report_error(where, "the output lies in the place of x with other strides");
       return;
     }
+  const Operand y("the output", output), stats("stats", inputs[3]), at_x("x", x), w("weight", inputs[1]), b("bias", inputs[2]);
+  if (output->data != x->data && !apart(y, {&at_x}, where)) return;
+  if (!apart(y, {&w, &b, &stats}, where) || !apart(stats, {&at_x, &w, &b}, where)) return;
   if (A.rows == 0 || !ensure_init()) return;
   A.y = output->data;
   with_float_type(inputs[0]->dtype, [&](auto t) { launch_forward<decltype(t)>(A); });
@@ -812,6 +815,14 @@ void layer_norm_hip_backward(Tensor **inputs, const Tensor *output, KernelParams
     report_error(where, "weight and bias have one gradient");
     return;
   }
+  // what is joined last may lie where operands were
+  const Operand to_x("the gradient of x", dx), to_w("the gradient of weight", A.dw ? inputs[1]->grad : nullptr),
+      to_b("the gradient of bias", A.db ? inputs[2]->grad : nullptr);
+  if (dx) {
+    const Operand at_x("x", x), up("the output's gradient", dy), w("weight", inputs[1]), stats("stats", inputs[3]);
+    if (!apart(to_x, {&at_x, &up, &w, &stats, &to_w, &to_b}, where)) return;
+  }
+  if (!apart(to_w, {&to_b}, where)) return;
   if (!dx && !A.dw && !A.db) return;
   const bool add = params.keepdim != 1;
   if (!ensure_init()) return;

@@ -1,8 +1,9 @@
 // rows.hpp — what the row operators over fp32, fp16 and bf16 share: where a row of strided leading axes starts, a row's
-// units of 16 bytes, and stores that another XCD's workgroup reads within the launch.
+// units of 16 bytes, stores that another XCD's workgroup reads within the launch, and operands that may not share memory.
 #pragma once
 
 #include "half_types.hpp"
+#include "places.hpp"
 
 namespace plast {
 
@@ -70,6 +71,21 @@ __device__ __forceinline__ V get_shared(const V *p) {
 
 inline bool f32_vector(const Tensor *t, uint64_t n) {
   return t && t->device == GPU && t->dtype == FLOAT32 && numel(t) == n && contiguous(t) && (t->data || n == 0);
+}
+
+// An operand that is written, and whether it lies apart from others: reported where one shares memory with it.
+struct Operand {
+  const char *name;
+  Place place;
+  Operand(const char *name, const Tensor *t) : name(name), place(t) {}
+};
+inline bool apart(const Operand &written, std::initializer_list<const Operand *> others, const char *where) {
+  for (const Operand *o : others)
+    if (share_memory(written.place, o->place)) {
+      report_error(where, "%s shares memory with %s", written.name, o->name);
+      return false;
+    }
+  return true;
 }
 
 }  // namespace plast
