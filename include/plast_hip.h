@@ -159,7 +159,7 @@ PLAST_HIP_KERNEL_PAIR(layer_norm)
  *             is 1.
  * output: h, of f's type and shape, the last axis contiguous, steps that do not overlap, in a place of its
  * own (its grad is the upstream gradient, none counts as zero). Steps of an operand are at most 2^22 elements
- * apart.
+ * apart. What a call writes shares no memory with what it reads or else writes, `last` in initial's place aside.
  * params.dim: 1 keeps the states for a backward pass, 0 does not; params.keepdim: 1 makes the backward
  * overwrite the gradients, 0 accumulate into them.
  * A gate so far out that the smaller of a and 1 - a is below FLOAT32's range (infinities, say) selects:

@@ -929,6 +929,11 @@ void gated_recurrence_hip_forward(const Tensor **inputs, Tensor *output, KernelP
     report_error(where, "the output lies in the place of f or v");
     return;
   }
+  const Operand h("the output", output), last("the last state", inputs[4]), states("states", params.dim == 1 ? inputs[5] : nullptr),
+      f("f", inputs[0]), v("v", inputs[1]), initial("the initial state", inputs[2]), lengths("lengths", inputs[3]);
+  if (!apart(h, {&f, &v, &initial, &lengths, &last, &states}, where) || !apart(last, {&f, &v, &lengths, &states}, where) ||
+      !apart(states, {&f, &v, &initial, &lengths}, where) || (A.last != A.initial && !apart(last, {&initial}, where)))
+    return;
   if (!ensure_init()) return;
   bool ok = false;
   with_float_type(inputs[0]->dtype, [&](auto t) { ok = launch_forward<decltype(t)>(A, where); });
@@ -989,6 +994,13 @@ void gated_recurrence_hip_backward(Tensor **inputs, const Tensor *output, Kernel
       return;
     }
   }
+  const Operand to_f("the gradient of f", A.df.p ? inputs[0]->grad : nullptr), to_v("the gradient of v", A.dv.p ? inputs[1]->grad : nullptr),
+      to_initial("the initial state's gradient", A.dinitial ? inputs[2]->grad : nullptr);
+  const Operand at_f("f", f), v("v", inputs[1]), up("the output's gradient", dy), up_last("the last state's gradient", dlast),
+      states("states", inputs[5]), lengths("lengths", inputs[3]);
+  if (!apart(to_f, {&to_v, &to_initial}, where) || !apart(to_v, {&to_initial}, where)) return;
+  for (const Operand *to : {&to_f, &to_v, &to_initial})
+    if (!apart(*to, {&at_f, &v, &up, &up_last, &states, &lengths}, where)) return;
   if ((!A.df.p && !A.dv.p && !A.dinitial) || !A.batch || !A.width || !ensure_init()) return;
   bool ok = false;
   with_float_type(f->dtype, [&](auto t) {
