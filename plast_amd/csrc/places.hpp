@@ -8,6 +8,8 @@
 
 namespace plast {
 
+inline int element_bytes(const Tensor *t) { return t->dtype == INT64 ? 8 : t->dtype == FLOAT16 || t->dtype == BFLOAT16 ? 2 : 4; }
+
 // The bytes of a tensor: runs of `run` bytes, at `at` and any of the multiples below n[d] of step[d] from there, the axes
 // by falling steps. Axes whose steps leave no gap are part of the run.
 struct Place {
@@ -19,7 +21,7 @@ struct Place {
   Place() = default;
   explicit Place(const Tensor *t) {
     if (!t || !t->data || t->ndim > PLAST_MAX_NDIM) return;
-    const int bytes = t->dtype == INT64 ? 8 : t->dtype == FLOAT16 || t->dtype == BFLOAT16 ? 2 : 4;
+    const int bytes = element_bytes(t);
     at = wide(reinterpret_cast<uintptr_t>(t->data));
     wide ext[PLAST_MAX_NDIM], st[PLAST_MAX_NDIM];
     int axes = 0;
@@ -81,5 +83,30 @@ inline bool share_memory(const Place &a, const Place &b) {
   int looks = kLooks;
   return places::meet(a, 0, a.at, b, 0, b.at, looks);
 }
+
+// The first byte of a tensor and the one behind its last, what tells most operands apart; all of memory where 64 bits do not hold
+// them. Of seven operands and their pairs they take 0.1 us of a call, Places 0.5.
+struct Span {
+  int64_t lo = 0, hi = 0;  // equal: no bytes
+  explicit Span(const Tensor *t) {
+    if (!t || !t->data || t->ndim > PLAST_MAX_NDIM) return;
+    const int64_t bytes = element_bytes(t);
+    int64_t below = 0, above = 1;
+    bool over = false;
+    for (uint64_t d = 0; d < t->ndim; ++d) {
+      if (t->shape[d] == 0) return;
+      int64_t s;
+      over |= __builtin_mul_overflow(int64_t(t->strides[d]), t->shape[d] - 1, &s);
+      over |= s < 0 ? __builtin_add_overflow(below, s, &below) : __builtin_add_overflow(above, s, &above);
+    }
+    const int64_t at = int64_t(reinterpret_cast<uintptr_t>(t->data));
+    over |= __builtin_mul_overflow(below, bytes, &below);
+    over |= __builtin_mul_overflow(above, bytes, &above);
+    over |= __builtin_add_overflow(at, below, &lo);
+    over |= __builtin_add_overflow(at, above, &hi);
+    if (over) lo = INT64_MIN, hi = INT64_MAX;
+  }
+  bool meets(const Span &o) const { return lo < o.hi && o.lo < hi && lo < hi && o.lo < o.hi; }
+};
 
 }  // namespace plast

@@ -76,12 +76,13 @@ inline bool f32_vector(const Tensor *t, uint64_t n) {
 // An operand that is written, and whether it lies apart from others: reported where one shares memory with it.
 struct Operand {
   const char *name;
-  Place place;
-  Operand(const char *name, const Tensor *t) : name(name), place(t) {}
+  const Tensor *t;
+  Span span;
+  Operand(const char *name, const Tensor *t) : name(name), t(t), span(t) {}
 };
 inline bool apart(const Operand &written, std::initializer_list<const Operand *> others, const char *where) {
   for (const Operand *o : others)
-    if (share_memory(written.place, o->place)) {
+    if (written.span.meets(o->span) && share_memory(Place(written.t), Place(o->t))) {
       report_error(where, "%s shares memory with %s", written.name, o->name);
       return false;
     }

@@ -71,6 +71,7 @@ int main() {
     for (size_t i = 0; i < 40000; ++i) want = want || (used[0][i] && used[1][i]);
     if (plast::share_memory(Place(&t[0]), Place(&t[1])) != want) return fail(want ? "not seen" : "seen", t[0], t[1]);
     if (plast::share_memory(Place(&t[1]), Place(&t[0])) != want) return fail("not the same the other way", t[0], t[1]);
+    if (want && !plast::Span(&t[0]).meets(plast::Span(&t[1]))) return fail("spans do not meet", t[0], t[1]);
     (want ? shared : apart) += 1;
   }
   if (shared < 2000 || apart < 2000) return std::printf("%d shared, %d apart\n", shared, apart), 1;
