@@ -640,16 +640,34 @@ void by_parts(const NormArgs &A, uint64_t per, uint64_t threads, F &&launch) {
   }
 }
 
-// f(lanes, units) for rows of `units` units that registers hold, MOST units a lane and MOST1024 of 1024 lanes; false for longer ones.
-template <int MOST, int MOST1024, class F>
+// The shapes of rows that registers hold, lanes a row and units a lane, the first that holds a row taken; up to MOST units a lane, MOST1024
+// of 1024 lanes.
+struct Held {
+  int lanes, units;
+};
+constexpr Held kHeld[] = {{16, 1},  {16, 2},  {16, 4},  {64, 2},   {64, 4},   {256, 1},  {256, 2},
+                          {256, 4}, {512, 1}, {512, 2}, {1024, 1}, {1024, 2}, {1024, 4}, {1024, 8}};
+constexpr int kHeldShapes = sizeof kHeld / sizeof *kHeld;
+// Whether any row takes shape i: none before it holds as much.
+template <int MOST, int MOST1024>
+constexpr bool taken(int i) {
+  const auto fits = [](Held h) { return h.units <= (h.lanes == 1024 ? MOST1024 : MOST); };
+  for (int k = 0; k < i; ++k)
+    if (fits(kHeld[k]) && kHeld[k].lanes * kHeld[k].units >= kHeld[i].lanes * kHeld[i].units) return false;
+  return fits(kHeld[i]);
+}
+// f(lanes, units) for rows of `units` units; false for longer ones.
+template <int MOST, int MOST1024, int I = 0, class F>
 bool with_held(uint32_t units, F &&f) {
   using std::integral_constant;
-#define HELD(l, n) \
-  if constexpr (n <= (l == 1024 ? MOST1024 : MOST)) \
-    if (units <= l * n) { f(integral_constant<int, l>{}, integral_constant<int, n>{}); return true; }
-  HELD(16, 1) HELD(16, 2) HELD(16, 4) HELD(64, 2) HELD(64, 4) HELD(256, 1) HELD(256, 2) HELD(256, 4) HELD(512, 1) HELD(512, 2) HELD(1024, 1)
-  HELD(1024, 2) HELD(1024, 4) HELD(1024, 8)
-#undef HELD
+  if constexpr (I < kHeldShapes) {
+    if constexpr (taken<MOST, MOST1024>(I))
+      if (units <= uint32_t(kHeld[I].lanes * kHeld[I].units)) {
+        f(integral_constant<int, kHeld[I].lanes>{}, integral_constant<int, kHeld[I].units>{});
+        return true;
+      }
+    return with_held<MOST, MOST1024, I + 1>(units, f);
+  }
   return false;
 }
 
