@@ -135,7 +135,7 @@ PLAST_HIP_KERNEL_PAIR(token_logprob)
  * output: y, of x's type and shape, the last axis contiguous, rows that do not overlap; it may be x itself,
  *         with its strides. Otherwise y and stats share no memory with the inputs or each other.
  * params.fval: eps, finite and above 0; params.keepdim: 1 makes the backward overwrite the gradients,
- * 0 accumulate into them. Sums are FLOAT32: the squares of a row's differences from its mean must fit.
+ * 0 accumulate into them. Sums are FLOAT32: a row's and that of the squares of its differences from its mean must fit.
  * A NaN or infinity makes its row NaN.
  * Backward, for the upstream gradient dy of x's type and shape, with n = (x - mean) * stats[1] and
  * g = dy * weight, each gradient only where its input requires one:
@@ -170,7 +170,8 @@ PLAST_HIP_KERNEL_PAIR(layer_norm)
  *   dh[t] = dy[t] + a[t+1] dh[t+1], the gradient of `last` added at the sequence's last step;
  *   v->grad (+)= (1 - a) dh,  f->grad (+)= dh (h[t-1] - v) a (1 - a),  initial->grad (+)= a[0] dh[0].
  * All results are the same bits on every call. Calls over several chunks leave what passes from one to the next
- * in records of the library: replays of captured calls on another stream than the library's race on them. */
+ * in records of the library: replays of captured calls on another stream than the library's race on them, and
+ * their results are then wrong or NaN, with no error. */
 #define PLAST_RECURRENCE_CHUNK 64
 PLAST_HIP_KERNEL_PAIR(gated_recurrence)
 

@@ -8,11 +8,13 @@
 //
 // The memory bounds it: x read and y written, x and dy read and dx written. So rows are held in registers between their sums and
 // their results, up to 32768 elements of fp32 and 65536 of 16 bits forward and 16384 backward, and workgroups go from row to row
-// with the next rows on their way, as one row's reads, sums and stores one after the other leave the memory idle. A lane keeps its
-// columns' sums for dw and db over all of its rows. us, and TB/s of what passes the L2 caches: forward [16384, 4096] in fp32 86, 6.3;
-// in bf16 46, 5.9; backward in bf16 66, 6.4, and 5 to join the workgroups' sums; [30011, 333] in fp32 15, 5.5 and 30, 4.1, its
-// rows off the 16-byte addresses and 84 of 128 units there. Longer rows are read by a workgroup each (three times; backward once for
-// the means and once by columns): backward [512, 20000] in fp16 9 + 18, and 4 to join.
+// with the next rows on their way (forward with up to 16 columns a lane), as one row's reads, sums and stores one after the other
+// leave the memory idle. A lane keeps its columns' sums for dw and db over all of its rows. us, and TB/s of what passes the L2 caches:
+// forward [16384, 4096] in fp32 86, 6.3; in bf16 46, 5.9; backward in bf16 66, 6.4, and 5 to join the workgroups' sums; [30011, 333] in
+// fp32 15, 5.5 and 30, 4.1, its rows off the 16-byte addresses and 84 of 128 units there. Backward of 8193 to 16384 elements, 16 columns a lane,
+// is more than registers hold: 76 to 153 spill in fp32, 4 to 115 in 16 bits ([4096, 9000] in bf16 112, 32 at a copy's rate). Longer
+// rows are read by a workgroup each (three times; backward once for the means and once by columns): backward [512, 20000] in fp16
+// 9 + 18, and 4 to join.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
