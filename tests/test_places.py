@@ -1,4 +1,4 @@
-"""Whether two strided operands share memory, on the CPU (plast_amd/csrc/places.hpp, built with g++ into a small checker that
+"""Whether two strided operands share memory, on the CPU (plast_amd/csrc/places.hpp, built with g++ into a small program that
 counts bytes)."""
 from __future__ import annotations
 
